@@ -15,6 +15,7 @@ from .model import (CANONICAL_AAS, BidirectionalRunState, DmsPositionRow, EsmCon
                     dequantize_on_device, forward_bidirectional, forward_bidirectional_gpu, forward_bidirectional_q4,
                     forward_bidirectional_q8, generate_sequence, log_softmax_canonical, matmul_tiled, prompt_tokens,
                     quantize_on_device, quantize_slice_to_q4, quantize_slice_to_q8, run_pipeline_dms, save_codq)
+from .ops import Kv8Batch, Kv8Cache, Rope, token_logprobs, token_logprobs_workspace
 
 _lib.lib()  # load now: no silent fallback
 

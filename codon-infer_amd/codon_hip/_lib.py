@@ -32,10 +32,15 @@ EXPORTED = [
     "cih_quantize_q4", "cih_dequantize_q8", "cih_dequantize_q4", "cih_tokenize", "cih_log_softmax_canonical",
     "cih_profile_enable", "cih_profile_read", "cih_last_error", "cih_abi_version", "cih_dms",
     "cih_decoder_create", "cih_decoder_destroy", "cih_decoder_reset", "cih_decode", "cih_generate",
-    "cih_matmul_tiled_noalloc",
+    "cih_matmul_tiled_noalloc", "cih_rope_init", "cih_kv8_append", "cih_kv8_read", "cih_kv8_attention",
+    "cih_kv8_attention_workspace", "cih_token_logprobs", "cih_token_logprobs_workspace",
 ]
 
 DMS_MASKED_MARGINAL, DMS_WILDTYPE_MARGINAL = 0, 1
+
+F32, F16, BF16 = 0, 1, 2
+KV8_PAGE = 64
+ROPE_NONE, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
 
 
 class CihError(RuntimeError):
@@ -73,6 +78,25 @@ class KernelStats(ctypes.Structure):
                 ("bytes", ctypes.c_double)]
 
 
+class Kv8CacheStruct(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("bad", ctypes.c_void_p),
+                ("n_pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class Kv8BatchStruct(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("cu_rows", "lens", "table", "slots")] + [
+        (n, ctypes.c_int32) for n in ("n_seq", "n_rows", "max_rows", "table_rows", "table_stride", "max_pages")]
+
+
+class RowsStruct(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class RopeStruct(ctypes.Structure):
+    _fields_ = [("rot_dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("gain", ctypes.c_float),
+                ("freq", ctypes.c_double * 64)]
+
+
 _lib = None
 
 
@@ -101,6 +125,13 @@ def lib():
                          ctypes.POINTER(ctypes.c_double)],
         "cih_matmul_tiled": [i32, vp, vp, vp, vp, i32, i32, i32],
         "cih_matmul_tiled_noalloc": [i32, vp, vp, vp, vp, i32, i32, i32, vp],
+        "cih_rope_init": [vp, i32, i32, ctypes.c_double, i32, ctypes.c_double, i32],
+        "cih_kv8_append": [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp],
+        "cih_kv8_read": [vp, vp, i32, vp, vp, vp],
+        "cih_kv8_attention": [vp, vp, i32, i32, vp, vp, vp, f32, i32, i32, vp, ctypes.c_size_t, vp],
+        "cih_kv8_attention_workspace": [vp, vp, i32, ctypes.POINTER(ctypes.c_size_t)],
+        "cih_token_logprobs": [i32, vp, i64, i32, i32, vp, vp, vp, i32, vp, vp, vp, ctypes.c_size_t, vp],
+        "cih_token_logprobs_workspace": [i32, i32, i32, ctypes.POINTER(ctypes.c_size_t)],
         "cih_dequantize_device": [i32, vp, i64, vp],
         "cih_quantize_device": [i32, vp, i64, vp],
         "cih_quantize_q8": [vp, i64, vp],

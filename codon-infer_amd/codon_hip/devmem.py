@@ -5,6 +5,8 @@ outputs in HBM (the benchmark, the device-I/O tests) uses.
 """
 import ctypes
 
+import numpy as np
+
 H2D, D2H, D2D = 1, 2, 3
 
 
@@ -45,3 +47,42 @@ class Hip:
 
     def free(self, p):
         self.L.hipFree(ctypes.c_void_p(p))
+
+
+class DeviceArray:
+    """A row-major array in device memory, as the device operators take them
+    (codon_hip.ops; torch tensors on the GPU serve as well): data_ptr(), shape,
+    stride() in elements and dtype.  dtype is a numpy type, or "bfloat16" with
+    the bits held as uint16 on the host."""
+
+    def __init__(self, hip, values, dtype=None):
+        a = np.ascontiguousarray(values)
+        self._hip, self._np = hip, a.dtype
+        self.dtype = dtype or a.dtype.name
+        self.shape = a.shape
+        self._ptr = hip.malloc(a.nbytes)
+        if a.nbytes:
+            hip.h2d(self._ptr, a)
+
+    def data_ptr(self):
+        return self._ptr
+
+    def stride(self):
+        st, n = [], 1
+        for d in reversed(self.shape):
+            st.append(n)
+            n *= max(d, 1)
+        return tuple(reversed(st))
+
+    def numpy(self):
+        """The values (after what was enqueued before has run)."""
+        a = np.empty(self.shape, self._np)
+        self._hip.sync()
+        if a.nbytes:
+            self._hip.d2h(a, self._ptr)
+        return a
+
+    def free(self):
+        if self._ptr:
+            self._hip.free(self._ptr)
+            self._ptr = 0

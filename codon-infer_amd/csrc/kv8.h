@@ -1,0 +1,102 @@
+// Internal launch interface of the 8-bit paged key/value cache and of the
+// token log probabilities (not part of the C ABI).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace cih {
+
+constexpr int KV8_PAGE = 64;
+
+// dims of a head as stored: what the matrix instructions' tiles need
+__host__ __device__ constexpr int kv8_dims(int head_dim) { return head_dim == 24 ? 32 : head_dim; }
+
+// K codes [page][head][64][dp], V codes [page][head][dp][64]: a lane of an int8
+// matrix instruction reads 16 consecutive codes, along the dims for q k and
+// along the tokens for p v.
+struct Kv8View {
+    signed char *k, *v;
+    float2 *scales;  // [page][head]: of K, of V
+    unsigned long long *bad;
+    int n_pages, hk, d, dp;
+};
+
+struct Kv8Seqs {
+    const int *cu, *lens, *table, *slots;
+    int n_seq, n_rows, max_rows, table_rows, table_stride, max_pages;
+};
+
+struct RowsView {
+    void *p;
+    int64_t rs, hs;  // elements between rows, heads
+};
+
+// Rotary positions by value in the kernel arguments: turns per position.
+struct RopeArg {
+    int rot = 0, inter = 0;
+    float gain = 1.0f;
+    double turns[64] = {};
+};
+
+// A sequence of the batch as the kernels see it.
+struct Kv8Seq {
+    int r0, n;        // first row, rows
+    int start, len;   // position of the first row (may be negative), tokens held (within the table)
+    const int *table; // nullptr: no such slot
+};
+__device__ __forceinline__ Kv8Seq kv8_seq(const Kv8Seqs &s, int i) {
+    Kv8Seq q;
+    q.r0 = min(max(s.cu[i], 0), s.n_rows);
+    q.n = min(min(max(s.cu[i + 1], q.r0), s.n_rows) - q.r0, s.max_rows);
+    const int len = max(s.lens[i], 0);
+    q.start = len - q.n;
+    q.len = (int)min((int64_t)len, (int64_t)s.max_pages * KV8_PAGE);
+    const int slot = s.slots ? s.slots[i] : i;
+    q.table = slot >= 0 && slot < s.table_rows ? s.table + (int64_t)slot * s.table_stride : nullptr;
+    return q;
+}
+// The page that holds tokens 64 pg ..; -1: none
+__device__ __forceinline__ int kv8_page(const Kv8View &c, const Kv8Seq &q, int pg) {
+    const int id = q.table ? q.table[pg] : -1;
+    return id >= 0 && id < c.n_pages ? id : -1;
+}
+
+// out_h2 (dtype F32 only): out is one matrix of f16-limb rows (x3.h) of hd
+// q_heads columns, rs and hs unused.
+struct Kv8Attention {
+    Kv8View c;
+    Kv8Seqs s;
+    RowsView q, out;
+    int dtype, heads, out_h2;
+    float *lse;
+    float scale;
+    int causal, window;
+};
+
+hipError_t launch_kv8_append(const Kv8View &c, const Kv8Seqs &s, int dtype, const RowsView &k, const RowsView &v,
+                             int heads, const RowsView &q, const RowsView &qo, const RopeArg &rope, hipStream_t st);
+hipError_t launch_kv8_read(const Kv8View &c, const Kv8Seqs &s, int dtype, const RowsView &k, const RowsView &v,
+                           hipStream_t st);
+// ws: kv8_attention_floats(...) floats
+hipError_t launch_kv8_attention(const Kv8Attention &a, float *ws, hipStream_t st);
+size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads);
+
+constexpr int LOGPROBS_MAX_TOP = 64;
+struct TokenLogprobs {
+    int dtype;
+    const void *logits;
+    int64_t stride;
+    int n, vocab, top;
+    const int *targets;
+    float *logprob, *entropy;
+    int *top_ids;
+    float *top_lp;
+};
+size_t token_logprobs_floats(int n, int vocab, int top);
+hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, hipStream_t st);
+
+// Element types of the row tensors.
+enum { FT_F32 = 0, FT_F16 = 1, FT_BF16 = 2 };
+template <class T> __device__ __forceinline__ float to_f32(T x) { return (float)x; }
+
+}  // namespace cih

@@ -250,6 +250,129 @@ int cih_dequantize_device(int32_t dtype, const void *blocks, int64_t nblocks, fl
  * n must be a multiple of 32; dst holds n/32 blocks. */
 int cih_quantize_device(int32_t dtype, const float *src, int64_t n, void *dst);
 
+/* ---- 8-bit paged key/value cache -------------------------------------------
+ * No counterpart in the reference, whose RunState keeps K and V in FP32
+ * (lib.rs:2464-2486).  Keys and values are held as 8-bit codes with one FP32
+ * scale for each page of CIH_KV8_PAGE tokens, head, and K or V: value = code *
+ * scale, codes -127..127.  A sequence's tokens live in the pages that its row
+ * of a page table names, in order: token p in page table[p / 64] at p % 64.
+ *
+ * Every pointer in the structures below is a DEVICE pointer on the current
+ * device; calls are enqueued on `stream` (a hipStream_t of that device; NULL =
+ * the null stream), return without waiting, allocate nothing and keep nothing
+ * between calls, so that they may be captured into a graph.  Sizes on the host
+ * (n_seq, n_rows, max_rows, max_pages) fix the grids; row offsets, lengths and
+ * tables are read on the device when the kernels run. */
+
+enum cih_float { CIH_F32 = 0, CIH_F16 = 1, CIH_BF16 = 2 };
+
+#define CIH_KV8_PAGE 64
+
+/* head_dim is 16, 24, 32, 64 or 128; dims = head_dim, but 32 for 24.  k and v
+ * 16-byte aligned, bad and scales 8-byte.  The memory need not be initialised:
+ * a page's first append writes its scales, and codes of tokens past a
+ * sequence's length are never used.  bad bit t: token t of the page had a
+ * value that is not finite in K or V of that head (its codes are 0 and it
+ * reads as NaN). */
+typedef struct cih_kv8_cache {
+    void *k;        /* int8 [n_pages][kv_heads][64][dims]  */
+    void *v;        /* int8 [n_pages][kv_heads][dims][64]  */
+    float *scales;  /* [n_pages][kv_heads][2]: of K, of V  */
+    uint64_t *bad;  /* [n_pages][kv_heads]                 */
+    int32_t n_pages, kv_heads, head_dim;
+} cih_kv8_cache;
+
+/* n_seq sequences with rows cu_rows[i] .. cu_rows[i + 1] of the row tensors
+ * (at most max_rows each; rows from n_rows on are never touched).  lens[i]:
+ * tokens the sequence holds including these rows, which are its last ones: its
+ * row r has position lens[i] - rows + r.  Sequence i uses row slots[i] (NULL:
+ * i) of the page table, which has table_rows rows of max_pages page ids,
+ * table_stride apart.  Tokens past max_pages * 64, and tokens whose page id is
+ * outside [0, n_pages) or whose slot is outside [0, table_rows), are treated
+ * as not there; rows at negative positions see nothing and are not stored. */
+typedef struct cih_kv8_batch {
+    const int32_t *cu_rows; /* [n_seq + 1] */
+    const int32_t *lens;    /* [n_seq]     */
+    const int32_t *table;   /* [table_rows][table_stride] */
+    const int32_t *slots;   /* [n_seq] or NULL */
+    int32_t n_seq, n_rows, max_rows;
+    int32_t table_rows, table_stride, max_pages;
+} cih_kv8_batch;
+
+/* Rows of heads: element (row, head, dim) at data[row * row_stride + head *
+ * head_stride + dim] (strides in elements; the data aligned to its type). */
+typedef struct cih_rows {
+    void *data;
+    int64_t row_stride, head_stride;
+} cih_rows;
+
+/* Rotary positions: pair j < rot_dim / 2 of a head turns by position * freq[j]
+ * radians, both values times gain.  The pair is (j, j + rot_dim / 2), or with
+ * interleaved (2 j, 2 j + 1); dims from rot_dim on stay as they are. */
+typedef struct cih_rope {
+    int32_t rot_dim, interleaved;
+    float gain;
+    double freq[64];
+} cih_rope;
+
+enum cih_rope_scaling { CIH_ROPE_NONE = 0, CIH_ROPE_LINEAR = 1, CIH_ROPE_NTK = 2, CIH_ROPE_YARN = 3 };
+
+/* Host: fills r for rot_dim dims (even, 2..128).  freq[j] = base^(-2j/rot_dim);
+ * LINEAR: divided by factor (position interpolation); NTK: base *
+ * factor^(rot_dim / (rot_dim - 2)) in place of base (rot_dim >= 4); YARN
+ * (Peng et al. 2023): with g = clamp((trained_len freq / 2 pi - 1) / 31, 0, 1),
+ * freq ((1 - g) / factor + g), gain = 0.1 ln(factor) + 1.  factor >= 1;
+ * trained_len >= 1 where YARN reads it. */
+int cih_rope_init(cih_rope *r, int32_t rot_dim, int32_t interleaved, double base, int32_t scaling, double factor,
+                  int32_t trained_len);
+
+/* Writes the batch's rows of K and V (kv_heads heads of head_dim, element type
+ * dtype, a cih_float) into the cache at their positions, K rotated if rope is
+ * not NULL.  A page that keeps tokens from before the sequence's first row
+ * keeps at least their scale; where a new row exceeds it the kept codes are
+ * rounded again to the larger one.  Later tokens of the page are forgotten.
+ * With q (q_heads heads; NULL: none) the rows of q are written to q_out (may
+ * be q), rotated by the same positions.  Two sequences of a batch must not
+ * write the same page. */
+int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
+                   const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out, const cih_rope *rope,
+                   void *stream);
+
+/* The batch's rows read back from the cache as values of type dtype (K as
+ * stored, rotated); a bad token's values are NaN.  Rows that are not there
+ * are left untouched. */
+int cih_kv8_read(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
+                 const cih_rows *v, void *stream);
+
+/* Attention of the batch's rows over the cache: head h of q_heads (a multiple
+ * of kv_heads) reads head h / (q_heads / kv_heads).  A row at position p sees
+ * tokens j < lens[i], with causal only j <= p, with window > 0 only j > p -
+ * window.  out = sum softmax(scale q.k) v in q's type; lse (NULL: none) [n_rows][q_heads] the
+ * logarithm of the sum of exp(scale q.k).  A row that sees nothing gets out 0
+ * and lse -inf, one that sees a bad token NaN.  workspace: 16-byte aligned, of the size
+ * cih_kv8_attention_workspace gives for the same sizes (it reads no device
+ * memory); calls that may run at the same time (other streams, two graphs)
+ * need one each. */
+int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
+                      const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal, int32_t window,
+                      void *workspace, size_t workspace_bytes, void *stream);
+int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t q_heads, size_t *bytes);
+
+/* ---- log probabilities of given tokens ----------------------------------------
+ * Beside log_softmax_canonical (lib.rs:4426-4441), over the whole vocabulary.
+ * For each row of logits [n_rows][vocab] (type dtype, rows row_stride elements
+ * apart): logprob = log softmax at targets[row]; entropy = -sum p log p (in
+ * nats); the top_k <= 64 largest logits (ties: lowest id first) as top_ids
+ * [n_rows][top_k] and their log probabilities top_logprobs.  logprob, entropy and the
+ * top pair may each be NULL.  Device pointers, as above.  A negative target
+ * gives 0, one >= vocab NaN.  -inf logits have probability 0: fewer than top_k
+ * others leave ids -1 and -inf at the end.  A row of -inf only: entropy 0,
+ * logprob -inf; a row with NaN or +inf: NaN and ids -1. */
+int cih_token_logprobs(int32_t dtype, const void *logits, int64_t row_stride, int32_t n_rows, int32_t vocab,
+                       const int32_t *targets, float *logprob, float *entropy, int32_t top_k, int32_t *top_ids,
+                       float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);
+int cih_token_logprobs_workspace(int32_t n_rows, int32_t vocab, int32_t top_k, size_t *bytes);
+
 /* ---- host helpers (no GPU) ---------------------------------------------- */
 
 /* quantize_slice_to_q8 / quantize_slice_to_q4 (lib.rs:670-673, 1085-1088);

@@ -112,6 +112,61 @@ pub struct cih_kernel_stats {
     pub bytes: f64,
 }
 
+pub const CIH_F32: i32 = 0;
+pub const CIH_F16: i32 = 1;
+pub const CIH_BF16: i32 = 2;
+pub const CIH_KV8_PAGE: i32 = 64;
+pub const CIH_ROPE_NONE: i32 = 0;
+pub const CIH_ROPE_LINEAR: i32 = 1;
+pub const CIH_ROPE_NTK: i32 = 2;
+pub const CIH_ROPE_YARN: i32 = 3;
+
+/// The 8-bit paged key/value cache (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct cih_kv8_cache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub scales: *mut f32,
+    pub bad: *mut u64,
+    pub n_pages: i32,
+    pub kv_heads: i32,
+    pub head_dim: i32,
+}
+
+/// Sequences with their new rows, lengths and page tables (device pointers).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct cih_kv8_batch {
+    pub cu_rows: *const i32,
+    pub lens: *const i32,
+    pub table: *const i32,
+    pub slots: *const i32,
+    pub n_seq: i32,
+    pub n_rows: i32,
+    pub max_rows: i32,
+    pub table_rows: i32,
+    pub table_stride: i32,
+    pub max_pages: i32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct cih_rows {
+    pub data: *mut c_void,
+    pub row_stride: i64,
+    pub head_stride: i64,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct cih_rope {
+    pub rot_dim: i32,
+    pub interleaved: i32,
+    pub gain: f32,
+    pub freq: [f64; 64],
+}
+
 #[repr(C)]
 pub struct cih_model {
     _private: [u8; 0],
@@ -152,6 +207,24 @@ extern "C" {
                             out_dim: i32, seq_len: i32) -> c_int;
     pub fn cih_matmul_tiled_noalloc(dtype: i32, out: *mut f32, x: *const f32, w: *const c_void, bias: *const f32,
                                     in_dim: i32, out_dim: i32, seq_len: i32, stream: *mut c_void) -> c_int;
+    pub fn cih_rope_init(r: *mut cih_rope, rot_dim: i32, interleaved: i32, base: f64, scaling: i32, factor: f64,
+                         trained_len: i32) -> c_int;
+    pub fn cih_kv8_append(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, dtype: i32, k: *const cih_rows,
+                          v: *const cih_rows, q_heads: i32, q: *const cih_rows, q_out: *const cih_rows,
+                          rope: *const cih_rope, stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_read(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, dtype: i32, k: *const cih_rows,
+                        v: *const cih_rows, stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_attention(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, dtype: i32, q_heads: i32,
+                             q: *const cih_rows, out: *const cih_rows, lse: *mut f32, scale: f32, causal: i32,
+                             window: i32, workspace: *mut c_void, workspace_bytes: usize,
+                             stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_attention_workspace(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, q_heads: i32,
+                                       bytes: *mut usize) -> c_int;
+    pub fn cih_token_logprobs(dtype: i32, logits: *const c_void, row_stride: i64, n_rows: i32, vocab: i32,
+                              targets: *const i32, logprob: *mut f32, entropy: *mut f32, top_k: i32,
+                              top_ids: *mut i32, top_logprobs: *mut f32, workspace: *mut c_void,
+                              workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn cih_token_logprobs_workspace(n_rows: i32, vocab: i32, top_k: i32, bytes: *mut usize) -> c_int;
     pub fn cih_dequantize_device(dtype: i32, blocks: *const c_void, nblocks: i64, out: *mut f32) -> c_int;
     pub fn cih_quantize_device(dtype: i32, src: *const f32, n: i64, dst: *mut c_void) -> c_int;
 

@@ -1,0 +1,105 @@
+"""Log probabilities of given tokens, entropy and top alternatives on the GPU
+(cih_token_logprobs) against the restatement in 64 bits.
+
+Tolerances: a sum of at most V exponentials in FP32 by lanes and trees of at
+most 2^-24 (V / 64 + 32) relative, log and exp 2^-22 each, the difference
+x - lse one rounding of |x| + |lse|: below 2^-18 (1 + |x| + |lse|) for V up to
+140000.  The entropy adds the products p x, with |x - max| up to the logits' range.
+"""
+import numpy as np
+import pytest
+
+import codon_hip as ch
+import kv8_ref as R
+from codon_hip.devmem import DeviceArray, Hip
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    return Hip()
+
+
+def run(hip, x, targets, k, dtype, stride=None, want=("logprob", "entropy", "top")):
+    n, vocab = x.shape
+    stride = stride or vocab
+    wide = np.full((n, stride), 1e4)
+    wide[:, :vocab] = x
+    base = R.put(hip, wide, dtype)
+    x = R.rounded(x, dtype)
+    logits = R.View(base, 0, (n, vocab), (stride, 1))
+    t = None if targets is None else DeviceArray(hip, np.asarray(targets, np.int32))
+    lp, en = [DeviceArray(hip, np.full(n, 7, np.float32)) for _ in range(2)]
+    ids, top = DeviceArray(hip, np.full((n, k), 7, np.int32)), DeviceArray(hip, np.full((n, k), 7, np.float32))
+    ws = DeviceArray(hip, np.full(ch.token_logprobs_workspace(n, vocab, k) + 16, 255, np.uint8))
+    pair = (ids, top) if "top" in want else (None, None)
+    ch.token_logprobs(logits, t, lp if "logprob" in want else None, en if "entropy" in want else None, *pair, workspace=ws)
+    g = [a.numpy() for a in (lp, en, ids, top)]
+    ref = R.logprobs(x, targets, k)
+    fin = np.where(np.isfinite(x), np.abs(x), 0).max(initial=0)
+    tol = 2.0 ** -18 * (1 + 2 * fin + np.log(vocab))
+    for name, got, want_ in (("logprob", g[0], ref[0]), ("entropy", g[1], ref[1]), ("top", g[3], ref[3])):
+        if name not in want:
+            assert (got == 7).all()
+            continue
+        assert np.array_equal(np.isnan(got), np.isnan(want_)), name
+        assert np.array_equal(np.isneginf(got), np.isneginf(want_)), name
+        f = np.isfinite(want_)
+        assert np.abs(got[f] - want_[f]).max(initial=0) <= tol, (name, np.abs(got[f] - want_[f]).max(), tol)
+    if "top" in want:
+        assert np.array_equal(g[2], ref[2]), np.argwhere(g[2] != ref[2])[:5]
+    R.free(base, lp, en, ids, top, ws, *([] if t is None else [t]))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n,vocab,k", [(1, 1, 1), (5, 2, 2), (8, 33, 5), (70, 33, 33), (3, 64, 20), (3, 65, 64), (9, 257, 8),
+                                       (4, 1000, 32), (2, 1023, 1), (2, 1025, 40), (3, 4097, 20), (2, 16385, 20), (2, 33000, 7),
+                                       (2, 70001, 64), (1, 140000, 20), (600, 1500, 3), (1100, 40, 4)])
+def test_random(hip, dtype, n, vocab, k):
+    rng = np.random.default_rng(vocab)
+    run(hip, 3 * rng.standard_normal((n, vocab)), rng.integers(0, vocab, n), k, dtype)
+
+
+@pytest.mark.parametrize("vocab", [33, 60, 300, 5000, 20000, 70000])
+def test_ties(hip, vocab):
+    """Equal logits: the lowest ids, also where every logit is the same."""
+    rng = np.random.default_rng(1)
+    x = rng.integers(0, 4, (4, vocab)).astype(float)
+    x[1] = 2.5
+    x[2] = -np.arange(vocab) // 7
+    x[3] = np.arange(vocab) // 7 * 0.25
+    run(hip, x, rng.integers(0, vocab, 4), min(vocab, 30), "float32")
+
+
+@pytest.mark.parametrize("vocab", [33, 200, 5000, 70000])
+def test_masked_lost_and_odd_rows(hip, vocab):
+    """Rows of -inf but one, few or none; the type's lowest values; NaN and infinities; targets outside; wide ranges."""
+    rng = np.random.default_rng(2)
+    x = 3 * rng.standard_normal((12, vocab))
+    x[0] = -np.inf
+    x[1, :-1] = -np.inf
+    x[2, 3:] = -np.inf
+    x[3, ::2] = -np.inf
+    x[4, 7] = np.nan
+    x[5, vocab - 1] = np.inf
+    x[6, :5] = np.finfo(np.float32).min
+    x[7] = np.finfo(np.float32).min
+    x[8] *= 30
+    x[9] += 1000
+    x[10, vocab // 2:] = np.nan
+    t = rng.integers(0, vocab, 12)
+    t[1], t[2], t[3] = vocab - 1, 5, 0
+    run(hip, x, t, 20, "float32")
+    t[:] = -1
+    t[9], t[10], t[11] = vocab, vocab + 5, -2 ** 31
+    run(hip, x, t, 1, "float32")
+
+
+def test_outputs_left_out_and_strides(hip):
+    rng = np.random.default_rng(3)
+    for vocab in (33, 1000, 40001):
+        x = rng.standard_normal((6, vocab))
+        for want in (("logprob",), ("entropy",), ("top",), ("logprob", "top")):
+            run(hip, x, rng.integers(0, vocab, 6) if "logprob" in want else None, 4, "bfloat16", stride=vocab + 7, want=want)
+        run(hip, x, rng.integers(0, vocab, 6), 0, "float16", stride=vocab + 1, want=("logprob", "entropy"))
