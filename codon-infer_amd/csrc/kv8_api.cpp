@@ -236,7 +236,7 @@ int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, in
 
 int cih_token_logprobs_workspace(int32_t n_rows, int32_t vocab, int32_t top_k, size_t *bytes) {
     if (!bytes) return set_error(CIH_ERR_ARG, "null bytes");
-    if (n_rows < 0 || vocab < 1) return set_error(CIH_ERR_SHAPE, "%d rows of %d logits", n_rows, vocab);
+    if (n_rows < 0 || vocab < 1 || vocab > 1 << 30) return set_error(CIH_ERR_SHAPE, "%d rows of %d logits", n_rows, vocab);
     if (top_k < 0 || top_k > LOGPROBS_MAX_TOP) return set_error(CIH_ERR_SHAPE, "top_k %d outside [0, %d]", top_k, LOGPROBS_MAX_TOP);
     *bytes = token_logprobs_floats(n_rows, vocab, top_k) * sizeof(float);
     return CIH_OK;

@@ -360,8 +360,8 @@ int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch 
 
 /* ---- log probabilities of given tokens ----------------------------------------
  * Beside log_softmax_canonical (lib.rs:4426-4441), over the whole vocabulary.
- * For each row of logits [n_rows][vocab] (type dtype, rows row_stride elements
- * apart): logprob = log softmax at targets[row]; entropy = -sum p log p (in
+ * For each row of logits [n_rows][vocab] (vocab <= 2^30, type dtype, rows
+ * row_stride elements apart): logprob = log softmax at targets[row]; entropy = -sum p log p (in
  * nats); the top_k <= 64 largest logits (ties: lowest id first) as top_ids
  * [n_rows][top_k] and their log probabilities top_logprobs.  logprob, entropy and the
  * top pair may each be NULL.  Device pointers, as above.  A negative target
