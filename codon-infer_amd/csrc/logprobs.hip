@@ -3,8 +3,7 @@
 // One pass over a row with the running maximum m: u = (x - m) log2 e, s = sum
 // 2^u, t = sum 2^u u; then
 //   log p(i) = x_i - m - ln 2 log2 s,  entropy = ln 2 (log2 s - t / s).
-// A NaN or +inf anywhere makes s NaN.  Bound by reading the logits once; what
-// the alternatives add is one comparison a thread and tile (see below).
+// A NaN or +inf anywhere makes s NaN.  Bound by reading the logits once.
 #include <limits.h>
 
 #include <algorithm>
@@ -137,169 +136,200 @@ template <class T> struct Vec {
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
 };
 
-constexpr int LP_VECS = 4;   // 16-byte loads of a thread in a tile
-constexpr int LP_CAP = 768;  // candidates
+// Logits of a thread in a tile, in 16-byte loads: 16 leave registers for 16
+// waves a CU (512 rows of 131072 bfloat16 logits: 42.4 us, with 32 logits 43.6, with 8 47.8).
+constexpr int LP_EACH = 16;
+constexpr int LP_CAP = 768;  // list entries
 
 // The row (or the chunk blockIdx % chunks of its tiles) by NT threads.
 //
-// Alternatives.  `bar` is a logit that top_k found ones reach.  A tile without
-// a logit above it costs one comparison a thread; otherwise the logits above
-// go to a list in LDS.  A tile with more than fit (the first, or one of a row
-// that ascends) first raises the bar to the top_k-th largest of 64 threads'
-// maxima, the best of the waves'; if that leaves too many (ties), the tile's
-// top_k are taken one by one.  The list is put in order, and the bar raised to
-// its top_k-th, when it is full and at the end.
+// Alternatives.  In the pass a thread keeps only its largest logit and the
+// 16-byte vector it came from.  Vectors are numbered in the logits' order, so
+// (logit, vector) orders the threads' bests as the logits are ordered: the
+// top_k-th of them, `least`, is a bound that the row's top_k reach, and they all
+// are among the vectors of the top_k threads that reach it.  Those threads' vectors
+// (top_k / NT of the row, in L2 by then) are read again, and what reaches `least`
+// goes to a list, about top_k logits.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void k_logprobs(TokenLogprobs a, int chunks, int tiles_per, float *__restrict__ ws) {
-    constexpr int VL = Vec<T>::N, TILE = NT * LP_VECS * VL, NW = NT / 64;
-    __shared__ u64 list[LP_CAP], best[LOGPROBS_MAX_TOP], kw[NW];
-    __shared__ int ranks[LP_CAP], iw[NW], s_cnt;
-    __shared__ float fw[NW], sw[NW][3];
+    constexpr int VL = Vec<T>::N, LP_VECS = LP_EACH / VL, TILE = NT * LP_EACH, NW = NT / 64;
+    static_assert(64 * VL + LOGPROBS_MAX_TOP <= LP_CAP && NW * LOGPROBS_MAX_TOP <= LP_CAP, "the list holds a wave's vectors");
+    __shared__ u64 list[LP_CAP], best[LOGPROBS_MAX_TOP];
+    __shared__ int ranks[LP_CAP], owner[LOGPROBS_MAX_TOP], iw[NW], s_cnt;
+    __shared__ float sw[NW][3];
     const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const T *p = static_cast<const T *>(a.logits) + row * a.stride;
     const int top = a.top;
-    const int64_t begin = (int64_t)chunk * tiles_per * TILE;
-    const int end = (int)min((int64_t)a.vocab, begin + (int64_t)tiles_per * TILE);
+    const int begin = (int)((int64_t)chunk * tiles_per * TILE);
+    const int end = (int)min((int64_t)a.vocab, (int64_t)begin + (int64_t)tiles_per * TILE);
     Sums v;
-    float bar = -INFINITY;
-    int cur = 0;  // list entries; uniform
-    if (tid == 0) s_cnt = 0;
+    float most = -INFINITY;
+    int from = 0;  // its vector's number / NT
 
-    // a count summed over the workgroup (every thread calls it)
-    auto total = [&](int c) {
-        int n = 0;
-        __syncthreads();
-        c = (int)wave_butterfly((float)c);
-        if (NW == 1) return c;
-        if (lane == 0) iw[wave] = c;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; w++) n += iw[w];
-        return n;
-    };
-    // the list's best in order in best[] and at its front, cut to top; an
-    // entry's place is the number of better ones, counted by NT / cur threads
-    auto sort_list = [&]() {
-        __syncthreads();
-        for (int i = tid; i < cur; i += NT) ranks[i] = 0;
-        __syncthreads();
-        if (cur > 0) {
-            const int parts = max(1, NT / cur), len = (cur + parts - 1) / parts;
-            for (int x = tid; x < cur * parts; x += NT) {
-                const int part = x / cur, i = x - part * cur, j1 = min(cur, (part + 1) * len);
-                const u64 k = list[i];
-                int r = 0;
-                for (int j = part * len; j < j1; j++) r += list[j] > k ? 1 : 0;
-                atomicAdd(&ranks[i], r);
-            }
-        }
-        __syncthreads();
-        for (int i = tid; i < cur; i += NT)
-            if (ranks[i] < top) best[ranks[i]] = list[i];
-        __syncthreads();
-        cur = min(cur, top);
-        if (tid < cur) list[tid] = best[tid];
-        if (tid == 0) s_cnt = cur;
-        if (cur == top) bar = key_value(best[top - 1]);
-        __syncthreads();
-    };
-
-    for (int base = (int)begin; base < end; base += TILE) {
-        float x[LP_VECS * VL];
-        int at[LP_VECS];
-#pragma unroll
-        for (int u = 0; u < LP_VECS; u++) {
-            at[u] = base + (u * NT + tid) * VL;
-            if (at[u] + VL <= end) {
-                const typename Vec<T>::type w = *reinterpret_cast<const typename Vec<T>::type *>(p + at[u]);
-#pragma unroll
-                for (int e = 0; e < VL; e++) x[u * VL + e] = to_f32(w[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VL; e++) x[u * VL + e] = at[u] + e < end ? to_f32(p[at[u] + e]) : -INFINITY;
-            }
-        }
+    auto add = [&](const float (&x)[LP_EACH], int tile) __attribute__((always_inline)) {
         float bm = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < LP_VECS * VL; e++) bm = fmaxf(bm, x[e]);
+        for (int u = 0; u < LP_VECS; u++) {
+            float m = x[u * VL];
+#pragma unroll
+            for (int e = 1; e < VL; e++) m = fmaxf(m, x[u * VL + e]);
+            if (m > most) {
+                most = m;
+                from = tile * LP_VECS + u;
+            }
+            bm = fmaxf(bm, m);
+        }
         v.rebase(bm);
         const float off = v.m == -INFINITY ? 0.0f : v.m;
 #pragma unroll
-        for (int e = 0; e < LP_VECS * VL; e++) {
+        for (int e = 0; e < LP_EACH; e++) {
             const float u = (x[e] - off) * LOG2E, y = __builtin_amdgcn_exp2f(u);
             v.s += y;
             v.t = fmaf(y, fmaxf(u, U_MIN), v.t);
         }
-        if (top == 0) continue;
-        if (!__syncthreads_or(bm > bar)) continue;
-        // logits that count: above bar, and not below floor
-        float floor = -INFINITY;
-        auto count = [&]() {
-            int c = 0;
+    };
+    const int whole = (end - begin) / TILE;
+    for (int t = 0; t < whole; t++) {
+        float x[LP_EACH];
 #pragma unroll
-            for (int e = 0; e < LP_VECS * VL; e++) c += x[e] > bar && x[e] >= floor ? 1 : 0;
-            return total(c);
-        };
-        int n = count();
-        if (cur + n > LP_CAP) {
-            // the top-th largest of a wave's 64 maxima, bit by bit
-            const unsigned key = order32(bm);
-            unsigned k = 0;
-#pragma unroll 1
-            for (int bit = 31; bit >= 0; bit--) {
-                const unsigned t = k | 1u << bit;
-                if (__popcll(__ballot(key >= t)) >= top) k = t;
-            }
-            floor = k == 0 ? -INFINITY : order32_value(k);
-            if (NW > 1) {
-                __syncthreads();
-                if (lane == 0) fw[wave] = floor;
-                __syncthreads();
+        for (int u = 0; u < LP_VECS; u++) {
+            const typename Vec<T>::type w =
+                *reinterpret_cast<const typename Vec<T>::type *>(p + begin + t * TILE + (u * NT + tid) * VL);
 #pragma unroll
-                for (int w = 0; w < NW; w++) floor = fmaxf(floor, fw[w]);
-            }
-            sort_list();
-            n = count();
+            for (int e = 0; e < VL; e++) x[u * VL + e] = to_f32(w[e]);
         }
-        if (cur + n <= LP_CAP) {
-#pragma unroll
-            for (int e = 0; e < LP_VECS * VL; e++)
-                if (x[e] > bar && x[e] >= floor) list[atomicAdd(&s_cnt, 1)] = place_key(x[e], at[e / VL] + e % VL);
-            cur += n;
-        } else {
-            u64 last = ~0ull;
-            for (int k = 0; k < top; k++) {
-                u64 y = 0;
-#pragma unroll
-                for (int e = 0; e < LP_VECS * VL; e++) {
-                    const u64 z = place_key(x[e], at[e / VL] + e % VL);
-                    if (x[e] > bar && z < last && z > y) y = z;
-                }
-#pragma unroll
-                for (int o = 32; o > 0; o >>= 1) y = max(y, (u64)__shfl_xor(y, o));
-                __syncthreads();
-                if (lane == 0) kw[wave] = y;
-                __syncthreads();
-                for (int w = 0; w < NW; w++) y = max(y, kw[w]);
-                if (y == 0) break;
-                last = y;
-                if (tid == 0) list[cur] = y;
-                cur++;
-            }
-            __syncthreads();
-            if (tid == 0) s_cnt = cur;
-        }
+        add(x, t);
     }
-
+    if (begin + whole * TILE < end) {
+        float x[LP_EACH];
+#pragma unroll
+        for (int u = 0; u < LP_VECS; u++) {
+            const int i = begin + whole * TILE + (u * NT + tid) * VL;
+            if (i + VL <= end) {
+                const typename Vec<T>::type w = *reinterpret_cast<const typename Vec<T>::type *>(p + i);
+#pragma unroll
+                for (int e = 0; e < VL; e++) x[u * VL + e] = to_f32(w[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VL; e++) x[u * VL + e] = i + e < end ? to_f32(p[i + e]) : -INFINITY;
+            }
+        }
+        add(x, whole);
+    }
     v = wave_sums(v);
     if (lane == 0) {
         sw[wave][0] = v.m;
         sw[wave][1] = v.s;
         sw[wave][2] = v.t;
     }
-    if (top > 0) sort_list();
-    else __syncthreads();
+
+    int cur = 0;  // list entries; uniform
+    u64 bar = 0;  // the last of the top_k that a cut left
+    if (top > 0) {
+        // the list's best in order in best[] and at its front, cut to top; an
+        // entry's place is the number of better ones, counted by NT / cur threads
+        auto sort_list = [&]() {
+            __syncthreads();
+            for (int i = tid; i < cur; i += NT) ranks[i] = 0;
+            __syncthreads();
+            if (cur > 0) {
+                const int parts = max(1, NT / cur), len = (cur + parts - 1) / parts;
+                for (int x = tid; x < cur * parts; x += NT) {
+                    const int part = x / cur, i = x - part * cur, j1 = min(cur, (part + 1) * len);
+                    const u64 k = list[i];
+                    int r = 0;
+                    for (int j = part * len; j < j1; j++) r += list[j] > k ? 1 : 0;
+                    atomicAdd(&ranks[i], r);
+                }
+            }
+            __syncthreads();
+            for (int i = tid; i < cur; i += NT)
+                if (ranks[i] < top) best[ranks[i]] = list[i];
+            __syncthreads();
+            cur = min(cur, top);
+            if (tid < cur) list[tid] = best[tid];
+            if (tid == 0) s_cnt = cur;
+            if (cur == top) bar = best[top - 1];
+            __syncthreads();
+        };
+        // a count summed over the workgroup
+        auto total = [&](int c) {
+            int n = 0;
+            c = (int)wave_butterfly((float)c);
+            if (NW == 1) return c;
+            __syncthreads();
+            if (lane == 0) iw[wave] = c;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NW; w++) n += iw[w];
+            return n;
+        };
+        // each wave's best threads, then the best of these
+        const u64 mine = most == -INFINITY ? 0 : (u64)order32(most) << 32 | (0xffffffffu - (unsigned)(from * NT + tid));
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < 64; j++) {
+            const u64 o = (u64)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 |
+                          (unsigned)__builtin_amdgcn_readlane((int)mine, j);
+            rank += o > mine ? 1 : 0;
+        }
+        if (tid == 0) s_cnt = 0;
+        __syncthreads();
+        if (mine != 0 && rank < top) list[atomicAdd(&s_cnt, 1)] = mine;
+        __syncthreads();
+        cur = s_cnt;
+        sort_list();
+        const int owners = cur;
+        const u64 least = owners > 0 ? best[owners - 1] : ~0ull;  // fewer than top_k: all that is finite counts
+        if (tid < owners) owner[tid] = (int)((0xffffffffu - (unsigned)best[tid]) % NT);
+        cur = 0;
+        bar = 0;
+        if (tid == 0) s_cnt = 0;
+        __syncthreads();
+        const int vecs = ((end - begin) + NT * VL - 1) / (NT * VL);  // of a thread
+        for (int w0 = 0; w0 < owners * vecs; w0 += NT) {
+            const int w = w0 + tid, f = w / vecs, s = w - f * vecs;
+            const int n = f < owners ? s * NT + owner[f] : 0, i = begin + n * VL;  // vector, its first logit
+            float x[VL];
+            if (f < owners && i + VL <= end) {
+                const typename Vec<T>::type q = *reinterpret_cast<const typename Vec<T>::type *>(p + i);
+#pragma unroll
+                for (int e = 0; e < VL; e++) x[e] = to_f32(q[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < VL; e++) x[e] = f < owners && i + e < end ? to_f32(p[i + e]) : -INFINITY;
+            }
+            auto counts = [&](int e) __attribute__((always_inline)) {
+                const u64 coarse = (u64)order32(x[e]) << 32 | (0xffffffffu - (unsigned)n);
+                return x[e] > -INFINITY && (coarse >= least || owners < top) && place_key(x[e], i + e) > bar;
+            };
+            int c = 0;
+#pragma unroll
+            for (int e = 0; e < VL; e++) c += counts(e) ? 1 : 0;
+            c = total(c);
+            auto push = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int e = 0; e < VL; e++)
+                    if (counts(e)) list[atomicAdd(&s_cnt, 1)] = place_key(x[e], i + e);
+            };
+            if (cur + c <= LP_CAP) {
+                push();
+                cur += c;
+            } else {  // wave by wave, each after a cut
+                for (int y = 0; y < NW; y++) {
+                    sort_list();
+                    if (wave == y) push();
+                    __syncthreads();
+                    cur = s_cnt;
+                }
+            }
+        }
+        sort_list();
+    } else {
+        __syncthreads();
+    }
+
     v = Sums{sw[0][0], sw[0][1], sw[0][2]};
 #pragma unroll
     for (int w = 1; w < NW; w++) v.add(Sums{sw[w][0], sw[w][1], sw[w][2]});
@@ -360,11 +390,10 @@ template <class T> __global__ __launch_bounds__(JOIN_THREADS) void k_logprobs_jo
 struct LpPlan {
     int nt, chunks, tiles_per;
 };
-LpPlan lp_plan(int n, int vocab, int top, int elem) {
-    const int per = LP_VECS * 16 / elem;  // logits of a thread in a tile
+LpPlan lp_plan(int n, int vocab, int top) {
     LpPlan p;
-    p.nt = vocab <= 64 * per ? 64 : vocab <= 512 * per ? 256 : 512;
-    const int tiles = (vocab + p.nt * per - 1) / (p.nt * per);
+    p.nt = vocab <= 2048 ? 64 : vocab <= 16384 ? 256 : 512;
+    const int tiles = (vocab + p.nt * LP_EACH - 1) / (p.nt * LP_EACH);
     const int most = top > 0 ? JOIN_MAX / top : 64;
     p.chunks = n >= 512 ? 1 : std::min(std::min(tiles, most), (767 + n) / n);
     p.tiles_per = (tiles + p.chunks - 1) / p.chunks;
@@ -378,7 +407,7 @@ template <class T> hipError_t launch_lp(const TokenLogprobs &a, float *ws, hipSt
                            st, a);
         return hipGetLastError();
     }
-    const LpPlan p = lp_plan(a.n, a.vocab, a.top, sizeof(T));
+    const LpPlan p = lp_plan(a.n, a.vocab, a.top);
     if ((int64_t)a.n * p.chunks > INT32_MAX) return hipErrorInvalidValue;
     const dim3 grid(a.n * p.chunks);
     if (p.nt == 64) hipLaunchKernelGGL((k_logprobs<T, 64>), grid, dim3(64), 0, st, a, p.chunks, p.tiles_per, ws);
@@ -394,12 +423,8 @@ template <class T> hipError_t launch_lp(const TokenLogprobs &a, float *ws, hipSt
 
 size_t token_logprobs_floats(int n, int vocab, int top) {
     if (n == 0 || vocab <= 64) return 0;
-    size_t most = 0;
-    for (int elem = 2; elem <= 4; elem += 2) {
-        const LpPlan p = lp_plan(n, vocab, top, elem);
-        if (p.chunks > 1) most = std::max(most, (size_t)n * p.chunks * (4 + 2 * top));
-    }
-    return most;
+    const LpPlan p = lp_plan(n, vocab, top);
+    return p.chunks > 1 ? (size_t)n * p.chunks * (4 + 2 * top) : 0;
 }
 
 hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, hipStream_t st) {

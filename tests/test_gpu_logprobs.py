@@ -72,6 +72,21 @@ def test_ties(hip, vocab):
     run(hip, x, rng.integers(0, vocab, 4), min(vocab, 30), "float32")
 
 
+@pytest.mark.parametrize("n,vocab", [(4, 1500), (4, 16000), (520, 16000), (2, 140001), (513, 70000)])
+@pytest.mark.parametrize("period", [64, 512, 2048, 4096, 8192])
+def test_large_logits_in_a_pattern(hip, n, vocab, period):
+    """The largest logits lie a period apart or ascend, so that a few threads see most of them."""
+    rng = np.random.default_rng(period)
+    x = rng.standard_normal((n, vocab))
+    i = np.arange(vocab)
+    x[0] += 50 * (i % period < 8)
+    x[1] = i * 1e-3 if n > 2 else -i * 1e-3
+    if n > 2:
+        x[2] += 50 * (i % period < 300)
+        x[3] = np.where(i % period < 100, 8.0, x[3])
+    run(hip, x, rng.integers(0, vocab, n), 64, "float32" if n > 500 else "bfloat16" if period % 3 else "float16")
+
+
 @pytest.mark.parametrize("vocab", [33, 200, 5000, 70000])
 def test_masked_lost_and_odd_rows(hip, vocab):
     """Rows of -inf but one, few or none; the type's lowest values; NaN and infinities; targets outside; wide ranges."""
