@@ -35,49 +35,73 @@ def _float(a, what):
         raise TypeError(f"{what} is {_dtype(a)}: float32, float16 or bfloat16 is needed") from None
 
 
-def _device(arrays, stream):
-    """The stream to enqueue on.  Every torch tensor among the arrays must be
-    on the current device."""
+def _where(arrays):
+    """The GPU that the torch tensors among the arrays are on; None without one."""
     torch = sys.modules.get("torch")
-    if torch is None:
+    at = None
+    if torch is not None:
+        for a in arrays:
+            if isinstance(a, torch.Tensor):
+                d = a.get_device()
+                if d < 0 or (at is not None and d != at):
+                    raise ValueError("tensors on the CPU or on different GPUs")
+                at = d
+    return at
+
+
+def _stream(at, stream):
+    """The stream to enqueue on for tensors on GPU `at`, which must be the current one."""
+    if at is None:
         return stream or 0
-    now = None
-    for a in arrays:
-        if isinstance(a, torch.Tensor):
-            if now is None:
-                if not a.is_cuda:
-                    raise ValueError(f"a tensor is on {a.device}, not on the GPU")
-                now = torch.cuda.current_device()
-            if a.get_device() != now:
-                raise ValueError(f"a tensor is on {a.device}, the current device is cuda:{now}")
+    torch = sys.modules["torch"]
+    if at != torch.cuda.current_device():
+        raise ValueError(f"a tensor is on cuda:{at}, the current device is cuda:{torch.cuda.current_device()}")
     if stream is not None:
         return stream
-    return 0 if now is None else torch.cuda.current_stream(now).cuda_stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without making a Stream object, 1 us
+    return raw(at) if raw else torch.cuda.current_stream(at).cuda_stream
+
+
+def _same(at, kept):
+    if at is None:
+        return kept
+    if kept is not None and kept != at:
+        raise ValueError("tensors on different GPUs")
+    return at
+
+
+def _dense(a):
+    try:
+        return a.is_contiguous()
+    except AttributeError:
+        pass
+    n = 1
+    for d, st in zip(reversed(a.shape), reversed(a.stride())):
+        if d != 1 and st != n:
+            return False
+        n *= d
+    return True
 
 
 def _plain(a, what, dtype, shape=None):
     """The address of an array without gaps, of this type (and shape)."""
     if _dtype(a) not in dtype:
         raise TypeError(f"{what} is {_dtype(a)}: {' or '.join(dtype)} is needed")
-    s = tuple(a.shape)
-    if shape is not None and s != tuple(shape):
-        raise ValueError(f"{what} has shape {s}: {tuple(shape)} is needed")
-    n = 1
-    for d, st in zip(reversed(s), reversed(a.stride())):
-        if d != 1 and st != n:
-            raise ValueError(f"{what} must be contiguous")
-        n *= d
+    if shape is not None and a.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(a.shape)}: {tuple(shape)} is needed")
+    if not _dense(a):
+        raise ValueError(f"{what} must be contiguous")
     return a.data_ptr()
 
 
-def _rows(a, what, rows, heads, dim):
+def _rows(a, what, shape):
     """A [rows][heads][dim] array as a cih_rows; the last axis without gaps."""
-    if tuple(a.shape) != (rows, heads, dim):
-        raise ValueError(f"{what} has shape {tuple(a.shape)}: {(rows, heads, dim)} is needed")
-    st = a.stride()
-    if st[2] != 1:
+    if a.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(a.shape)}: {shape} is needed")
+    rs, hs, one = a.stride()
+    if one != 1:
         raise ValueError(f"{what}: the last axis must be contiguous")
-    return C.RowsStruct(a.data_ptr(), st[0], st[1])
+    return C.RowsStruct(a.data_ptr(), rs, hs)
 
 
 class Rope:
@@ -124,6 +148,7 @@ class Kv8Batch:
                                        table.data_ptr(), None if slots is None else _plain(slots, "slots", i32, (n,)),
                                        n, n_rows, max_rows, table.shape[0], stride, table.shape[1])
         self._at = ctypes.addressof(self.struct)
+        self._gpu = _where(self._arrays)
 
 
 class Kv8Cache:
@@ -142,6 +167,7 @@ class Kv8Cache:
                                        _plain(scales, "scales", ("float32",), (n, h, 2)),
                                        _plain(bad, "bad", ("int64", "uint64"), (n, h)), n, h, head_dim)
         self._at = ctypes.addressof(self.struct)
+        self._gpu = _where(self._arrays)
         self._scale = head_dim ** -0.5
 
     @staticmethod
@@ -153,8 +179,8 @@ class Kv8Cache:
         """Writes the batch's rows k and v [n_rows][kv_heads][head_dim] into the
         cache at their positions, k rotated by rope; q [n_rows][q_heads][head_dim]
         rotated goes to q_out (default: q itself)."""
-        n, d, t = batch.n_rows, self.head_dim, _float(k, "k")
-        ks, vs = _rows(k, "k", n, self.kv_heads, d), _rows(v, "v", n, self.kv_heads, d)
+        t, shape = _float(k, "k"), (batch.n_rows, self.kv_heads, self.head_dim)
+        ks, vs = _rows(k, "k", shape), _rows(v, "v", shape)
         if _float(v, "v") != t:
             raise TypeError("k and v differ in type")
         qs = qo = None
@@ -162,22 +188,24 @@ class Kv8Cache:
         if q is not None:
             q_out = q if q_out is None else q_out
             heads = q.shape[1]
-            qs, qo = _rows(q, "q", n, heads, d), _rows(q_out, "q_out", n, heads, d)
+            shape = (batch.n_rows, heads, self.head_dim)
+            qs, qo = _rows(q, "q", shape), _rows(q_out, "q_out", shape)
             if _float(q, "q") != t or _float(q_out, "q_out") != t:
                 raise TypeError("q, q_out and k differ in type")
-        st = _device((k, v) + (() if q is None else (q, q_out)) + self._arrays + batch._arrays, stream)
+        at = _same(_same(_where((k, v) if q is None else (k, v, q, q_out)), self._gpu), batch._gpu)
         a = ctypes.addressof
         C.check(C.lib().cih_kv8_append(self._at, batch._at, t, a(ks), a(vs), heads, a(qs) if qs else None,
-                                       a(qo) if qo else None, a(rope.struct) if rope else None, st))
+                                       a(qo) if qo else None, a(rope.struct) if rope else None, _stream(at, stream)))
 
     def read(self, batch, k, v, stream=None):
         """The batch's rows read back into k and v [n_rows][kv_heads][head_dim]."""
-        n, d, t = batch.n_rows, self.head_dim, _float(k, "k")
-        ks, vs = _rows(k, "k", n, self.kv_heads, d), _rows(v, "v", n, self.kv_heads, d)
+        t, shape = _float(k, "k"), (batch.n_rows, self.kv_heads, self.head_dim)
+        ks, vs = _rows(k, "k", shape), _rows(v, "v", shape)
         if _float(v, "v") != t:
             raise TypeError("k and v differ in type")
-        st = _device((k, v) + self._arrays + batch._arrays, stream)
-        C.check(C.lib().cih_kv8_read(self._at, batch._at, t, ctypes.addressof(ks), ctypes.addressof(vs), st))
+        at = _same(_same(_where((k, v)), self._gpu), batch._gpu)
+        C.check(C.lib().cih_kv8_read(self._at, batch._at, t, ctypes.addressof(ks), ctypes.addressof(vs),
+                                     _stream(at, stream)))
 
     def attend_workspace(self, batch, q_heads):
         """Bytes of workspace that attend needs for a batch of these sizes."""
@@ -190,17 +218,17 @@ class Kv8Cache:
         cache into out (q's shape and type) and lse float32 [n_rows][q_heads].
         scale: default 1 / sqrt(head_dim).  workspace: uint8, of attend_workspace
         bytes at least."""
-        n, d, t, heads = batch.n_rows, self.head_dim, _float(q, "q"), q.shape[1]
-        qs, os = _rows(q, "q", n, heads, d), _rows(out, "out", n, heads, d)
+        t, heads = _float(q, "q"), q.shape[1]
+        shape = (batch.n_rows, heads, self.head_dim)
+        qs, os = _rows(q, "q", shape), _rows(out, "out", shape)
         if _float(out, "out") != t:
             raise TypeError("q and out differ in type")
-        at = None if lse is None else _plain(lse, "lse", ("float32",), (n, heads))
+        ls = None if lse is None else _plain(lse, "lse", ("float32",), shape[:2])
         ws, size = _workspace(workspace)
-        st = _device((q, out) + (() if lse is None else (lse,)) + (() if workspace is None else (workspace,)) +
-                     self._arrays + batch._arrays, stream)
-        C.check(C.lib().cih_kv8_attention(self._at, batch._at, t, heads, ctypes.addressof(qs), ctypes.addressof(os), at,
+        at = _same(_same(_where((q, out, lse, workspace)), self._gpu), batch._gpu)
+        C.check(C.lib().cih_kv8_attention(self._at, batch._at, t, heads, ctypes.addressof(qs), ctypes.addressof(os), ls,
                                           self._scale if scale is None else scale, 1 if causal else 0, window, ws, size,
-                                          st))
+                                          _stream(at, stream)))
 
 
 def _workspace(w):
@@ -237,7 +265,6 @@ def token_logprobs(logits, targets=None, logprob=None, entropy=None, top_ids=Non
         ids = _plain(top_ids, "top_ids", ("int32",), (n, k))
         tl = _plain(top_logprobs, "top_logprobs", f32, (n, k))
     ws, size = _workspace(workspace)
-    st = _device([a for a in (logits, targets, logprob, entropy, top_ids, top_logprobs, workspace) if a is not None],
-                 stream)
+    at = _where((logits, targets, logprob, entropy, top_ids, top_logprobs, workspace))
     C.check(C.lib().cih_token_logprobs(_float(logits, "logits"), logits.data_ptr(), logits.stride()[0], n, vocab, tg, lp,
-                                       en, k, ids, tl, ws, size, st))
+                                       en, k, ids, tl, ws, size, _stream(at, stream)))
