@@ -71,6 +71,7 @@ struct Kv8Attention {
     float *lse;
     float scale;
     int causal, window;
+    int q16, out16;  // set by the launch: queries in 16-byte loads, output in stores of 4 dims
 };
 
 hipError_t launch_kv8_append(const Kv8View &c, const Kv8Seqs &s, int dtype, const RowsView &k, const RowsView &v,

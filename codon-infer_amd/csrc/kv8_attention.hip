@@ -1,23 +1,29 @@
 // Attention over the 8-bit paged key/value cache.
 //
-// Both products run on the int8 matrix instruction (16 x 16 x 64), which takes
-// the codes as they lie in the cache: nothing is converted.  The other operand
-// is an integer in limbs of 7 bits,
-//   q = (max |q| / M) (128^2 q0 + 128 q1 + q2),  M = 126 128^2
-//   p = (1 / P) (128^2 p0 + 128 p1 + p2),        P = 127 128^2
-// (FP32 rows; 16-bit rows take two limbs, M = 126 128, P = 127 128), so that the
-// sums over dims and over a page's tokens are exact and only the limbs round: a
-// query to 2^-21 of its largest value, a weight to 2^-21 of the largest of its
-// page.  Each page has weights of its own, p = exp(s - max of the page), and joins the
-// running output with exp(max of the page - running max) times the page's V
-// scale, in FP32.
+// q k runs on the int8 matrix instruction (16 x 16 x 64), which takes K's codes
+// as they lie in the cache.  The query is an integer in signed bytes,
+//   q = (max |q| / M) (256^2 q0 + 256 q1 + q2),  M = 126 256^2
+// for FP32 rows, two bytes (M = 126 256) for 16-bit ones, so that the sums over
+// the dims are exact and only the query rounds, to 2^-24 (2^-16) of its largest
+// value.
 //
 // Lanes.  S^T = K Q^T: keys are the rows of a tile, the 16 columns are (row, head
 // of the group) pairs that share the kv head; row i of key tile t is key (i / 4)
 // 16 + 4 t + i % 4 of the page, so a lane's 16 scores are those of 16
-// consecutive keys, l / 16 * 16 .., of column l % 16: as bytes, just its
-// operand of O^T = V^T P^T.  Nothing crosses lanes but the page's maximum.
+// consecutive keys, l / 16 * 16 .., of column l % 16, which is its share of the
+// second operand of O^T = V^T P^T, for int8 and for f16.
+//
+// k_kv8_attend (few columns: single tokens).  Keys are split over waves and
+// workgroups.  The weights are bytes as well, P = 127 256^2 (127 256) at the
+// largest of the page: p v is exact, and each page joins the running output
+// with exp(max of the page - running max) times its V scale in FP32.
+//
+// k_kv8_prompt (many columns).  V's codes become f16, once for 32 columns, and
+// the weights f16 (FP32 rows: two f16, hi + lo), so that the matrix
+// instruction adds to the running output itself.
 #include <float.h>
+#include <stdlib.h>
+#include <string.h>
 
 #include <type_traits>
 
@@ -29,6 +35,8 @@ namespace cih {
 namespace {
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -71,6 +79,20 @@ __device__ __forceinline__ Column column(const Kv8Attention &a, const Kv8Seq &q,
     return c;
 }
 
+// Four dims i .. of one row (i % 4 == 0).
+template <class T>
+__device__ __forceinline__ void store_out4(const Kv8Attention &a, int row, int head, int i, f32x4 x) {
+    typedef T vec __attribute__((ext_vector_type(4)));
+    if (std::is_same<T, float>::value && a.out_h2) {
+        h2_store4(static_cast<unsigned short *>(a.out.p), row, head * a.c.d + i, a.heads * a.c.d, make_float4(x[0], x[1], x[2], x[3]));
+        return;
+    }
+    T *p = static_cast<T *>(a.out.p) + row * a.out.rs + head * a.out.hs + i;
+    if (a.out16) *reinterpret_cast<vec *>(p) = vec{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+    else
+#pragma unroll
+        for (int r = 0; r < 4; r++) p[r] = (T)x[r];
+}
 template <class T>
 __device__ __forceinline__ void store_out(const Kv8Attention &a, int row, int head, int i, float x) {
     if (std::is_same<T, float>::value && a.out_h2)
@@ -79,41 +101,142 @@ __device__ __forceinline__ void store_out(const Kv8Attention &a, int row, int he
         static_cast<T *>(a.out.p)[row * a.out.rs + head * a.out.hs + i] = (T)x;
 }
 
+// A value that all lanes read at the same address and nothing writes meanwhile: by a scalar load.
+template <class V> __device__ __forceinline__ V uniform(const V *p) {
+    return *(const __attribute__((address_space(4))) V *)(unsigned long long)p;
+}
+// A page's address, the same in all lanes, in scalar registers.
+typedef const __attribute__((address_space(1))) signed char *page_ptr;
+__device__ __forceinline__ page_ptr scalar_address(const signed char *p) {
+    const unsigned long long u = (unsigned long long)p;
+    const unsigned lo = __builtin_amdgcn_readfirstlane((int)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
+    return (page_ptr)((unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ i32x4 load16(page_ptr p) { return *(const __attribute__((address_space(1))) i32x4 *)p; }
+__device__ __forceinline__ int page_id(const Kv8View &c, const Kv8Seq &q, int pg) {
+    const int id = q.table ? uniform(q.table + pg) : -1;
+    return __builtin_amdgcn_readfirstlane(id >= 0 && id < c.n_pages ? id : -1);
+}
+
+// Which of the 16 keys j0 .. are visible, as bits.
+__device__ __forceinline__ unsigned visible16(int begin, int end, int j0) {
+    const int lo = min(max(begin - j0, 0), 16), hi = min(max(end - j0, 0), 16);
+    return ((1u << hi) - 1) & ~((1u << lo) - 1);
+}
+
 // A page of one head in registers: the A operands of both products.
 template <int DP> struct Tile {
     static constexpr int KS = DP > 64 ? DP / 64 : 1;  // k steps of q k
     i32x4 k[4][KS], v[DP / 16];
-    float2 sc;
+    float sk, sv;
     unsigned long long bad;
 };
+// First of the 16 dims a lane reads of a key; dims past a narrow head's meet zeros of the query.
+template <int DP> __device__ __forceinline__ int k_dim(int g4) { return (DP >= 64 ? g4 : g4 % (DP / 16)) * 16; }
 template <int DP>
 __device__ __forceinline__ void load_tile(Tile<DP> &t, const Kv8View &c, int id, int kvh, int lane) {
     const int64_t ph = (int64_t)max(id, 0) * c.hk + kvh;
-    const signed char *k = c.k + ph * (KV8_PAGE * DP), *v = c.v + ph * (KV8_PAGE * DP);
+    const page_ptr k = scalar_address(c.k + ph * (KV8_PAGE * DP)), v = scalar_address(c.v + ph * (KV8_PAGE * DP));
     const int i = lane & 15, g4 = lane >> 4;
+    // the page's address in scalar registers, the lane's offset in one vector register
+    const unsigned koff = ((i >> 2) * 16 + (i & 3)) * DP + k_dim<DP>(g4), voff = i * KV8_PAGE + g4 * 16;
 #pragma unroll
     for (int s = 0; s < Tile<DP>::KS; s++)
 #pragma unroll
-        for (int kt = 0; kt < 4; kt++) {
-            const int key = (i >> 2) * 16 + kt * 4 + (i & 3);
-            if (DP >= 64 || g4 < DP / 16) t.k[kt][s] = *reinterpret_cast<const i32x4 *>(k + key * DP + s * 64 + g4 * 16);
-            else t.k[kt][s] = i32x4{0, 0, 0, 0};
-        }
+        for (int kt = 0; kt < 4; kt++) t.k[kt][s] = load16(k + koff + (kt * 4 * DP + s * 64));
 #pragma unroll
-    for (int dt = 0; dt < DP / 16; dt++)
-        t.v[dt] = *reinterpret_cast<const i32x4 *>(v + (dt * 16 + i) * KV8_PAGE + g4 * 16);
-    t.sc = c.scales[ph];
-    t.bad = c.bad[ph];
+    for (int dt = 0; dt < DP / 16; dt++) t.v[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
+    t.sk = uniform(&c.scales[ph].x);
+    t.sv = uniform(&c.scales[ph].y);
+    t.bad = uniform(c.bad + ph);
+}
+
+// A column's query as bytes, ready as the second operand, and the factor that
+// makes scores in units of log2 of its sums with a page's codes (times the K
+// scale); NaN if the query is not finite.
+template <int NL, int KS, class T>
+__device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column &col, int g4, i32x4 (&ql)[NL][KS]) {
+    constexpr float M = NL == 3 ? 126.0f * 65536 : 126.0f * 256;
+    constexpr int HALF = NL == 3 ? 0x8080 : 0x80;  // bytes below the first are v + 128
+    constexpr int VL = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(VL)));
+    float x[KS][16];
+    unsigned top = 0;
+    const T *qp = static_cast<const T *>(a.q.p) + (col.row >= 0 ? col.row * a.q.rs + col.head * a.q.hs : 0);
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 16; e += VL) {  // a head has whole groups of VL dims
+            const int i = s * 64 + g4 * 16 + e;
+            const T *p = qp + (i < a.c.d ? i : 0);
+            T w[VL];
+            if (a.q16) {
+                const vec y = *reinterpret_cast<const vec *>(p);
+#pragma unroll
+                for (int u = 0; u < VL; u++) w[u] = y[u];
+            } else {
+#pragma unroll
+                for (int u = 0; u < VL; u++) w[u] = p[u];
+            }
+#pragma unroll
+            for (int u = 0; u < VL; u++) {
+                x[s][e + u] = col.row >= 0 && i < a.c.d ? to_f32(w[u]) : 0.0f;
+                top = max(top, __float_as_uint(x[s][e + u]) & 0x7fffffffu);  // NaN above infinity above the rest
+            }
+        }
+    float mx = __uint_as_float(top);
+    const bool lost = groups_max(mx <= FLT_MAX ? 0.0f : 1.0f) > 0.0f;
+    mx = groups_max(mx);
+    const float up = mx < 0x1p-64f ? 0x1p64f : 1.0f;  // so that the reciprocal is finite
+    mx *= up;
+    // a negative scale turns the query, so that the factor is never negative
+    const float inv = mx < 0x1p-60f ? 0.0f : a.scale < 0.0f ? -M / mx : M / mx;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) x[s][e] = lost ? 0.0f : x[s][e] * up;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            unsigned o[3] = {0, 0, 0};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int v = (int)rintf(x[s][4 * w + e] * inv) + HALF;
+#pragma unroll
+                for (int n = 0; n < NL; n++) o[n] |= (unsigned)(v >> (8 * (NL - 1 - n)) & 255) << (8 * e);
+            }
+#pragma unroll
+            for (int n = 0; n < NL; n++) ql[n][s][w] = (int)(n == 0 ? o[n] : o[n] ^ 0x80808080u);
+        }
+    return lost ? NAN : mx / M / up * fabsf(a.scale) * LOG2E;
+}
+
+// Scores of 16 keys with one column (times M), from the sums with each byte.
+template <int NL, int KS>
+__device__ __forceinline__ void score_tile(const i32x4 (&k)[KS], const i32x4 (&ql)[NL][KS], float (&s)[4]) {
+    i32x4 d[NL];
+#pragma unroll
+    for (int n = 0; n < NL; n++) {
+        d[n] = i32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int x = 0; x < KS; x++) d[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[n][x], d[n], 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const float hi = (float)(d[0][r] * 256 + d[1][r]);  // below 2^30
+        s[r] = NL == 3 ? fmaf(hi, 256.0f, (float)d[NL - 1][r]) : hi;
+    }
 }
 
 // One workgroup of W waves per (sequence, kv head, 16 columns, split of the
 // pages); its waves take the split's pages in turn and join their sums at the
 // end.  splits > 1: unnormalised results [row][head][split][DP + 2] in ws.
 template <int DP, int NL, class T, int W>
-__global__ __launch_bounds__(64 * W) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
+__global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
-    constexpr float M = NL == 3 ? 126.0f * 16384 : 126.0f * 128, P = NL == 3 ? 127.0f * 16384 : 127.0f * 128;
+    constexpr float P = NL == 3 ? 127.0f * 65536 : 127.0f * 256;
     __shared__ __attribute__((aligned(16))) float so[W][16][DP + 4];
     __shared__ float sml[W][2][16];
     int b = blockIdx.x;
@@ -135,48 +258,8 @@ __global__ __launch_bounds__(64 * W) void k_kv8_attend(Kv8Attention a, int g, in
     const int first = pg0 + split * pps, last = pg0 + min(np, (split + 1) * pps);
     if (split > 0 && first >= last) return;  // the join knows
 
-    // the query's limbs, as B operands, and its factor
     i32x4 ql[NL][KS];
-    float f;
-    {
-        float x[KS][16];
-        unsigned top = 0;
-        const T *qp = static_cast<const T *>(a.q.p) + col.row * a.q.rs + col.head * a.q.hs;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int i = s * 64 + g4 * 16 + e;
-                x[s][e] = col.row >= 0 && i < a.c.d ? to_f32(qp[i]) : 0.0f;
-                top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);  // NaN above infinity above the rest
-            }
-        float mx = __uint_as_float(top);
-        const bool lost = groups_max(mx <= FLT_MAX ? 0.0f : 1.0f) > 0.0f;
-        mx = groups_max(mx);
-        const float up = mx < 0x1p-64f ? 0x1p64f : 1.0f;  // so that the reciprocal is finite
-        mx *= up;
-        const float inv = lost || mx < 0x1p-60f ? 0.0f : M / mx;
-        f = lost ? NAN : mx / M / up * a.scale * LOG2E;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                unsigned o[3] = {0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    int v = lost ? 0 : (int)rintf(x[s][4 * w + e] * up * inv);
-#pragma unroll
-                    for (int n = NL - 1; n > 0; n--) {
-                        const int r = ((v + 64) & 127) - 64;
-                        o[n] |= (unsigned)(r & 255) << (8 * e);
-                        v = (v - r) >> 7;
-                    }
-                    o[0] |= (unsigned)(v & 255) << (8 * e);
-                }
-#pragma unroll
-                for (int n = 0; n < NL; n++) ql[n][s][w] = (int)o[n];
-            }
-    }
+    const float f = query_bytes<NL, KS, T>(a, col, g4, ql);
 
     float m = -INFINITY, l = 0.0f;
     float o[DT][4];
@@ -189,35 +272,23 @@ __global__ __launch_bounds__(64 * W) void k_kv8_attend(Kv8Attention a, int g, in
         if (id < 0) return;
         // scores in units of log2
         float s[4][4];
-        const float fk = f * t.sc.x;
+        const float fk = f * t.sk;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            i32x4 d[NL];
+            score_tile<NL, KS>(t.k[kt], ql, s[kt]);
 #pragma unroll
-            for (int n = 0; n < NL; n++) {
-                d[n] = i32x4{0, 0, 0, 0};
-#pragma unroll
-                for (int x = 0; x < KS; x++) d[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(t.k[kt][x], ql[n][x], d[n], 0, 0, 0);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const float hi = (float)(d[0][r] * 128 + d[1][r]);  // below 2^30
-                s[kt][r] = (NL == 3 ? fmaf(hi, 128.0f, (float)d[NL - 1][r]) : hi) * fk;
-            }
+            for (int r = 0; r < 4; r++) s[kt][r] *= fk;
         }
         const int j0 = pg * KV8_PAGE;
         unsigned long long bad = t.bad;
-        if (!(t.sc.x <= FLT_MAX && t.sc.y <= FLT_MAX)) bad = ~0ull;
+        if (!(t.sk >= 0.0f && t.sk <= FLT_MAX && t.sv >= 0.0f && t.sv <= FLT_MAX)) bad = ~0ull;
         if (j0 < all0 || j0 + KV8_PAGE > all1 || bad) {
+            const unsigned see = visible16(col.begin, col.end, j0 + g4 * 16), lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
+            if (see & lost) l = NAN;
 #pragma unroll
             for (int kt = 0; kt < 4; kt++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int k = g4 * 16 + kt * 4 + r, j = j0 + k;
-                    const bool see = j >= col.begin && j < col.end, lost = bad >> k & 1;
-                    if (see && lost) l = NAN;
-                    if (!see || lost) s[kt][r] = -INFINITY;
-                }
+                for (int r = 0; r < 4; r++) s[kt][r] = (see & ~lost) >> (kt * 4 + r) & 1 ? s[kt][r] : -INFINITY;
         }
         float mp = -INFINITY;
 #pragma unroll
@@ -227,34 +298,39 @@ __global__ __launch_bounds__(64 * W) void k_kv8_attend(Kv8Attention a, int g, in
         mp = groups_max(mp);
         if (mp == INFINITY) l = NAN;
         const float base = mp == -INFINITY ? 0.0f : mp;
-        // the page's weights, as B operands, and their sum (exact)
+        // the page's weights as bytes, and their sum (exact)
         i32x4 pl[NL];
-        int sum = 0;
+        unsigned sum = 0;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            unsigned w[3] = {0, 0, 0};
+            unsigned v[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const unsigned v = (unsigned)rintf(__builtin_amdgcn_exp2f(s[kt][r] - base) * P);
-                sum += v;
-                if (NL == 3) {
-                    w[0] |= (v >> 14) << (8 * r);
-                    w[1] |= (v >> 7 & 127) << (8 * r);
-                    w[2] |= (v & 127) << (8 * r);
-                } else {
-                    w[0] |= (v >> 7) << (8 * r);
-                    w[1] |= (v & 127) << (8 * r);
-                }
+                const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
+                v[r] = (unsigned)rintf(e * P);
+                sum += v[r];
+                v[r] += NL == 3 ? 0x8080 : 0x80;
             }
-#pragma unroll
-            for (int n = 0; n < NL; n++) pl[n][kt] = (int)w[n];
+            if (NL == 3) {
+                const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010602u);  // bytes 2 | bytes 1
+                const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010602u);
+                const unsigned b01 = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), b23 = __builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u);
+                pl[0][kt] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+                pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
+                pl[NL - 1][kt] = (int)(__builtin_amdgcn_perm(b23, b01, 0x05040100u) ^ 0x80808080u);
+            } else {
+                const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x04000501u);  // bytes 1 | bytes 0
+                const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x04000501u);
+                pl[0][kt] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+                pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
+            }
         }
         const float mn = fmaxf(m, base == mp ? mp : m);
         const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
         const float add = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn) * (1.0f / P);
         l = fmaf(l, keep, (float)sum * add);
         m = mn;
-        const float av = add * t.sc.y;
+        const float av = add * t.sv;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             i32x4 d[NL];
@@ -263,14 +339,14 @@ __global__ __launch_bounds__(64 * W) void k_kv8_attend(Kv8Attention a, int g, in
                 d[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(t.v[dt], pl[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float hi = (float)(d[0][r] * 128 + d[1][r]);
-                o[dt][r] = fmaf(o[dt][r], keep, (NL == 3 ? fmaf(hi, 128.0f, (float)d[NL - 1][r]) : hi) * av);
+                const float hi = (float)(d[0][r] * 256 + d[1][r]);
+                o[dt][r] = fmaf(o[dt][r], keep, (NL == 3 ? fmaf(hi, 256.0f, (float)d[NL - 1][r]) : hi) * av);
             }
         }
     };
 
     // two pages in registers: the next one's loads are under way while one is worked on
-    auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? kv8_page(a.c, q, pg) : -1; };
+    auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? page_id(a.c, q, pg) : -1; };
     Tile<DP> ta, tb;
     int pg = first + wave, ia = id_of(pg), ib = id_of(pg + W);
     if (pg < last) load_tile<DP>(ta, a.c, ia, kvh, lane);
@@ -363,8 +439,181 @@ __global__ __launch_bounds__(64) void k_kv8_join(Kv8Attention a, int g, int spli
     if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
+// Four waves of CT x 16 columns each, over all pages that these see.  The
+// running maximum follows only when a score exceeds it by 2^8, and the output's
+// unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
+// 2^3 at the running maximum and have room for both.
+template <int DP, int NL, class T, int CT>
+__global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int per_xcd) {
+    constexpr int KS = Tile<DP>::KS, DT = DP / 16, PL = NL - 1;  // PL: f16 a weight
+    constexpr float SLACK = 8.0f, P0 = 3.0f, UNIT = 16.0f;
+    // consecutive workgroups go to the 8 XCDs in turn: each gets whole heads,
+    // whose K and V its L2 then holds; a head's longest rows first
+    int b = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
+    if (b >= a.c.hk * a.s.n_seq * tiles) return;
+    const int tile = tiles - 1 - b % tiles;
+    b /= tiles;
+    const int kvh = b / a.s.n_seq;
+    const Kv8Seq q = kv8_seq(a.s, b % a.s.n_seq);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, g4 = lane >> 4;
+    const int f0 = (tile * 4 + wave) * CT * 16, f1 = min(f0 + CT * 16, q.n * g) - 1;  // columns of the wave
+    if (f0 > f1) return;
+    const Column c0 = column(a, q, kvh, g, f0), c1 = column(a, q, kvh, g, f1);
+    const int any0 = __builtin_amdgcn_readfirstlane(c0.begin), any1 = __builtin_amdgcn_readfirstlane(c1.end);
+    const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
+    const int first = any0 / KV8_PAGE, last = (any1 + KV8_PAGE - 1) / KV8_PAGE;
+
+    i32x4 ql[CT][NL][KS];
+    float f[CT], m[CT], l[CT];
+    int begin[CT], end[CT];
+    f32x4 o[CT][DT];
+#pragma unroll
+    for (int t = 0; t < CT; t++) {
+        const Column col = column(a, q, kvh, g, f0 + t * 16 + c);
+        f[t] = query_bytes<NL, KS, T>(a, col, g4, ql[t]);
+        begin[t] = col.begin;
+        end[t] = col.end;
+        m[t] = -INFINITY;
+        l[t] = f[t] != f[t] ? NAN : 0.0f;  // a query that is not finite
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) o[t][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    float unit = 0.0f;  // o is in units of it (0: nothing added yet)
+
+    i32x4 kr[4][KS], vr[DT];
+    float sk = 0.0f, sv = 0.0f, skn = 0.0f, svn = 0.0f;
+    unsigned long long bad = 0, badn = 0;
+    // the lane's offsets in a page: with the page's address in scalar registers a load takes one vector register
+    const unsigned koff = ((c >> 2) * 16 + (c & 3)) * DP + k_dim<DP>(g4), voff = c * KV8_PAGE + g4 * 16;
+    auto load_k = [&](int id) __attribute__((always_inline)) {
+        const int64_t ph = (int64_t)max(id, 0) * a.c.hk + kvh;
+        const page_ptr k = scalar_address(a.c.k + ph * (KV8_PAGE * DP));
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+                kr[kt][s] = load16(k + koff + (kt * 4 * DP + s * 64));
+        skn = uniform(&a.c.scales[ph].x);
+        svn = uniform(&a.c.scales[ph].y);
+        badn = uniform(a.c.bad + ph);
+    };
+    int id = first < last ? page_id(a.c, q, first) : -1;
+    if (first < last) load_k(id);
+    for (int pg = first; pg < last; pg++) {
+        sk = skn;
+        sv = svn;
+        bad = badn;
+        {
+            const page_ptr v = scalar_address(a.c.v + ((int64_t)max(id, 0) * a.c.hk + kvh) * (KV8_PAGE * DP));
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++) vr[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
+        }
+        float s[CT][4][4];
+#pragma unroll
+        for (int t = 0; t < CT; t++)
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++) score_tile<NL, KS>(kr[kt], ql[t], s[t][kt]);
+        const bool missing = id < 0;
+        if (pg + 1 < last) {
+            id = page_id(a.c, q, pg + 1);
+            load_k(id);
+        }
+        if (!(sk >= 0.0f && sk <= FLT_MAX && sv >= 0.0f && sv <= FLT_MAX)) bad = ~0ull;
+        const int j0 = pg * KV8_PAGE;
+        if (j0 < all0 || j0 + KV8_PAGE > all1 || bad || missing) {  // hidden keys
+#pragma unroll
+            for (int t = 0; t < CT; t++) {
+                unsigned see = missing ? 0 : visible16(begin[t], end[t], j0 + g4 * 16);
+                const unsigned lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
+                l[t] = see & lost ? NAN : l[t];
+                see &= ~lost;
+#pragma unroll
+                for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) s[t][kt][r] = see >> (kt * 4 + r) & 1 ? s[t][kt][r] : -INFINITY;
+            }
+        }
+        float fk[CT], x[CT];
+        bool move = false;
+#pragma unroll
+        for (int t = 0; t < CT; t++) {
+            fk[t] = fmaxf(f[t] * sk, 0x1p-120f);  // above 0: what is hidden stays at -inf
+            x[t] = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) x[t] = fmaxf(x[t], s[t][kt][r]);
+            x[t] *= fk[t];
+            move |= x[t] > m[t] + SLACK;
+        }
+        const float svu = sv > 0.0f ? sv : unit;  // a page of zeros fits any unit
+        move |= svu > unit * UNIT || svu * UNIT < unit;
+        if (__any(move)) {
+            const float w = unit > 0.0f ? unit / svu : 0.0f;
+            unit = svu;
+#pragma unroll
+            for (int t = 0; t < CT; t++) {
+                const float mn = fmaxf(m[t], groups_max(x[t]));
+                const float y = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - mn), z = y * w;
+                m[t] = mn;
+                l[t] *= y;
+#pragma unroll
+                for (int dt = 0; dt < DT; dt++) o[t][dt] *= z;
+            }
+        }
+        const float ratio = unit > 0.0f ? svu / unit : 1.0f;
+        const float up = P0 + __builtin_amdgcn_logf(ratio), down = __builtin_amdgcn_exp2f(-P0) / ratio;
+        f16x8 p[CT][PL][2];
+#pragma unroll
+        for (int t = 0; t < CT; t++) {
+            const float off = up - (m[t] == -INFINITY ? 0.0f : m[t]);
+            float sum = 0.0f;
+#pragma unroll
+            for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[t][kt][r], fk[t], off));
+                    sum += e;
+                    const _Float16 hi = (_Float16)e;
+                    p[t][0][kt / 2][kt % 2 * 4 + r] = hi;
+                    if (PL == 2) p[t][PL - 1][kt / 2][kt % 2 * 4 + r] = (_Float16)(e - (float)hi);
+                }
+            l[t] = fmaf(sum, down, l[t]);
+        }
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const f16x8 v = quants_f16<1>(qu32x2_t{(unsigned)vr[dt][2 * h], (unsigned)vr[dt][2 * h + 1]}, 0);
+#pragma unroll
+                for (int t = 0; t < CT; t++)
+#pragma unroll
+                    for (int n = 0; n < PL; n++)
+                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[t][n][h], o[t][dt], 0, 0, 0);
+            }
+    }
+
+#pragma unroll
+    for (int t = 0; t < CT; t++) {
+        const Column col = column(a, q, kvh, g, f0 + t * 16 + c);
+        float sum = groups_sum(l[t]);
+        if (begin[t] >= end[t]) sum = 0.0f;
+        if (col.row < 0) continue;
+        const float x = unit / sum * __builtin_amdgcn_exp2f(-P0);
+#pragma unroll
+        for (int dt = 0; dt < DT; dt++) {
+            const int i = dt * 16 + g4 * 4;
+            if (i < a.c.d) store_out4<T>(a, col.row, col.head, i, sum == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o[t][dt] * x);
+        }
+        if (g4 == 0 && a.lse)
+            a.lse[(int64_t)col.row * a.heads + col.head] = sum == 0.0f ? -INFINITY : (m[t] + log2f(sum)) * LN2;
+    }
+}
+
 // Workgroups: how the pages of a sequence are split.
 struct Plan {
+    bool prompt;
     int g, tiles, splits, pps;
     int64_t blocks;
 };
@@ -373,8 +622,10 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window)
     p.g = heads / c.hk;
     p.tiles = (int)(((int64_t)s.max_rows * p.g + 15) / 16);
     const int64_t tasks = (int64_t)s.n_seq * c.hk * p.tiles;
+    const char *e = getenv("CIH_KV8_PROMPT");
+    p.prompt = e ? !strcmp(e, "1") : p.tiles > 1 && tasks >= 1024;
     int64_t pps = max((int64_t)16, min(s.max_pages * tasks / 2048, (int64_t)64));
-    if (tasks >= 4096) pps = s.max_pages;
+    if (tasks >= 4096 || p.prompt) pps = s.max_pages;
     // pages that the keys of 16 columns touch at most
     int64_t pages = s.max_pages;
     if (window > 0) pages = min(pages, ((int64_t)window + (causal ? 16 / p.g + 1 : s.max_rows) + KV8_PAGE - 2) / KV8_PAGE + 1);
@@ -384,9 +635,22 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window)
     return p;
 }
 
+// Columns of a prompt wave, / 16.
+template <int DP, class T> constexpr int prompt_tiles() {
+    return DP == 128 && std::is_same<T, float>::value ? 1 : 2;
+}
+
 template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, hipStream_t st) {
-    constexpr int NL = std::is_same<T, float>::value ? 3 : 2;
+    constexpr int NL = std::is_same<T, float>::value ? 3 : 2, CT = prompt_tiles<DP, T>();
     const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window);
+    if (p.prompt) {
+        const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
+        const int64_t per_xcd = (tiles * a.s.n_seq * a.c.hk + 7) / 8;
+        if (per_xcd * 8 > INT32_MAX) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((k_kv8_prompt<DP, NL, T, CT>), dim3(per_xcd * 8), dim3(256), 0, st, a, p.g, (int)tiles,
+                           (int)per_xcd);
+        return hipGetLastError();
+    }
     if (p.blocks > INT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_kv8_attend<DP, NL, T, 4>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles, p.splits, p.pps, ws);
     hipError_t e = hipGetLastError();
@@ -416,8 +680,15 @@ size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads) {
     return p.splits == 1 ? 0 : (size_t)s.n_rows * heads * p.splits * (c.dp + 2);
 }
 
-hipError_t launch_kv8_attention(const Kv8Attention &a, float *ws, hipStream_t st) {
-    if (a.s.n_rows == 0 || a.s.n_seq == 0 || a.s.max_rows == 0) return hipSuccess;
+hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, hipStream_t st) {
+    if (call.s.n_rows == 0 || call.s.n_seq == 0 || call.s.max_rows == 0) return hipSuccess;
+    Kv8Attention a = call;
+    const int64_t size = a.dtype == FT_F32 ? 4 : 2;
+    auto aligned = [&](const RowsView &v, int64_t n) {
+        return (reinterpret_cast<uintptr_t>(v.p) | (uintptr_t)(v.rs * size) | (uintptr_t)(v.hs * size)) % n == 0;
+    };
+    a.q16 = aligned(a.q, 16);
+    a.out16 = aligned(a.out, 4 * size);
     switch (a.dtype) {
         case FT_F32: return launch_dims<float>(a, ws, st);
         case FT_F16: return launch_dims<_Float16>(a, ws, st);

@@ -28,6 +28,12 @@ def hip():
     return Hip()
 
 
+@pytest.fixture(params=["0", "1"], ids=["few", "prompt"])
+def kernel(request, monkeypatch):
+    """Both kernels, whichever the sizes would choose."""
+    monkeypatch.setenv("CIH_KV8_PROMPT", request.param)
+
+
 def offsets(rows):
     return np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
 
@@ -105,7 +111,7 @@ def run_attention(hip, rng, lens, rows, hk, g, d, dtype, causal=True, window=0, 
 
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("d,hk,g", [(16, 3, 1), (24, 2, 2), (32, 1, 5), (64, 4, 1), (64, 1, 8), (128, 2, 3), (128, 1, 16)])
-def test_steps(hip, dtype, d, hk, g):
+def test_steps(hip, kernel, dtype, d, hk, g):
     """One row a sequence, lengths around the pages' ends, an idle stream among them."""
     rng = np.random.default_rng(d + g)
     lens = [1, 2, 63, 64, 65, 0, 127, 128, 129, 300, 1000]
@@ -115,7 +121,7 @@ def test_steps(hip, dtype, d, hk, g):
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("d,hk,g", [(16, 2, 1), (24, 2, 3), (32, 2, 1), (64, 2, 1), (64, 1, 4), (128, 1, 4)])
 @pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 50), (False, 33)])
-def test_prompts_and_chunks(hip, dtype, d, hk, g, causal, window):
+def test_prompts_and_chunks(hip, kernel, dtype, d, hk, g, causal, window):
     """Ragged prompts, chunks behind a context, drafted rows: all masks."""
     rng = np.random.default_rng(d + g + window)
     run_attention(hip, rng, [1, 17, 64, 130, 200, 333, 90], [1, 17, 64, 130, 65, 3, 0], hk, g, d, dtype, causal, window,
@@ -124,7 +130,7 @@ def test_prompts_and_chunks(hip, dtype, d, hk, g, causal, window):
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("window", [0, 700, 1])
-def test_long_sequences(hip, dtype, window):
+def test_long_sequences(hip, kernel, dtype, window):
     """Few rows over many pages: the keys are split and joined again."""
     rng = np.random.default_rng(3)
     run_attention(hip, rng, [9001, 5], [1, 1], 1, 1, 64, dtype, window=window, layout="heads")
@@ -132,7 +138,7 @@ def test_long_sequences(hip, dtype, window):
 
 
 @pytest.mark.parametrize("rows", [1, 40])
-def test_bad_tokens(hip, rows):
+def test_bad_tokens(hip, kernel, rows):
     """A token that is not finite makes the rows that see it NaN, and no other."""
     rng = np.random.default_rng(5)
 
@@ -146,7 +152,7 @@ def test_bad_tokens(hip, rows):
 
 
 @pytest.mark.parametrize("rows", [1, 30])
-def test_garbage_past_the_end_and_missing_pages(hip, rows):
+def test_garbage_past_the_end_and_missing_pages(hip, kernel, rows):
     """Codes past a sequence's length, scales of pages it does not own, page ids outside the cache."""
     rng = np.random.default_rng(6)
 
@@ -164,7 +170,7 @@ def test_garbage_past_the_end_and_missing_pages(hip, rows):
                   max_pages=5, layout="heads")
 
 
-def test_rows_before_the_first_position(hip):
+def test_rows_before_the_first_position(hip, kernel):
     """A padded batch: more rows than tokens; the rows at negative positions give 0 and -inf."""
     rng = np.random.default_rng(7)
     got = run_attention(hip, rng, [3, 0, 70], [5, 4, 1], 2, 1, 64, "float32", layout="heads")
@@ -172,7 +178,7 @@ def test_rows_before_the_first_position(hip):
     run_attention(hip, rng, [3, 0, 70], [5, 4, 1], 2, 1, 64, "float32", causal=False, layout="heads")
 
 
-def test_lengths_past_the_table(hip):
+def test_lengths_past_the_table(hip, kernel):
     """A length beyond the table's pages reads what the table has."""
     rng = np.random.default_rng(8)
     c = R.Cache(hip, rng, 4, 1, 32)
@@ -189,7 +195,7 @@ def test_lengths_past_the_table(hip):
     R.free(*arr, qd, od, ws, *c.dev)
 
 
-def test_slots_shared_pages_and_no_lse(hip):
+def test_slots_shared_pages_and_no_lse(hip, kernel):
     rng = np.random.default_rng(9)
     run_attention(hip, rng, [100, 1, 64], [1, 1, 2], 2, 2, 64, "float16", slots=True, layout="heads", want_lse=False)
 
@@ -200,14 +206,14 @@ def test_slots_shared_pages_and_no_lse(hip):
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
-def test_scales(hip, scale):
+def test_scales(hip, kernel, scale):
     """Uniform weights, turned order, nearly one-hot rows."""
     rng = np.random.default_rng(10)
     run_attention(hip, rng, [150, 77], [1, 77], 2, 1, 64, "float32", scale=scale, layout="heads")
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_query_extremes(hip, dtype):
+def test_query_extremes(hip, kernel, dtype):
     """Rows of zeros and of very small and large values (scores stay finite)."""
     rng = np.random.default_rng(11)
     c = R.Cache(hip, rng, 5, 1, 64)
@@ -226,7 +232,7 @@ def test_query_extremes(hip, dtype):
     R.free(*arr, qd, od, lse, ws, *c.dev)
 
 
-def test_query_not_finite(hip):
+def test_query_not_finite(hip, kernel):
     """A query row with NaN or infinity gives NaN for its own head only."""
     rng = np.random.default_rng(12)
     for rows in (1, 33):
@@ -246,6 +252,46 @@ def test_query_not_finite(hip):
         want[0, 0] = want[-1, 1] = True
         assert np.array_equal(bad, want), (rows, np.argwhere(bad != want))
         R.free(*arr, qd, od, ws, *c.dev)
+
+
+def test_v_scales_far_apart(hip, kernel):
+    """Pages whose V is huge or zero beside ordinary ones: rows that do not see the huge page keep their precision."""
+    rng = np.random.default_rng(14)
+
+    def change(c, table):
+        c.scales[table[0, 1], :, 1] = 1e30   # tokens 64 .. 127: seen by the later rows only
+        c.scales[table[1, 0], :, 1] = 0      # a page of zeros first
+        c.v[table[1, 0]] = 0
+        c.scales[table[2, 1], :, 1] = 1e-20
+
+    for rows, n in ((64, 64), (100, 130)):
+        c = R.Cache(hip, rng, 12, 2, 64)
+        table = R.tables(rng, [n] * 3, 12, 3)
+        if n > 64:
+            change(c, table)
+        q = R.rounded(rng.standard_normal((3 * rows, 2, 64)), "float32")
+        arr = [DeviceArray(hip, x) for x in (offsets([rows] * 3), np.array([n] * 3, np.int32), table)]
+        qd, od = R.put(hip, q, "float32"), R.put(hip, q * 0, "float32")
+        cache = c.upload()
+        b = ch.Kv8Batch(*arr, 3 * rows, rows)
+        ws = DeviceArray(hip, np.zeros(cache.attend_workspace(b, 2) + 16, np.uint8))
+        cache.attend(b, qd, od, workspace=ws)
+        got = R.get(od)
+        for i in range(3):
+            for r in range(rows):
+                pos = n - rows + r
+                a = slice(i * rows + r, i * rows + r + 1)
+                ref, rlse, err = R.attention(c, table[i], n, np.array([pos]), q[a], 1 / 8, True, 0, 1)
+                vmax = 127 * max(float(c.scales[table[i, p], :, 1].max()) for p in range(pos // 64 + 1))
+                check_attention(got[a], rlse, ref, rlse, err, "float32", vmax)
+        R.free(*arr, qd, od, ws, *c.dev)
+
+
+def test_the_sizes_choose_the_prompt_kernel(hip):
+    """Enough columns for it without being told so."""
+    rng = np.random.default_rng(15)
+    lens = [int(x) for x in rng.integers(60, 100, 24)]
+    run_attention(hip, rng, lens, [max(n - 5 * i, 1) for i, n in enumerate(lens)], 8, 1, 32, "bfloat16", layout="heads")
 
 
 # ---- append and read ---------------------------------------------------------
