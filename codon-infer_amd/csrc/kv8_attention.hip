@@ -1,11 +1,12 @@
 // Attention over the 8-bit paged key/value cache.
 //
 // q k runs on the int8 matrix instruction (16 x 16 x 64), which takes K's codes
-// as they lie in the cache.  The query is an integer in signed bytes,
-//   q = (max |q| / M) (256^2 q0 + 256 q1 + q2),  M = 126 256^2
-// for FP32 rows, two bytes (M = 126 256) for 16-bit ones, so that the sums over
-// the dims are exact and only the query rounds, to 2^-24 (2^-16) of its largest
-// value.
+// as they lie in the cache.  The query is an integer in signed bytes, q = 2^-e
+// (256^2 q0 + 256 q1 + q2), so that the sums over the dims are exact and only
+// the query rounds, to 2^-23 of its largest value; the sum with q2, without its
+// last 8 bits, starts the one with q1, which leaves 2^-22 of an ordinary score.
+// For 16-bit rows of prompts two bytes do: the scale is a power of 2, so that
+// what is not below 2^-7 (float16: 2^-4) of the largest value is exact.
 //
 // Lanes.  S^T = K Q^T: keys are the rows of a tile, the 16 columns are (row, head
 // of the group) pairs that share the kv head; row i of key tile t is key (i / 4)
@@ -14,8 +15,8 @@
 // second operand of O^T = V^T P^T, for int8 and for f16.
 //
 // k_kv8_attend (few columns: single tokens).  Keys are split over waves and
-// workgroups.  The weights are bytes as well, P = 127 256^2 (127 256) at the
-// largest of the page: p v is exact, and each page joins the running output
+// workgroups.  The weights are bytes as well, three for FP32 rows and two for
+// 16-bit ones, P = 127 256^2 (127 256) at the largest of the page: p v is exact, and each page joins the running output
 // with exp(max of the page - running max) times its V scale in FP32.
 //
 // k_kv8_prompt (many columns).  V's codes become f16, once for 32 columns, and
@@ -151,13 +152,13 @@ __device__ __forceinline__ void load_tile(Tile<DP> &t, const Kv8View &c, int id,
     t.bad = uniform(c.bad + ph);
 }
 
-// A column's query as bytes, ready as the second operand, and the factor that
-// makes scores in units of log2 of its sums with a page's codes (times the K
-// scale); NaN if the query is not finite.
-template <int NL, int KS, class T>
-__device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column &col, int g4, i32x4 (&ql)[NL][KS]) {
-    constexpr float M = NL == 3 ? 126.0f * 65536 : 126.0f * 256;
-    constexpr int HALF = NL == 3 ? 0x8080 : 0x80;  // bytes below the first are v + 128
+// A column's query as QB bytes a value, ready as the second operand, and the
+// factor that makes scores in units of log2 of its sums with a page's codes
+// (times the K scale); NaN if the query is not finite.
+template <int QB, int KS, class T>
+__device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column &col, int g4, i32x4 (&ql)[QB][KS]) {
+    constexpr int BITS = 8 * QB - 1, HALF = QB == 3 ? 0x8080 : 0x80;  // the lower bytes are + 128 at first
+    constexpr float MOST = (1 << BITS) - 1 - HALF;
     constexpr int VL = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(VL)));
     float x[KS][16];
@@ -187,56 +188,52 @@ __device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column
     float mx = __uint_as_float(top);
     const bool lost = groups_max(mx <= FLT_MAX ? 0.0f : 1.0f) > 0.0f;
     mx = groups_max(mx);
-    const float up = mx < 0x1p-64f ? 0x1p64f : 1.0f;  // so that the reciprocal is finite
-    mx *= up;
+    int e = BITS - __builtin_amdgcn_frexp_expf(mx);
+    if (ldexpf(mx, e) > MOST) e--;
     // a negative scale turns the query, so that the factor is never negative
-    const float inv = mx < 0x1p-60f ? 0.0f : a.scale < 0.0f ? -M / mx : M / mx;
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) x[s][e] = lost ? 0.0f : x[s][e] * up;
+    const float sign = lost ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            unsigned o[3] = {0, 0, 0};
+            unsigned o[QB] = {};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int v = (int)rintf(x[s][4 * w + e] * inv) + HALF;
+            for (int u = 0; u < 4; u++) {
+                const int v = (int)rintf(ldexpf(lost ? 0.0f : x[s][4 * w + u] * sign, e)) + HALF;
 #pragma unroll
-                for (int n = 0; n < NL; n++) o[n] |= (unsigned)(v >> (8 * (NL - 1 - n)) & 255) << (8 * e);
+                for (int n = 0; n < QB; n++) o[n] |= (unsigned)(v >> (8 * (QB - 1 - n)) & 255) << (8 * u);
             }
 #pragma unroll
-            for (int n = 0; n < NL; n++) ql[n][s][w] = (int)(n == 0 ? o[n] : o[n] ^ 0x80808080u);
+            for (int n = 0; n < QB; n++) ql[n][s][w] = (int)(n == 0 ? o[n] : o[n] ^ 0x80808080u);
         }
-    return lost ? NAN : mx / M / up * fabsf(a.scale) * LOG2E;
+    return lost ? NAN : ldexpf(fabsf(a.scale) * LOG2E, (QB == 3 ? 8 : 0) - e);
 }
 
-// Scores of 16 keys with one column (times M), from the sums with each byte.
-template <int NL, int KS>
-__device__ __forceinline__ void score_tile(const i32x4 (&k)[KS], const i32x4 (&ql)[NL][KS], float (&s)[4]) {
-    i32x4 d[NL];
+// Scores of 16 keys with one column, in the units of the last byte but (three bytes) one.
+template <int QB, int KS>
+__device__ __forceinline__ void score_tile(const i32x4 (&k)[KS], const i32x4 (&ql)[QB][KS], float (&s)[4]) {
+    i32x4 d = {0, 0, 0, 0}, h = {0, 0, 0, 0};
+    if (QB == 3) {
 #pragma unroll
-    for (int n = 0; n < NL; n++) {
-        d[n] = i32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int x = 0; x < KS; x++) d[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[n][x], d[n], 0, 0, 0);
+        for (int x = 0; x < KS; x++) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[QB - 1][x], d, 0, 0, 0);
+        d >>= 8;
     }
 #pragma unroll
-    for (int r = 0; r < 4; r++) {
-        const float hi = (float)(d[0][r] * 256 + d[1][r]);  // below 2^30
-        s[r] = NL == 3 ? fmaf(hi, 256.0f, (float)d[NL - 1][r]) : hi;
-    }
+    for (int x = 0; x < KS; x++) h = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[0][x], h, 0, 0, 0);
+#pragma unroll
+    for (int x = 0; x < KS; x++) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[1][x], d, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; r++) s[r] = (float)(h[r] * 256 + d[r]);  // below 2^30
 }
 
 // One workgroup of W waves per (sequence, kv head, 16 columns, split of the
 // pages); its waves take the split's pages in turn and join their sums at the
 // end.  splits > 1: unnormalised results [row][head][split][DP + 2] in ws.
-template <int DP, int NL, class T, int W>
+template <int DP, int PL, class T, int W>
 __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
-    constexpr float P = NL == 3 ? 127.0f * 65536 : 127.0f * 256;
+    constexpr float P = PL == 3 ? 127.0f * 65536 : 127.0f * 256;
     __shared__ __attribute__((aligned(16))) float so[W][16][DP + 4];
     __shared__ float sml[W][2][16];
     int b = blockIdx.x;
@@ -258,8 +255,8 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
     const int first = pg0 + split * pps, last = pg0 + min(np, (split + 1) * pps);
     if (split > 0 && first >= last) return;  // the join knows
 
-    i32x4 ql[NL][KS];
-    const float f = query_bytes<NL, KS, T>(a, col, g4, ql);
+    i32x4 ql[3][KS];
+    const float f = query_bytes<3, KS, T>(a, col, g4, ql);
 
     float m = -INFINITY, l = 0.0f;
     float o[DT][4];
@@ -275,7 +272,7 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
         const float fk = f * t.sk;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
-            score_tile<NL, KS>(t.k[kt], ql, s[kt]);
+            score_tile<3, KS>(t.k[kt], ql, s[kt]);
 #pragma unroll
             for (int r = 0; r < 4; r++) s[kt][r] *= fk;
         }
@@ -299,7 +296,7 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
         if (mp == INFINITY) l = NAN;
         const float base = mp == -INFINITY ? 0.0f : mp;
         // the page's weights as bytes, and their sum (exact)
-        i32x4 pl[NL];
+        i32x4 pl[PL];
         unsigned sum = 0;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
@@ -309,15 +306,15 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
                 const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
                 v[r] = (unsigned)rintf(e * P);
                 sum += v[r];
-                v[r] += NL == 3 ? 0x8080 : 0x80;
+                v[r] += PL == 3 ? 0x8080 : 0x80;
             }
-            if (NL == 3) {
+            if (PL == 3) {
                 const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010602u);  // bytes 2 | bytes 1
                 const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010602u);
                 const unsigned b01 = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), b23 = __builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u);
                 pl[0][kt] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
                 pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
-                pl[NL - 1][kt] = (int)(__builtin_amdgcn_perm(b23, b01, 0x05040100u) ^ 0x80808080u);
+                pl[PL - 1][kt] = (int)(__builtin_amdgcn_perm(b23, b01, 0x05040100u) ^ 0x80808080u);
             } else {
                 const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x04000501u);  // bytes 1 | bytes 0
                 const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x04000501u);
@@ -333,14 +330,14 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
         const float av = add * t.sv;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
-            i32x4 d[NL];
+            i32x4 d[PL];
 #pragma unroll
-            for (int n = 0; n < NL; n++)
+            for (int n = 0; n < PL; n++)
                 d[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(t.v[dt], pl[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float hi = (float)(d[0][r] * 256 + d[1][r]);
-                o[dt][r] = fmaf(o[dt][r], keep, (NL == 3 ? fmaf(hi, 256.0f, (float)d[NL - 1][r]) : hi) * av);
+                o[dt][r] = fmaf(o[dt][r], keep, (PL == 3 ? fmaf(hi, 256.0f, (float)d[PL - 1][r]) : hi) * av);
             }
         }
     };
@@ -439,13 +436,14 @@ __global__ __launch_bounds__(64) void k_kv8_join(Kv8Attention a, int g, int spli
     if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
-// Four waves of CT x 16 columns each, over all pages that these see.  The
+// Four waves of CT x 16 columns each, over all pages that these see, with PL f16
+// a weight.  The
 // running maximum follows only when a score exceeds it by 2^8, and the output's
 // unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
 // 2^3 at the running maximum and have room for both.
-template <int DP, int NL, class T, int CT>
+template <int DP, int PL, class T, int CT>
 __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int per_xcd) {
-    constexpr int KS = Tile<DP>::KS, DT = DP / 16, PL = NL - 1;  // PL: f16 a weight
+    constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr float SLACK = 8.0f, P0 = 3.0f, UNIT = 16.0f;
     // consecutive workgroups go to the 8 XCDs in turn: each gets whole heads,
     // whose K and V its L2 then holds; a head's longest rows first
@@ -464,14 +462,15 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
     const int first = any0 / KV8_PAGE, last = (any1 + KV8_PAGE - 1) / KV8_PAGE;
 
-    i32x4 ql[CT][NL][KS];
+    constexpr int QB = PL + 1;  // bytes of a query
+    i32x4 ql[CT][QB][KS];
     float f[CT], m[CT], l[CT];
     int begin[CT], end[CT];
     f32x4 o[CT][DT];
 #pragma unroll
     for (int t = 0; t < CT; t++) {
         const Column col = column(a, q, kvh, g, f0 + t * 16 + c);
-        f[t] = query_bytes<NL, KS, T>(a, col, g4, ql[t]);
+        f[t] = query_bytes<QB, KS, T>(a, col, g4, ql[t]);
         begin[t] = col.begin;
         end[t] = col.end;
         m[t] = -INFINITY;
@@ -513,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 #pragma unroll
         for (int t = 0; t < CT; t++)
 #pragma unroll
-            for (int kt = 0; kt < 4; kt++) score_tile<NL, KS>(kr[kt], ql[t], s[t][kt]);
+            for (int kt = 0; kt < 4; kt++) score_tile<QB, KS>(kr[kt], ql[t], s[t][kt]);
         const bool missing = id < 0;
         if (pg + 1 < last) {
             id = page_id(a.c, q, pg + 1);
@@ -641,18 +640,19 @@ template <int DP, class T> constexpr int prompt_tiles() {
 }
 
 template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, hipStream_t st) {
-    constexpr int NL = std::is_same<T, float>::value ? 3 : 2, CT = prompt_tiles<DP, T>();
+    constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
+    constexpr int CT = prompt_tiles<DP, T>();
     const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window);
     if (p.prompt) {
         const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
         const int64_t per_xcd = (tiles * a.s.n_seq * a.c.hk + 7) / 8;
         if (per_xcd * 8 > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((k_kv8_prompt<DP, NL, T, CT>), dim3(per_xcd * 8), dim3(256), 0, st, a, p.g, (int)tiles,
+        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(per_xcd * 8), dim3(256), 0, st, a, p.g, (int)tiles,
                            (int)per_xcd);
         return hipGetLastError();
     }
     if (p.blocks > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_kv8_attend<DP, NL, T, 4>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles, p.splits, p.pps, ws);
+    hipLaunchKernelGGL((k_kv8_attend<DP, full ? 3 : 2, T, 4>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles, p.splits, p.pps, ws);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;
