@@ -135,21 +135,27 @@ template <int DP> struct Tile {
 // First of the 16 dims a lane reads of a key; dims past a narrow head's meet zeros of the query.
 template <int DP> __device__ __forceinline__ int k_dim(int g4) { return (DP >= 64 ? g4 : g4 % (DP / 16)) * 16; }
 template <int DP>
-__device__ __forceinline__ void load_tile(Tile<DP> &t, const Kv8View &c, int id, int kvh, int lane) {
+__device__ __forceinline__ void load_k(Tile<DP> &t, const Kv8View &c, int id, int kvh, int lane) {
     const int64_t ph = (int64_t)max(id, 0) * c.hk + kvh;
-    const page_ptr k = scalar_address(c.k + ph * (KV8_PAGE * DP)), v = scalar_address(c.v + ph * (KV8_PAGE * DP));
+    const page_ptr k = scalar_address(c.k + ph * (KV8_PAGE * DP));
     const int i = lane & 15, g4 = lane >> 4;
     // the page's address in scalar registers, the lane's offset in one vector register
-    const unsigned koff = ((i >> 2) * 16 + (i & 3)) * DP + k_dim<DP>(g4), voff = i * KV8_PAGE + g4 * 16;
+    const unsigned koff = ((i >> 2) * 16 + (i & 3)) * DP + k_dim<DP>(g4);
 #pragma unroll
     for (int s = 0; s < Tile<DP>::KS; s++)
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) t.k[kt][s] = load16(k + koff + (kt * 4 * DP + s * 64));
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; dt++) t.v[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
     t.sk = uniform(&c.scales[ph].x);
     t.sv = uniform(&c.scales[ph].y);
     t.bad = uniform(c.bad + ph);
+}
+template <int DP>
+__device__ __forceinline__ void load_v(Tile<DP> &t, const Kv8View &c, int id, int kvh, int lane) {
+    const int64_t ph = (int64_t)max(id, 0) * c.hk + kvh;
+    const page_ptr v = scalar_address(c.v + ph * (KV8_PAGE * DP));
+    const unsigned voff = (lane & 15) * KV8_PAGE + (lane >> 4) * 16;
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; dt++) t.v[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
 }
 
 // A column's query as QB bytes a value, ready as the second operand, and the
@@ -230,7 +236,7 @@ __device__ __forceinline__ void score_tile(const i32x4 (&k)[KS], const i32x4 (&q
 // pages); its waves take the split's pages in turn and join their sums at the
 // end.  splits > 1: unnormalised results [row][head][split][DP + 2] in ws.
 template <int DP, int PL, class T, int W>
-__global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
+__global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr float P = PL == 3 ? 127.0f * 65536 : 127.0f * 256;
@@ -265,8 +271,8 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
 #pragma unroll
         for (int r = 0; r < 4; r++) o[dt][r] = 0.0f;
 
-    auto page = [&](const Tile<DP> &t, int id, int pg) __attribute__((always_inline)) {
-        if (id < 0) return;
+    auto page = [&](Tile<DP> &t, int id, int pg, int next) __attribute__((always_inline)) {
+        const bool missing = id < 0;
         // scores in units of log2
         float s[4][4];
         const float fk = f * t.sk;
@@ -276,11 +282,16 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
 #pragma unroll
             for (int r = 0; r < 4; r++) s[kt][r] *= fk;
         }
-        const int j0 = pg * KV8_PAGE;
+        float sv = t.sv;
         unsigned long long bad = t.bad;
-        if (!(t.sk >= 0.0f && t.sk <= FLT_MAX && t.sv >= 0.0f && t.sv <= FLT_MAX)) bad = ~0ull;
-        if (j0 < all0 || j0 + KV8_PAGE > all1 || bad) {
-            const unsigned see = visible16(col.begin, col.end, j0 + g4 * 16), lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
+        if (!(t.sk >= 0.0f && t.sk <= FLT_MAX && sv >= 0.0f && sv <= FLT_MAX)) {
+            bad = ~0ull;
+            sv = 0.0f;  // columns that do not see the page add nothing
+        }
+        if (pg + W < last) load_k(t, a.c, next, kvh, lane);
+        const int j0 = pg * KV8_PAGE;
+        if (j0 < all0 || j0 + KV8_PAGE > all1 || bad || missing) {
+            const unsigned see = missing ? 0 : visible16(col.begin, col.end, j0 + g4 * 16), lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
             if (see & lost) l = NAN;
 #pragma unroll
             for (int kt = 0; kt < 4; kt++)
@@ -327,7 +338,7 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
         const float add = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn) * (1.0f / P);
         l = fmaf(l, keep, (float)sum * add);
         m = mn;
-        const float av = add * t.sv;
+        const float av = add * sv;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             i32x4 d[PL];
@@ -342,23 +353,15 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
         }
     };
 
-    // two pages in registers: the next one's loads are under way while one is worked on
     auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? page_id(a.c, q, pg) : -1; };
-    Tile<DP> ta, tb;
-    int pg = first + wave, ia = id_of(pg), ib = id_of(pg + W);
-    if (pg < last) load_tile<DP>(ta, a.c, ia, kvh, lane);
-    while (pg < last) {
-        const int ic = id_of(pg + 2 * W);
-        if (pg + W < last) load_tile<DP>(tb, a.c, ib, kvh, lane);
-        page(ta, ia, pg);
-        pg += W;
-        if (pg >= last) break;
-        const int id = id_of(pg + 2 * W);
-        if (pg + W < last) load_tile<DP>(ta, a.c, ic, kvh, lane);
-        page(tb, ib, pg);
-        pg += W;
-        ia = ic;
-        ib = id;
+    Tile<DP> t;
+    int pg = first + wave, id = id_of(pg);
+    if (pg < last) load_k(t, a.c, id, kvh, lane);
+    for (; pg < last; pg += W) {
+        load_v(t, a.c, id, kvh, lane);
+        const int next = id_of(pg + W);
+        page(t, id, pg, next);
+        id = next;
     }
 
     if (f != f && any1 > any0) l = NAN;  // a query that is not finite
@@ -401,12 +404,16 @@ __global__ __launch_bounds__(64 * W, DP == 128 ? 1 : 2) void k_kv8_attend(Kv8Att
     }
 }
 
-// Joins a row's splits: one wave per (row of a sequence, head).
+// Joins a row's splits: one workgroup per (row of a sequence, head), the
+// splits dealt out to its waves.
+constexpr int JOIN_WAVES = 4;
 template <int DP, class T>
-__global__ __launch_bounds__(64) void k_kv8_join(Kv8Attention a, int g, int splits, int pps,
-                                                 const float *__restrict__ ws) {
+__global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, int g, int splits, int pps,
+                                                              const float *__restrict__ ws) {
+    constexpr int DL = DP > 64 ? DP / 64 : 1;  // dims a lane
+    __shared__ float so[JOIN_WAVES][DP], sl[JOIN_WAVES];
     const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads;
-    const int r = b % a.s.max_rows, lane = threadIdx.x;
+    const int r = b % a.s.max_rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Kv8Seq q = kv8_seq(a.s, b / a.s.max_rows);
     if (r >= q.n) return;
     // the splits of its 16 columns that had pages
@@ -421,19 +428,32 @@ __global__ __launch_bounds__(64) void k_kv8_join(Kv8Attention a, int g, int spli
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor(mm, x));
     const float base = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, oo[(DP + 63) / 64] = {};
-    for (int s = 0; s < used; s++) {
+    float ll = 0.0f, oo[DL] = {};
+#pragma unroll 4
+    for (int s = wave; s < used; s += JOIN_WAVES) {
         const float *ps = p + s * (DP + 2);
-        const float x = __builtin_amdgcn_exp2f(ps[DP] - base);
-        ll += ps[DP + 1] != ps[DP + 1] ? NAN : ps[DP + 1] * x;
+        const float l = ps[DP + 1], x = __builtin_amdgcn_exp2f(ps[DP] - base);
+        ll += l != l ? NAN : l * x;
 #pragma unroll
-        for (int u = 0; u < (DP + 63) / 64; u++)
-            if (lane + 64 * u < DP) oo[u] = fmaf(ps[lane + 64 * u], x, oo[u]);
+        for (int u = 0; u < DL; u++)
+            if (DP >= 64 || lane < DP) oo[u] = fmaf(ps[lane + 64 * u], x, oo[u]);
     }
 #pragma unroll
-    for (int u = 0; u < (DP + 63) / 64; u++)
-        if (lane + 64 * u < a.c.d) store_out<T>(a, row, h, lane + 64 * u, ll == 0.0f ? 0.0f : oo[u] / ll);
-    if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
+    for (int u = 0; u < DL; u++)
+        if (DP >= 64 || lane < DP) so[wave][lane + 64 * u] = oo[u];
+    if (lane == 0) sl[wave] = ll;
+    __syncthreads();
+    ll = 0.0f;
+#pragma unroll
+    for (int w = 0; w < JOIN_WAVES; w++) ll += sl[w];
+    const int i = threadIdx.x;
+    if (i < a.c.d) {
+        float o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < JOIN_WAVES; w++) o += so[w][i];
+        store_out<T>(a, row, h, i, ll == 0.0f ? 0.0f : o / ll);
+    }
+    if (a.lse && i == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
 // Four waves of CT x 16 columns each, over all pages that these see, with PL f16
@@ -518,7 +538,10 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
             id = page_id(a.c, q, pg + 1);
             load_k(id);
         }
-        if (!(sk >= 0.0f && sk <= FLT_MAX && sv >= 0.0f && sv <= FLT_MAX)) bad = ~0ull;
+        if (!(sk >= 0.0f && sk <= FLT_MAX && sv >= 0.0f && sv <= FLT_MAX)) {
+            bad = ~0ull;
+            sk = sv = 0.0f;  // columns that do not see the page add nothing
+        }
         const int j0 = pg * KV8_PAGE;
         if (j0 < all0 || j0 + KV8_PAGE > all1 || bad || missing) {  // hidden keys
 #pragma unroll
@@ -657,7 +680,7 @@ template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, h
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;
     if (rows > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_kv8_join<DP, T>), dim3(rows), dim3(64), 0, st, a, p.g, p.splits, p.pps, ws);
+    hipLaunchKernelGGL((k_kv8_join<DP, T>), dim3(rows), dim3(64 * JOIN_WAVES), 0, st, a, p.g, p.splits, p.pps, ws);
     return hipGetLastError();
 }
 
