@@ -325,7 +325,7 @@ def append_ref(c, table, start, k, v):
     return want
 
 
-def run_append(hip, rng, lens, rows, hk, g, d, dtype, rope=None, edit=None, q=True, inplace=False, n_pages=None):
+def run_append(hip, rng, lens, rows, hk, g, d, dtype, rope=None, edit=None, q=True, inplace=False, n_pages=None, gap=0):
     need = sum(-(-n // R.PAGE) for n in lens)
     c = R.Cache(hip, rng, n_pages or need + 2, hk, d)
     table = R.tables(rng, lens, len(c.k))
@@ -336,8 +336,8 @@ def run_append(hip, rng, lens, rows, hk, g, d, dtype, rope=None, edit=None, q=Tr
     qx = R.rounded(rng.standard_normal((n, h, d)), dtype)
     if edit:
         edit(k, v, c, table)
-    width = (h + 2 * hk) * d
-    base = R.put(hip, np.concatenate([x.reshape(n, -1) for x in (qx, k, v)], 1), dtype)
+    width = (h + 2 * hk) * d + gap
+    base = R.put(hip, np.concatenate([x.reshape(n, -1) for x in (qx, k, v)] + [np.zeros((n, gap))], 1), dtype)
     qo = base if inplace else R.put(hip, np.full((n, h, d), 5.0), dtype)
     arr = [DeviceArray(hip, x) for x in (cu, np.asarray(lens, np.int32), table)]
     cache = c.upload()
@@ -414,6 +414,25 @@ def test_append(hip, dtype, d, hk, g, kind):
                inplace=kind == 2, q=kind != 3)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("d,hk,g", [(16, 3, 1), (24, 2, 2), (32, 1, 4), (64, 2, 1), (128, 2, 3)])
+@pytest.mark.parametrize("kind", [0, 1, 2])
+def test_append_few_rows(hip, dtype, d, hk, g, kind):
+    """One to four rows a sequence, over a page's end, an idle stream among them; kept codes of all word offsets."""
+    rng = np.random.default_rng(d + kind)
+    rope = None if ROPES[kind] is None else ch.Rope(d, **ROPES[kind])
+    run_append(hip, rng, [1, 2, 7, 64, 66, 65, 130, 0, 99], [1, 2, 3, 4, 4, 1, 2, 0, 1], hk, g, d, dtype, rope)
+    run_append(hip, rng, [6, 64, 130], [1, 1, 1], hk, g, d, dtype, rope)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("rows", [1, 70])
+def test_append_rows_of_any_alignment(hip, dtype, rows):
+    rng = np.random.default_rng(rows)
+    run_append(hip, rng, [100, 71], [rows, rows], 2, 2, 64, dtype, ch.Rope(64), gap=1)
+    run_append(hip, rng, [100, 71], [rows, rows], 2, 1, 32, dtype, ch.Rope(10, interleaved=True))
+
+
 def test_append_far_positions(hip):
     """Angles of positions that FP32 products of position and frequency lose."""
     rng = np.random.default_rng(1)
@@ -445,6 +464,7 @@ def test_append_not_finite_and_extremes(hip):
         k[70:, 1] *= 1e-44                                       # values that have no scale
         v[70:, 0] *= 1e30
     run_append(hip, rng, [70, 40], [70, 40], 2, 1, 64, "float32", ch.Rope(64), edit=edit)
+    run_append(hip, rng, [70, 40], [70, 40], 2, 1, 64, "float32", ch.Rope(64), edit=edit, gap=3)
 
     def keep(k, v, c, table):  # a page whose kept tokens are small, bad, or without a scale
         c.scales[table[0, 0], 0] = 1e-6
@@ -453,6 +473,12 @@ def test_append_not_finite_and_extremes(hip):
         c.bad[table[0, 0], 0] = np.uint64(0xF0F0F0F0F0F0F0F0)
         k[0, 1], v[0, 1] = 0, 0
     run_append(hip, rng, [30], [1], 2, 2, 64, "float32", edit=keep)
+
+    def lost(k, v, c, table):
+        keep(k, v, c, table)
+        k[0, 0, 5], v[2, 0, 63] = np.inf, np.nan
+    run_append(hip, rng, [31], [3], 2, 2, 64, "float32", edit=lost)
+    run_append(hip, rng, [50], [20], 2, 2, 64, "float32", edit=lost)
     run_append(hip, rng, [30], [9], 2, 2, 128, "bfloat16", edit=keep)
 
 
