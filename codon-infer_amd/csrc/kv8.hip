@@ -260,31 +260,36 @@ __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, Row
     // V: pieces of four tokens n4 .., aligned to the page's words
     const T *vp = static_cast<const T *>(v.p) + t.h * v.hs;
     const int q0 = t.lo / 4, nq = (t.hi + 3) / 4 - q0, chunks = d / VL;
-    float vx[VIT][4][VL];
-    unsigned mv = 0;
+    // (loads without branches, at the nearest row there is, so that all are under way at once)
+    float vx[VIT][4][VL], kx[KIT][2][VL];
+    unsigned mv = 0, mk = 0;
+    const int items = d / (2 * VL), turned = rope.rot / (2 * VL);
 #pragma unroll
     for (int it = 0; it < VIT; it++) {
+        if (it * NT >= chunks * nq) continue;
         const int x = tid + it * NT, ch = x / nq, n4 = 4 * (q0 + x - ch * nq);
 #pragma unroll
-        for (int u = 0; u < 4; u++) {
-            const int n = n4 + u;
-            if (ch < chunks && n >= t.lo && n < t.hi) {
-                load_chunk<T>(vp + (row0 + n - t.lo) * v.rs + ch * VL, vx[it][u]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VL; e++) vx[it][u][e] = 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < VL; e++) mv = max(mv, abs_bits(vx[it][u][e]));
-        }
+        for (int u = 0; u < 4; u++)
+            load_chunk<T>(vp + (row0 + min(max(n4 + u, t.lo), t.hi - 1) - t.lo) * v.rs + min(ch, chunks - 1) * VL, vx[it][u]);
     }
     // K and Q: items of two pieces
     const T *kp = static_cast<const T *>(k.p) + t.h * k.hs;
-    const int items = d / (2 * VL), turned = rope.rot / (2 * VL);
-    float kx[KIT][2][VL];
-    unsigned mk = 0;
 #pragma unroll
     for (int it = 0; it < KIT; it++) {
+        if (it * NT >= nt * items) continue;
+        const int x = tid + it * NT, n = min(x / items, nt - 1), i = x % items;
+        const bool turn = i < turned;
+        const int da = turn && !rope.inter ? i * VL : i * 2 * VL, db = turn && !rope.inter ? da + rope.rot / 2 : da + VL;
+        load_chunk<T>(kp + (row0 + n) * k.rs + da, kx[it][0]);
+        load_chunk<T>(kp + (row0 + n) * k.rs + db, kx[it][1]);
+    }
+#pragma unroll
+    for (int it = 0; it < KIT; it++) {
+        if (it * NT >= nt * items) {
+#pragma unroll
+            for (int e = 0; e < VL; e++) kx[it][0][e] = kx[it][1][e] = 0.0f;
+            continue;
+        }
         const int x = tid + it * NT, n = x / items, i = x - n * items;
         const bool live = n < nt, turn = i < turned;
         const int da = turn && !rope.inter ? i * VL : i * 2 * VL, db = turn && !rope.inter ? da + rope.rot / 2 : da + VL;
@@ -310,35 +315,65 @@ __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, Row
             }
         };
         if (live) {
-            load_chunk<T>(kp + (row0 + n) * k.rs + da, kx[it][0]);
-            load_chunk<T>(kp + (row0 + n) * k.rs + db, kx[it][1]);
+            const T *qr = static_cast<const T *>(q.p) + (row0 + n) * q.rs + t.h * g * q.hs;
+            T *qw = static_cast<T *>(qo.p) + (row0 + n) * qo.rs + t.h * g * qo.hs;
+            float qa[VL], qb[VL];  // the next head's
+            if (q.p) {
+                load_chunk<T>(qr + da, qa);
+                load_chunk<T>(qr + db, qb);
+            }
             float cs[VL], sn[VL];
             if (turn) {
 #pragma unroll
                 for (int e = 0; e < VL; e++) rope_cs(rope, p0 + n, (rope.inter ? da / 2 : da) + e, cs[e], sn[e]);
                 rotate(kx[it][0], kx[it][1], cs, sn);
             }
-            if (q.p) {
-                const T *qr = static_cast<const T *>(q.p) + (row0 + n) * q.rs + t.h * g * q.hs;
-                T *qw = static_cast<T *>(qo.p) + (row0 + n) * qo.rs + t.h * g * qo.hs;
-#pragma unroll 2
+            if (q.p)
                 for (int hq = 0; hq < g; hq++) {
                     float a[VL], b[VL];
-                    load_chunk<T>(qr + hq * q.hs + da, a);
-                    load_chunk<T>(qr + hq * q.hs + db, b);
+#pragma unroll
+                    for (int e = 0; e < VL; e++) {
+                        a[e] = qa[e];
+                        b[e] = qb[e];
+                    }
+                    if (hq + 1 < g) {
+                        load_chunk<T>(qr + (hq + 1) * q.hs + da, qa);
+                        load_chunk<T>(qr + (hq + 1) * q.hs + db, qb);
+                    }
                     if (turn) rotate(a, b, cs, sn);
                     store_chunk<T>(qw + hq * qo.hs + da, a);
                     store_chunk<T>(qw + hq * qo.hs + db, b);
                 }
-            }
-        } else {
+        }
 #pragma unroll
-            for (int e = 0; e < VL; e++) kx[it][0][e] = kx[it][1][e] = 0.0f;
+        for (int e = 0; e < VL; e++) {
+            kx[it][0][e] = live ? kx[it][0][e] : 0.0f;
+            kx[it][1][e] = live ? kx[it][1][e] : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < VL; e++) mk = max(mk, max(abs_bits(kx[it][0][e]), abs_bits(kx[it][1][e])));
     }
     if (id < 0) return;
+#pragma unroll
+    for (int it = 0; it < VIT; it++) {
+        if (it * NT >= chunks * nq) {
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+#pragma unroll
+                for (int e = 0; e < VL; e++) vx[it][u][e] = 0.0f;
+            continue;
+        }
+        const int x = tid + it * NT, ch = x / nq, n4 = 4 * (q0 + x - ch * nq);
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const bool live = ch < chunks && n4 + u >= t.lo && n4 + u < t.hi;
+#pragma unroll
+            for (int e = 0; e < VL; e++) {
+                vx[it][u][e] = live ? vx[it][u][e] : 0.0f;
+                mv = max(mv, abs_bits(vx[it][u][e]));
+            }
+        }
+    }
     auto all = [&]() {  // mk and mv over the workgroup
         mk = wave_max_bits(mk);
         mv = wave_max_bits(mv);
