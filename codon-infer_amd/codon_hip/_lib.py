@@ -34,6 +34,7 @@ EXPORTED = [
     "cih_decoder_create", "cih_decoder_destroy", "cih_decoder_reset", "cih_decode", "cih_generate",
     "cih_matmul_tiled_noalloc", "cih_rope_init", "cih_kv8_append", "cih_kv8_read", "cih_kv8_attention",
     "cih_kv8_attention_workspace", "cih_token_logprobs", "cih_token_logprobs_workspace",
+    "cih_decoder_create_kv8", "cih_decoder_score", "cih_decoder_read_cache",
 ]
 
 DMS_MASKED_MARGINAL, DMS_WILDTYPE_MARGINAL = 0, 1
@@ -118,6 +119,9 @@ def lib():
         "cih_forward": [vp, vp, vp, i32, i32, ctypes.c_uint32, ctypes.POINTER(Outputs)],
         "cih_dms": [vp, vp, i32, i32, i32, i32, i32, vp, vp],
         "cih_decoder_create": [vp, i32, i32, i32, pmodel],
+        "cih_decoder_create_kv8": [vp, i32, i32, i32, i32, vp, pmodel],
+        "cih_decoder_score": [vp, i32, vp, vp, vp, i32, vp, vp, vp, vp],
+        "cih_decoder_read_cache": [vp, i32, i32, i32, i32, vp, vp],
         "cih_decoder_destroy": [vp],
         "cih_decoder_reset": [vp, i32],
         "cih_decode": [vp, vp, vp, vp, i32, vp],

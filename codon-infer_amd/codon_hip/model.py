@@ -494,13 +494,24 @@ class GenerationMetrics:
 class GpuDecoder:
     """RunState (lib.rs:2459-2486) on the GPU for n_slots sequences: per-slot
     KV caches, forward_* for batches of rows (decode), and the
-    generate_sequence* loop (generate)."""
+    generate_sequence* loop (generate).
 
-    def __init__(self, model, n_slots=1, max_len=None, max_rows=64):
+    kv8: keys and values in 8 bits (cih_decoder_create_kv8), in pages of 64
+    positions from a pool of n_pages (0: enough for every slot's max_len);
+    rope: a Rope that replaces the model's rotary positions."""
+
+    def __init__(self, model, n_slots=1, max_len=None, max_rows=64, kv8=False, n_pages=0, rope=None):
         self.model = model
         self.max_len = max_len or model.cfg.max_seq_len
         self._h = ctypes.c_void_p()
-        C.check(C.lib().cih_decoder_create(model._h, n_slots, self.max_len, max_rows, ctypes.byref(self._h)))
+        if kv8:
+            C.check(C.lib().cih_decoder_create_kv8(model._h, n_slots, self.max_len, max_rows, n_pages,
+                                                   None if rope is None else ctypes.addressof(rope.struct),
+                                                   ctypes.byref(self._h)))
+        elif n_pages or rope is not None:
+            raise ValueError("n_pages and rope need kv8")
+        else:
+            C.check(C.lib().cih_decoder_create(model._h, n_slots, self.max_len, max_rows, ctypes.byref(self._h)))
         self.n_slots, self.max_rows = n_slots, max_rows
 
     def close(self):
@@ -528,6 +539,30 @@ class GpuDecoder:
         C.check(C.lib().cih_decode(self._h, slots.ctypes.data, tokens.ctypes.data, pos.ctypes.data, n,
                                    out.ctypes.data))
         return out
+
+    def score(self, seqs, top_k=0, slots=None):
+        """How likely sequences of token ids are (cih_decoder_score): for each
+        a dict of logprob (of the token after each, 0 at the last), entropy,
+        top_ids and top_logprobs [len][top_k]."""
+        n = len(seqs)
+        slots = np.arange(n, dtype=np.int32) if slots is None else np.ascontiguousarray(slots, np.int32)
+        if slots.size != n:
+            raise ValueError("one slot a sequence")
+        flat = np.concatenate([np.asarray(s, np.int32).ravel() for s in seqs]).astype(np.int32)
+        offs = np.zeros(n + 1, np.int32)
+        offs[1:] = np.cumsum([len(s) for s in seqs])
+        lp, en = np.empty(flat.size, np.float32), np.empty(flat.size, np.float32)
+        ids, tl = np.empty((flat.size, top_k), np.int32), np.empty((flat.size, top_k), np.float32)
+        C.check(C.lib().cih_decoder_score(self._h, n, slots.ctypes.data, flat.ctypes.data, offs.ctypes.data, top_k,
+                                          lp.ctypes.data, en.ctypes.data, ids.ctypes.data, tl.ctypes.data))
+        return [{"logprob": lp[a:b], "entropy": en[a:b], "top_ids": ids[a:b], "top_logprobs": tl[a:b]}
+                for a, b in zip(offs[:-1], offs[1:])]
+
+    def read_cache(self, layer, slot, pos, n):
+        """K (rotated) and V of n positions of a slot: two [n][dim] arrays."""
+        k, v = (np.empty((n, self.model.cfg.dim), np.float32) for _ in range(2))
+        C.check(C.lib().cih_decoder_read_cache(self._h, layer, slot, pos, n, k.ctypes.data, v.ctypes.data))
+        return k, v
 
     def generate(self, prompts, temperature=0.0, max_new_tokens=None, seeds=None, slots=None, max_seq_len=0):
         """generate_sequence* (lib.rs:6551-6827) for a list of prompt id

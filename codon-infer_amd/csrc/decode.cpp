@@ -7,13 +7,37 @@
 // number of rows, each (slot, token, position): the weights are read once
 // for all rows (the GEMV for up to 8 rows, the MFMA GEMM above), so
 // independent sequences decode together and a prompt prefills in one call.
+//
+// cih_decoder_create_kv8's decoder holds its keys and values in the 8-bit paged
+// cache (kv8.h): the slots take pages of 64 positions from one pool as they
+// grow, the same page ids in every layer, and rotary positions may be scaled.
 #include <chrono>
 #include <cmath>
 #include <cstring>
+#include <exception>
 #include <map>
 #include <tuple>
 
+#include "kv8.h"
 #include "model.h"
+
+// The 8-bit cache of a decoder.
+struct DecoderKv8 {
+    bool on = false;
+    int n_pages = 0, max_pages = 0;            // of the pool, of a slot
+    cih::Kv8View view{};                       // layer 0; the layers follow one another
+    int *d_table = nullptr, *d_seq = nullptr;  // [slots][max_pages]; cu_rows | lens | slots of the call's sequences
+    int *h_table = nullptr, *h_seq = nullptr;  // pinned
+    float *ws = nullptr;
+    size_t ws_floats = 0;
+    cih::RopeArg rope;
+    std::vector<int> free_pages;
+    std::vector<std::vector<int>> pages;  // of each slot, in order
+    std::vector<int> changed;             // slots whose row of the table has to be copied
+    // staged call: sequences, the most rows of one, staged row of each row of the caller
+    int n_seq = 0, max_rows = 0;
+    std::vector<int> order;
+};
 
 struct cih_decoder {
     cih_model *m = nullptr;
@@ -28,6 +52,11 @@ struct cih_decoder {
     int *d_flag = nullptr;  // device status word of a step (FLAG_* bits)
     cih::PartialBuf part;
     std::vector<int> filled;  // positions written per slot (0..filled-1 valid)
+    DecoderKv8 kv;
+    // cih_decoder_score: targets in; log probability | entropy | top log probabilities [64] | top ids [64] out
+    int *d_targets = nullptr, *d_top_ids = nullptr;
+    float *d_score = nullptr, *d_top_lp = nullptr, *d_lp_ws = nullptr;
+    int *h_score = nullptr;  // pinned: [max_rows][3 + 2 * 64]
     bool unique = false;      // staged rows: every slot at most once
     // (rows, fused, kernel switches) -> captured step
     std::map<std::tuple<int, bool, std::string>, hipGraphExec_t> graphs;
@@ -38,6 +67,13 @@ using namespace cih;
 
 namespace {
 
+// workspace of the log probabilities of up to `rows` rows (a few rows are split over more chunks than many)
+size_t score_ws_floats(int rows, int vocab) {
+    size_t most = 0;
+    for (int n = 1; n <= rows && n < 512; n++) most = std::max(most, token_logprobs_floats(n, vocab, LOGPROBS_MAX_TOP));
+    return std::max(most, token_logprobs_floats(rows, vocab, LOGPROBS_MAX_TOP));
+}
+
 void destroy(cih_decoder *dc) {
     if (!dc) return;
     if (dc->m && dc->m->stream) hipStreamSynchronize(dc->m->stream);
@@ -45,6 +81,8 @@ void destroy(cih_decoder *dc) {
     free_list(dc->allocs);
     if (dc->h_meta) hipHostFree(dc->h_meta);
     if (dc->h_logits) hipHostFree(dc->h_logits);
+    for (int *h : {dc->h_score, dc->kv.h_table, dc->kv.h_seq})
+        if (h) hipHostFree(h);
     delete dc;
 }
 
@@ -65,6 +103,34 @@ bool step_gemv16(const cih_decoder *dc, int n) {
 // that is no longer finite, and run again in full range.
 bool step_limbs(const cih_decoder *dc, int n) { return n > GEMV_MAX_M ? !full_range_mode() : step_gemv16(dc, n); }
 
+// Rows of the 8-bit cache: Q, K and V of dc->qkv rotated and appended, then the
+// attention, to dc->ao in FP32 or f16 limbs.
+int enqueue_kv8(cih_decoder *dc, int l, int n, int out_fmt) {
+    const cih_model *m = dc->m;
+    const int64_t d = m->cfg.dim, hd = m->hd, H = m->cfg.n_heads;
+    DecoderKv8 &kv = dc->kv;
+    const int64_t heads = (int64_t)l * kv.n_pages * H;  // (page, head)s before this layer's
+    Kv8Attention a{};
+    a.c = kv.view;
+    a.c.k += heads * KV8_PAGE * a.c.dp;
+    a.c.v += heads * KV8_PAGE * a.c.dp;
+    a.c.scales += heads;
+    a.c.bad += heads;
+    a.s = {kv.d_seq,    kv.d_seq + kv.n_seq + 1, kv.d_table, kv.d_seq + 2 * kv.n_seq + 1, kv.n_seq, n,
+           kv.max_rows, dc->slots,               kv.max_pages, kv.max_pages};
+    a.q = {dc->qkv, 3 * d, hd};
+    a.out = {dc->ao, d, hd};
+    a.dtype = FT_F32;
+    a.heads = (int)H;
+    a.out_h2 = out_fmt == AF_H2;
+    a.scale = 1.0f / std::sqrt((float)hd);
+    a.causal = 1;
+    HIPCHK(launch_kv8_append(a.c, a.s, FT_F32, RowsView{dc->qkv + d, 3 * d, hd}, RowsView{dc->qkv + 2 * d, 3 * d, hd},
+                             (int)H, a.q, a.q, kv.rope, m->stream));
+    HIPCHK(launch_kv8_attention(a, kv.ws, kv.ws_floats, m->stream));
+    return 0;
+}
+
 // The rows' forward from the staged device tokens / rows: embedding
 // (constant 0.88 scale, <mask> -> 0), the layers with cached causal
 // attention, final LN and LM head -> dc->logits.  Kernel launches only, so
@@ -84,6 +150,7 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
     // algorithmic attention work of the rows: keys 0..pos of their slot
     double keys = 0;
     for (int i = 0; i < n; i++) keys += dc->h_meta[dc->max_rows + 2 * i + 1] + 1;
+    const double key_bytes = dc->kv.on ? 2 : 8;  // of a key and its value, a dim
     const bool g16 = step_gemv16(dc, n);
     const size_t part_half = dc->part.floats / 2 / 64 * 64;
     float *const part_a = dc->part.part, *const part_b = dc->part.part + part_half;
@@ -96,7 +163,7 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
     const char *few_wo_env = getenv("CIH_FEW_WO");
     const bool fuse_wo = n <= 2 && (m->hd == 32 || m->hd == 64) && L > 0 &&
                          (m->layers[0].wo.fmt == WF_Q8 || m->layers[0].wo.fmt == WF_Q4) &&
-                         (size_t)H * n * d <= part_half && !(few_wo_env && !strcmp(few_wo_env, "0"));
+                         !dc->kv.on && (size_t)H * n * d <= part_half && !(few_wo_env && !strcmp(few_wo_env, "0"));
     // one row: the residual LayerNorms are formed inside the QKV and FC1
     // GEMVs (every workgroup normalises the row itself; the new residual goes
     // to xb, then back to x), two launches fewer per layer; CIH_DECODE_LN=0: apart
@@ -122,8 +189,11 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
         }
         float *kc = dc->kc + l * layer, *vc = dc->vc + l * layer;
         {
-            ProfScope ps(m, CIH_KC_ATTENTION, 4.0 * keys * d, 8.0 * keys * d + 24.0 * n * d);
-            if (fused && fuse_wo) {
+            ProfScope ps(m, CIH_KC_ATTENTION, 4.0 * keys * d, key_bytes * keys * d + 24.0 * n * d);
+            if (dc->kv.on) {
+                HIPCHK(launch_gemv16_fold(part_b, sq, n, 3 * d, ly.bqkv, dc->qkv, 3 * d, EPI_NONE, st));
+                if (int rc = enqueue_kv8(dc, l, n, AF_H2)) return rc;
+            } else if (fused && fuse_wo) {
                 // attention and each head's share of Wo in one kernel: the heads are Wo's splits
                 HIPCHK(launch_decode_attention_fused_wo(dc->qkv, part_b, sq, ly.bqkv, d, H, dc->d_rows, n,
                                                         dc->max_len, dc->rope_c, dc->rope_s, kc, vc, dc->slot_stride,
@@ -182,7 +252,7 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
         }
         // one row per sequence through the GEMV: the attention kernel adds
         // the QKV partial sums itself (no separate reduction)
-        const bool qkv_parts = fused && use_gemv(n, AF_F32, EPI_NONE);
+        const bool qkv_parts = fused && !dc->kv.on && use_gemv(n, AF_F32, EPI_NONE);
         int splits = 0;
         if (qkv_parts) {
             ProfScope ps(m, ly.wqkv.fmt == WF_F32 ? CIH_KC_GEMM_FP32 : CIH_KC_GEMM_QUANT, 2.0 * n * ly.wqkv.N * d,
@@ -194,8 +264,10 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
         float *kc = dc->kc + l * layer, *vc = dc->vc + l * layer;
         {
             // K and V read once per key, Q read, rows written
-            ProfScope ps(m, CIH_KC_ATTENTION, 4.0 * keys * d, 8.0 * keys * d + 24.0 * n * d);
-            if (fused) {
+            ProfScope ps(m, CIH_KC_ATTENTION, 4.0 * keys * d, key_bytes * keys * d + 24.0 * n * d);
+            if (dc->kv.on) {
+                if (int rc = enqueue_kv8(dc, l, n, af)) return rc;
+            } else if (fused) {
                 HIPCHK(launch_decode_attention_fused(dc->qkv, qkv_parts ? dc->part.part : nullptr, splits, ly.bqkv, d,
                                                      H, dc->d_rows, n, dc->max_len, dc->rope_c, dc->rope_s, kc, vc,
                                                      dc->slot_stride, dc->ao, st, af));
@@ -263,6 +335,17 @@ int run_rows(cih_decoder *dc, int n) {
     const bool fused = dc->unique;
     HIPCHK(hipMemcpyAsync(dc->d_tokens, dc->h_meta, (size_t)n * 4, hipMemcpyHostToDevice, st));
     HIPCHK(hipMemcpyAsync(dc->d_rows, dc->h_meta + dc->max_rows, (size_t)n * 8, hipMemcpyHostToDevice, st));
+    std::string switches = kernel_switches();
+    if (dc->kv.on) {
+        DecoderKv8 &kv = dc->kv;
+        HIPCHK(hipMemcpyAsync(kv.d_seq, kv.h_seq, (size_t)(3 * kv.n_seq + 1) * 4, hipMemcpyHostToDevice, st));
+        for (int slot : kv.changed) {
+            const size_t at = (size_t)slot * kv.max_pages;
+            HIPCHK(hipMemcpyAsync(kv.d_table + at, kv.h_table + at, (size_t)kv.max_pages * 4, hipMemcpyHostToDevice, st));
+        }
+        kv.changed.clear();
+        switches += std::to_string(kv.n_seq) + "," + std::to_string(kv.max_rows);  // what the grids and buffers go by
+    }
     // Rows whose activations travel as f16 limbs: a non-finite residual (an
     // overflowed limb) runs the rows again in full-range mode, kernel by
     // kernel, rewriting the same cache positions.
@@ -279,7 +362,7 @@ int run_rows(cih_decoder *dc, int n) {
         if (int rc = enqueue_rows(dc, n, fused)) return rc;
         return limbs ? check() : 0;
     }
-    auto key = std::make_tuple(n, fused, kernel_switches());
+    auto key = std::make_tuple(n, fused, switches);
     auto it = dc->graphs.find(key);
     if (it == dc->graphs.end()) {
         hipGraph_t g = nullptr;
@@ -300,11 +383,74 @@ int run_rows(cih_decoder *dc, int n) {
     return limbs ? check() : 0;
 }
 
+// Stages validated rows for the 8-bit cache: the rows of a slot together, in
+// the order in which the slots first appear, and the slots' pages: next[slot]
+// positions each.  Nothing changes where the pool has too few.
+int stage_kv8(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, const int32_t *pos, int n,
+              const std::map<int, int> &next) {
+    DecoderKv8 &kv = dc->kv;
+    int64_t spare = (int64_t)kv.free_pages.size(), want = 0;
+    for (auto &s : next) {
+        const int64_t need = (s.second + KV8_PAGE - 1) / KV8_PAGE;
+        want += need - (int64_t)kv.pages[s.first].size();
+    }
+    if (want > spare)
+        return set_error(CIH_ERR_CAPACITY, "the rows need %lld more pages of 64 positions, %lld are free", (long long)want,
+                         (long long)spare);
+    // later positions of a slot are forgotten, and their pages go back
+    for (int give = 1; give >= 0; give--)
+        for (auto &s : next) {
+            std::vector<int> &pg = kv.pages[s.first];
+            const size_t need = (s.second + KV8_PAGE - 1) / KV8_PAGE;
+            if (pg.size() == need || (pg.size() > need) != (give == 1)) continue;
+            while (pg.size() > need) {
+                kv.free_pages.push_back(pg.back());
+                pg.pop_back();
+            }
+            while (pg.size() < need) {
+                pg.push_back(kv.free_pages.back());
+                kv.free_pages.pop_back();
+            }
+            std::copy(pg.begin(), pg.end(), kv.h_table + (size_t)s.first * kv.max_pages);
+            kv.changed.push_back(s.first);
+        }
+    std::map<int, int> index;  // slot -> its place among the call's sequences
+    std::vector<int> count;
+    for (int i = 0; i < n; i++) {
+        auto it = index.emplace(slots[i], (int)index.size());
+        if (it.second) count.push_back(0);
+        count[it.first->second]++;
+    }
+    kv.n_seq = (int)count.size();
+    kv.max_rows = *std::max_element(count.begin(), count.end());
+    int *cu = kv.h_seq, *lens = cu + kv.n_seq + 1, *sl = lens + kv.n_seq;
+    cu[0] = 0;
+    for (int i = 0; i < kv.n_seq; i++) cu[i + 1] = cu[i] + count[i];
+    std::vector<int> at(cu, cu + kv.n_seq);
+    kv.order.resize(n);
+    for (int i = 0; i < n; i++) {
+        const int q = index[slots[i]], to = at[q]++;
+        kv.order[i] = to;
+        dc->h_meta[to] = tokens[i];
+        dc->h_meta[dc->max_rows + 2 * to] = slots[i];
+        dc->h_meta[dc->max_rows + 2 * to + 1] = pos[i];
+        lens[q] = next.at(slots[i]);
+        sl[q] = slots[i];
+    }
+    for (auto &s : next) dc->filled[s.first] = s.second;
+    return 0;
+}
+
+// The staged row of the caller's row i.
+int staged_row(const cih_decoder *dc, int i) { return dc->kv.on ? dc->kv.order[i] : i; }
+
 // Validates rows and stages them; rows of one slot must continue its
 // cache: consecutive positions starting at most at the slot's filled count.
 int stage_rows(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, const int32_t *pos, int n) {
     const int V = dc->m->cfg.vocab_size;
     if (n < 1 || n > dc->max_rows) return set_error(CIH_ERR_CAPACITY, "%d rows outside [1, %d]", n, dc->max_rows);
+    // a call before this one may still be copying the staged arrays
+    if (dc->kv.on) HIPCHK(hipStreamSynchronize(dc->m->stream));
     std::map<int, int> next;  // slot -> next position this call may write
     for (int i = 0; i < n; i++) {
         const int s = slots[i], p = pos[i], t = tokens[i];
@@ -322,8 +468,9 @@ int stage_rows(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, con
         dc->h_meta[dc->max_rows + 2 * i] = s;
         dc->h_meta[dc->max_rows + 2 * i + 1] = p;
     }
-    for (auto &kv : next) dc->filled[kv.first] = std::max(dc->filled[kv.first], kv.second);
     dc->unique = (int)next.size() == n;
+    if (dc->kv.on) return stage_kv8(dc, slots, tokens, pos, n, next);
+    for (auto &kv : next) dc->filled[kv.first] = std::max(dc->filled[kv.first], kv.second);
     return 0;
 }
 
@@ -373,21 +520,26 @@ int sample(float *lg, int V, float temperature, Rng &rng) {
     return 4;
 }
 
-double ms_since(std::chrono::steady_clock::time_point t0) {
-    return std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
-}
-
-}  // namespace
-
-extern "C" {
-
-int cih_decoder_create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, cih_decoder **out) {
+int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, bool kv8, int32_t n_pages,
+           const cih_rope *rope, cih_decoder **out) {
     if (!m || !out) return set_error(CIH_ERR_ARG, "null argument");
     *out = nullptr;
     if (n_slots < 1 || max_len < 1 || max_rows < 1) return set_error(CIH_ERR_ARG, "n_slots, max_len, max_rows must be >= 1");
-    if (max_len > 15000) return set_error(CIH_ERR_SHAPE, "max_len %d above the attention kernel's 15000", max_len);
+    if (!kv8 && max_len > 15000) return set_error(CIH_ERR_SHAPE, "max_len %d above the attention kernel's 15000", max_len);
+    if (kv8 && max_len > 1 << 20) return set_error(CIH_ERR_SHAPE, "max_len %d above 2^20", max_len);
+    if (n_pages < 0) return set_error(CIH_ERR_ARG, "n_pages must be >= 0");
     const size_t d = m->cfg.dim, F = m->cfg.hidden_dim, V = m->cfg.vocab_size, L = m->cfg.n_layers;
     const size_t R = max_rows;
+    cih_rope plain{};
+    if (kv8) {
+        // RoPE of the reference (apply_rope, lib.rs:3533-3552), with the angles in 64 bits
+        if (!rope) {
+            if (int rc = cih_rope_init(&plain, m->hd, 0, 10000.0, CIH_ROPE_NONE, 1.0, 1)) return rc;
+            rope = &plain;
+        }
+        if (rope->rot_dim < 2 || rope->rot_dim > m->hd || rope->rot_dim % 2)
+            return set_error(CIH_ERR_SHAPE, "%d rotary dims in a head of %d", rope->rot_dim, m->hd);
+    }
     cih_decoder *dc = new cih_decoder();
     dc->m = m;
     dc->slots = n_slots;
@@ -396,30 +548,77 @@ int cih_decoder_create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t m
     dc->slot_stride = (int64_t)max_len * d;
     dc->filled.assign(n_slots, 0);
     auto &al = dc->allocs;
-    const size_t cache = L * n_slots * (size_t)max_len * d;
-    bool good = dalloc(dc->kc, cache, al) == hipSuccess && dalloc(dc->vc, cache, al) == hipSuccess &&
-                dalloc(dc->rope_c, (size_t)max_len * (m->hd / 2), al) == hipSuccess &&
-                dalloc(dc->rope_s, (size_t)max_len * (m->hd / 2), al) == hipSuccess &&
-                dalloc(dc->x, R * d, al) == hipSuccess && dalloc(dc->xb, R * d, al) == hipSuccess &&
-                dalloc(dc->qkv, R * 3 * d, al) == hipSuccess && dalloc(dc->ao, R * d, al) == hipSuccess &&
-                dalloc(dc->h, R * std::max(F, d), al) == hipSuccess && dalloc(dc->logits, R * V, al) == hipSuccess &&
-                dalloc(dc->d_tokens, R, al) == hipSuccess && dalloc(dc->d_rows, 2 * R, al) == hipSuccess &&
-                dalloc(dc->d_cu, R, al) == hipSuccess && dalloc(dc->d_lens, R, al) == hipSuccess &&
-                dalloc(dc->d_flag, 1, al) == hipSuccess;
+    bool good = true;
+    size_t cache;
+    if (kv8) {
+        DecoderKv8 &kv = dc->kv;
+        kv.on = true;
+        kv.max_pages = (max_len + KV8_PAGE - 1) / KV8_PAGE;
+        const int64_t most = (int64_t)kv.max_pages * n_slots;
+        if (n_pages == 0 && most > INT32_MAX) {
+            destroy(dc);
+            return set_error(CIH_ERR_CAPACITY, "%lld pages for every slot's max_len", (long long)most);
+        }
+        kv.n_pages = n_pages > 0 ? (int)std::min<int64_t>(n_pages, most) : (int)most;
+        const size_t H = m->cfg.n_heads, dp = kv8_dims(m->hd), ph = L * kv.n_pages * H;
+        cache = ph * KV8_PAGE * dp;
+        kv.view = {nullptr, nullptr, nullptr, nullptr, kv.n_pages, (int)H, m->hd, (int)dp};
+        kv.rope.rot = rope->rot_dim;
+        kv.rope.inter = rope->interleaved != 0;
+        kv.rope.gain = rope->gain;
+        for (int j = 0; j < kv.rope.rot / 2; j++) kv.rope.turns[j] = rope->freq[j] / 6.283185307179586476925;
+        // partial results of split keys: at most a split for every 16 pages, and no more than 64 MiB (fewer splits then)
+        kv.ws_floats = std::min<size_t>((size_t)R * H * ((kv.max_pages + 15) / 16) * (dp + 2), (size_t)16 << 20);
+        good = dalloc(kv.view.k, cache, al) == hipSuccess && dalloc(kv.view.v, cache, al) == hipSuccess &&
+               dalloc(kv.view.scales, ph, al) == hipSuccess && dalloc(kv.view.bad, ph, al) == hipSuccess &&
+               dalloc(kv.d_table, (size_t)most, al) == hipSuccess && dalloc(kv.d_seq, 3 * R + 1, al) == hipSuccess &&
+               dalloc(kv.ws, kv.ws_floats, al) == hipSuccess &&
+               hipHostMalloc((void **)&kv.h_table, (size_t)most * sizeof(int)) == hipSuccess &&
+               hipHostMalloc((void **)&kv.h_seq, (3 * R + 1) * sizeof(int)) == hipSuccess;
+        cache *= 2;
+        if (good) {
+            std::fill(kv.h_table, kv.h_table + most, -1);
+            kv.pages.resize(n_slots);
+            for (int i = kv.n_pages - 1; i >= 0; i--) kv.free_pages.push_back(i);
+        }
+    } else {
+        cache = L * n_slots * (size_t)max_len * d;
+        good = dalloc(dc->kc, cache, al) == hipSuccess && dalloc(dc->vc, cache, al) == hipSuccess &&
+               dalloc(dc->rope_c, (size_t)max_len * (m->hd / 2), al) == hipSuccess &&
+               dalloc(dc->rope_s, (size_t)max_len * (m->hd / 2), al) == hipSuccess;
+        cache *= 8;
+    }
+    good = good && dalloc(dc->x, R * d, al) == hipSuccess && dalloc(dc->xb, R * d, al) == hipSuccess &&
+           dalloc(dc->qkv, R * 3 * d, al) == hipSuccess && dalloc(dc->ao, R * d, al) == hipSuccess &&
+           dalloc(dc->h, R * std::max(F, d), al) == hipSuccess && dalloc(dc->logits, R * V, al) == hipSuccess &&
+           dalloc(dc->d_tokens, R, al) == hipSuccess && dalloc(dc->d_rows, 2 * R, al) == hipSuccess &&
+           dalloc(dc->d_cu, R, al) == hipSuccess && dalloc(dc->d_lens, R, al) == hipSuccess &&
+           dalloc(dc->d_flag, 1, al) == hipSuccess;
     dc->part.floats = model_part_floats(m, R);  // a prompt's residual projections split over K too
     good = good && dalloc(dc->part.part, dc->part.floats, al) == hipSuccess &&
            hipHostMalloc((void **)&dc->h_meta, (3 * R + 1) * sizeof(int)) == hipSuccess &&
            hipHostMalloc((void **)&dc->h_logits, R * V * sizeof(float)) == hipSuccess;
+    // cih_decoder_score's rows
+    good = good && dalloc(dc->d_targets, R, al) == hipSuccess && dalloc(dc->d_score, 2 * R, al) == hipSuccess &&
+           dalloc(dc->d_top_lp, R * LOGPROBS_MAX_TOP, al) == hipSuccess &&
+           dalloc(dc->d_top_ids, R * LOGPROBS_MAX_TOP, al) == hipSuccess &&
+           dalloc(dc->d_lp_ws, score_ws_floats((int)R, (int)V), al) == hipSuccess &&
+           hipHostMalloc((void **)&dc->h_score, R * (3 + 2 * LOGPROBS_MAX_TOP) * sizeof(int)) == hipSuccess;
     if (!good) {
         destroy(dc);
-        return set_error(CIH_ERR_HIP, "decoder allocation failed (%zu MiB of KV cache)", 2 * cache * 4 >> 20);
+        return set_error(CIH_ERR_HIP, "decoder allocation failed (%zu MiB of KV cache)", cache >> 20);
     }
-    std::vector<float> c, s;
-    rope_tables_host(max_len, m->hd, c, s);
     std::vector<int> cu(R), lens(R, 1);
     for (size_t i = 0; i < R; i++) cu[i] = (int)i;
-    hipError_t e = hipMemcpy(dc->rope_c, c.data(), c.size() * 4, hipMemcpyHostToDevice);
-    if (e == hipSuccess) e = hipMemcpy(dc->rope_s, s.data(), s.size() * 4, hipMemcpyHostToDevice);
+    hipError_t e = hipSuccess;
+    if (kv8) {
+        e = hipMemcpy(dc->kv.d_table, dc->kv.h_table, (size_t)dc->kv.max_pages * n_slots * 4, hipMemcpyHostToDevice);
+    } else {
+        std::vector<float> c, s;
+        rope_tables_host(max_len, m->hd, c, s);
+        e = hipMemcpy(dc->rope_c, c.data(), c.size() * 4, hipMemcpyHostToDevice);
+        if (e == hipSuccess) e = hipMemcpy(dc->rope_s, s.data(), s.size() * 4, hipMemcpyHostToDevice);
+    }
     if (e == hipSuccess) e = hipMemcpy(dc->d_cu, cu.data(), R * 4, hipMemcpyHostToDevice);
     if (e == hipSuccess) e = hipMemcpy(dc->d_lens, lens.data(), R * 4, hipMemcpyHostToDevice);
     if (e != hipSuccess) {
@@ -430,6 +629,38 @@ int cih_decoder_create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t m
     return CIH_OK;
 }
 
+// A slot's pages back to the pool.
+void release_slot(cih_decoder *dc, int slot) {
+    dc->filled[slot] = 0;
+    if (!dc->kv.on) return;
+    std::vector<int> &pg = dc->kv.pages[slot];
+    while (!pg.empty()) {
+        dc->kv.free_pages.push_back(pg.back());
+        pg.pop_back();
+    }
+}
+
+double ms_since(std::chrono::steady_clock::time_point t0) {
+    return std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now() - t0).count();
+}
+
+}  // namespace
+
+extern "C" {
+
+int cih_decoder_create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, cih_decoder **out) {
+    return create(m, n_slots, max_len, max_rows, false, 0, nullptr, out);
+}
+
+int cih_decoder_create_kv8(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, int32_t n_pages,
+                           const cih_rope *rope, cih_decoder **out) {
+    try {
+        return create(m, n_slots, max_len, max_rows, true, n_pages, rope, out);
+    } catch (const std::exception &e) {  // host memory
+        return set_error(CIH_ERR_HIP, "decoder set-up failed: %s", e.what());
+    }
+}
+
 int cih_decoder_destroy(cih_decoder *dc) {
     destroy(dc);
     return CIH_OK;
@@ -437,8 +668,9 @@ int cih_decoder_destroy(cih_decoder *dc) {
 
 int cih_decoder_reset(cih_decoder *dc, int32_t slot) {
     if (!dc) return set_error(CIH_ERR_ARG, "null decoder");
-    if (slot < 0) std::fill(dc->filled.begin(), dc->filled.end(), 0);
-    else if (slot < dc->slots) dc->filled[slot] = 0;
+    if (slot < 0)
+        for (int i = 0; i < dc->slots; i++) release_slot(dc, i);
+    else if (slot < dc->slots) release_slot(dc, slot);
     else return set_error(CIH_ERR_ARG, "slot %d outside [0, %d)", slot, dc->slots);
     return CIH_OK;
 }
@@ -451,8 +683,125 @@ int cih_decode(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, con
     const size_t lb = (size_t)n * dc->m->cfg.vocab_size * 4;
     if (logits) HIPCHK(hipMemcpyAsync(dc->h_logits, dc->logits, lb, hipMemcpyDeviceToHost, dc->m->stream));
     HIPCHK(hipStreamSynchronize(dc->m->stream));
-    if (logits) std::memcpy(logits, dc->h_logits, lb);
+    const size_t V = dc->m->cfg.vocab_size;
+    if (logits && dc->kv.on)
+        for (int i = 0; i < n; i++) std::memcpy(logits + i * V, dc->h_logits + staged_row(dc, i) * V, V * 4);
+    else if (logits) std::memcpy(logits, dc->h_logits, lb);
     profile_collect(dc->m);
+    return CIH_OK;
+}
+
+int cih_decoder_score(cih_decoder *dc, int32_t n, const int32_t *slots, const int32_t *tokens, const int32_t *offsets,
+                      int32_t top_k, float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs) try {
+    if (!dc || !slots || !tokens || !offsets || (top_k > 0 && (!top_ids || !top_logprobs)))
+        return set_error(CIH_ERR_ARG, "null argument");
+    const int V = dc->m->cfg.vocab_size;
+    if (n < 1) return set_error(CIH_ERR_ARG, "n must be >= 1");
+    if (top_k < 0 || top_k > std::min(V, LOGPROBS_MAX_TOP))
+        return set_error(CIH_ERR_SHAPE, "top_k %d outside [0, %d]", top_k, std::min(V, LOGPROBS_MAX_TOP));
+    std::vector<char> seen(dc->slots, 0);
+    for (int i = 0; i < n; i++) {
+        if (slots[i] < 0 || slots[i] >= dc->slots) return set_error(CIH_ERR_ARG, "slot %d out of range", slots[i]);
+        if (seen[slots[i]]++) return set_error(CIH_ERR_ARG, "slot %d used by two sequences", slots[i]);
+        if (offsets[i + 1] <= offsets[i]) return set_error(CIH_ERR_ARG, "sequence %d has no tokens", i);
+        if (offsets[i + 1] - offsets[i] > dc->max_len)
+            return set_error(CIH_ERR_CAPACITY, "sequence %d has %d tokens, max_len is %d", i, offsets[i + 1] - offsets[i],
+                             dc->max_len);
+        for (int k = offsets[i]; k < offsets[i + 1]; k++)
+            if (tokens[k] < 0 || tokens[k] >= V) return set_error(CIH_ERR_TOKEN, "token %d out of range", tokens[k]);
+    }
+    hipStream_t st = dc->m->stream;
+    for (int i = 0; i < n; i++) release_slot(dc, slots[i]);
+    // the sequences' rows one after the other, max_rows a call
+    std::vector<int32_t> sl, tk, ps, tg;
+    int first = offsets[0];  // of the rows gathered
+    auto flush = [&]() -> int {
+        const int k = (int)sl.size();
+        if (int rc = stage_rows(dc, sl.data(), tk.data(), ps.data(), k)) return rc;
+        if (int rc = run_rows(dc, k)) return rc;
+        int *h = dc->h_score;  // targets | log probabilities | entropies | top log probabilities | top ids
+        HIPCHK(hipStreamSynchronize(st));
+        for (int i = 0; i < k; i++) h[staged_row(dc, i)] = tg[i];
+        HIPCHK(hipMemcpyAsync(dc->d_targets, h, (size_t)k * 4, hipMemcpyHostToDevice, st));
+        {
+            ProfScope pr(dc->m, CIH_KC_OTHER, 5.0 * k * V, 4.0 * k * V);
+            const TokenLogprobs a{FT_F32,      dc->logits,          V,           k,            V, top_k, dc->d_targets,
+                                  dc->d_score, dc->d_score + k, dc->d_top_ids, dc->d_top_lp};
+            HIPCHK(launch_token_logprobs(a, dc->d_lp_ws, st));
+        }
+        float *hf = reinterpret_cast<float *>(h + k);
+        HIPCHK(hipMemcpyAsync(hf, dc->d_score, (size_t)k * 8, hipMemcpyDeviceToHost, st));
+        if (top_k > 0) {
+            HIPCHK(hipMemcpyAsync(hf + 2 * k, dc->d_top_lp, (size_t)k * top_k * 4, hipMemcpyDeviceToHost, st));
+            HIPCHK(hipMemcpyAsync(h + 3 * k + (size_t)k * top_k, dc->d_top_ids, (size_t)k * top_k * 4,
+                                  hipMemcpyDeviceToHost, st));
+        }
+        HIPCHK(hipStreamSynchronize(st));
+        profile_collect(dc->m);
+        for (int i = 0; i < k; i++) {
+            const int r = staged_row(dc, i), to = first - offsets[0] + i;
+            if (logprob) logprob[to] = hf[r];
+            if (entropy) entropy[to] = hf[k + r];
+            for (int j = 0; j < top_k; j++) {
+                top_logprobs[(size_t)to * top_k + j] = hf[2 * k + (size_t)r * top_k + j];
+                top_ids[(size_t)to * top_k + j] = h[3 * k + (size_t)k * top_k + (size_t)r * top_k + j];
+            }
+        }
+        first += k;
+        sl.clear(); tk.clear(); ps.clear(); tg.clear();
+        return 0;
+    };
+    for (int i = 0; i < n; i++)
+        for (int k = offsets[i]; k < offsets[i + 1]; k++) {
+            sl.push_back(slots[i]);
+            tk.push_back(tokens[k]);
+            ps.push_back(k - offsets[i]);
+            tg.push_back(k + 1 < offsets[i + 1] ? tokens[k + 1] : -1);
+            if ((int)sl.size() == dc->max_rows)
+                if (int rc = flush()) return rc;
+        }
+    return sl.empty() ? CIH_OK : flush();
+} catch (const std::exception &e) {  // host memory
+    return set_error(CIH_ERR_HIP, "scoring failed: %s", e.what());
+}
+
+int cih_decoder_read_cache(cih_decoder *dc, int32_t layer, int32_t slot, int32_t pos, int32_t n, float *k, float *v) {
+    if (!dc || !k || !v) return set_error(CIH_ERR_ARG, "null argument");
+    const cih_model *m = dc->m;
+    if (layer < 0 || layer >= m->cfg.n_layers) return set_error(CIH_ERR_ARG, "layer %d outside [0, %d)", layer, m->cfg.n_layers);
+    if (slot < 0 || slot >= dc->slots) return set_error(CIH_ERR_ARG, "slot %d outside [0, %d)", slot, dc->slots);
+    if (pos < 0 || n < 0 || (int64_t)pos + n > dc->filled[slot])
+        return set_error(CIH_ERR_ARG, "positions %d .. %lld of a slot that holds %d", pos, (long long)pos + n, dc->filled[slot]);
+    const int64_t d = m->cfg.dim, hd = m->hd;
+    hipStream_t st = m->stream;
+    HIPCHK(hipStreamSynchronize(st));
+    if (!dc->kv.on) {
+        const int64_t at = ((int64_t)layer * dc->slots + slot) * dc->slot_stride + pos * d;
+        HIPCHK(hipMemcpy(k, dc->kc + at, (size_t)n * d * 4, hipMemcpyDeviceToHost));
+        HIPCHK(hipMemcpy(v, dc->vc + at, (size_t)n * d * 4, hipMemcpyDeviceToHost));
+        return CIH_OK;
+    }
+    DecoderKv8 &kv = dc->kv;
+    Kv8View c = kv.view;
+    const int64_t heads = (int64_t)layer * kv.n_pages * c.hk;
+    c.k += heads * KV8_PAGE * c.dp;
+    c.v += heads * KV8_PAGE * c.dp;
+    c.scales += heads;
+    c.bad += heads;
+    for (int p0 = 0; p0 < n; p0 += dc->max_rows) {
+        const int r = std::min(dc->max_rows, n - p0);
+        int *seq = kv.h_seq;  // one sequence of r rows that end at pos + p0 + r
+        seq[0] = 0;
+        seq[1] = r;
+        seq[2] = pos + p0 + r;
+        seq[3] = slot;
+        HIPCHK(hipMemcpyAsync(kv.d_seq, seq, 16, hipMemcpyHostToDevice, st));
+        const Kv8Seqs s{kv.d_seq, kv.d_seq + 2, kv.d_table, kv.d_seq + 3, 1, r, r, dc->slots, kv.max_pages, kv.max_pages};
+        HIPCHK(launch_kv8_read(c, s, FT_F32, RowsView{dc->qkv, d, hd}, RowsView{dc->qkv + r * d, d, hd}, st));
+        HIPCHK(hipStreamSynchronize(st));
+        HIPCHK(hipMemcpy(k + p0 * d, dc->qkv, (size_t)r * d * 4, hipMemcpyDeviceToHost));
+        HIPCHK(hipMemcpy(v + p0 * d, dc->qkv + r * d, (size_t)r * d * 4, hipMemcpyDeviceToHost));
+    }
     return CIH_OK;
 }
 
@@ -485,7 +834,7 @@ int cih_generate(cih_decoder *dc, int32_t n, const int32_t *slots, const int32_t
     // which other streams run with it
     const auto t0 = std::chrono::steady_clock::now();
     for (int i = 0; i < n; i++) {
-        dc->filled[slots[i]] = 0;
+        release_slot(dc, slots[i]);
         for (int p0 = 0; p0 < pos[i]; p0 += dc->max_rows) {
             const int k = std::min(dc->max_rows, pos[i] - p0);
             std::vector<int32_t> sl(k, slots[i]), tk(prompts + offsets[i] + p0, prompts + offsets[i] + p0 + k), ps(k);

@@ -78,8 +78,8 @@ hipError_t launch_kv8_append(const Kv8View &c, const Kv8Seqs &s, int dtype, cons
                              int heads, const RowsView &q, const RowsView &qo, const RopeArg &rope, hipStream_t st);
 hipError_t launch_kv8_read(const Kv8View &c, const Kv8Seqs &s, int dtype, const RowsView &k, const RowsView &v,
                            hipStream_t st);
-// ws: kv8_attention_floats(...) floats
-hipError_t launch_kv8_attention(const Kv8Attention &a, float *ws, hipStream_t st);
+// ws_floats below kv8_attention_floats(...): the keys are split less
+hipError_t launch_kv8_attention(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st);
 size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads);
 
 constexpr int LOGPROBS_MAX_TOP = 64;

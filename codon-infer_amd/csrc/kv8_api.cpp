@@ -229,7 +229,7 @@ int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, in
     a.window = window;
     hipStream_t st = static_cast<hipStream_t>(stream);
     CIH_TRY(check_stream(st));
-    const hipError_t e = launch_kv8_attention(a, static_cast<float *>(workspace), st);
+    const hipError_t e = launch_kv8_attention(a, static_cast<float *>(workspace), workspace_bytes / sizeof(float), st);
     if (e != hipSuccess) return set_error(CIH_ERR_HIP, "attention over the cache failed: %s", hipGetErrorString(e));
     return CIH_OK;
 }

@@ -639,7 +639,7 @@ struct Plan {
     int g, tiles, splits, pps;
     int64_t blocks;
 };
-Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window) {
+Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window, size_t ws_floats) {
     Plan p;
     p.g = heads / c.hk;
     p.tiles = (int)(((int64_t)s.max_rows * p.g + 15) / 16);
@@ -651,7 +651,10 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window)
     // pages that the keys of 16 columns touch at most
     int64_t pages = s.max_pages;
     if (window > 0) pages = min(pages, ((int64_t)window + (causal ? 16 / p.g + 1 : s.max_rows) + KV8_PAGE - 2) / KV8_PAGE + 1);
-    p.splits = (int)max((int64_t)1, (pages + pps - 1) / pps);
+    for (;; pps *= 2) {
+        p.splits = (int)max((int64_t)1, (pages + pps - 1) / pps);
+        if (p.splits == 1 || (size_t)s.n_rows * heads * p.splits * (c.dp + 2) <= ws_floats) break;
+    }
     p.pps = (int)(p.splits == 1 ? (int64_t)1 << 24 : pps);
     p.blocks = tasks * p.splits;
     return p;
@@ -662,10 +665,10 @@ template <int DP, class T> constexpr int prompt_tiles() {
     return DP == 128 && std::is_same<T, float>::value ? 1 : 2;
 }
 
-template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, hipStream_t st) {
+template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st) {
     constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
     constexpr int CT = prompt_tiles<DP, T>();
-    const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window);
+    const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, ws_floats);
     if (p.prompt) {
         const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
         const int64_t per_xcd = (tiles * a.s.n_seq * a.c.hk + 7) / 8;
@@ -684,12 +687,12 @@ template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, h
     return hipGetLastError();
 }
 
-template <class T> hipError_t launch_dims(const Kv8Attention &a, float *ws, hipStream_t st) {
+template <class T> hipError_t launch_dims(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st) {
     switch (a.c.dp) {
-        case 16: return launch<16, T>(a, ws, st);
-        case 32: return launch<32, T>(a, ws, st);
-        case 64: return launch<64, T>(a, ws, st);
-        case 128: return launch<128, T>(a, ws, st);
+        case 16: return launch<16, T>(a, ws, ws_floats, st);
+        case 32: return launch<32, T>(a, ws, ws_floats, st);
+        case 64: return launch<64, T>(a, ws, ws_floats, st);
+        case 128: return launch<128, T>(a, ws, ws_floats, st);
     }
     return hipErrorInvalidValue;
 }
@@ -699,11 +702,11 @@ template <class T> hipError_t launch_dims(const Kv8Attention &a, float *ws, hipS
 size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads) {
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return 0;
     // a window leaves fewer pages at as many pages a split: what is enough without one is enough
-    const Plan p = plan(c, s, heads, 1, 0);
+    const Plan p = plan(c, s, heads, 1, 0, SIZE_MAX);
     return p.splits == 1 ? 0 : (size_t)s.n_rows * heads * p.splits * (c.dp + 2);
 }
 
-hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, hipStream_t st) {
+hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, size_t ws_floats, hipStream_t st) {
     if (call.s.n_rows == 0 || call.s.n_seq == 0 || call.s.max_rows == 0) return hipSuccess;
     Kv8Attention a = call;
     const int64_t size = a.dtype == FT_F32 ? 4 : 2;
@@ -713,9 +716,9 @@ hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, hipStream_t
     a.q16 = aligned(a.q, 16);
     a.out16 = aligned(a.out, 4 * size);
     switch (a.dtype) {
-        case FT_F32: return launch_dims<float>(a, ws, st);
-        case FT_F16: return launch_dims<_Float16>(a, ws, st);
-        case FT_BF16: return launch_dims<__bf16>(a, ws, st);
+        case FT_F32: return launch_dims<float>(a, ws, ws_floats, st);
+        case FT_F16: return launch_dims<_Float16>(a, ws, ws_floats, st);
+        case FT_BF16: return launch_dims<__bf16>(a, ws, ws_floats, st);
     }
     return hipErrorInvalidValue;
 }

@@ -214,42 +214,6 @@ enum cih_dms_mode { CIH_DMS_MASKED_MARGINAL = 0, CIH_DMS_WILDTYPE_MARGINAL = 1 }
 int cih_dms(cih_model *m, const int32_t *residues, int32_t n, int32_t window, int32_t stride, int32_t mode,
             int32_t chunk, float *deltas, float *entropy);
 
-/* ---- kernel-level entry points (host pointers; each call stages through
- * freshly allocated device memory — for tests, not for the hot loop) ------ */
-
-/* matmul_tiled_{fp32,q8,q4}_parallel (lib.rs:4803, 4870, 4937):
- * out[p][i] = sum_k W[i][k] x[p][k] + bias[i] for p < seq_len.
- * w: [out_dim][in_dim] FP32 or packed blocks of that matrix. */
-int cih_matmul_tiled(int32_t dtype, float *out, const float *x, const void *w,
-                     const float *bias, int32_t in_dim, int32_t out_dim, int32_t seq_len);
-
-/* No counterpart in the reference: a variant of cih_matmul_tiled for callers
- * that cannot allocate device memory (code under HIP graph capture, tight
- * serving loops, harnesses that forbid hipMalloc).  out, x, w and bias are
- * DEVICE pointers (w 4-byte aligned, x 16-byte aligned; w in the same
- * reference layout as above); the call is enqueued on `stream` (a
- * hipStream_t; NULL = the null stream) and returns without waiting.  It
- * calls no allocator: the repacked weight matrix and the partial sums of a
- * k-split live in one fixed device array per GPU (48 MiB, held from the time
- * the library's code is loaded on that GPU until the process ends), so a
- * matrix whose repacked form exceeds 32 MiB returns CIH_ERR_CAPACITY (650M
- * FC1 in Q8_0 is 7.4 MB; a 3B FC1 in Q8_0 29.5 MB).  Every call on one GPU
- * uses the same array: calls that overlap on one GPU (other streams, other
- * threads) race; calls in order on one stream do not.  Results equal
- * cih_matmul_tiled's bit for bit. */
-int cih_matmul_tiled_noalloc(int32_t dtype, float *out, const float *x, const void *w, const float *bias,
-                             int32_t in_dim, int32_t out_dim, int32_t seq_len, void *stream);
-
-/* Dequantizes nblocks blocks on the GPU with the decode routine the GEMMs
- * use (BlockQ8_0/BlockQ4_0::dequantize_to, lib.rs:663-667, 1074-1082). */
-int cih_dequantize_device(int32_t dtype, const void *blocks, int64_t nblocks, float *out);
-
-/* quantize_slice_to_q8 / quantize_slice_to_q4 (lib.rs:670-673, 1085-1088)
- * on the GPU, with the kernel that cih_model_create_from_file(quantize_to)
- * runs on FP32 weights; bit-identical to cih_quantize_q8 / cih_quantize_q4.
- * n must be a multiple of 32; dst holds n/32 blocks. */
-int cih_quantize_device(int32_t dtype, const float *src, int64_t n, void *dst);
-
 /* ---- 8-bit paged key/value cache -------------------------------------------
  * No counterpart in the reference, whose RunState keeps K and V in FP32
  * (lib.rs:2464-2486).  Keys and values are held as 8-bit codes with one FP32
@@ -372,6 +336,71 @@ int cih_token_logprobs(int32_t dtype, const void *logits, int64_t row_stride, in
                        const int32_t *targets, float *logprob, float *entropy, int32_t top_k, int32_t *top_ids,
                        float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);
 int cih_token_logprobs_workspace(int32_t n_rows, int32_t vocab, int32_t top_k, size_t *bytes);
+
+/* ---- decoding over the 8-bit cache; scores --------------------------------- */
+
+/* A decoder whose keys and values live in the 8-bit paged cache above: 2 bytes
+ * a dim and position in place of 8, pages of 64 positions taken from one pool
+ * of n_pages (0: enough for every slot's max_len) as the slots grow, given
+ * back by cih_decoder_reset, cih_generate and cih_decoder_score, which start slots anew.
+ * rope (NULL: as the reference's, the whole head, base 10000) may scale the
+ * positions for contexts beyond those the model was trained on; max_len <=
+ * 2^20.  cih_decode and cih_generate work as on any decoder, but: rows that
+ * rewrite a position make the slot forget the ones after it, a call that needs more pages
+ * than are free returns CIH_ERR_CAPACITY and changes nothing, and results
+ * carry the rounding of K and V to 8 bits. */
+int cih_decoder_create_kv8(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, int32_t n_pages,
+                           const cih_rope *rope, cih_decoder **out);
+
+/* How likely given sequences are, on any decoder: sequence i is tokens
+ * [offsets[i], offsets[i + 1]) (at least one), read from position 0 of slot
+ * slots[i].  For each token, counted from offsets[0]: logprob of the token
+ * after it (0 at a sequence's last one), entropy of the distribution of that
+ * token in nats, and its top_k <= min(vocab, 64) likeliest ids with their log
+ * probabilities [token][top_k].  Host arrays; logprob and entropy may be NULL.
+ * The slots hold the sequences afterwards.  Synchronous. */
+int cih_decoder_score(cih_decoder *d, int32_t n, const int32_t *slots, const int32_t *tokens, const int32_t *offsets,
+                      int32_t top_k, float *logprob, float *entropy, int32_t *top_ids, float *top_logprobs);
+
+/* K (rotated) and V of n positions from pos on of a slot in one layer, as the
+ * rows read them: host arrays [n][dim].  Synchronous. */
+int cih_decoder_read_cache(cih_decoder *d, int32_t layer, int32_t slot, int32_t pos, int32_t n, float *k, float *v);
+
+/* ---- kernel-level entry points (host pointers; each call stages through
+ * freshly allocated device memory — for tests, not for the hot loop) ------ */
+
+/* matmul_tiled_{fp32,q8,q4}_parallel (lib.rs:4803, 4870, 4937):
+ * out[p][i] = sum_k W[i][k] x[p][k] + bias[i] for p < seq_len.
+ * w: [out_dim][in_dim] FP32 or packed blocks of that matrix. */
+int cih_matmul_tiled(int32_t dtype, float *out, const float *x, const void *w,
+                     const float *bias, int32_t in_dim, int32_t out_dim, int32_t seq_len);
+
+/* No counterpart in the reference: a variant of cih_matmul_tiled for callers
+ * that cannot allocate device memory (code under HIP graph capture, tight
+ * serving loops, harnesses that forbid hipMalloc).  out, x, w and bias are
+ * DEVICE pointers (w 4-byte aligned, x 16-byte aligned; w in the same
+ * reference layout as above); the call is enqueued on `stream` (a
+ * hipStream_t; NULL = the null stream) and returns without waiting.  It
+ * calls no allocator: the repacked weight matrix and the partial sums of a
+ * k-split live in one fixed device array per GPU (48 MiB, held from the time
+ * the library's code is loaded on that GPU until the process ends), so a
+ * matrix whose repacked form exceeds 32 MiB returns CIH_ERR_CAPACITY (650M
+ * FC1 in Q8_0 is 7.4 MB; a 3B FC1 in Q8_0 29.5 MB).  Every call on one GPU
+ * uses the same array: calls that overlap on one GPU (other streams, other
+ * threads) race; calls in order on one stream do not.  Results equal
+ * cih_matmul_tiled's bit for bit. */
+int cih_matmul_tiled_noalloc(int32_t dtype, float *out, const float *x, const void *w, const float *bias,
+                             int32_t in_dim, int32_t out_dim, int32_t seq_len, void *stream);
+
+/* Dequantizes nblocks blocks on the GPU with the decode routine the GEMMs
+ * use (BlockQ8_0/BlockQ4_0::dequantize_to, lib.rs:663-667, 1074-1082). */
+int cih_dequantize_device(int32_t dtype, const void *blocks, int64_t nblocks, float *out);
+
+/* quantize_slice_to_q8 / quantize_slice_to_q4 (lib.rs:670-673, 1085-1088)
+ * on the GPU, with the kernel that cih_model_create_from_file(quantize_to)
+ * runs on FP32 weights; bit-identical to cih_quantize_q8 / cih_quantize_q4.
+ * n must be a multiple of 32; dst holds n/32 blocks. */
+int cih_quantize_device(int32_t dtype, const float *src, int64_t n, void *dst);
 
 /* ---- host helpers (no GPU) ---------------------------------------------- */
 

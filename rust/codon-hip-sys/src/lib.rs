@@ -191,6 +191,13 @@ extern "C" {
 
     pub fn cih_decoder_create(m: *mut cih_model, n_slots: i32, max_len: i32, max_rows: i32,
                               out: *mut *mut cih_decoder) -> c_int;
+    pub fn cih_decoder_create_kv8(m: *mut cih_model, n_slots: i32, max_len: i32, max_rows: i32, n_pages: i32,
+                                  rope: *const cih_rope, out: *mut *mut cih_decoder) -> c_int;
+    pub fn cih_decoder_score(d: *mut cih_decoder, n: i32, slots: *const i32, tokens: *const i32, offsets: *const i32,
+                             top_k: i32, logprob: *mut f32, entropy: *mut f32, top_ids: *mut i32,
+                             top_logprobs: *mut f32) -> c_int;
+    pub fn cih_decoder_read_cache(d: *mut cih_decoder, layer: i32, slot: i32, pos: i32, n: i32, k: *mut f32,
+                                  v: *mut f32) -> c_int;
     pub fn cih_decoder_destroy(d: *mut cih_decoder) -> c_int;
     pub fn cih_decoder_reset(d: *mut cih_decoder, slot: i32) -> c_int;
     pub fn cih_decode(d: *mut cih_decoder, slots: *const i32, tokens: *const i32, pos: *const i32, n: i32,

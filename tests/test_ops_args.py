@@ -177,3 +177,11 @@ def test_rope_refusals(kw):
     assert C.lib().cih_rope_init(ctypes.addressof(r), 32, 0, 1e4, 9, 1.0, 1) == -1
     with pytest.raises(ValueError):
         ch.Rope(32, scaling="other")
+
+
+def test_decoder_refusals_without_a_model():
+    lib, out, r = C.lib(), ctypes.c_void_p(), C.RopeStruct()
+    assert lib.cih_decoder_create_kv8(None, 1, 64, 8, 0, None, ctypes.byref(out)) == -1
+    assert lib.cih_decoder_create_kv8(None, 1, 64, 8, 0, ctypes.addressof(r), None) == -1
+    assert lib.cih_decoder_score(None, 1, None, None, None, 0, None, None, None, None) == -1
+    assert lib.cih_decoder_read_cache(None, 0, 0, 0, 1, None, None) == -1
