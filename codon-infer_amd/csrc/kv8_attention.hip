@@ -462,17 +462,15 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 // unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
 // 2^3 at the running maximum and have room for both.
 template <int DP, int PL, class T, int CT>
-__global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int per_xcd) {
+__global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr float SLACK = 8.0f, P0 = 3.0f, UNIT = 16.0f;
-    // consecutive workgroups go to the 8 XCDs in turn: each gets whole heads,
-    // whose K and V its L2 then holds; a head's longest rows first
-    int b = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-    if (b >= a.c.hk * a.s.n_seq * tiles) return;
-    const int tile = tiles - 1 - b % tiles;
-    b /= tiles;
-    const int kvh = b / a.s.n_seq;
-    const Kv8Seq q = kv8_seq(a.s, b % a.s.n_seq);
+    // The last rows, which see most keys, go first, over all (sequence, kv head)
+    // pairs (a pair after the other left the longest to a quarter of the CUs:
+    // prompts of 131 to 512 rows 28.4 -> 25.4 us; whole pairs to one XCD: no difference).
+    const int pairs = a.c.hk * a.s.n_seq, pair = blockIdx.x % pairs, tile = tiles - 1 - blockIdx.x / pairs;
+    const int kvh = pair % a.c.hk;
+    const Kv8Seq q = kv8_seq(a.s, pair / a.c.hk);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g4 = lane >> 4;
     const int f0 = (tile * 4 + wave) * CT * 16, f1 = min(f0 + CT * 16, q.n * g) - 1;  // columns of the wave
@@ -660,21 +658,21 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window,
     return p;
 }
 
-// Columns of a prompt wave, / 16.
-template <int DP, class T> constexpr int prompt_tiles() {
-    return DP == 128 && std::is_same<T, float>::value ? 1 : 2;
-}
+// Columns of a prompt wave, / 16: heads of 128 share V's conversion over 32
+// (bfloat16, 20 heads: 4096 rows 238 -> 147 us; 131 to 512 rows 36 -> 31), narrower
+// ones gain more from twice the waves (64 wide: 92 and 96, 20 -> 17; 32 wide 80
+// and 79, 17 -> 15).
+template <int DP> constexpr int prompt_tiles() { return DP == 128 ? 2 : 1; }
 
 template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st) {
     constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
-    constexpr int CT = prompt_tiles<DP, T>();
+    constexpr int CT = prompt_tiles<DP>();
     const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, ws_floats);
     if (p.prompt) {
         const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
-        const int64_t per_xcd = (tiles * a.s.n_seq * a.c.hk + 7) / 8;
-        if (per_xcd * 8 > INT32_MAX) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(per_xcd * 8), dim3(256), 0, st, a, p.g, (int)tiles,
-                           (int)per_xcd);
+        const int64_t blocks = tiles * a.s.n_seq * a.c.hk;
+        if (blocks > INT32_MAX) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(blocks), dim3(256), 0, st, a, p.g, (int)tiles);
         return hipGetLastError();
     }
     if (p.blocks > INT32_MAX) return hipErrorInvalidValue;
