@@ -190,15 +190,20 @@ __global__ __launch_bounds__(NT) void k_logprobs(TokenLogprobs a, int chunks, in
         }
     };
     const int whole = (end - begin) / TILE;
+    typename Vec<T>::type w[LP_VECS];  // the next tile's logits
+    auto fetch = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < LP_VECS; u++)
+            w[u] = *reinterpret_cast<const typename Vec<T>::type *>(p + begin + t * TILE + (u * NT + tid) * VL);
+    };
+    if (whole > 0) fetch(0);
     for (int t = 0; t < whole; t++) {
         float x[LP_EACH];
 #pragma unroll
-        for (int u = 0; u < LP_VECS; u++) {
-            const typename Vec<T>::type w =
-                *reinterpret_cast<const typename Vec<T>::type *>(p + begin + t * TILE + (u * NT + tid) * VL);
+        for (int u = 0; u < LP_VECS; u++)
 #pragma unroll
-            for (int e = 0; e < VL; e++) x[u * VL + e] = to_f32(w[e]);
-        }
+            for (int e = 0; e < VL; e++) x[u * VL + e] = to_f32(w[u][e]);
+        if (t + 1 < whole) fetch(t + 1);
         add(x, t);
     }
     if (begin + whole * TILE < end) {
