@@ -38,12 +38,14 @@ def _float(a, what):
 def _where(arrays):
     """The GPU that the torch tensors among the arrays are on; None without one."""
     torch = sys.modules.get("torch")
-    at = None
-    if torch is not None:
-        for a in arrays:
-            if isinstance(a, torch.Tensor):
-                d = a.get_device()
-                if d < 0 or (at is not None and d != at):
+    if torch is None:
+        return None
+    at, tensor = None, torch.Tensor
+    for a in arrays:
+        if isinstance(a, tensor):
+            d = a.get_device()
+            if d != at:
+                if d < 0 or at is not None:
                     raise ValueError("tensors on the CPU or on different GPUs")
                 at = d
     return at
@@ -53,13 +55,26 @@ def _stream(at, stream):
     """The stream to enqueue on for tensors on GPU `at`, which must be the current one."""
     if at is None:
         return stream or 0
-    torch = sys.modules["torch"]
-    if at != torch.cuda.current_device():
-        raise ValueError(f"a tensor is on cuda:{at}, the current device is cuda:{torch.cuda.current_device()}")
-    if stream is not None:
-        return stream
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # without making a Stream object, 1 us
-    return raw(at) if raw else torch.cuda.current_stream(at).cuda_stream
+    now, raw = _torch_now()
+    if at != now():
+        raise ValueError(f"a tensor is on cuda:{at}, the current device is cuda:{now()}")
+    return raw(at) if stream is None else stream
+
+
+_now = None
+
+
+def _torch_now():
+    """torch's current device, and its current stream on a device: the plain
+    integers where this torch gives them (a Stream object costs 1 us)."""
+    global _now
+    if _now is None:
+        torch = sys.modules["torch"]
+        torch.cuda.current_device()  # torch is set up
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _now = (getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+                raw or (lambda d: torch.cuda.current_stream(d).cuda_stream))
+    return _now
 
 
 def _same(at, kept):
@@ -94,14 +109,18 @@ def _plain(a, what, dtype, shape=None):
     return a.data_ptr()
 
 
-def _rows(a, what, shape):
+def _rows(a, what, shape, new=C.RowsStruct):
     """A [rows][heads][dim] array as a cih_rows; the last axis without gaps."""
     if a.shape != shape:
         raise ValueError(f"{what} has shape {tuple(a.shape)}: {shape} is needed")
     rs, hs, one = a.stride()
     if one != 1:
         raise ValueError(f"{what}: the last axis must be contiguous")
-    return C.RowsStruct(a.data_ptr(), rs, hs)
+    return new(a.data_ptr(), rs, hs)
+
+
+_lib = C.lib()
+_at = ctypes.addressof
 
 
 class Rope:
@@ -115,7 +134,7 @@ class Rope:
         if scaling not in self.SCALINGS:
             raise ValueError(f"scaling {scaling!r} is none of {', '.join(self.SCALINGS)}")
         self.struct = C.RopeStruct()
-        C.check(C.lib().cih_rope_init(ctypes.addressof(self.struct), rot_dim, int(interleaved), float(base),
+        C.check(_lib.cih_rope_init(_at(self.struct), rot_dim, int(interleaved), float(base),
                                       self.SCALINGS[scaling], float(factor), int(trained_len)))
 
     @property
@@ -147,7 +166,7 @@ class Kv8Batch:
         self.struct = C.Kv8BatchStruct(_plain(cu_rows, "cu_rows", i32, (n + 1,)), _plain(lens, "lens", i32, (n,)),
                                        table.data_ptr(), None if slots is None else _plain(slots, "slots", i32, (n,)),
                                        n, n_rows, max_rows, table.shape[0], stride, table.shape[1])
-        self._at = ctypes.addressof(self.struct)
+        self._at = _at(self.struct)
         self._gpu = _where(self._arrays)
 
 
@@ -166,7 +185,7 @@ class Kv8Cache:
         self.struct = C.Kv8CacheStruct(_plain(k, "k", ("int8",)), _plain(v, "v", ("int8",), (n, h, d, page)),
                                        _plain(scales, "scales", ("float32",), (n, h, 2)),
                                        _plain(bad, "bad", ("int64", "uint64"), (n, h)), n, h, head_dim)
-        self._at = ctypes.addressof(self.struct)
+        self._at = _at(self.struct)
         self._gpu = _where(self._arrays)
         self._scale = head_dim ** -0.5
 
@@ -193,8 +212,8 @@ class Kv8Cache:
             if _float(q, "q") != t or _float(q_out, "q_out") != t:
                 raise TypeError("q, q_out and k differ in type")
         at = _same(_same(_where((k, v) if q is None else (k, v, q, q_out)), self._gpu), batch._gpu)
-        a = ctypes.addressof
-        C.check(C.lib().cih_kv8_append(self._at, batch._at, t, a(ks), a(vs), heads, a(qs) if qs else None,
+        a = _at
+        C.check(_lib.cih_kv8_append(self._at, batch._at, t, a(ks), a(vs), heads, a(qs) if qs else None,
                                        a(qo) if qo else None, a(rope.struct) if rope else None, _stream(at, stream)))
 
     def read(self, batch, k, v, stream=None):
@@ -204,13 +223,13 @@ class Kv8Cache:
         if _float(v, "v") != t:
             raise TypeError("k and v differ in type")
         at = _same(_same(_where((k, v)), self._gpu), batch._gpu)
-        C.check(C.lib().cih_kv8_read(self._at, batch._at, t, ctypes.addressof(ks), ctypes.addressof(vs),
+        C.check(_lib.cih_kv8_read(self._at, batch._at, t, _at(ks), _at(vs),
                                      _stream(at, stream)))
 
     def attend_workspace(self, batch, q_heads):
         """Bytes of workspace that attend needs for a batch of these sizes."""
         n = ctypes.c_size_t()
-        C.check(C.lib().cih_kv8_attention_workspace(self._at, batch._at, q_heads, ctypes.byref(n)))
+        C.check(_lib.cih_kv8_attention_workspace(self._at, batch._at, q_heads, ctypes.byref(n)))
         return n.value
 
     def attend(self, batch, q, out, lse=None, scale=None, causal=True, window=0, workspace=None, stream=None):
@@ -226,7 +245,7 @@ class Kv8Cache:
         ls = None if lse is None else _plain(lse, "lse", ("float32",), shape[:2])
         ws, size = _workspace(workspace)
         at = _same(_same(_where((q, out, lse, workspace)), self._gpu), batch._gpu)
-        C.check(C.lib().cih_kv8_attention(self._at, batch._at, t, heads, ctypes.addressof(qs), ctypes.addressof(os), ls,
+        C.check(_lib.cih_kv8_attention(self._at, batch._at, t, heads, _at(qs), _at(os), ls,
                                           self._scale if scale is None else scale, 1 if causal else 0, window, ws, size,
                                           _stream(at, stream)))
 
@@ -238,7 +257,7 @@ def _workspace(w):
 def token_logprobs_workspace(n_rows, vocab, top_k):
     """Bytes of workspace that token_logprobs needs."""
     n = ctypes.c_size_t()
-    C.check(C.lib().cih_token_logprobs_workspace(n_rows, vocab, top_k, ctypes.byref(n)))
+    C.check(_lib.cih_token_logprobs_workspace(n_rows, vocab, top_k, ctypes.byref(n)))
     return n.value
 
 
@@ -266,5 +285,5 @@ def token_logprobs(logits, targets=None, logprob=None, entropy=None, top_ids=Non
         tl = _plain(top_logprobs, "top_logprobs", f32, (n, k))
     ws, size = _workspace(workspace)
     at = _where((logits, targets, logprob, entropy, top_ids, top_logprobs, workspace))
-    C.check(C.lib().cih_token_logprobs(_float(logits, "logits"), logits.data_ptr(), logits.stride()[0], n, vocab, tg, lp,
+    C.check(_lib.cih_token_logprobs(_float(logits, "logits"), logits.data_ptr(), logits.stride()[0], n, vocab, tg, lp,
                                        en, k, ids, tl, ws, size, _stream(at, stream)))
