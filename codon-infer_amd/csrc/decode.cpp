@@ -103,9 +103,10 @@ bool step_gemv16(const cih_decoder *dc, int n) {
 // that is no longer finite, and run again in full range.
 bool step_limbs(const cih_decoder *dc, int n) { return n > GEMV_MAX_M ? !full_range_mode() : step_gemv16(dc, n); }
 
-// Rows of the 8-bit cache: Q, K and V of dc->qkv rotated and appended, then the
-// attention, to dc->ao in FP32 or f16 limbs.
-int enqueue_kv8(cih_decoder *dc, int l, int n, int out_fmt) {
+// Rows of the 8-bit cache: Q, K and V (dc->qkv, or the projection's partial
+// sums) rotated, K and V appended, then the attention, to dc->ao in FP32 or f16
+// limbs; one launch where every row is its own sequence's.
+int enqueue_kv8(cih_decoder *dc, int l, int n, int out_fmt, const float *part, int splits, const float *bias) {
     const cih_model *m = dc->m;
     const int64_t d = m->cfg.dim, hd = m->hd, H = m->cfg.n_heads;
     DecoderKv8 &kv = dc->kv;
@@ -125,6 +126,12 @@ int enqueue_kv8(cih_decoder *dc, int l, int n, int out_fmt) {
     a.out_h2 = out_fmt == AF_H2;
     a.scale = 1.0f / std::sqrt((float)hd);
     a.causal = 1;
+    if (dc->unique) {
+        const Kv8Step step{dc->qkv, part, bias, splits, kv.rope};
+        HIPCHK(launch_kv8_step(a, step, kv.ws, kv.ws_floats, m->stream));
+        return 0;
+    }
+    if (part) HIPCHK(launch_gemv16_fold(part, splits, n, (int)(3 * d), bias, dc->qkv, (int)(3 * d), EPI_NONE, m->stream));
     HIPCHK(launch_kv8_append(a.c, a.s, FT_F32, RowsView{dc->qkv + d, 3 * d, hd}, RowsView{dc->qkv + 2 * d, 3 * d, hd},
                              (int)H, a.q, a.q, kv.rope, m->stream));
     HIPCHK(launch_kv8_attention(a, kv.ws, kv.ws_floats, m->stream));
@@ -191,8 +198,7 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
         {
             ProfScope ps(m, CIH_KC_ATTENTION, 4.0 * keys * d, key_bytes * keys * d + 24.0 * n * d);
             if (dc->kv.on) {
-                HIPCHK(launch_gemv16_fold(part_b, sq, n, 3 * d, ly.bqkv, dc->qkv, 3 * d, EPI_NONE, st));
-                if (int rc = enqueue_kv8(dc, l, n, AF_H2)) return rc;
+                if (int rc = enqueue_kv8(dc, l, n, AF_H2, part_b, sq, ly.bqkv)) return rc;
             } else if (fused && fuse_wo) {
                 // attention and each head's share of Wo in one kernel: the heads are Wo's splits
                 HIPCHK(launch_decode_attention_fused_wo(dc->qkv, part_b, sq, ly.bqkv, d, H, dc->d_rows, n,
@@ -252,7 +258,7 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
         }
         // one row per sequence through the GEMV: the attention kernel adds
         // the QKV partial sums itself (no separate reduction)
-        const bool qkv_parts = fused && !dc->kv.on && use_gemv(n, AF_F32, EPI_NONE);
+        const bool qkv_parts = fused && use_gemv(n, AF_F32, EPI_NONE);
         int splits = 0;
         if (qkv_parts) {
             ProfScope ps(m, ly.wqkv.fmt == WF_F32 ? CIH_KC_GEMM_FP32 : CIH_KC_GEMM_QUANT, 2.0 * n * ly.wqkv.N * d,
@@ -266,7 +272,7 @@ int enqueue_rows(cih_decoder *dc, int n, bool fused) {
             // K and V read once per key, Q read, rows written
             ProfScope ps(m, CIH_KC_ATTENTION, 4.0 * keys * d, key_bytes * keys * d + 24.0 * n * d);
             if (dc->kv.on) {
-                if (int rc = enqueue_kv8(dc, l, n, af)) return rc;
+                if (int rc = enqueue_kv8(dc, l, n, af, qkv_parts ? dc->part.part : nullptr, splits, ly.bqkv)) return rc;
             } else if (fused) {
                 HIPCHK(launch_decode_attention_fused(dc->qkv, qkv_parts ? dc->part.part : nullptr, splits, ly.bqkv, d,
                                                      H, dc->d_rows, n, dc->max_len, dc->rope_c, dc->rope_s, kc, vc,

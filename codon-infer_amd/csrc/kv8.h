@@ -1,7 +1,9 @@
 // Internal launch interface of the 8-bit paged key/value cache and of the
 // token log probabilities (not part of the C ABI).
 #pragma once
+#include <float.h>
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 namespace cih {
@@ -61,6 +63,37 @@ __device__ __forceinline__ int kv8_page(const Kv8View &c, const Kv8Seq &q, int p
     return id >= 0 && id < c.n_pages ? id : -1;
 }
 
+// cos and sin (times gain) of position p's angle at pair j.  The angle in
+// turns is reduced in 64 bits: at position 1e6 a 32-bit product is off by
+// 0.06 radians.
+__device__ __forceinline__ void rope_cs(const RopeArg &r, int p, int j, float &c, float &s) {
+    const double a = (double)p * r.turns[j];
+    const float t = (float)(a - rint(a));
+    sincospif(2.0f * t, &s, &c);
+    c *= r.gain;
+    s *= r.gain;
+}
+
+__device__ __forceinline__ int code8(float x, float inv) {
+    return (int)fminf(fmaxf(rintf(x * inv), -127.0f), 127.0f) & 0xff;
+}
+// four codes scaled again
+__device__ __forceinline__ unsigned recode4(unsigned w, float ratio) {
+    unsigned o = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o |= (unsigned)code8((float)(signed char)(w >> (8 * e)), ratio) << (8 * e);
+    return o;
+}
+
+// A page's scales from the largest new |K| and |V| (as bits) and the kept
+// tokens' (0 where none are kept): too small to be inverted, they are 0, and so are the codes.
+__device__ __forceinline__ float2 kv8_scales(unsigned mk, unsigned mv, float2 old) {
+    float2 sc = {__uint_as_float(mk) / 127.0f, __uint_as_float(mv) / 127.0f};
+    if (!(sc.x >= FLT_MIN)) sc.x = 0.0f;
+    if (!(sc.y >= FLT_MIN)) sc.y = 0.0f;
+    return {fmaxf(sc.x, old.x), fmaxf(sc.y, old.y)};
+}
+
 // out_h2 (dtype F32 only): out is one matrix of f16-limb rows (x3.h) of hd
 // q_heads columns, rs and hs unused.
 struct Kv8Attention {
@@ -73,6 +106,16 @@ struct Kv8Attention {
     int causal, window;
     int q16, out16;  // set by the launch: queries in 16-byte loads, output in stores of 4 dims
 };
+
+// A decoder's step (one FP32 row a sequence, no shared heads): append and
+// attention in one launch.  The rows are qkv [n_rows][3 d] or, with part, the
+// projection's sums over `splits` [splits][n_rows][3 d] plus bias.
+struct Kv8Step {
+    const float *qkv = nullptr, *part = nullptr, *bias = nullptr;
+    int splits = 0;
+    RopeArg rope;
+};
+hipError_t launch_kv8_step(const Kv8Attention &a, const Kv8Step &step, float *ws, size_t ws_floats, hipStream_t st);
 
 hipError_t launch_kv8_append(const Kv8View &c, const Kv8Seqs &s, int dtype, const RowsView &k, const RowsView &v,
                              int heads, const RowsView &q, const RowsView &qo, const RopeArg &rope, hipStream_t st);

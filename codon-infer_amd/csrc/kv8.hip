@@ -17,17 +17,6 @@ namespace {
 constexpr int KV_THREADS = 256;
 constexpr int VQ = KV8_PAGE + 4;  // bytes of a dim's codes in LDS
 
-// cos and sin (times gain) of position p's angle at pair j.  The angle in
-// turns is reduced in 64 bits: at position 1e6 a 32-bit product is off by
-// 0.06 radians.
-__device__ __forceinline__ void rope_cs(const RopeArg &r, int p, int j, float &c, float &s) {
-    const double a = (double)p * r.turns[j];
-    const float t = (float)(a - rint(a));
-    sincospif(2.0f * t, &s, &c);
-    c *= r.gain;
-    s *= r.gain;
-}
-
 // The two dims of pair j of a head: rotated pairs first, then neighbours.
 __device__ __forceinline__ void pair_dims(const RopeArg &r, int j, int &i0, int &i1) {
     const int half = r.rot / 2;
@@ -38,17 +27,6 @@ __device__ __forceinline__ void pair_dims(const RopeArg &r, int j, int &i0, int 
         i0 = j;
         i1 = j + half;
     }
-}
-
-__device__ __forceinline__ int code8(float x, float inv) {
-    return (int)fminf(fmaxf(rintf(x * inv), -127.0f), 127.0f) & 0xff;
-}
-// four codes scaled again
-__device__ __forceinline__ unsigned recode4(unsigned w, float ratio) {
-    unsigned o = 0;
-#pragma unroll
-    for (int e = 0; e < 4; e++) o |= (unsigned)code8((float)(signed char)(w >> (8 * e)), ratio) << (8 * e);
-    return o;
 }
 
 // Which (sequence, page, head) a workgroup owns, and the page's new tokens
@@ -142,19 +120,14 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv8_append(Kv8View c, Kv8Seqs s,
         mk = fmaxf(mk, red[0][w]);
         mv = fmaxf(mv, red[1][w]);
     }
-    // scales too small to be inverted are 0, and so are their codes
-    float2 sc = {mk / 127.0f, mv / 127.0f};
-    if (!(sc.x >= FLT_MIN)) sc.x = 0.0f;
-    if (!(sc.y >= FLT_MIN)) sc.y = 0.0f;
     const int64_t ph = (int64_t)id * c.hk + t.h;
     float2 old = {0.0f, 0.0f};
     unsigned long long kept_bad = 0;
     if (t.lo > 0) {
         old = c.scales[ph];
         kept_bad = c.bad[ph] & ((1ull << t.lo) - 1);
-        sc.x = fmaxf(sc.x, old.x);
-        sc.y = fmaxf(sc.y, old.y);
     }
+    const float2 sc = kv8_scales(__float_as_uint(mk), __float_as_uint(mv), old);
     __syncthreads();  // the old scales are read before they are replaced
     if (tid == 0) {
         c.scales[ph] = sc;
@@ -439,14 +412,7 @@ __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, Row
         }
         all();
     }
-    // scales too small to be inverted are 0, and so are their codes
-    float2 sc = {__uint_as_float(mk) / 127.0f, __uint_as_float(mv) / 127.0f};
-    if (!(sc.x >= FLT_MIN)) sc.x = 0.0f;
-    if (!(sc.y >= FLT_MIN)) sc.y = 0.0f;
-    if (t.lo > 0) {
-        sc.x = fmaxf(sc.x, old.x);
-        sc.y = fmaxf(sc.y, old.y);
-    }
+    const float2 sc = kv8_scales(mk, mv, old);
     if (NW > 1) __syncthreads();  // the old scales are read before they are replaced
     if (tid == 0) {
         c.scales[ph] = sc;

@@ -28,6 +28,7 @@
 
 #include <type_traits>
 
+#include "kernels.h"
 #include "kv8.h"
 #include "x3.h"
 
@@ -57,6 +58,11 @@ template <class OP> __device__ __forceinline__ float groups(float v, OP op) {
 }
 __device__ __forceinline__ float groups_max(float v) {
     return groups(v, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {  // over all lanes
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
+    return v;
 }
 __device__ __forceinline__ float groups_sum(float v) {
     return groups(v, [](float a, float b) { return a + b; });
@@ -158,17 +164,11 @@ __device__ __forceinline__ void load_v(Tile<DP> &t, const Kv8View &c, int id, in
     for (int dt = 0; dt < DP / 16; dt++) t.v[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
 }
 
-// A column's query as QB bytes a value, ready as the second operand, and the
-// factor that makes scores in units of log2 of its sums with a page's codes
-// (times the K scale); NaN if the query is not finite.
-template <int QB, int KS, class T>
-__device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column &col, int g4, i32x4 (&ql)[QB][KS]) {
-    constexpr int BITS = 8 * QB - 1, HALF = QB == 3 ? 0x8080 : 0x80;  // the lower bytes are + 128 at first
-    constexpr float MOST = (1 << BITS) - 1 - HALF;
+// A column's query, the 16 values of a lane of each k step.
+template <int KS, class T>
+__device__ __forceinline__ void load_query(const Kv8Attention &a, const Column &col, int g4, float (&x)[KS][16]) {
     constexpr int VL = 16 / sizeof(T);
     typedef T vec __attribute__((ext_vector_type(VL)));
-    float x[KS][16];
-    unsigned top = 0;
     const T *qp = static_cast<const T *>(a.q.p) + (col.row >= 0 ? col.row * a.q.rs + col.head * a.q.hs : 0);
 #pragma unroll
     for (int s = 0; s < KS; s++)
@@ -188,16 +188,29 @@ __device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column
 #pragma unroll
             for (int u = 0; u < VL; u++) {
                 x[s][e + u] = col.row >= 0 && i < a.c.d ? to_f32(w[u]) : 0.0f;
-                top = max(top, __float_as_uint(x[s][e + u]) & 0x7fffffffu);  // NaN above infinity above the rest
             }
         }
+}
+
+// A column's query as QB bytes a value, ready as the second operand, and the
+// factor that makes scores in units of log2 of its sums with a page's codes
+// (times the K scale); NaN if the query is not finite.
+template <int QB, int KS>
+__device__ __forceinline__ float query_bytes(const float (&x)[KS][16], float scale, i32x4 (&ql)[QB][KS]) {
+    constexpr int BITS = 8 * QB - 1, HALF = QB == 3 ? 0x8080 : 0x80;  // the lower bytes are + 128 at first
+    constexpr float MOST = (1 << BITS) - 1 - HALF;
+    unsigned top = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);  // NaN above infinity above the rest
     float mx = __uint_as_float(top);
     const bool lost = groups_max(mx <= FLT_MAX ? 0.0f : 1.0f) > 0.0f;
     mx = groups_max(mx);
     int e = BITS - __builtin_amdgcn_frexp_expf(mx);
     if (ldexpf(mx, e) > MOST) e--;
     // a negative scale turns the query, so that the factor is never negative
-    const float sign = lost ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
+    const float sign = lost ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -212,7 +225,7 @@ __device__ __forceinline__ float query_bytes(const Kv8Attention &a, const Column
 #pragma unroll
             for (int n = 0; n < QB; n++) ql[n][s][w] = (int)(n == 0 ? o[n] : o[n] ^ 0x80808080u);
         }
-    return lost ? NAN : ldexpf(fabsf(a.scale) * LOG2E, (QB == 3 ? 8 : 0) - e);
+    return lost ? NAN : ldexpf(fabsf(scale) * LOG2E, (QB == 3 ? 8 : 0) - e);
 }
 
 // Scores of 16 keys with one column, in the units of the last byte but (three bytes) one.
@@ -232,12 +245,109 @@ __device__ __forceinline__ void score_tile(const i32x4 (&k)[KS], const i32x4 (&q
     for (int r = 0; r < 4; r++) s[r] = (float)(h[r] * 256 + d[r]);  // below 2^30
 }
 
+struct NoStep {};
+template <bool STEP> using StepArg = typename std::conditional<STEP, Kv8Step, NoStep>::type;
+
+// A row's query, key and value of one head: rotated, in LDS.
+template <int DP, int W>
+__device__ __forceinline__ void step_row(const Kv8Attention &a, const Kv8Step &step, int r, int h, int pos, bool kv,
+                                         float (&row)[3][DP]) {
+    const int hd = a.c.d, d = a.heads * hd, n = a.s.n_rows;
+    for (int t = threadIdx.x; t < (kv ? 3 : 1) * hd; t += 64 * W) {
+        const int which = t / hd, i = t - which * hd, col = which * d + h * hd + i;
+        float v;
+        if (step.part) v = fold_splits(step.part + (size_t)r * 3 * d + col, step.splits, (size_t)n * 3 * d) + step.bias[col];
+        else v = step.qkv[(size_t)r * 3 * d + col];
+        row[which][i] = v;
+    }
+    __syncthreads();
+    const int pairs = step.rope.rot / 2, t = threadIdx.x;
+    if (t < pairs) {
+        const int i0 = step.rope.inter ? 2 * t : t, i1 = step.rope.inter ? i0 + 1 : t + pairs;
+        float c, s;
+        rope_cs(step.rope, pos, t, c, s);
+        const float q0 = row[0][i0], q1 = row[0][i1];
+        row[0][i0] = q0 * c - q1 * s;
+        row[0][i1] = q1 * c + q0 * s;
+        if (kv) {
+            const float k0 = row[1][i0], k1 = row[1][i1];
+            row[1][i0] = k0 * c - k1 * s;
+            row[1][i1] = k1 * c + k0 * s;
+        }
+    }
+    __syncthreads();
+}
+
+// What a page's record is after a step's key and value went into it.
+struct Kv8Own {
+    int pg;
+    float2 sc;
+    unsigned long long bad;
+};
+// Token `lo` of a page of one head, from rows in LDS (k_kv8_append's arithmetic).
+template <int DP, int W>
+__device__ __forceinline__ Kv8Own step_append(const Kv8View &c, int id, int h, int lo, const float (&k)[DP],
+                                              const float (&v)[DP]) {
+    Kv8Own o{-1, {0.0f, 0.0f}, 0};
+    if (id < 0) return o;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t ph = (int64_t)id * c.hk + h;
+    float2 old = {0.0f, 0.0f};
+    unsigned long long kept_bad = 0;
+    if (lo > 0) {
+        old = c.scales[ph];
+        kept_bad = c.bad[ph] & ((1ull << lo) - 1);
+    }
+    unsigned mk = 0, mv = 0;
+    for (int i = lane; i < c.d; i += 64) {
+        mk = max(mk, __float_as_uint(k[i]) & 0x7fffffffu);
+        mv = max(mv, __float_as_uint(v[i]) & 0x7fffffffu);
+    }
+    mk = wave_max_bits(mk);
+    mv = wave_max_bits(mv);
+    const bool lost = max(mk, mv) >= 0x7f800000u;
+    o.sc = kv8_scales(lost ? 0 : mk, lost ? 0 : mv, old);
+    o.bad = kept_bad | (lost ? 1ull << lo : 0);
+    const float ik = o.sc.x > 0.0f && !lost ? 1.0f / o.sc.x : 0.0f, iv = o.sc.y > 0.0f && !lost ? 1.0f / o.sc.y : 0.0f;
+    signed char *kc = c.k + ph * (KV8_PAGE * DP), *vc = c.v + ph * (KV8_PAGE * DP);
+    __syncthreads();  // every wave has the old record
+    if (tid == 0) {
+        c.scales[ph] = o.sc;
+        c.bad[ph] = o.bad;
+    }
+    if (lo > 0) {
+        const float rk = o.sc.x > 0.0f ? old.x / o.sc.x : 0.0f, rv = o.sc.y > 0.0f ? old.y / o.sc.y : 0.0f;
+        if (rk != 1.0f)
+            for (int e = tid; e < lo * DP / 4; e += 64 * W) {
+                unsigned *w = reinterpret_cast<unsigned *>(kc) + e;
+                *w = recode4(*w, rk);
+            }
+        if (rv != 1.0f) {
+            const int words = (lo + 3) / 4;
+            for (int e = tid; e < c.d * words; e += 64 * W) {
+                unsigned *w = reinterpret_cast<unsigned *>(vc + e / words * KV8_PAGE) + e % words;
+                *w = recode4(*w, rv);
+            }
+            __syncthreads();  // before the new codes, which share words with kept ones
+        }
+    }
+    for (int i = tid; i < DP; i += 64 * W) kc[lo * DP + i] = i < c.d && !lost ? code8(k[i], ik) : 0;
+    for (int i = tid; i < c.d; i += 64 * W) vc[i * KV8_PAGE + lo] = lost ? 0 : code8(v[i], iv);
+    return o;
+}
+
 // One workgroup of W waves per (sequence, kv head, 16 columns, split of the
 // pages); its waves take the split's pages in turn and join their sums at the
 // end.  splits > 1: unnormalised results [row][head][split][DP + 2] in ws.
-template <int DP, int PL, class T, int W>
+//
+// STEP (a decoder's row a sequence, FP32, no shared heads): the rows come as
+// Q | K | V, or as the partial sums of their projection; the workgroup rotates its
+// head's query, and the one that has the row's own page quantizes its key and value
+// into it (as k_kv8_append) before it reads the page.  The page's scales and codes
+// have no other reader in the launch.
+template <int DP, int PL, class T, int W, bool STEP>
 __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
-                                                       float *__restrict__ ws) {
+                                                       float *__restrict__ ws, StepArg<STEP> step) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr float P = PL == 3 ? 127.0f * 65536 : 127.0f * 256;
     __shared__ __attribute__((aligned(16))) float so[W][16][DP + 4];
@@ -261,8 +371,39 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     const int first = pg0 + split * pps, last = pg0 + min(np, (split + 1) * pps);
     if (split > 0 && first >= last) return;  // the join knows
 
+    // the split's pages, dealt out to the waves
+    auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? page_id(a.c, q, pg) : -1; };
+    Tile<DP> t;
+    int pg = first + wave, id = id_of(pg);
+    float x[KS][16];
+    Kv8Own own;
+    own.pg = -1;
+    if constexpr (STEP) {
+        const int pos = q.start, mine = pos / KV8_PAGE;
+        const bool writes = mine >= first && mine < last;
+        // pages that hold nothing new are on their way meanwhile
+        if (pg < last && pg != mine) load_k(t, a.c, id, kvh, lane);
+        __shared__ float row[3][DP];
+        step_row<DP, W>(a, step, q.r0, kvh, pos, writes, row);
+        if (writes) {
+            own = step_append<DP, W>(a.c, page_id(a.c, q, mine), kvh, pos % KV8_PAGE, row[1], row[2]);
+            own.pg = mine;
+            __syncthreads();  // the codes are written
+        }
+        if (pg < last && pg == mine) load_k(t, a.c, id, kvh, lane);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int i = s * 64 + g4 * 16 + e;
+                x[s][e] = c == 0 && i < a.c.d ? row[0][min(i, DP - 1)] : 0.0f;
+            }
+    } else {
+        if (pg < last) load_k(t, a.c, id, kvh, lane);
+        load_query<KS, T>(a, col, g4, x);
+    }
     i32x4 ql[3][KS];
-    const float f = query_bytes<3, KS, T>(a, col, g4, ql);
+    const float f = query_bytes<3, KS>(x, a.scale, ql);
 
     float m = -INFINITY, l = 0.0f;
     float o[DT][4];
@@ -353,11 +494,12 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         }
     };
 
-    auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? page_id(a.c, q, pg) : -1; };
-    Tile<DP> t;
-    int pg = first + wave, id = id_of(pg);
-    if (pg < last) load_k(t, a.c, id, kvh, lane);
     for (; pg < last; pg += W) {
+        if (STEP && pg == own.pg) {  // what was just written is not in the scalar cache
+            t.sk = own.sc.x;
+            t.sv = own.sc.y;
+            t.bad = own.bad;
+        }
         load_v(t, a.c, id, kvh, lane);
         const int next = id_of(pg + W);
         page(t, id, pg, next);
@@ -488,7 +630,9 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 #pragma unroll
     for (int t = 0; t < CT; t++) {
         const Column col = column(a, q, kvh, g, f0 + t * 16 + c);
-        f[t] = query_bytes<QB, KS, T>(a, col, g4, ql[t]);
+        float x[KS][16];
+        load_query<KS, T>(a, col, g4, x);
+        f[t] = query_bytes<QB, KS>(x, a.scale, ql[t]);
         begin[t] = col.begin;
         end[t] = col.end;
         m[t] = -INFINITY;
@@ -664,11 +808,12 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window,
 // and 79, 17 -> 15).
 template <int DP> constexpr int prompt_tiles() { return DP == 128 ? 2 : 1; }
 
-template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st) {
+template <int DP, class T>
+hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t ws_floats, hipStream_t st) {
     constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
     constexpr int CT = prompt_tiles<DP>();
     const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, ws_floats);
-    if (p.prompt) {
+    if (p.prompt && !step) {
         const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
         const int64_t blocks = tiles * a.s.n_seq * a.c.hk;
         if (blocks > INT32_MAX) return hipErrorInvalidValue;
@@ -676,7 +821,13 @@ template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, s
         return hipGetLastError();
     }
     if (p.blocks > INT32_MAX) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_kv8_attend<DP, full ? 3 : 2, T, 4>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles, p.splits, p.pps, ws);
+    if constexpr (full)
+        if (step)
+            hipLaunchKernelGGL((k_kv8_attend<DP, 3, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
+                               p.splits, p.pps, ws, *step);
+    if (!step)
+        hipLaunchKernelGGL((k_kv8_attend<DP, full ? 3 : 2, T, 4, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g,
+                           p.tiles, p.splits, p.pps, ws, NoStep{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;
@@ -685,12 +836,13 @@ template <int DP, class T> hipError_t launch(const Kv8Attention &a, float *ws, s
     return hipGetLastError();
 }
 
-template <class T> hipError_t launch_dims(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st) {
+template <class T>
+hipError_t launch_dims(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t ws_floats, hipStream_t st) {
     switch (a.c.dp) {
-        case 16: return launch<16, T>(a, ws, ws_floats, st);
-        case 32: return launch<32, T>(a, ws, ws_floats, st);
-        case 64: return launch<64, T>(a, ws, ws_floats, st);
-        case 128: return launch<128, T>(a, ws, ws_floats, st);
+        case 16: return launch<16, T>(a, step, ws, ws_floats, st);
+        case 32: return launch<32, T>(a, step, ws, ws_floats, st);
+        case 64: return launch<64, T>(a, step, ws, ws_floats, st);
+        case 128: return launch<128, T>(a, step, ws, ws_floats, st);
     }
     return hipErrorInvalidValue;
 }
@@ -714,11 +866,22 @@ hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, size_t ws_f
     a.q16 = aligned(a.q, 16);
     a.out16 = aligned(a.out, 4 * size);
     switch (a.dtype) {
-        case FT_F32: return launch_dims<float>(a, ws, ws_floats, st);
-        case FT_F16: return launch_dims<_Float16>(a, ws, ws_floats, st);
-        case FT_BF16: return launch_dims<__bf16>(a, ws, ws_floats, st);
+        case FT_F32: return launch_dims<float>(a, nullptr, ws, ws_floats, st);
+        case FT_F16: return launch_dims<_Float16>(a, nullptr, ws, ws_floats, st);
+        case FT_BF16: return launch_dims<__bf16>(a, nullptr, ws, ws_floats, st);
     }
     return hipErrorInvalidValue;
+}
+
+hipError_t launch_kv8_step(const Kv8Attention &call, const Kv8Step &step, float *ws, size_t ws_floats, hipStream_t st) {
+    if (call.s.n_rows == 0 || call.s.n_seq == 0) return hipSuccess;
+    if (call.dtype != FT_F32 || call.heads != call.c.hk || call.s.max_rows != 1 || call.s.n_rows != call.s.n_seq ||
+        (step.part && (!step.bias || step.splits < 1)) || step.rope.rot > call.c.d)
+        return hipErrorInvalidValue;
+    Kv8Attention a = call;
+    a.q16 = 0;
+    a.out16 = 0;
+    return launch_dims<float>(a, &step, ws, ws_floats, st);
 }
 
 }  // namespace cih

@@ -195,6 +195,28 @@ def test_graph_replays_match_eager(fmt, streams, monkeypatch):
     m.close()
 
 
+@pytest.mark.parametrize("hd,fmt", [(64, "q8"), (24, "fp32")])
+def test_many_streams(hd, fmt):
+    """More streams than the GEMV takes, each at its own position; pages that start, fill and end."""
+    cfg, w, m = make(hd, fmt, heads=8 if hd == 24 else 4)
+    W = dense_weights(cfg, w)
+    n = 20
+    dec = ch.GpuDecoder(m, n_slots=n, max_len=2048, max_rows=64, kv8=True, n_pages=60)
+    t = [tokens(140, 40 + s) for s in range(n)]
+    at = [(7 * s) % 64 + 64 * (s % 2) for s in range(n)]
+    for s in range(n):
+        for p in range(0, at[s], 50):
+            k = min(50, at[s] - p)
+            dec.decode([s] * k, t[s][p:p + k], np.arange(p, p + k))
+    for i in range(3):
+        got = dec.decode(list(range(n)), [t[s][at[s] + i] for s in range(n)], [at[s] + i for s in range(n)])
+        for s in range(n):
+            ref = rows64(cfg, W, [t[s][at[s] + i]], [at[s] + i], held(dec, cfg, s, at[s] + i + 1))
+            assert np.abs(got[s] - ref[0]).max() <= TOL, (i, s)
+    dec.close()
+    m.close()
+
+
 @pytest.mark.parametrize("rows", [1, 12])
 def test_limb_overflow_runs_full_range(rows):
     """Steps and prompts whose activations overflow the f16 limbs run again in full range and write the same positions:
