@@ -16,6 +16,7 @@
 #include <cstring>
 #include <exception>
 #include <map>
+#include <memory>
 #include <tuple>
 
 #include "kv8.h"
@@ -56,6 +57,7 @@ struct cih_decoder {
     // cih_decoder_score: targets in; log probability | entropy | top log probabilities [64] | top ids [64] out
     int *d_targets = nullptr, *d_top_ids = nullptr;
     float *d_score = nullptr, *d_top_lp = nullptr, *d_lp_ws = nullptr;
+    size_t lp_ws_floats = 0;
     int *h_score = nullptr;  // pinned: [max_rows][3 + 2 * 64]
     bool unique = false;      // staged rows: every slot at most once
     // (rows, fused, kernel switches) -> captured step
@@ -67,11 +69,13 @@ using namespace cih;
 
 namespace {
 
-// workspace of the log probabilities of up to `rows` rows (a few rows are split over more chunks than many)
+// workspace of the log probabilities of up to `rows` rows with up to 64
+// alternatives (few rows, and rows with few alternatives, are split over more chunks)
 size_t score_ws_floats(int rows, int vocab) {
     size_t most = 0;
-    for (int n = 1; n <= rows && n < 512; n++) most = std::max(most, token_logprobs_floats(n, vocab, LOGPROBS_MAX_TOP));
-    return std::max(most, token_logprobs_floats(rows, vocab, LOGPROBS_MAX_TOP));
+    for (int top = 0; top <= LOGPROBS_MAX_TOP; top++)
+        for (int n = 1; n <= std::min(rows, 512); n++) most = std::max(most, token_logprobs_floats(n, vocab, top));
+    return most;
 }
 
 void destroy(cih_decoder *dc) {
@@ -546,7 +550,8 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
         if (rope->rot_dim < 2 || rope->rot_dim > m->hd || rope->rot_dim % 2)
             return set_error(CIH_ERR_SHAPE, "%d rotary dims in a head of %d", rope->rot_dim, m->hd);
     }
-    cih_decoder *dc = new cih_decoder();
+    std::unique_ptr<cih_decoder, void (*)(cih_decoder *)> held(new cih_decoder(), destroy);
+    cih_decoder *dc = held.get();
     dc->m = m;
     dc->slots = n_slots;
     dc->max_len = max_len;
@@ -561,10 +566,8 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
         kv.on = true;
         kv.max_pages = (max_len + KV8_PAGE - 1) / KV8_PAGE;
         const int64_t most = (int64_t)kv.max_pages * n_slots;
-        if (n_pages == 0 && most > INT32_MAX) {
-            destroy(dc);
+        if (n_pages == 0 && most > INT32_MAX)
             return set_error(CIH_ERR_CAPACITY, "%lld pages for every slot's max_len", (long long)most);
-        }
         kv.n_pages = n_pages > 0 ? (int)std::min<int64_t>(n_pages, most) : (int)most;
         const size_t H = m->cfg.n_heads, dp = kv8_dims(m->hd), ph = L * kv.n_pages * H;
         cache = ph * KV8_PAGE * dp;
@@ -605,15 +608,13 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
            hipHostMalloc((void **)&dc->h_meta, (3 * R + 1) * sizeof(int)) == hipSuccess &&
            hipHostMalloc((void **)&dc->h_logits, R * V * sizeof(float)) == hipSuccess;
     // cih_decoder_score's rows
+    dc->lp_ws_floats = score_ws_floats((int)R, (int)V);
     good = good && dalloc(dc->d_targets, R, al) == hipSuccess && dalloc(dc->d_score, 2 * R, al) == hipSuccess &&
            dalloc(dc->d_top_lp, R * LOGPROBS_MAX_TOP, al) == hipSuccess &&
            dalloc(dc->d_top_ids, R * LOGPROBS_MAX_TOP, al) == hipSuccess &&
-           dalloc(dc->d_lp_ws, score_ws_floats((int)R, (int)V), al) == hipSuccess &&
+           dalloc(dc->d_lp_ws, dc->lp_ws_floats, al) == hipSuccess &&
            hipHostMalloc((void **)&dc->h_score, R * (3 + 2 * LOGPROBS_MAX_TOP) * sizeof(int)) == hipSuccess;
-    if (!good) {
-        destroy(dc);
-        return set_error(CIH_ERR_HIP, "decoder allocation failed (%zu MiB of KV cache)", cache >> 20);
-    }
+    if (!good) return set_error(CIH_ERR_HIP, "decoder allocation failed (%zu MiB of KV cache)", cache >> 20);
     std::vector<int> cu(R), lens(R, 1);
     for (size_t i = 0; i < R; i++) cu[i] = (int)i;
     hipError_t e = hipSuccess;
@@ -627,11 +628,8 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
     }
     if (e == hipSuccess) e = hipMemcpy(dc->d_cu, cu.data(), R * 4, hipMemcpyHostToDevice);
     if (e == hipSuccess) e = hipMemcpy(dc->d_lens, lens.data(), R * 4, hipMemcpyHostToDevice);
-    if (e != hipSuccess) {
-        destroy(dc);
-        return set_error(CIH_ERR_HIP, "decoder set-up failed: %s", hipGetErrorString(e));
-    }
-    *out = dc;
+    if (e != hipSuccess) return set_error(CIH_ERR_HIP, "decoder set-up failed: %s", hipGetErrorString(e));
+    *out = held.release();
     return CIH_OK;
 }
 
@@ -655,7 +653,11 @@ double ms_since(std::chrono::steady_clock::time_point t0) {
 extern "C" {
 
 int cih_decoder_create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, cih_decoder **out) {
-    return create(m, n_slots, max_len, max_rows, false, 0, nullptr, out);
+    try {
+        return create(m, n_slots, max_len, max_rows, false, 0, nullptr, out);
+    } catch (const std::exception &e) {  // host memory
+        return set_error(CIH_ERR_HIP, "decoder set-up failed: %s", e.what());
+    }
 }
 
 int cih_decoder_create_kv8(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, int32_t n_pages,
@@ -682,7 +684,7 @@ int cih_decoder_reset(cih_decoder *dc, int32_t slot) {
 }
 
 int cih_decode(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, const int32_t *pos, int32_t n,
-               float *logits) {
+               float *logits) try {
     if (!dc || !slots || !tokens || !pos) return set_error(CIH_ERR_ARG, "null argument");
     if (int rc = stage_rows(dc, slots, tokens, pos, n)) return rc;
     if (int rc = run_rows(dc, n)) return rc;
@@ -695,6 +697,8 @@ int cih_decode(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, con
     else if (logits) std::memcpy(logits, dc->h_logits, lb);
     profile_collect(dc->m);
     return CIH_OK;
+} catch (const std::exception &e) {  // host memory
+    return set_error(CIH_ERR_HIP, "decoding failed: %s", e.what());
 }
 
 int cih_decoder_score(cih_decoder *dc, int32_t n, const int32_t *slots, const int32_t *tokens, const int32_t *offsets,
@@ -703,6 +707,7 @@ int cih_decoder_score(cih_decoder *dc, int32_t n, const int32_t *slots, const in
         return set_error(CIH_ERR_ARG, "null argument");
     const int V = dc->m->cfg.vocab_size;
     if (n < 1) return set_error(CIH_ERR_ARG, "n must be >= 1");
+    if (offsets[0] < 0) return set_error(CIH_ERR_ARG, "offsets[0] is negative");
     if (top_k < 0 || top_k > std::min(V, LOGPROBS_MAX_TOP))
         return set_error(CIH_ERR_SHAPE, "top_k %d outside [0, %d]", top_k, std::min(V, LOGPROBS_MAX_TOP));
     std::vector<char> seen(dc->slots, 0);
@@ -733,7 +738,7 @@ int cih_decoder_score(cih_decoder *dc, int32_t n, const int32_t *slots, const in
             ProfScope pr(dc->m, CIH_KC_OTHER, 5.0 * k * V, 4.0 * k * V);
             const TokenLogprobs a{FT_F32,      dc->logits,          V,           k,            V, top_k, dc->d_targets,
                                   dc->d_score, dc->d_score + k, dc->d_top_ids, dc->d_top_lp};
-            HIPCHK(launch_token_logprobs(a, dc->d_lp_ws, st));
+            HIPCHK(launch_token_logprobs(a, dc->d_lp_ws, dc->lp_ws_floats, st));
         }
         float *hf = reinterpret_cast<float *>(h + k);
         HIPCHK(hipMemcpyAsync(hf, dc->d_score, (size_t)k * 8, hipMemcpyDeviceToHost, st));
@@ -814,7 +819,7 @@ int cih_decoder_read_cache(cih_decoder *dc, int32_t layer, int32_t slot, int32_t
 int cih_generate(cih_decoder *dc, int32_t n, const int32_t *slots, const int32_t *prompts, const int32_t *offsets,
                  float temperature, int32_t max_new_tokens, const uint64_t *seeds, int32_t max_seq_len,
                  int32_t *out_tokens, int32_t out_cap, int32_t *n_generated, double *prefill_ms,
-                 double *generation_ms) {
+                 double *generation_ms) try {
     if (!dc || !slots || !prompts || !offsets || !seeds || !out_tokens || !n_generated)
         return set_error(CIH_ERR_ARG, "null argument");
     if (n < 1) return set_error(CIH_ERR_ARG, "n must be >= 1");
@@ -893,6 +898,8 @@ int cih_generate(cih_decoder *dc, int32_t n, const int32_t *slots, const int32_t
     if (prefill_ms) *prefill_ms = t_prefill;
     if (generation_ms) *generation_ms = ms_since(t1);
     return CIH_OK;
+} catch (const std::exception &e) {  // host memory
+    return set_error(CIH_ERR_HIP, "generation failed: %s", e.what());
 }
 
 }  // extern "C"

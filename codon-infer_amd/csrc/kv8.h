@@ -40,6 +40,9 @@ struct RopeArg {
     double turns[64] = {};
 };
 
+// Workgroups of `threads` that one launch may have: its threads are counted in 32 bits.
+inline bool kv8_grid(int64_t blocks, int threads) { return blocks > 0 && blocks <= INT32_MAX && blocks <= (int64_t)UINT32_MAX / threads; }
+
 // A sequence of the batch as the kernels see it.
 struct Kv8Seq {
     int r0, n;        // first row, rows
@@ -137,7 +140,7 @@ struct TokenLogprobs {
     float *top_lp;
 };
 size_t token_logprobs_floats(int n, int vocab, int top);
-hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, hipStream_t st);
+hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, size_t ws_floats, hipStream_t st);
 
 // Element types of the row tensors.
 enum { FT_F32 = 0, FT_F16 = 1, FT_BF16 = 2 };

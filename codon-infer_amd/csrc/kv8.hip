@@ -592,7 +592,7 @@ hipError_t launch_kv8_append(const Kv8View &c, const Kv8Seqs &s, int dtype, cons
     const int per = pages_per_seq(s.max_rows), g = heads / c.hk;
     const int64_t blocks = (int64_t)s.n_seq * per * c.hk;
     if (blocks == 0) return hipSuccess;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (!kv8_grid(blocks, KV_THREADS)) return hipErrorInvalidValue;
     switch (dtype) {
         case FT_F32: return launch_append<float>(c, s, k, v, g, q, qo, rope, per, blocks, st);
         case FT_F16: return launch_append<_Float16>(c, s, k, v, g, q, qo, rope, per, blocks, st);
@@ -606,7 +606,7 @@ hipError_t launch_kv8_read(const Kv8View &c, const Kv8Seqs &s, int dtype, const 
     const int per = pages_per_seq(s.max_rows);
     const int64_t blocks = (int64_t)s.n_seq * per * c.hk;
     if (blocks == 0) return hipSuccess;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (!kv8_grid(blocks, KV_THREADS)) return hipErrorInvalidValue;
     switch (dtype) {
         case FT_F32: return launch_read<float>(c, s, k, v, per, blocks, st);
         case FT_F16: return launch_read<_Float16>(c, s, k, v, per, blocks, st);

@@ -61,15 +61,13 @@ int check_batch(const cih_kv8_batch *b, Kv8Seqs &s, bool memory) {
     return 0;
 }
 
-// One past the largest element offset of `heads` heads stays below 2^62.
-int check_rows(const cih_rows *r, const char *what, int dtype, int d, RowsView &v) {
+int check_rows(const cih_rows *r, const char *what, int dtype, RowsView &v) {
     if (!r || !r->data) return set_error(CIH_ERR_ARG, "null %s", what);
     if (!aligned(r->data, float_size(dtype))) return set_error(CIH_ERR_ARG, "%s is not aligned to its type", what);
     const int64_t most = (int64_t)1 << 31;
     if (r->row_stride < 0 || r->head_stride < 0 || r->row_stride > most || r->head_stride > most)
         return set_error(CIH_ERR_SHAPE, "%s: strides of %lld and %lld elements", what, (long long)r->row_stride,
                          (long long)r->head_stride);
-    (void)d;
     v = {r->data, r->row_stride, r->head_stride};
     return 0;
 }
@@ -99,9 +97,11 @@ int check_rope(const cih_rope *r, int d, RopeArg &a) {
     return 0;
 }
 
-int check_heads(int heads, int hk) {
+int check_heads(int heads, int hk, const Kv8Seqs &s) {
     if (heads < 1 || heads > 65535 || heads % hk)
         return set_error(CIH_ERR_SHAPE, "%d query heads over %d key/value heads", heads, hk);
+    if ((int64_t)s.max_rows * (heads / hk) > 1 << 30)
+        return set_error(CIH_ERR_SHAPE, "%d rows of %d query heads a key/value head", s.max_rows, heads / hk);
     return 0;
 }
 
@@ -155,12 +155,12 @@ int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32
     CIH_TRY(check_batch(batch, s, true));
     CIH_TRY(check_rope(rope, c.d, ra));
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return CIH_OK;
-    CIH_TRY(check_rows(k, "k", dtype, c.d, kv));
-    CIH_TRY(check_rows(v, "v", dtype, c.d, vv));
+    CIH_TRY(check_rows(k, "k", dtype, kv));
+    CIH_TRY(check_rows(v, "v", dtype, vv));
     if (q) {
-        CIH_TRY(check_heads(q_heads, c.hk));
-        CIH_TRY(check_rows(q, "q", dtype, c.d, qv));
-        CIH_TRY(check_rows(q_out, "q_out", dtype, c.d, qo));
+        CIH_TRY(check_heads(q_heads, c.hk, s));
+        CIH_TRY(check_rows(q, "q", dtype, qv));
+        CIH_TRY(check_rows(q_out, "q_out", dtype, qo));
         CIH_TRY(check_out(qo, "q_out", s.n_rows, q_heads, c.d));
         if (qo.p == qv.p && (qo.rs != qv.rs || qo.hs != qv.hs))
             return set_error(CIH_ERR_ARG, "q_out in q's place must have q's strides");
@@ -181,8 +181,8 @@ int cih_kv8_read(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t
     CIH_TRY(check_cache(cache, c, true));
     CIH_TRY(check_batch(batch, s, true));
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return CIH_OK;
-    CIH_TRY(check_rows(k, "k", dtype, c.d, kv));
-    CIH_TRY(check_rows(v, "v", dtype, c.d, vv));
+    CIH_TRY(check_rows(k, "k", dtype, kv));
+    CIH_TRY(check_rows(v, "v", dtype, vv));
     CIH_TRY(check_out(kv, "k", s.n_rows, c.hk, c.d));
     CIH_TRY(check_out(vv, "v", s.n_rows, c.hk, c.d));
     hipStream_t st = static_cast<hipStream_t>(stream);
@@ -198,7 +198,7 @@ int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch 
     if (!bytes) return set_error(CIH_ERR_ARG, "null bytes");
     CIH_TRY(check_cache(cache, c, false));
     CIH_TRY(check_batch(batch, s, false));
-    CIH_TRY(check_heads(q_heads, c.hk));
+    CIH_TRY(check_heads(q_heads, c.hk, s));
     *bytes = kv8_attention_floats(c, s, q_heads) * sizeof(float);
     return CIH_OK;
 }
@@ -210,13 +210,15 @@ int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, in
     CIH_TRY(check_float(dtype));
     CIH_TRY(check_cache(cache, a.c, true));
     CIH_TRY(check_batch(batch, a.s, true));
-    CIH_TRY(check_heads(q_heads, a.c.hk));
+    CIH_TRY(check_heads(q_heads, a.c.hk, a.s));
     if (window < 0) return set_error(CIH_ERR_ARG, "window %d", window);
     if (!std::isfinite(scale)) return set_error(CIH_ERR_ARG, "the scale is not finite");
     if (a.s.n_rows == 0 || a.s.n_seq == 0 || a.s.max_rows == 0) return CIH_OK;
-    CIH_TRY(check_rows(q, "q", dtype, a.c.d, a.q));
-    CIH_TRY(check_rows(out, "out", dtype, a.c.d, a.out));
+    CIH_TRY(check_rows(q, "q", dtype, a.q));
+    CIH_TRY(check_rows(out, "out", dtype, a.out));
     CIH_TRY(check_out(a.out, "out", a.s.n_rows, q_heads, a.c.d));
+    if (a.out.p == a.q.p && (a.out.rs != a.q.rs || a.out.hs != a.q.hs))
+        return set_error(CIH_ERR_ARG, "out in q's place must have q's strides");
     if (lse && !aligned(lse, 4)) return set_error(CIH_ERR_ARG, "lse must be 4-byte aligned");
     const size_t need = kv8_attention_floats(a.c, a.s, q_heads) * sizeof(float);
     if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
@@ -236,7 +238,8 @@ int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, in
 
 int cih_token_logprobs_workspace(int32_t n_rows, int32_t vocab, int32_t top_k, size_t *bytes) {
     if (!bytes) return set_error(CIH_ERR_ARG, "null bytes");
-    if (n_rows < 0 || vocab < 1 || vocab > 1 << 30) return set_error(CIH_ERR_SHAPE, "%d rows of %d logits", n_rows, vocab);
+    if (n_rows < 0 || n_rows > 1 << 30 || vocab < 1 || vocab > 1 << 30)
+        return set_error(CIH_ERR_SHAPE, "%d rows of %d logits", n_rows, vocab);
     if (top_k < 0 || top_k > LOGPROBS_MAX_TOP) return set_error(CIH_ERR_SHAPE, "top_k %d outside [0, %d]", top_k, LOGPROBS_MAX_TOP);
     *bytes = token_logprobs_floats(n_rows, vocab, top_k) * sizeof(float);
     return CIH_OK;
@@ -260,7 +263,7 @@ int cih_token_logprobs(int32_t dtype, const void *logits, int64_t row_stride, in
     hipStream_t st = static_cast<hipStream_t>(stream);
     CIH_TRY(check_stream(st));
     const TokenLogprobs a{dtype, logits, n_rows > 1 ? row_stride : 0, n_rows, vocab, top_k, targets, logprob, entropy, top_ids, top_logprobs};
-    const hipError_t e = launch_token_logprobs(a, static_cast<float *>(workspace), st);
+    const hipError_t e = launch_token_logprobs(a, static_cast<float *>(workspace), workspace_bytes / sizeof(float), st);
     if (e != hipSuccess) return set_error(CIH_ERR_HIP, "token log probabilities failed: %s", hipGetErrorString(e));
     return CIH_OK;
 }

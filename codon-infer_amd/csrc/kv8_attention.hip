@@ -816,11 +816,12 @@ hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t 
     if (p.prompt && !step) {
         const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
         const int64_t blocks = tiles * a.s.n_seq * a.c.hk;
-        if (blocks > INT32_MAX) return hipErrorInvalidValue;
+        if (!kv8_grid(blocks, 256)) return hipErrorInvalidValue;
         hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(blocks), dim3(256), 0, st, a, p.g, (int)tiles);
         return hipGetLastError();
     }
-    if (p.blocks > INT32_MAX) return hipErrorInvalidValue;
+    const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;  // of the join
+    if (!kv8_grid(p.blocks, 256) || (p.splits > 1 && !kv8_grid(rows, 64 * JOIN_WAVES))) return hipErrorInvalidValue;
     if constexpr (full)
         if (step)
             hipLaunchKernelGGL((k_kv8_attend<DP, 3, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
@@ -830,8 +831,6 @@ hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t 
                            p.tiles, p.splits, p.pps, ws, NoStep{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;
-    if (rows > INT32_MAX) return hipErrorInvalidValue;
     hipLaunchKernelGGL((k_kv8_join<DP, T>), dim3(rows), dim3(64 * JOIN_WAVES), 0, st, a, p.g, p.splits, p.pps, ws);
     return hipGetLastError();
 }

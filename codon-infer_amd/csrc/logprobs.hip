@@ -408,12 +408,12 @@ LpPlan lp_plan(int n, int vocab, int top) {
 
 template <class T> hipError_t launch_lp(const TokenLogprobs &a, float *ws, hipStream_t st) {
     if (a.vocab <= 64) {
-        hipLaunchKernelGGL(k_logprobs_narrow<T>, dim3((a.n + NARROW_ROWS - 1) / NARROW_ROWS), dim3(64 * NARROW_ROWS), 0,
+        hipLaunchKernelGGL(k_logprobs_narrow<T>, dim3(a.n / NARROW_ROWS + (a.n % NARROW_ROWS != 0)), dim3(64 * NARROW_ROWS), 0,
                            st, a);
         return hipGetLastError();
     }
     const LpPlan p = lp_plan(a.n, a.vocab, a.top);
-    if ((int64_t)a.n * p.chunks > INT32_MAX) return hipErrorInvalidValue;
+    if (!kv8_grid((int64_t)a.n * p.chunks, p.nt)) return hipErrorInvalidValue;
     const dim3 grid(a.n * p.chunks);
     if (p.nt == 64) hipLaunchKernelGGL((k_logprobs<T, 64>), grid, dim3(64), 0, st, a, p.chunks, p.tiles_per, ws);
     else if (p.nt == 256) hipLaunchKernelGGL((k_logprobs<T, 256>), grid, dim3(256), 0, st, a, p.chunks, p.tiles_per, ws);
@@ -432,8 +432,9 @@ size_t token_logprobs_floats(int n, int vocab, int top) {
     return p.chunks > 1 ? (size_t)n * p.chunks * (4 + 2 * top) : 0;
 }
 
-hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, hipStream_t st) {
+hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, size_t ws_floats, hipStream_t st) {
     if (a.n == 0) return hipSuccess;
+    if (token_logprobs_floats(a.n, a.vocab, a.top) > ws_floats) return hipErrorInvalidValue;
     switch (a.dtype) {
         case FT_F32: return launch_lp<float>(a, ws, st);
         case FT_F16: return launch_lp<_Float16>(a, ws, st);

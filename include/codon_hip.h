@@ -297,7 +297,9 @@ int cih_rope_init(cih_rope *r, int32_t rot_dim, int32_t interleaved, double base
  * rounded again to the larger one.  Later tokens of the page are forgotten.
  * With q (q_heads heads; NULL: none) the rows of q are written to q_out (may
  * be q), rotated by the same positions.  Two sequences of a batch must not
- * write the same page. */
+ * write the same page.  Rows without a position in the table (negative, or from
+ * max_pages * 64 on) leave q_out as it was.  k, v and q_out must not overlap
+ * each other. */
 int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
                    const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out, const cih_rope *rope,
                    void *stream);
@@ -313,9 +315,11 @@ int cih_kv8_read(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t
  * tokens j < lens[i], with causal only j <= p, with window > 0 only j > p -
  * window.  out = sum softmax(scale q.k) v in q's type; lse (NULL: none) [n_rows][q_heads] the
  * logarithm of the sum of exp(scale q.k).  A row that sees nothing gets out 0
- * and lse -inf, one that sees a bad token NaN.  workspace: 16-byte aligned, of the size
+ * and lse -inf, one that sees a bad token NaN.  out may be q
+ * (with its strides).  Rows of very different counts, such as prompts beside
+ * single tokens, are served better by a call each.  workspace: 16-byte aligned, of the size
  * cih_kv8_attention_workspace gives for the same sizes (it reads no device
- * memory); calls that may run at the same time (other streams, two graphs)
+ * memory; max_rows * q_heads / kv_heads <= 2^30); calls that may run at the same time (other streams, two graphs)
  * need one each. */
 int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
                       const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal, int32_t window,
@@ -324,7 +328,7 @@ int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch 
 
 /* ---- log probabilities of given tokens ----------------------------------------
  * Beside log_softmax_canonical (lib.rs:4426-4441), over the whole vocabulary.
- * For each row of logits [n_rows][vocab] (vocab <= 2^30, type dtype, rows
+ * For each row of logits [n_rows][vocab] (both <= 2^30, type dtype, rows
  * row_stride elements apart): logprob = log softmax at targets[row]; entropy = -sum p log p (in
  * nats); the top_k <= 64 largest logits (ties: lowest id first) as top_ids
  * [n_rows][top_k] and their log probabilities top_logprobs.  logprob, entropy and the
@@ -346,9 +350,10 @@ int cih_token_logprobs_workspace(int32_t n_rows, int32_t vocab, int32_t top_k, s
  * rope (NULL: as the reference's, the whole head, base 10000) may scale the
  * positions for contexts beyond those the model was trained on; max_len <=
  * 2^20.  cih_decode and cih_generate work as on any decoder, but: rows that
- * rewrite a position make the slot forget the ones after it, a call that needs more pages
- * than are free returns CIH_ERR_CAPACITY and changes nothing, and results
- * carry the rounding of K and V to 8 bits. */
+ * rewrite a position make the slot forget the ones after it, a cih_decode that needs
+ * more pages than are free returns CIH_ERR_CAPACITY and changes nothing (a
+ * cih_generate or cih_decoder_score stops there, its slots started anew), and
+ * results carry the rounding of K and V to 8 bits. */
 int cih_decoder_create_kv8(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, int32_t n_pages,
                            const cih_rope *rope, cih_decoder **out);
 

@@ -10,6 +10,7 @@ import numpy as np
 import pytest
 
 import codon_hip as ch
+from codon_hip import _lib as C
 from ref64 import _gelu, _ln, dense_weights
 from test_gpu_decode import overflow_model
 
@@ -305,6 +306,24 @@ def test_score(kv8):
     m.close()
 
 
+def test_score_large_vocabulary():
+    """Rows of 500,000 logits, which are split over 62 workgroups with 33 alternatives and over 32 with 64."""
+    cfg = ch.EsmConfig(64, 256, 1, 2, vocab_size=500_000)
+    m = ch.GpuModel(cfg, ch.EsmWeights.random(cfg, seed=5, std=0.06, bias_std=0.02), max_batch=1, max_len=16)
+    dec = ch.GpuDecoder(m, n_slots=1, max_len=64, max_rows=4, kv8=True)
+    lg = dec.decode([0], [400_000], [0]).astype(np.float64)[0]
+    lse = lg.max() + np.log(np.exp(lg - lg.max()).sum())
+    tol = 2.0 ** -18 * (1 + 2 * np.abs(lg).max() + np.log(lg.size))
+    for top in (0, 33, 64):
+        r = dec.score([[400_000]], top)[0]
+        best = np.argsort(-lg, kind="stable")[:top]
+        assert np.array_equal(r["top_ids"][0], best)
+        assert np.abs(r["top_logprobs"][0] - (lg[best] - lse)).max(initial=0) <= tol
+        assert abs(r["entropy"][0] - (lse - np.exp(lg - lse) @ lg)) <= tol
+    dec.close()
+    m.close()
+
+
 def test_refusals():
     cfg, w, m = make(16)
     for kw in (dict(max_len=1 << 21), dict(n_pages=-1), dict(n_slots=0), dict(rope=ch.Rope(32))):
@@ -318,6 +337,9 @@ def test_refusals():
         with pytest.raises(ch.CihError) as e:
             dec.score(seqs, **kw)
         assert e.value.code == code, (seqs, kw)
+    zero, offs = np.zeros(8, np.int32), np.array([-1, 1], np.int32)
+    assert C.lib().cih_decoder_score(dec._h, 1, zero.ctypes.data, zero.ctypes.data + 4, offs.ctypes.data, 0, None, None, None,
+                                     None) == -1
     dec.decode([0, 0], [0, 5], [0, 1])
     for a in ((2, 0, 0, 1), (-1, 0, 0, 1), (0, 2, 0, 1), (0, 0, 0, 3), (0, 0, -1, 1), (0, 1, 0, 1)):
         with pytest.raises(ch.CihError):

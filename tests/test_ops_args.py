@@ -113,6 +113,9 @@ def test_attention_refusals():
         assert code(c.attend, long, one, one, workspace=Fake((need - 1,), "uint8")) == -3
         assert code(c.attend, long, one, one) == -3
         assert code(c.attend, long, one, one, workspace=Fake((need,), "uint8", at=8)) == -3
+    many = batch(n_rows=1 << 30, max_rows=1 << 30)  # 2^31 rows of a key/value head
+    assert code(c.attend_workspace, many, 4) == -2
+    assert code(c.attend, b, q(at=1 << 20), q(at=1 << 20, stride=(512, 64, 1)), workspace=ws) == -1  # in place, other strides
     lib = C.lib()
     assert lib.cih_kv8_attention(None, b._at, 0, 4, None, None, None, 1.0, 1, 0, None, 0, None) == -1
     assert lib.cih_kv8_attention(c._at, b._at, 7, 4, None, None, None, 1.0, 1, 0, None, 0, None) == -1
@@ -141,6 +144,7 @@ def test_logprobs_refusals():
     assert code(ch.token_logprobs, Fake((3, 100), at=0), t, f, workspace=ws) == -1
     assert code(ch.token_logprobs_workspace, 3, 0, 1) == -2
     assert code(ch.token_logprobs_workspace, -1, 10, 1) == -2
+    assert code(ch.token_logprobs_workspace, (1 << 30) + 1, 10, 1) == -2
     need = ch.token_logprobs_workspace(1, 131072, 20)
     if need:
         assert code(ch.token_logprobs, Fake((1, 131072)), Fake((1,), "int32"), Fake((1,)), top_ids=Fake((1, 20), "int32"),
