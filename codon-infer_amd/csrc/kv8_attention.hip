@@ -546,56 +546,91 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     }
 }
 
-// Joins a row's splits: one workgroup per (row of a sequence, head), the
-// splits dealt out to its waves.
+// Joins a row's splits: a row of one head by W waves, the splits dealt out to
+// them (W = 1: four rows a workgroup).  cols: columns whose pages were split together.
 constexpr int JOIN_WAVES = 4;
-template <int DP, class T>
-__global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, int g, int splits, int pps,
+template <int DP, class T, int W>
+__global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, int g, int cols, int splits, int pps,
                                                               const float *__restrict__ ws) {
     constexpr int DL = DP > 64 ? DP / 64 : 1;  // dims a lane
-    __shared__ float so[JOIN_WAVES][DP], sl[JOIN_WAVES];
-    const int h = blockIdx.x % a.heads, b = blockIdx.x / a.heads;
-    const int r = b % a.s.max_rows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Kv8Seq q = kv8_seq(a.s, b / a.s.max_rows);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const unsigned at = W == 1 ? blockIdx.x * JOIN_WAVES + wave : blockIdx.x;  // (below 2^24)
+    const unsigned b = at / (unsigned)a.heads;
+    const int h = at - b * a.heads, seq = b / (unsigned)a.s.max_rows, r = b - seq * a.s.max_rows;
+    if (seq >= a.s.n_seq) return;
+    const Kv8Seq q = kv8_seq(a.s, seq);
     if (r >= q.n) return;
-    // the splits of its 16 columns that had pages
-    const int kvh = h / g, f = r * g + (h - kvh * g), t0 = f / 16 * 16;
-    const Column c0 = column(a, q, kvh, g, t0), c1 = column(a, q, kvh, g, min(t0 + 15, q.n * g - 1));
+    // the splits of its columns that had pages
+    const int kvh = h / g, f = r * g + (h - kvh * g), t0 = f / cols * cols;
+    const Column c0 = column(a, q, kvh, g, t0), c1 = column(a, q, kvh, g, min(t0 + cols - 1, q.n * g - 1));
     const int pg0 = c0.begin / KV8_PAGE, np = (c1.end + KV8_PAGE - 1) / KV8_PAGE - pg0;
     const int used = min(splits, max(1, (np + pps - 1) / pps));
     const int row = q.r0 + r;
     const float *p = ws + ((int64_t)row * a.heads + h) * splits * (DP + 2);
-    float mm = -INFINITY;
-    for (int s = lane; s < used; s += 64) mm = fmaxf(mm, p[s * (DP + 2) + DP]);
+    float mm = -INFINITY, ll = 0.0f, oo[DL] = {};
+    if constexpr (W == 1) {
+        // four splits' values at a time, requested together; the maximum moves with them
+        for (int s0 = 0; s0 < used; s0 += 4) {
+            float m[4], l[4], o[4][DL];
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor(mm, x));
-    const float base = mm == -INFINITY ? 0.0f : mm;
-    float ll = 0.0f, oo[DL] = {};
+            for (int s = 0; s < 4; s++) {
+                const float *ps = p + min(s0 + s, used - 1) * (DP + 2);
+                const float2 ml = *reinterpret_cast<const float2 *>(ps + DP);
+                m[s] = s0 + s < used ? ml.x : -INFINITY;
+                l[s] = ml.y;
+#pragma unroll
+                for (int u = 0; u < DL; u++) o[s][u] = ps[(DP >= 64 ? lane : lane % DP) + 64 * u];
+            }
+            const float mn = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), mm);
+            const float base = mn == -INFINITY ? 0.0f : mn, y = __builtin_amdgcn_exp2f(mm - base);
+            mm = mn;
+            ll *= y;
+#pragma unroll
+            for (int u = 0; u < DL; u++) oo[u] *= y;
+#pragma unroll
+            for (int s = 0; s < 4; s++) {
+                const float x = __builtin_amdgcn_exp2f(m[s] - base);
+                ll += s0 + s < used ? l[s] * x : 0.0f;  // (x may be 0: 0 NaN is NaN)
+#pragma unroll
+                for (int u = 0; u < DL; u++) oo[u] = s0 + s < used ? fmaf(o[s][u], x, oo[u]) : oo[u];
+            }
+        }
+    } else {
+        for (int s = lane; s < used; s += 64) mm = fmaxf(mm, p[s * (DP + 2) + DP]);
+#pragma unroll
+        for (int x = 32; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor(mm, x));
+        const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll 4
-    for (int s = wave; s < used; s += JOIN_WAVES) {
-        const float *ps = p + s * (DP + 2);
-        const float l = ps[DP + 1], x = __builtin_amdgcn_exp2f(ps[DP] - base);
-        ll += l != l ? NAN : l * x;
+        for (int s = wave; s < used; s += W) {
+            const float *ps = p + s * (DP + 2);
+            const float x = __builtin_amdgcn_exp2f(ps[DP] - base);
+            ll += ps[DP + 1] * x;
+#pragma unroll
+            for (int u = 0; u < DL; u++)
+                if (DP >= 64 || lane < DP) oo[u] = fmaf(ps[lane + 64 * u], x, oo[u]);
+        }
+        __shared__ float so[W][DP], sl[W];
 #pragma unroll
         for (int u = 0; u < DL; u++)
-            if (DP >= 64 || lane < DP) oo[u] = fmaf(ps[lane + 64 * u], x, oo[u]);
+            if (DP >= 64 || lane < DP) so[wave][lane + 64 * u] = oo[u];
+        if (lane == 0) sl[wave] = ll;
+        __syncthreads();
+        if (wave > 0) return;  // (behind the last barrier)
+        ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) ll += sl[w];
+#pragma unroll
+        for (int u = 0; u < DL; u++) {
+            oo[u] = 0.0f;
+            if (DP >= 64 || lane < DP)
+#pragma unroll
+                for (int w = 0; w < W; w++) oo[u] += so[w][lane + 64 * u];
+        }
     }
 #pragma unroll
     for (int u = 0; u < DL; u++)
-        if (DP >= 64 || lane < DP) so[wave][lane + 64 * u] = oo[u];
-    if (lane == 0) sl[wave] = ll;
-    __syncthreads();
-    ll = 0.0f;
-#pragma unroll
-    for (int w = 0; w < JOIN_WAVES; w++) ll += sl[w];
-    const int i = threadIdx.x;
-    if (i < a.c.d) {
-        float o = 0.0f;
-#pragma unroll
-        for (int w = 0; w < JOIN_WAVES; w++) o += so[w][i];
-        store_out<T>(a, row, h, i, ll == 0.0f ? 0.0f : o / ll);
-    }
-    if (a.lse && i == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
+        if (lane + 64 * u < a.c.d) store_out<T>(a, row, h, lane + 64 * u, ll == 0.0f ? 0.0f : oo[u] / ll);
+    if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
 // Four waves of CT x 16 columns each, over all pages that these see, with PL f16
@@ -604,13 +639,15 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 // unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
 // 2^3 at the running maximum and have room for both.
 template <int DP, int PL, class T, int CT>
-__global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles) {
+__global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int splits, int pps,
+                                                       float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr float SLACK = 8.0f, P0 = 3.0f, UNIT = 16.0f;
     // The last rows, which see most keys, go first, over all (sequence, kv head)
     // pairs (a pair after the other left the longest to a quarter of the CUs:
     // prompts of 131 to 512 rows 28.4 -> 25.4 us; whole pairs to one XCD: no difference).
-    const int pairs = a.c.hk * a.s.n_seq, pair = blockIdx.x % pairs, tile = tiles - 1 - blockIdx.x / pairs;
+    const int split = blockIdx.x % splits, task = blockIdx.x / splits;
+    const int pairs = a.c.hk * a.s.n_seq, pair = task % pairs, tile = tiles - 1 - task / pairs;
     const int kvh = pair % a.c.hk;
     const Kv8Seq q = kv8_seq(a.s, pair / a.c.hk);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -620,7 +657,9 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     const Column c0 = column(a, q, kvh, g, f0), c1 = column(a, q, kvh, g, f1);
     const int any0 = __builtin_amdgcn_readfirstlane(c0.begin), any1 = __builtin_amdgcn_readfirstlane(c1.end);
     const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
-    const int first = any0 / KV8_PAGE, last = (any1 + KV8_PAGE - 1) / KV8_PAGE;
+    const int pg0 = any0 / KV8_PAGE, np = (any1 + KV8_PAGE - 1) / KV8_PAGE - pg0;
+    const int first = pg0 + split * pps, last = pg0 + min(np, (split + 1) * pps);
+    if (split > 0 && first >= last) return;  // the join knows
 
     constexpr int QB = PL + 1;  // bytes of a query
     i32x4 ql[CT][QB][KS];
@@ -764,6 +803,17 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         float sum = groups_sum(l[t]);
         if (begin[t] >= end[t]) sum = 0.0f;
         if (col.row < 0) continue;
+        if (splits > 1) {
+            float *p = ws + (((int64_t)col.row * a.heads + col.head) * splits + split) * (DP + 2);
+            const float x = unit * __builtin_amdgcn_exp2f(-P0);
+#pragma unroll
+            for (int dt = 0; dt < DT; dt++)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2)
+                    *reinterpret_cast<float2 *>(p + dt * 16 + g4 * 4 + r) = make_float2(o[t][dt][r] * x, o[t][dt][r + 1] * x);
+            if (g4 == 0) *reinterpret_cast<float2 *>(p + DP) = make_float2(m[t], sum);
+            continue;
+        }
         const float x = unit / sum * __builtin_amdgcn_exp2f(-P0);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
@@ -775,24 +825,55 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     }
 }
 
-// Workgroups: how the pages of a sequence are split.
+// Columns of a prompt wave, / 16: heads of 128 share V's conversion over 32
+// (bfloat16, 20 heads: 4096 rows 238 -> 147 us; 131 to 512 rows 36 -> 31), narrower
+// ones gain more from twice the waves (64 wide: 92 and 96, 20 -> 17; 32 wide 80
+// and 79, 17 -> 15).
+constexpr int prompt_tiles(int dp) { return dp == 128 ? 2 : 1; }
+
+// Which kernel, and how the pages of a sequence are split.
 struct Plan {
     bool prompt;
-    int g, tiles, splits, pps;
+    int g, tiles, splits, pps;  // tiles of cols columns (a workgroup of a prompt has four)
+    int cols;
     int64_t blocks;
 };
-Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window, size_t ws_floats) {
+// Prompts: k_kv8_prompt where the columns alone fill the GPU, or are more than
+// a workgroup's and the keys long enough to be split (us, FP32 rows, 20
+// heads of 64, the one kernel and the other: 2 sequences of 512 rows 18.8
+// and 13.1, 256 rows of 4096 keys 36.7 and 30.1, but 512 of 1024 16.9 and 19.8, 64 of
+// 1024 10.3 and 15.7).  Its pages are split until the workgroups are as many as
+// run at once (heads of 128: two a CU, and one does as well for 16-bit rows: bfloat16, 2
+// x 512 rows of 4096 keys, 32 over 8 heads, 98 unsplit, 117 in two; narrower heads four a
+// CU), not below 8 pages each (512 rows of 65536 keys, 32 over 8 heads of 128: FP32
+// 3082 unsplit, 1006; bfloat16 1420, 702), and only from 32 pages
+// on (1000 rows of 1000 keys: 18.1 unsplit, 29.8).
+//
+// Few columns: splits of 16 to 64 pages, a wave's 4 to 16, so that there are some
+// 2048 workgroups; shorter ones cost more in the join than they gain (8 single tokens of 700, 20
+// heads of 64: 8.4 us, with 8 pages 12.1), and from 4096 tiles on none is split.
+Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, bool full, int causal, int window, bool step, size_t ws_floats) {
     Plan p;
     p.g = heads / c.hk;
-    p.tiles = (int)(((int64_t)s.max_rows * p.g + 15) / 16);
-    const int64_t tasks = (int64_t)s.n_seq * c.hk * p.tiles;
+    const int64_t columns = (int64_t)s.max_rows * p.g, pairs = (int64_t)s.n_seq * c.hk;
+    const bool fits = pairs * ((columns + 15) / 16) >= 1024, split = s.max_pages >= 32;
     const char *e = getenv("CIH_KV8_PROMPT");
-    p.prompt = e ? !strcmp(e, "1") : p.tiles > 1 && tasks >= 1024;
-    int64_t pps = max((int64_t)16, min(s.max_pages * tasks / 2048, (int64_t)64));
-    if (tasks >= 4096 || p.prompt) pps = s.max_pages;
-    // pages that the keys of 16 columns touch at most
+    p.prompt = step ? false : e ? !strcmp(e, "1") : columns > 16 && (fits || (columns > 64 && split));
+    p.cols = p.prompt ? 16 * prompt_tiles(c.dp) : 16;
+    const int wg = p.prompt ? 4 * p.cols : p.cols;
+    p.tiles = (int)((columns + wg - 1) / wg);
+    const int64_t tasks = pairs * p.tiles;
+    int64_t pps = s.max_pages;
+    if (p.prompt && split) {
+        const int64_t want = max((int64_t)1, (c.dp < 128 ? 1024 : full ? 512 : 256) / tasks);
+        pps = max((int64_t)8, (s.max_pages + want - 1) / want);
+    } else if (!p.prompt && tasks < 4096) {
+        pps = max((int64_t)16, min(s.max_pages * tasks / 2048, (int64_t)64));
+    }
+    // pages that the keys of a tile's columns touch at most
     int64_t pages = s.max_pages;
-    if (window > 0) pages = min(pages, ((int64_t)window + (causal ? 16 / p.g + 1 : s.max_rows) + KV8_PAGE - 2) / KV8_PAGE + 1);
+    if (window > 0)
+        pages = min(pages, ((int64_t)window + (causal ? p.cols / p.g + 1 : s.max_rows) + KV8_PAGE - 2) / KV8_PAGE + 1);
     for (;; pps *= 2) {
         p.splits = (int)max((int64_t)1, (pages + pps - 1) / pps);
         if (p.splits == 1 || (size_t)s.n_rows * heads * p.splits * (c.dp + 2) <= ws_floats) break;
@@ -802,36 +883,33 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window,
     return p;
 }
 
-// Columns of a prompt wave, / 16: heads of 128 share V's conversion over 32
-// (bfloat16, 20 heads: 4096 rows 238 -> 147 us; 131 to 512 rows 36 -> 31), narrower
-// ones gain more from twice the waves (64 wide: 92 and 96, 20 -> 17; 32 wide 80
-// and 79, 17 -> 15).
-template <int DP> constexpr int prompt_tiles() { return DP == 128 ? 2 : 1; }
-
 template <int DP, class T>
 hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t ws_floats, hipStream_t st) {
     constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
-    constexpr int CT = prompt_tiles<DP>();
-    const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, ws_floats);
-    if (p.prompt && !step) {
-        const int64_t tiles = ((int64_t)a.s.max_rows * p.g + 64 * CT - 1) / (64 * CT);
-        const int64_t blocks = tiles * a.s.n_seq * a.c.hk;
-        if (!kv8_grid(blocks, 256)) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(blocks), dim3(256), 0, st, a, p.g, (int)tiles);
-        return hipGetLastError();
-    }
+    constexpr int CT = prompt_tiles(DP);
+    const Plan p = plan(a.c, a.s, a.heads, full, a.causal, a.window, step != nullptr, ws_floats);
     const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;  // of the join
     if (!kv8_grid(p.blocks, 256) || (p.splits > 1 && !kv8_grid(rows, 64 * JOIN_WAVES))) return hipErrorInvalidValue;
     if constexpr (full)
         if (step)
             hipLaunchKernelGGL((k_kv8_attend<DP, 3, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                                p.splits, p.pps, ws, *step);
-    if (!step)
+    if (!step && p.prompt)
+        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
+                           p.splits, p.pps, ws);
+    else if (!step)
         hipLaunchKernelGGL((k_kv8_attend<DP, full ? 3 : 2, T, 4, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g,
                            p.tiles, p.splits, p.pps, ws, NoStep{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
-    hipLaunchKernelGGL((k_kv8_join<DP, T>), dim3(rows), dim3(64 * JOIN_WAVES), 0, st, a, p.g, p.splits, p.pps, ws);
+    // A wave a row where the rows fill the GPU or the splits are few (20 heads of 64, 1024 rows
+    // in three splits: 76 us, by four waves 104), else four (128 rows of heads, 16 splits: 26.9, by one 28.6).
+    if (p.splits <= 8 || rows >= 8192)
+        hipLaunchKernelGGL((k_kv8_join<DP, T, 1>), dim3((rows + JOIN_WAVES - 1) / JOIN_WAVES), dim3(64 * JOIN_WAVES), 0, st, a,
+                           p.g, p.cols, p.splits, p.pps, ws);
+    else
+        hipLaunchKernelGGL((k_kv8_join<DP, T, JOIN_WAVES>), dim3(rows), dim3(64 * JOIN_WAVES), 0, st, a, p.g, p.cols,
+                           p.splits, p.pps, ws);
     return hipGetLastError();
 }
 
@@ -850,8 +928,8 @@ hipError_t launch_dims(const Kv8Attention &a, const Kv8Step *step, float *ws, si
 
 size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads) {
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return 0;
-    // a window leaves fewer pages at as many pages a split: what is enough without one is enough
-    const Plan p = plan(c, s, heads, 1, 0, SIZE_MAX);
+    // a window leaves fewer pages at as many pages a split, and 16-bit rows are split less
+    const Plan p = plan(c, s, heads, true, 1, 0, false, SIZE_MAX);
     return p.splits == 1 ? 0 : (size_t)s.n_rows * heads * p.splits * (c.dp + 2);
 }
 

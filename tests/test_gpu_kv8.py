@@ -294,6 +294,29 @@ def test_the_sizes_choose_the_prompt_kernel(hip):
     run_attention(hip, rng, lens, [max(n - 5 * i, 1) for i, n in enumerate(lens)], 8, 1, 32, "bfloat16", layout="heads")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("d,hk,g", [(16, 2, 1), (24, 2, 2), (64, 1, 4), (128, 1, 3)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 900), (False, 1500)])
+def test_prompts_over_split_keys(hip, kernel, dtype, d, hk, g, causal, window):
+    """Chunks of rows over long keys, which are split and joined: splits that a sequence is too short for, that the
+    window hides, with bad tokens and missing pages in them."""
+    rng = np.random.default_rng(16 + d)
+
+    def change(c, table):
+        c.bad[table[0, 30], 0] = np.uint64(1 << 9)    # token 1929 of sequence 0, head 0
+        table[2, 17:19] = -1                          # 1088 .. 1215 of sequence 2
+        c.scales[table[2, 30:34], :, 1] *= 2.0 ** -12  # a split whose values are far below the others'
+
+    run_attention(hip, rng, [2111, 70, 3000, 1], [85, 70, 40, 1], hk, g, d, dtype, causal, window, change=change, layout="heads")
+
+
+def test_the_sizes_choose_split_prompts(hip):
+    rng = np.random.default_rng(17)
+    for dtype in ("float32", "bfloat16"):
+        run_attention(hip, rng, [2500], [100], 2, 1, 64, dtype)
+        run_attention(hip, rng, [2100, 2500], [30, 33], 1, 4, 128, dtype, layout="heads")
+
+
 # ---- append and read ---------------------------------------------------------
 
 def append_ref(c, table, start, k, v):
