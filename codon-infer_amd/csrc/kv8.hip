@@ -6,6 +6,10 @@
 //   s = max(s_old where tokens are kept, max |new| / 127)
 //   kept codes  q <- rint(q s_old / s)   only where s grew
 //   new codes   q  = rint(x / s)
+//
+// Bound by the rows' bytes for many of them: 12,300 bfloat16 rows of 32 + 8 heads of
+// 128, append 70 us (4.3 TB/s with the rotated queries) and read 19 us; by latency for
+// few: one FP32 row of 8 sequences, 20 heads of 64, 6.1 and 4.5 us.
 #include <float.h>
 
 #include "kv8.h"
@@ -209,7 +213,7 @@ template <class T> __device__ __forceinline__ void store_chunk(T *p, const float
 // that hold VL whole pairs (neighbouring ones, or half the rotated dims apart).  V:
 // a thread takes one piece of four tokens, whose codes of a dim are one word
 // of the page.  Bound by the rows' bytes; NT = 64 for at most 4 rows a
-// sequence, where a page's 256 threads would mostly idle.
+// sequence, where a page's 256 threads would mostly idle (8 rows of 20 heads of 64: 6.1 us).
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, RowsView k, RowsView v, RowsView q,
                                                        RowsView qo, int g, int per_seq, RopeArg rope) {

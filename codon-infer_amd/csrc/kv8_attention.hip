@@ -12,16 +12,24 @@
 // of the group) pairs that share the kv head; row i of key tile t is key (i / 4)
 // 16 + 4 t + i % 4 of the page, so a lane's 16 scores are those of 16
 // consecutive keys, l / 16 * 16 .., of column l % 16, which is its share of the
-// second operand of O^T = V^T P^T, for int8 and for f16.
+// second operand of O^T = V^T P^T, for int8 and for f16: the weights never leave
+// their lane.
 //
 // k_kv8_attend (few columns: single tokens).  Keys are split over waves and
 // workgroups.  The weights are bytes as well, three for FP32 rows and two for
-// 16-bit ones, P = 127 256^2 (127 256) at the largest of the page: p v is exact, and each page joins the running output
-// with exp(max of the page - running max) times its V scale in FP32.
+// 16-bit ones, P = 127 256^2 (127 256) at the largest of the page: p v is exact,
+// and each page joins the running output with exp(max of the page - running max)
+// times its V scale in FP32.  Bound by reading the codes once: 64 sequences of
+// 1025 to 7500 tokens, 32 heads over 8 of 128, bfloat16, 143 us (4.2 TB/s); one
+// of 65003, 40 heads of 64, float16, 70 us (4.75 TB/s, what a copy reaches).
+// One page of 20 heads of 16 takes 4 us, all latency.
 //
-// k_kv8_prompt (many columns).  V's codes become f16, once for 32 columns, and
-// the weights f16 (FP32 rows: two f16, hi + lo), so that the matrix
-// instruction adds to the running output itself.
+// k_kv8_prompt (many columns).  V's codes become f16 and the weights f16 (FP32
+// rows: two f16, hi + lo), so that the matrix instruction adds to the running
+// output itself.  Bound by instruction issue, the exponentials, the weights'
+// conversions and V's (VALU 62% busy, matrix instructions 30%): 2047 rows of 16000 keys, 32
+// heads over 8 of 128, bfloat16, 655 us (767 TFLOP/s); 131 to 512 rows of 8
+// sequences, 20 heads of 64, FP32, 22 us.
 #include <float.h>
 #include <stdlib.h>
 #include <string.h>
@@ -337,7 +345,7 @@ __device__ __forceinline__ Kv8Own step_append(const Kv8View &c, int id, int h, i
 }
 
 // One workgroup of W waves per (sequence, kv head, 16 columns, split of the
-// pages); its waves take the split's pages in turn and join their sums at the
+// pages): with four waves a page's latency (1 us) is paid for four pages at once.  Its waves take the split's pages in turn and join their sums at the
 // end.  splits > 1: unnormalised results [row][head][split][DP + 2] in ws.
 //
 // STEP (a decoder's row a sequence, FP32, no shared heads): the rows come as
@@ -633,9 +641,8 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
     if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
-// Four waves of CT x 16 columns each, over all pages that these see, with PL f16
-// a weight.  The
-// running maximum follows only when a score exceeds it by 2^8, and the output's
+// Four waves of CT x 16 columns each, over the pages of a split that these see,
+// with PL f16 a weight.  The running maximum follows only when a score exceeds it by 2^8, and the output's
 // unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
 // 2^3 at the running maximum and have room for both.
 template <int DP, int PL, class T, int CT>
@@ -826,7 +833,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 }
 
 // Columns of a prompt wave, / 16: heads of 128 share V's conversion over 32
-// (bfloat16, 20 heads: 4096 rows 238 -> 147 us; 131 to 512 rows 36 -> 31), narrower
+// (20 heads, 4096 rows: bfloat16 238 -> 147 us, FP32 245 -> 215), narrower
 // ones gain more from twice the waves (64 wide: 92 and 96, 20 -> 17; 32 wide 80
 // and 79, 17 -> 15).
 constexpr int prompt_tiles(int dp) { return dp == 128 ? 2 : 1; }

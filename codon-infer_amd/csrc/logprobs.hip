@@ -3,7 +3,9 @@
 // One pass over a row with the running maximum m: u = (x - m) log2 e, s = sum
 // 2^u, t = sum 2^u u; then
 //   log p(i) = x_i - m - ln 2 log2 s,  entropy = ln 2 (log2 s - t / s).
-// A NaN or +inf anywhere makes s NaN.  Bound by reading the logits once.
+// A NaN or +inf anywhere makes s NaN.  Bound by reading the logits once, and close
+// to it by the seven operations a logit: 512 rows of 131072 bfloat16 logits, 20 alternatives, 38
+// us (3.5 TB/s, VALU 59% busy); 8192 rows of 33, 7.6 us, mostly latency.
 #include <limits.h>
 
 #include <algorithm>
