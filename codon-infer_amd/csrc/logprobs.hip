@@ -4,8 +4,8 @@
 // 2^u, t = sum 2^u u; then
 //   log p(i) = x_i - m - ln 2 log2 s,  entropy = ln 2 (log2 s - t / s).
 // A NaN or +inf anywhere makes s NaN.  Bound by reading the logits once, and close
-// to it by the seven operations a logit: 512 rows of 131072 bfloat16 logits, 20 alternatives, 38
-// us (3.5 TB/s, VALU 59% busy); 8192 rows of 33, 7.6 us, mostly latency.
+// to it by the seven operations a logit: 512 rows of 131072 bfloat16 logits 26 us without
+// alternatives, 31 with 20 (4.3 TB/s), 40 with 64; 8192 rows of 33, 7.6 us, mostly latency.
 #include <limits.h>
 
 #include <algorithm>
@@ -37,6 +37,12 @@ template <class OP> __device__ __forceinline__ float wave_all(float v, OP op) {
     v = op(v, dpp_or<0x4E, 0xf>(v, v));
     v = op(v, dpp_or<0xB1, 0xf>(v, v));
     return v;
+}
+// the same of integers
+template <class OP> __device__ __forceinline__ unsigned wave_bits(unsigned v, OP op) {
+    return __builtin_amdgcn_readfirstlane((int)__float_as_uint(wave_all(__uint_as_float(v), [&](float a, float b) {
+        return __uint_as_float(op(__float_as_uint(a), __float_as_uint(b)));
+    })));
 }
 __device__ __forceinline__ float wave_max(float v) {
     return wave_all(v, [](float a, float b) { return fmaxf(a, b); });
@@ -139,25 +145,70 @@ template <class T> struct Vec {
 };
 
 // Logits of a thread in a tile, in 16-byte loads: 16 leave registers for 16
-// waves a CU (512 rows of 131072 bfloat16 logits: 42.4 us, with 32 logits 43.6, with 8 47.8).
+// waves a CU (512 rows of 131072 bfloat16 logits, with an earlier choice of the alternatives:
+// 42.4 us, with 32 logits 43.6, with 8 47.8).
 constexpr int LP_EACH = 16;
 constexpr int LP_CAP = 768;  // list entries
+
+// A key that between top and top + LP_SLACK of a wave's keys reach (1 where no
+// more than that are above 0), bit by bit from the highest in which they differ: a ballot
+// for each step and key.  Keys above 0 are distinct.
+constexpr int LP_SLACK = 8;
+template <int K> __device__ __forceinline__ u64 top_bound(const u64 (&key)[K], int top) {
+    auto reach = [&](u64 t) __attribute__((always_inline)) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < K; i++) n += __popcll(__ballot(key[i] >= t));
+        return n;
+    };
+    if (reach(1) <= top + LP_SLACK) return 1;
+    u64 any = 0, all = ~0ull;  // of the keys above 0
+#pragma unroll
+    for (int i = 0; i < K; i++) {
+        any |= key[i];
+        all &= key[i] ? key[i] : ~0ull;
+    }
+    unsigned lo[2] = {(unsigned)(any >> 32), (unsigned)any}, hi[2] = {(unsigned)(all >> 32), (unsigned)all};
+    u64 t = 0;
+    int b = -1;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        const unsigned o = wave_bits(lo[h], [](unsigned x, unsigned y) { return x | y; });
+        const unsigned a = wave_bits(hi[h], [](unsigned x, unsigned y) { return x & y; });
+        if (b < 0) {
+            t |= (u64)(o & a) << (32 - 32 * h);
+            if (o != a) {
+                b = 63 - 32 * h - __builtin_clz(o ^ a);
+                t = t >> (b + 1) << (b + 1);
+            }
+        }
+    }
+    for (; b >= 0; b--) {
+        const u64 up = t | 1ull << b;
+        const int n = reach(up);
+        if (n >= top) {
+            t = up;
+            if (n <= top + LP_SLACK) break;
+        }
+    }
+    return t;
+}
 
 // The row (or the chunk blockIdx % chunks of its tiles) by NT threads.
 //
 // Alternatives.  In the pass a thread keeps only its largest logit and the
 // 16-byte vector it came from.  Vectors are numbered in the logits' order, so
-// (logit, vector) orders the threads' bests as the logits are ordered: the
-// top_k-th of them, `least`, is a bound that the row's top_k reach, and they all
-// are among the vectors of the top_k threads that reach it.  Those threads' vectors
-// (top_k / NT of the row, in L2 by then) are read again, and what reaches `least`
-// goes to a list, about top_k logits.
+// (logit, vector) orders the threads' bests as the logits are ordered: what top_k
+// of them reach, `least`, the row's top_k reach as well, and they all are among the vectors of the
+// threads that reach it.  Those threads' vectors (some top_k / NT of the row, in L2 by then) are
+// read again, and what reaches `least` goes to a list, about top_k logits.
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void k_logprobs(TokenLogprobs a, int chunks, int tiles_per, float *__restrict__ ws) {
     constexpr int VL = Vec<T>::N, LP_VECS = LP_EACH / VL, TILE = NT * LP_EACH, NW = NT / 64;
     static_assert(64 * VL + LOGPROBS_MAX_TOP <= LP_CAP && NW * LOGPROBS_MAX_TOP <= LP_CAP, "the list holds a wave's vectors");
     __shared__ u64 list[LP_CAP], best[LOGPROBS_MAX_TOP];
-    __shared__ int ranks[LP_CAP], owner[LOGPROBS_MAX_TOP], iw[NW], s_cnt;
+    __shared__ int ranks[LP_CAP], owner[LOGPROBS_MAX_TOP + LP_SLACK], iw[NW], s_cnt, s_owners;
+    __shared__ u64 s_least;
     __shared__ float sw[NW][3];
     const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -272,63 +323,86 @@ __global__ __launch_bounds__(NT) void k_logprobs(TokenLogprobs a, int chunks, in
             for (int w = 0; w < NW; w++) n += iw[w];
             return n;
         };
-        // each wave's best threads, then the best of these
         const u64 mine = most == -INFINITY ? 0 : (u64)order32(most) << 32 | (0xffffffffu - (unsigned)(from * NT + tid));
-        int rank = 0;
-#pragma unroll 4
-        for (int j = 0; j < 64; j++) {
-            const u64 o = (u64)(unsigned)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 |
-                          (unsigned)__builtin_amdgcn_readlane((int)mine, j);
-            rank += o > mine ? 1 : 0;
-        }
-        if (tid == 0) s_cnt = 0;
-        __syncthreads();
-        if (mine != 0 && rank < top) list[atomicAdd(&s_cnt, 1)] = mine;
-        __syncthreads();
-        cur = s_cnt;
-        sort_list();
-        const int owners = cur;
-        const u64 least = owners > 0 ? best[owners - 1] : ~0ull;  // fewer than top_k: all that is finite counts
-        if (tid < owners) owner[tid] = (int)((0xffffffffu - (unsigned)best[tid]) % NT);
-        cur = 0;
-        bar = 0;
-        if (tid == 0) s_cnt = 0;
-        __syncthreads();
-        const int vecs = ((end - begin) + NT * VL - 1) / (NT * VL);  // of a thread
-        for (int w0 = 0; w0 < owners * vecs; w0 += NT) {
-            const int w = w0 + tid, f = w / vecs, s = w - f * vecs;
-            const int n = f < owners ? s * NT + owner[f] : 0, i = begin + n * VL;  // vector, its first logit
-            float x[VL];
-            if (f < owners && i + VL <= end) {
-                const typename Vec<T>::type q = *reinterpret_cast<const typename Vec<T>::type *>(p + i);
+        if constexpr (NW > 1) {
+            list[tid] = mine;
+            __syncthreads();
+            if (wave == 0) {
+                u64 keys[NW];
 #pragma unroll
-                for (int e = 0; e < VL; e++) x[e] = to_f32(q[e]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < VL; e++) x[e] = f < owners && i + e < end ? to_f32(p[i + e]) : -INFINITY;
+                for (int w = 0; w < NW; w++) keys[w] = list[w * 64 + lane];
+                const u64 t = top_bound(keys, top);
+                if (lane == 0) s_least = t;
             }
-            auto counts = [&](int e) __attribute__((always_inline)) {
-                const u64 coarse = (u64)order32(x[e]) << 32 | (0xffffffffu - (unsigned)n);
-                return x[e] > -INFINITY && (coarse >= least || owners < top) && place_key(x[e], i + e) > bar;
-            };
-            int c = 0;
+        } else {
+            const u64 keys[1] = {mine}, t = top_bound(keys, top);
+            if (lane == 0) s_least = t;
+        }
+        if (tid == 0) s_cnt = s_owners = 0;
+        __syncthreads();
+        const u64 least = s_least;
+        if (mine >= least) owner[atomicAdd(&s_owners, 1)] = tid;
+        __syncthreads();
+        const int owners = s_owners;
+        const int vecs = ((end - begin) + NT * VL - 1) / (NT * VL);  // of a thread
+        // Item w: VL logits from i on, of which those from i0 on are of the owner's vector n (a row's last
+        // vector: its last VL logits; a row has more than 64).
+        auto fetch_item = [&](int w, int &n, int &i, int &i0) __attribute__((always_inline)) {
+            const int f = w / vecs;
+            n = f < owners ? (w - f * vecs) * NT + owner[f] : 0;
+            i0 = f < owners ? begin + n * VL : INT_MAX;
+            i = min(f < owners ? i0 : begin, end - VL);
+            return *reinterpret_cast<const typename Vec<T>::type *>(p + i);
+        };
+        auto reaches = [&](float x, int n) __attribute__((always_inline)) {
+            return x > -INFINITY && ((u64)order32(x) << 32 | (0xffffffffu - (unsigned)n)) >= least;
+        };
+        for (int w0 = 0; w0 < owners * vecs; w0 += 2 * NT) {
+            int n[2], i[2], i0[2];
+            typename Vec<T>::type x[2];
 #pragma unroll
-            for (int e = 0; e < VL; e++) c += counts(e) ? 1 : 0;
-            c = total(c);
-            auto push = [&]() __attribute__((always_inline)) {
+            for (int u = 0; u < 2; u++) x[u] = fetch_item(w0 + u * NT + tid, n[u], i[u], i0[u]);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int e = 0; e < VL; e++)
-                    if (counts(e)) list[atomicAdd(&s_cnt, 1)] = place_key(x[e], i + e);
-            };
-            if (cur + c <= LP_CAP) {
-                push();
-                cur += c;
-            } else {  // wave by wave, each after a cut
-                for (int y = 0; y < NW; y++) {
-                    sort_list();
-                    if (wave == y) push();
-                    __syncthreads();
-                    cur = s_cnt;
+                    if (i[u] + e >= i0[u] && reaches(to_f32(x[u][e]), n[u])) {
+                        const int at = atomicAdd(&s_cnt, 1);
+                        if (at < LP_CAP) list[at] = place_key(to_f32(x[u][e]), i[u] + e);
+                    }
+        }
+        __syncthreads();
+        cur = s_cnt;
+        if (cur > LP_CAP) {  // large logits side by side in the same threads: again, the list cut whenever it is full
+            __syncthreads();
+            cur = 0;
+            if (tid == 0) s_cnt = 0;
+            __syncthreads();
+            for (int w0 = 0; w0 < owners * vecs; w0 += NT) {
+                int n, i, i0;
+                const typename Vec<T>::type x = fetch_item(w0 + tid, n, i, i0);
+                auto counts = [&](int e) __attribute__((always_inline)) {
+                    return i + e >= i0 && reaches(to_f32(x[e]), n) && place_key(to_f32(x[e]), i + e) > bar;
+                };
+                int c = 0;
+#pragma unroll
+                for (int e = 0; e < VL; e++) c += counts(e) ? 1 : 0;
+                c = total(c);
+                auto push = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                    for (int e = 0; e < VL; e++)
+                        if (counts(e)) list[atomicAdd(&s_cnt, 1)] = place_key(to_f32(x[e]), i + e);
+                };
+                if (cur + c <= LP_CAP) {
+                    push();
+                    cur += c;
+                } else {  // wave by wave, each after a cut
+                    for (int y = 0; y < NW; y++) {
+                        sort_list();
+                        if (wave == y) push();
+                        __syncthreads();
+                        cur = s_cnt;
+                    }
                 }
             }
         }
@@ -393,16 +467,21 @@ template <class T> __global__ __launch_bounds__(JOIN_THREADS) void k_logprobs_jo
     for (int k = n + tid; k < top; k += JOIN_THREADS) store_top(a, row, k, -INFINITY, -1, st);
 }
 
-// Threads a row, chunks a row.
+// Threads a row, chunks a row (bfloat16, us).  A workgroup's joins cost about as much as
+// a thread's 64 logits, so a wave takes up to 4096 logits (4096 rows of 3000: 12, 256 threads 23)
+// and 256 threads up to 65536 (4096 rows of 30000: 51, a wave 67, 512 threads 66).  A
+// row is split where the rows leave CUs idle and it has 12 tiles or more, into
+// chunks of at least four (one row of 131072: 15.7, in four 12.7, in 16 14.8; 64 rows of 30000:
+// 10.3, in two 12.5; 200 rows of 131072: 18, in two 22).
 struct LpPlan {
     int nt, chunks, tiles_per;
 };
 LpPlan lp_plan(int n, int vocab, int top) {
     LpPlan p;
-    p.nt = vocab <= 2048 ? 64 : vocab <= 16384 ? 256 : 512;
+    p.nt = vocab <= 4096 ? 64 : vocab <= 65536 ? 256 : 512;
     const int tiles = (vocab + p.nt * LP_EACH - 1) / (p.nt * LP_EACH);
     const int most = top > 0 ? JOIN_MAX / top : 64;
-    p.chunks = n >= 512 ? 1 : std::min(std::min(tiles, most), (767 + n) / n);
+    p.chunks = tiles < 12 ? 1 : std::max(1, std::min(std::min(tiles / 4, most), 256 / n));
     p.tiles_per = (tiles + p.chunks - 1) / p.chunks;
     p.chunks = (tiles + p.tiles_per - 1) / p.tiles_per;
     return p;

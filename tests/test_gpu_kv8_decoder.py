@@ -307,7 +307,7 @@ def test_score(kv8):
 
 
 def test_score_large_vocabulary():
-    """Rows of 500,000 logits, which are split over 62 workgroups with 33 alternatives and over 32 with 64."""
+    """Rows of 500,000 logits, which are split over workgroups and joined, with as many alternatives as there may be."""
     cfg = ch.EsmConfig(64, 256, 1, 2, vocab_size=500_000)
     m = ch.GpuModel(cfg, ch.EsmWeights.random(cfg, seed=5, std=0.06, bias_std=0.02), max_batch=1, max_len=16)
     dec = ch.GpuDecoder(m, n_slots=1, max_len=64, max_rows=4, kv8=True)

@@ -61,6 +61,14 @@ def test_random(hip, dtype, n, vocab, k):
     run(hip, 3 * rng.standard_normal((n, vocab)), rng.integers(0, vocab, n), k, dtype)
 
 
+@pytest.mark.parametrize("n,vocab,k", [(3, 4096, 64), (70, 4095, 9), (2, 49153, 64), (90, 49999, 5), (2, 65536, 33),
+                                       (2, 65537, 64), (1, 98305, 64), (257, 98304, 2), (128, 131072, 20)])
+def test_around_the_sizes_that_choose(hip, n, vocab, k):
+    """Threads a row and chunks a row change between these."""
+    rng = np.random.default_rng(vocab + k)
+    run(hip, 3 * rng.standard_normal((n, vocab)), rng.integers(0, vocab, n), k, "bfloat16" if n % 2 else "float32")
+
+
 @pytest.mark.parametrize("vocab", [33, 60, 300, 5000, 20000, 70000])
 def test_ties(hip, vocab):
     """Equal logits: the lowest ids, also where every logit is the same."""
