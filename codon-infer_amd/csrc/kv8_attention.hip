@@ -455,9 +455,9 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         mp = groups_max(mp);
         if (mp == INFINITY) l = NAN;
         const float base = mp == -INFINITY ? 0.0f : mp;
-        // the page's weights as bytes, and their sum (exact)
+        // the page's weights as bytes; their sum before that rounding, which lse does not share
         i32x4 pl[PL];
-        unsigned sum = 0;
+        float sum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
             unsigned v[4];
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
             for (int r = 0; r < 4; r++) {
                 const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
                 v[r] = (unsigned)rintf(e * P);
-                sum += v[r];
+                sum += e;
                 v[r] += PL == 3 ? 0x8080 : 0x80;
             }
             if (PL == 3) {
@@ -484,10 +484,10 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         }
         const float mn = fmaxf(m, base == mp ? mp : m);
         const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float add = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn) * (1.0f / P);
-        l = fmaf(l, keep, (float)sum * add);
+        const float add = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn);
+        l = fmaf(l, keep, sum * add);
         m = mn;
-        const float av = add * sv;
+        const float av = add * (1.0f / P) * sv;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             i32x4 d[PL];
