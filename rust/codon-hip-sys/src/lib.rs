@@ -362,6 +362,30 @@ impl Decoder {
         Ok(Decoder { raw })
     }
 
+    /// Keys and values in 8 bits, in pages of 64 positions from a pool of `n_pages` (0: enough for every slot's
+    /// `max_len`); `rope` (None: the model's) may scale the positions.
+    pub fn new_kv8(model: &mut Model, n_slots: usize, max_len: usize, max_rows: usize, n_pages: usize,
+                   rope: Option<&cih_rope>) -> io::Result<Self> {
+        let mut raw = ptr::null_mut();
+        check(unsafe {
+            cih_decoder_create_kv8(model.raw, n_slots as i32, max_len as i32, max_rows as i32, n_pages as i32,
+                                   rope.map_or(ptr::null(), |r| r as *const cih_rope), &mut raw)
+        })?;
+        Ok(Decoder { raw })
+    }
+
+    /// One sequence of ids through slot 0: the log probability of the token after each (0 at the last) and the
+    /// entropy of its distribution.
+    pub fn score(&mut self, tokens: &[i32]) -> io::Result<(Vec<f32>, Vec<f32>)> {
+        let offs = [0i32, tokens.len() as i32];
+        let (mut logprob, mut entropy) = (vec![0f32; tokens.len()], vec![0f32; tokens.len()]);
+        check(unsafe {
+            cih_decoder_score(self.raw, 1, [0i32].as_ptr(), tokens.as_ptr(), offs.as_ptr(), 0, logprob.as_mut_ptr(),
+                              entropy.as_mut_ptr(), ptr::null_mut(), ptr::null_mut())
+        })?;
+        Ok((logprob, entropy))
+    }
+
     /// One stream: the prompt ids without the trailing `<eos>`; returns the
     /// generated ids and the prefill / generation times in ms.
     pub fn generate(&mut self, prompt: &[i32], temperature: f32, max_new_tokens: Option<usize>, seed: u64,
