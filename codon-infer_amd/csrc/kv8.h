@@ -33,6 +33,30 @@ struct RowsView {
     int64_t rs, hs;  // elements between rows, heads
 };
 
+// The largest v of the wave's lanes, in all of them, without LDS trips (permlane
+// swaps of lane halves, then DPP: lanes ^ 32, 16, 8, 4, 2, 1).
+template <int C, int BANK> __device__ __forceinline__ unsigned dpp_bits(unsigned old, unsigned v) {
+    return (unsigned)__builtin_amdgcn_update_dpp((int)old, (int)v, C, 0xf, BANK, false);
+}
+__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
+    unsigned w = v;
+    asm volatile("" : "+v"(w));  // a register of its own
+    const auto r = __builtin_amdgcn_permlane32_swap(v, w, false, false);
+    const unsigned r0 = r[0], r1 = r[1];
+    v = r0 > r1 ? r0 : r1;
+    w = v;
+    asm volatile("" : "+v"(w));
+    const auto t = __builtin_amdgcn_permlane16_swap(v, w, false, false);
+    const unsigned t0 = t[0], t1 = t[1];
+    v = t0 > t1 ? t0 : t1;
+    auto up = [&](unsigned o) { v = o > v ? o : v; };
+    up(dpp_bits<0x128, 0xf>(v, v));
+    up(dpp_bits<0x114, 0xa>(dpp_bits<0x104, 0x5>(v, v), v));
+    up(dpp_bits<0x4E, 0xf>(v, v));
+    up(dpp_bits<0xB1, 0xf>(v, v));
+    return v;
+}
+
 // Rotary positions by value in the kernel arguments: turns per position.
 struct RopeArg {
     int rot = 0, inter = 0;
@@ -69,12 +93,15 @@ __device__ __forceinline__ int kv8_page(const Kv8View &c, const Kv8Seq &q, int p
 // cos and sin (times gain) of position p's angle at pair j.  The angle in
 // turns is reduced in 64 bits: at position 1e6 a 32-bit product is off by
 // 0.06 radians.
-__device__ __forceinline__ void rope_cs(const RopeArg &r, int p, int j, float &c, float &s) {
-    const double a = (double)p * r.turns[j];
+__device__ __forceinline__ void turn_cs(double turns, float gain, int p, float &c, float &s) {
+    const double a = (double)p * turns;
     const float t = (float)(a - rint(a));
     sincospif(2.0f * t, &s, &c);
-    c *= r.gain;
-    s *= r.gain;
+    c *= gain;
+    s *= gain;
+}
+__device__ __forceinline__ void rope_cs(const RopeArg &r, int p, int j, float &c, float &s) {
+    turn_cs(r.turns[j], r.gain, p, c, s);
 }
 
 __device__ __forceinline__ int code8(float x, float inv) {
@@ -116,7 +143,9 @@ struct Kv8Attention {
 struct Kv8Step {
     const float *qkv = nullptr, *part = nullptr, *bias = nullptr;
     int splits = 0;
-    RopeArg rope;
+    int rot = 0, inter = 0;
+    float gain = 1.0f;
+    const double *turns = nullptr;  // device: of each pair (a lane's own of the kernel arguments came 3 us later)
 };
 hipError_t launch_kv8_step(const Kv8Attention &a, const Kv8Step &step, float *ws, size_t ws_floats, hipStream_t st);
 

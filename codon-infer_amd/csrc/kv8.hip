@@ -186,12 +186,6 @@ __device__ __forceinline__ unsigned pack4(const float (&x)[4], float inv) {
     return o;
 }
 __device__ __forceinline__ unsigned abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }  // NaN > inf > the rest
-__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
-    return v;
-}
-
 template <class T> struct Chunk {
     static constexpr int N = 16 / sizeof(T);
     typedef T type __attribute__((ext_vector_type(16 / sizeof(T))));

@@ -67,11 +67,6 @@ template <class OP> __device__ __forceinline__ float groups(float v, OP op) {
 __device__ __forceinline__ float groups_max(float v) {
     return groups(v, [](float a, float b) { return fmaxf(a, b); });
 }
-__device__ __forceinline__ unsigned wave_max_bits(unsigned v) {  // over all lanes
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, (unsigned)__shfl_xor((int)v, o));
-    return v;
-}
 __device__ __forceinline__ float groups_sum(float v) {
     return groups(v, [](float a, float b) { return a + b; });
 }
@@ -260,20 +255,31 @@ template <bool STEP> using StepArg = typename std::conditional<STEP, Kv8Step, No
 template <int DP, int W>
 __device__ __forceinline__ void step_row(const Kv8Attention &a, const Kv8Step &step, int r, int h, int pos, bool kv,
                                          float (&row)[3][DP]) {
-    const int hd = a.c.d, d = a.heads * hd, n = a.s.n_rows;
-    for (int t = threadIdx.x; t < (kv ? 3 : 1) * hd; t += 64 * W) {
-        const int which = t / hd, i = t - which * hd, col = which * d + h * hd + i;
-        float v;
-        if (step.part) v = fold_splits(step.part + (size_t)r * 3 * d + col, step.splits, (size_t)n * 3 * d) + step.bias[col];
-        else v = step.qkv[(size_t)r * 3 * d + col];
+    const int hd = a.c.d, d = a.heads * hd, n = a.s.n_rows, pairs = step.rot / 2, t = threadIdx.x;
+    float c = 1.0f, s = 0.0f;
+    if (t < pairs) turn_cs(step.turns[t], step.gain, pos, c, s);
+    for (int e = t; e < (kv ? 3 : 1) * hd; e += 64 * W) {
+        const int which = e / hd, i = e - which * hd, col = which * d + h * hd + i;
+        float v = 0.0f;
+        if (step.part) {  // (fold_splits, in less code: a launch reads it anew)
+            const float *p = step.part + (size_t)r * 3 * d + col;
+            const int64_t stride = (int64_t)n * 3 * d;
+            for (int s0 = 0; s0 < step.splits; s0 += 8) {
+                float x[8];
+#pragma unroll
+                for (int u = 0; u < 8; u++) x[u] = p[min(s0 + u, step.splits - 1) * stride];
+#pragma unroll
+                for (int u = 0; u < 8; u++) v += s0 + u < step.splits ? x[u] : 0.0f;
+            }
+            v += step.bias[col];
+        } else {
+            v = step.qkv[(size_t)r * 3 * d + col];
+        }
         row[which][i] = v;
     }
     __syncthreads();
-    const int pairs = step.rope.rot / 2, t = threadIdx.x;
     if (t < pairs) {
-        const int i0 = step.rope.inter ? 2 * t : t, i1 = step.rope.inter ? i0 + 1 : t + pairs;
-        float c, s;
-        rope_cs(step.rope, pos, t, c, s);
+        const int i0 = step.inter ? 2 * t : t, i1 = step.inter ? i0 + 1 : t + pairs;
         const float q0 = row[0][i0], q1 = row[0][i1];
         row[0][i0] = q0 * c - q1 * s;
         row[0][i1] = q1 * c + q0 * s;
@@ -286,26 +292,25 @@ __device__ __forceinline__ void step_row(const Kv8Attention &a, const Kv8Step &s
     __syncthreads();
 }
 
-// What a page's record is after a step's key and value went into it.
+// What a page's record is after a step's key and value went into it.  patch:
+// the kept codes stayed, so that a wave that has the page from before puts
+// the new codes in itself (from code[]) and no one waits for the stores.
 struct Kv8Own {
-    int pg;
+    int pg, lo;
+    bool patch;
     float2 sc;
     unsigned long long bad;
 };
-// Token `lo` of a page of one head, from rows in LDS (k_kv8_append's arithmetic).
+// Token `lo` of a page of one head, from rows in LDS (k_kv8_append's arithmetic); old, was_bad: the page's record.
 template <int DP, int W>
-__device__ __forceinline__ Kv8Own step_append(const Kv8View &c, int id, int h, int lo, const float (&k)[DP],
-                                              const float (&v)[DP]) {
-    Kv8Own o{-1, {0.0f, 0.0f}, 0};
+__device__ __forceinline__ Kv8Own step_append(const Kv8View &c, int id, int h, int lo, float2 old,
+                                              unsigned long long was_bad, const float (&k)[DP], const float (&v)[DP],
+                                              unsigned char (&code)[2][DP]) {
+    Kv8Own o{-1, lo, true, {0.0f, 0.0f}, 0};
     if (id < 0) return o;
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t ph = (int64_t)id * c.hk + h;
-    float2 old = {0.0f, 0.0f};
-    unsigned long long kept_bad = 0;
-    if (lo > 0) {
-        old = c.scales[ph];
-        kept_bad = c.bad[ph] & ((1ull << lo) - 1);
-    }
+    if (lo == 0) old = {0.0f, 0.0f};
     unsigned mk = 0, mv = 0;
     for (int i = lane; i < c.d; i += 64) {
         mk = max(mk, __float_as_uint(k[i]) & 0x7fffffffu);
@@ -315,16 +320,18 @@ __device__ __forceinline__ Kv8Own step_append(const Kv8View &c, int id, int h, i
     mv = wave_max_bits(mv);
     const bool lost = max(mk, mv) >= 0x7f800000u;
     o.sc = kv8_scales(lost ? 0 : mk, lost ? 0 : mv, old);
-    o.bad = kept_bad | (lost ? 1ull << lo : 0);
+    o.bad = (was_bad & ((1ull << lo) - 1)) | (lost ? 1ull << lo : 0);
     const float ik = o.sc.x > 0.0f && !lost ? 1.0f / o.sc.x : 0.0f, iv = o.sc.y > 0.0f && !lost ? 1.0f / o.sc.y : 0.0f;
     signed char *kc = c.k + ph * (KV8_PAGE * DP), *vc = c.v + ph * (KV8_PAGE * DP);
-    __syncthreads();  // every wave has the old record
-    if (tid == 0) {
-        c.scales[ph] = o.sc;
-        c.bad[ph] = o.bad;
+    const float rk = lo > 0 && o.sc.x > 0.0f ? old.x / o.sc.x : lo > 0 ? 0.0f : 1.0f;
+    const float rv = lo > 0 && o.sc.y > 0.0f ? old.y / o.sc.y : lo > 0 ? 0.0f : 1.0f;
+    o.patch = __builtin_amdgcn_readfirstlane(rk == 1.0f && rv == 1.0f);
+    for (int i = tid; i < 2 * DP; i += 64 * W) {
+        const int j = i % DP;
+        code[i / DP][j] = j < c.d && !lost ? code8(i < DP ? k[j] : v[j], i < DP ? ik : iv) : 0;
     }
-    if (lo > 0) {
-        const float rk = o.sc.x > 0.0f ? old.x / o.sc.x : 0.0f, rv = o.sc.y > 0.0f ? old.y / o.sc.y : 0.0f;
+    __syncthreads();  // every wave has the old record as well
+    if (!o.patch) {  // a scale grew
         if (rk != 1.0f)
             for (int e = tid; e < lo * DP / 4; e += 64 * W) {
                 unsigned *w = reinterpret_cast<unsigned *>(kc) + e;
@@ -336,12 +343,44 @@ __device__ __forceinline__ Kv8Own step_append(const Kv8View &c, int id, int h, i
                 unsigned *w = reinterpret_cast<unsigned *>(vc + e / words * KV8_PAGE) + e % words;
                 *w = recode4(*w, rv);
             }
-            __syncthreads();  // before the new codes, which share words with kept ones
         }
+        __syncthreads();  // before the new codes, which share words with kept ones
     }
-    for (int i = tid; i < DP; i += 64 * W) kc[lo * DP + i] = i < c.d && !lost ? code8(k[i], ik) : 0;
-    for (int i = tid; i < c.d; i += 64 * W) vc[i * KV8_PAGE + lo] = lost ? 0 : code8(v[i], iv);
+    if (tid == 0) {
+        c.scales[ph] = o.sc;
+        c.bad[ph] = o.bad;
+    }
+    for (int i = tid; i < DP; i += 64 * W) kc[lo * DP + i] = code[0][i];
+    for (int i = tid; i < c.d; i += 64 * W) vc[i * KV8_PAGE + lo] = code[1][i];
+    if (!o.patch) __syncthreads();  // the codes are written
     return o;
+}
+// The new key's codes in a tile that may not have them, and the new value's.
+template <int DP>
+__device__ __forceinline__ void patch_k(Tile<DP> &t, int lo, const unsigned char (&code)[DP], int lane) {
+    const int c = lane & 15, g4 = lane >> 4;
+    const bool mine = c == (lo >> 4) * 4 + (lo & 3);
+#pragma unroll
+    for (int s = 0; s < Tile<DP>::KS; s++) {
+        const i32x4 x = *reinterpret_cast<const i32x4 *>(&code[k_dim<DP>(g4) + s * 64]);
+#pragma unroll
+        for (int kt = 0; kt < 4; kt++)
+            if (kt == (lo >> 2 & 3))
+#pragma unroll
+                for (int w = 0; w < 4; w++) t.k[kt][s][w] = mine ? x[w] : t.k[kt][s][w];
+    }
+}
+template <int DP>
+__device__ __forceinline__ void patch_v(Tile<DP> &t, int lo, const unsigned char (&code)[DP], int lane) {
+    const int c = lane & 15, g4 = lane >> 4, at = 8 * (lo & 3);
+    const bool mine = g4 == lo >> 4;
+#pragma unroll
+    for (int dt = 0; dt < DP / 16; dt++) {
+        const unsigned x = (unsigned)code[dt * 16 + c] << at;
+#pragma unroll
+        for (int w = 0; w < 4; w++)
+            if (w == (lo >> 2 & 3)) t.v[dt][w] = mine ? (int)((t.v[dt][w] & ~(0xffu << at)) | x) : t.v[dt][w];
+    }
 }
 
 // One workgroup of W waves per (sequence, kv head, 16 columns, split of the
@@ -386,19 +425,28 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     float x[KS][16];
     Kv8Own own;
     own.pg = -1;
+    own.patch = false;
+    __shared__ __attribute__((aligned(16))) unsigned char code[2][DP];  // the own token's (STEP)
     if constexpr (STEP) {
         const int pos = q.start, mine = pos / KV8_PAGE;
         const bool writes = mine >= first && mine < last;
-        // pages that hold nothing new are on their way meanwhile
-        if (pg < last && pg != mine) load_k(t, a.c, id, kvh, lane);
+        // the pages and the own page's record are on their way meanwhile
+        if (pg < last) load_k(t, a.c, id, kvh, lane);
+        const int own_id = writes ? page_id(a.c, q, mine) : -1;
+        float2 old = {0.0f, 0.0f};
+        unsigned long long was_bad = 0;
+        if (own_id >= 0) {
+            const int64_t ph = (int64_t)own_id * a.c.hk + kvh;
+            old = a.c.scales[ph];
+            was_bad = a.c.bad[ph];
+        }
         __shared__ float row[3][DP];
         step_row<DP, W>(a, step, q.r0, kvh, pos, writes, row);
         if (writes) {
-            own = step_append<DP, W>(a.c, page_id(a.c, q, mine), kvh, pos % KV8_PAGE, row[1], row[2]);
+            own = step_append<DP, W>(a.c, own_id, kvh, pos % KV8_PAGE, old, was_bad, row[1], row[2], code);
             own.pg = mine;
-            __syncthreads();  // the codes are written
         }
-        if (pg < last && pg == mine) load_k(t, a.c, id, kvh, lane);
+        if (pg < last && pg == mine && !own.patch) load_k(t, a.c, id, kvh, lane);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -488,6 +536,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         l = fmaf(l, keep, sum * add);
         m = mn;
         const float av = add * (1.0f / P) * sv;
+        if (STEP && pg == own.pg && own.patch && !missing) patch_v(t, own.lo, code[1], lane);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             i32x4 d[PL];
@@ -507,6 +556,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
             t.sk = own.sc.x;
             t.sv = own.sc.y;
             t.bad = own.bad;
+            if (own.patch && id >= 0) patch_k(t, own.lo, code[0], lane);
         }
         load_v(t, a.c, id, kvh, lane);
         const int next = id_of(pg + W);
@@ -960,7 +1010,7 @@ hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, size_t ws_f
 hipError_t launch_kv8_step(const Kv8Attention &call, const Kv8Step &step, float *ws, size_t ws_floats, hipStream_t st) {
     if (call.s.n_rows == 0 || call.s.n_seq == 0) return hipSuccess;
     if (call.dtype != FT_F32 || call.heads != call.c.hk || call.s.max_rows != 1 || call.s.n_rows != call.s.n_seq ||
-        (step.part && (!step.bias || step.splits < 1)) || step.rope.rot > call.c.d)
+        (step.part && (!step.bias || step.splits < 1)) || step.rot > call.c.d || !step.turns)
         return hipErrorInvalidValue;
     Kv8Attention a = call;
     a.q16 = 0;
