@@ -32,7 +32,6 @@ struct DecoderKv8 {
     float *ws = nullptr;
     size_t ws_floats = 0;
     cih::RopeArg rope;
-    double *d_turns = nullptr;  // rope.turns on the device
     std::vector<int> free_pages;
     std::vector<std::vector<int>> pages;  // of each slot, in order
     std::vector<int> changed;             // slots whose row of the table has to be copied
@@ -132,7 +131,7 @@ int enqueue_kv8(cih_decoder *dc, int l, int n, int out_fmt, const float *part, i
     a.scale = 1.0f / std::sqrt((float)hd);
     a.causal = 1;
     if (dc->unique) {
-        const Kv8Step step{dc->qkv, part, bias, splits, kv.rope.rot, kv.rope.inter, kv.rope.gain, kv.d_turns};
+        const Kv8Step step{dc->qkv, part, bias, splits, kv.rope};
         HIPCHK(launch_kv8_step(a, step, kv.ws, kv.ws_floats, m->stream));
         return 0;
     }
@@ -582,7 +581,7 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
         good = dalloc(kv.view.k, cache, al) == hipSuccess && dalloc(kv.view.v, cache, al) == hipSuccess &&
                dalloc(kv.view.scales, ph, al) == hipSuccess && dalloc(kv.view.bad, ph, al) == hipSuccess &&
                dalloc(kv.d_table, (size_t)most, al) == hipSuccess && dalloc(kv.d_seq, 3 * R + 1, al) == hipSuccess &&
-               dalloc(kv.ws, kv.ws_floats, al) == hipSuccess && dalloc(kv.d_turns, 64, al) == hipSuccess &&
+               dalloc(kv.ws, kv.ws_floats, al) == hipSuccess &&
                hipHostMalloc((void **)&kv.h_table, (size_t)most * sizeof(int)) == hipSuccess &&
                hipHostMalloc((void **)&kv.h_seq, (3 * R + 1) * sizeof(int)) == hipSuccess;
         cache *= 2;
@@ -621,7 +620,6 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
     hipError_t e = hipSuccess;
     if (kv8) {
         e = hipMemcpy(dc->kv.d_table, dc->kv.h_table, (size_t)dc->kv.max_pages * n_slots * 4, hipMemcpyHostToDevice);
-        if (e == hipSuccess) e = hipMemcpy(dc->kv.d_turns, dc->kv.rope.turns, sizeof(dc->kv.rope.turns), hipMemcpyHostToDevice);
     } else {
         std::vector<float> c, s;
         rope_tables_host(max_len, m->hd, c, s);

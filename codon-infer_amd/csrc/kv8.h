@@ -93,15 +93,12 @@ __device__ __forceinline__ int kv8_page(const Kv8View &c, const Kv8Seq &q, int p
 // cos and sin (times gain) of position p's angle at pair j.  The angle in
 // turns is reduced in 64 bits: at position 1e6 a 32-bit product is off by
 // 0.06 radians.
-__device__ __forceinline__ void turn_cs(double turns, float gain, int p, float &c, float &s) {
-    const double a = (double)p * turns;
+__device__ __forceinline__ void rope_cs(const RopeArg &r, int p, int j, float &c, float &s) {
+    const double a = (double)p * r.turns[j];
     const float t = (float)(a - rint(a));
     sincospif(2.0f * t, &s, &c);
-    c *= gain;
-    s *= gain;
-}
-__device__ __forceinline__ void rope_cs(const RopeArg &r, int p, int j, float &c, float &s) {
-    turn_cs(r.turns[j], r.gain, p, c, s);
+    c *= r.gain;
+    s *= r.gain;
 }
 
 __device__ __forceinline__ int code8(float x, float inv) {
@@ -143,9 +140,7 @@ struct Kv8Attention {
 struct Kv8Step {
     const float *qkv = nullptr, *part = nullptr, *bias = nullptr;
     int splits = 0;
-    int rot = 0, inter = 0;
-    float gain = 1.0f;
-    const double *turns = nullptr;  // device: of each pair (a lane's own of the kernel arguments came 3 us later)
+    RopeArg rope;
 };
 hipError_t launch_kv8_step(const Kv8Attention &a, const Kv8Step &step, float *ws, size_t ws_floats, hipStream_t st);
 

@@ -255,9 +255,9 @@ template <bool STEP> using StepArg = typename std::conditional<STEP, Kv8Step, No
 template <int DP, int W>
 __device__ __forceinline__ void step_row(const Kv8Attention &a, const Kv8Step &step, int r, int h, int pos, bool kv,
                                          float (&row)[3][DP]) {
-    const int hd = a.c.d, d = a.heads * hd, n = a.s.n_rows, pairs = step.rot / 2, t = threadIdx.x;
+    const int hd = a.c.d, d = a.heads * hd, n = a.s.n_rows, pairs = step.rope.rot / 2, t = threadIdx.x;
     float c = 1.0f, s = 0.0f;
-    if (t < pairs) turn_cs(step.turns[t], step.gain, pos, c, s);
+    if (t < pairs) rope_cs(step.rope, pos, t, c, s);
     for (int e = t; e < (kv ? 3 : 1) * hd; e += 64 * W) {
         const int which = e / hd, i = e - which * hd, col = which * d + h * hd + i;
         float v = 0.0f;
@@ -279,7 +279,7 @@ __device__ __forceinline__ void step_row(const Kv8Attention &a, const Kv8Step &s
     }
     __syncthreads();
     if (t < pairs) {
-        const int i0 = step.inter ? 2 * t : t, i1 = step.inter ? i0 + 1 : t + pairs;
+        const int i0 = step.rope.inter ? 2 * t : t, i1 = step.rope.inter ? i0 + 1 : t + pairs;
         const float q0 = row[0][i0], q1 = row[0][i1];
         row[0][i0] = q0 * c - q1 * s;
         row[0][i1] = q1 * c + q0 * s;
@@ -1010,7 +1010,7 @@ hipError_t launch_kv8_attention(const Kv8Attention &call, float *ws, size_t ws_f
 hipError_t launch_kv8_step(const Kv8Attention &call, const Kv8Step &step, float *ws, size_t ws_floats, hipStream_t st) {
     if (call.s.n_rows == 0 || call.s.n_seq == 0) return hipSuccess;
     if (call.dtype != FT_F32 || call.heads != call.c.hk || call.s.max_rows != 1 || call.s.n_rows != call.s.n_seq ||
-        (step.part && (!step.bias || step.splits < 1)) || step.rot > call.c.d || !step.turns)
+        (step.part && (!step.bias || step.splits < 1)) || step.rope.rot > call.c.d)
         return hipErrorInvalidValue;
     Kv8Attention a = call;
     a.q16 = 0;
