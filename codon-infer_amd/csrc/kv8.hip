@@ -207,7 +207,8 @@ template <class T> __device__ __forceinline__ void store_chunk(T *p, const float
 // that hold VL whole pairs (neighbouring ones, or half the rotated dims apart).  V:
 // a thread takes one piece of four tokens, whose codes of a dim are one word
 // of the page.  Bound by the rows' bytes; NT = 64 for at most 4 rows a
-// sequence, where a page's 256 threads would mostly idle (8 rows of 20 heads of 64: 6.1 us).
+// sequence, where a page's 256 threads would mostly idle (a row each of 512 sequences, 20 heads of 64: append
+// and read 85 us, with 256 threads 118; of 8 sequences no difference).
 template <class T, int NT>
 __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, RowsView k, RowsView v, RowsView q,
                                                        RowsView qo, int g, int per_seq, RopeArg rope) {
@@ -560,7 +561,7 @@ hipError_t launch_append(const Kv8View &c, const Kv8Seqs &s, const RowsView &k, 
     constexpr int VL = Chunk<T>::N;
     // In 16-byte pieces where the rows are aligned to them and a pair's halves
     // lie in the same two pieces: 12,300 bfloat16 rows of 32 + 8 heads of 128,
-    // half of them rotated, 223 us value by value.
+    // half of them rotated, 70 us, value by value 223.
     const bool vec = pieces(k, sizeof(T)) && pieces(v, sizeof(T)) && pieces(q, sizeof(T)) && pieces(qo, sizeof(T)) &&
                      c.d % (2 * VL) == 0 && rope.rot % (2 * VL) == 0;
     if (vec && s.max_rows <= 4)

@@ -390,8 +390,10 @@ __device__ __forceinline__ void patch_v(Tile<DP> &t, int lo, const unsigned char
 // STEP (a decoder's row a sequence, FP32, no shared heads): the rows come as
 // Q | K | V, or as the partial sums of their projection; the workgroup rotates its
 // head's query, and the one that has the row's own page quantizes its key and value
-// into it (as k_kv8_append) before it reads the page.  The page's scales and codes
-// have no other reader in the launch.
+// into it as k_kv8_append does: while the page's scale stays, the waves patch the
+// new codes into the tile that they requested before, else they read the page anew.  The
+// page has no other reader in the launch.  650M, one row at position 280: 11.4 us (append
+// 2 and the projection's sums 1.5 of it), the attention alone 5.5.
 template <int DP, int PL, class T, int W, bool STEP>
 __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws, StepArg<STEP> step) {

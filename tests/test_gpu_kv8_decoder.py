@@ -218,6 +218,21 @@ def test_many_streams(hd, fmt):
     m.close()
 
 
+@pytest.mark.parametrize("hd,fmt", [(16, "q8"), (24, "q4"), (32, "fp32"), (64, "q8")])
+def test_steps_from_the_first_token(hd, fmt):
+    """A sequence token by token, through every place of a page and into the next, then again from the middle of it."""
+    cfg, w, m = make(hd, fmt, heads=8 if hd == 24 else 4)
+    W = dense_weights(cfg, w)
+    dec = ch.GpuDecoder(m, n_slots=2, max_len=130, max_rows=8, kv8=True)
+    t = tokens(140, 50 + hd)
+    for p in [*range(70), *range(45, 52)]:
+        got = dec.decode([1], [t[p]], [p])
+        ref = rows64(cfg, W, [t[p]], [p], held(dec, cfg, 1, p + 1))
+        assert np.abs(got[0] - ref[0]).max() <= TOL, p
+    dec.close()
+    m.close()
+
+
 @pytest.mark.parametrize("rows", [1, 12])
 def test_limb_overflow_runs_full_range(rows):
     """Steps and prompts whose activations overflow the f16 limbs run again in full range and write the same positions:
