@@ -15,7 +15,7 @@ size_t float_size(int dtype) { return dtype == CIH_F32 ? 4 : 2; }
 
 // A launch goes to the stream's device, the kernels to the current one.
 int check_stream(hipStream_t st) {
-    if (!st) return 0;
+    if (!st || st == hipStreamPerThread) return 0;  // the current device's
     int now = -1;
     hipDevice_t of = -1;
     HIPCHK(hipGetDevice(&now));

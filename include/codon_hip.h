@@ -296,10 +296,10 @@ int cih_rope_init(cih_rope *r, int32_t rot_dim, int32_t interleaved, double base
  * keeps at least their scale; where a new row exceeds it the kept codes are
  * rounded again to the larger one.  Later tokens of the page are forgotten.
  * With q (q_heads heads; NULL: none) the rows of q are written to q_out (may
- * be q), rotated by the same positions.  Two sequences of a batch must not
- * write the same page.  Rows without a position in the table (negative, or from
- * max_pages * 64 on) leave q_out as it was.  k, v and q_out must not overlap
- * each other. */
+ * be q; no overlap with k or v), rotated by the same positions; rows without a
+ * position in the table (negative, or from max_pages * 64 on) leave it as it
+ * was.  No page may be written twice in a batch, by two sequences or by one
+ * whose table names it twice. */
 int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
                    const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out, const cih_rope *rope,
                    void *stream);
@@ -313,13 +313,14 @@ int cih_kv8_read(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t
 /* Attention of the batch's rows over the cache: head h of q_heads (a multiple
  * of kv_heads) reads head h / (q_heads / kv_heads).  A row at position p sees
  * tokens j < lens[i], with causal only j <= p, with window > 0 only j > p -
- * window.  out = sum softmax(scale q.k) v in q's type; lse (NULL: none) [n_rows][q_heads] the
- * logarithm of the sum of exp(scale q.k).  A row that sees nothing gets out 0
- * and lse -inf, one that sees a bad token NaN.  out may be q
- * (with its strides).  Rows of very different counts, such as prompts beside
- * single tokens, are served better by a call each.  workspace: 16-byte aligned, of the size
+ * window.  out = sum softmax(scale q.k) v in q's type (may be q, with its
+ * strides); lse (NULL: none) [n_rows][q_heads] the logarithm of the sum of
+ * exp(scale q.k).  A row that sees nothing gets out 0 and lse -inf, one that
+ * sees a bad token NaN.  max_rows * q_heads / kv_heads <= 2^30.  Rows of very
+ * different counts, such as prompts beside single tokens, are served better by
+ * a call each.  workspace: 16-byte aligned, of the size
  * cih_kv8_attention_workspace gives for the same sizes (it reads no device
- * memory; max_rows * q_heads / kv_heads <= 2^30); calls that may run at the same time (other streams, two graphs)
+ * memory); calls that may run at the same time (other streams, two graphs)
  * need one each. */
 int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
                       const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal, int32_t window,
@@ -329,13 +330,14 @@ int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch 
 /* ---- log probabilities of given tokens ----------------------------------------
  * Beside log_softmax_canonical (lib.rs:4426-4441), over the whole vocabulary.
  * For each row of logits [n_rows][vocab] (both <= 2^30, type dtype, rows
- * row_stride elements apart): logprob = log softmax at targets[row]; entropy = -sum p log p (in
- * nats); the top_k <= 64 largest logits (ties: lowest id first) as top_ids
- * [n_rows][top_k] and their log probabilities top_logprobs.  logprob, entropy and the
- * top pair may each be NULL.  Device pointers, as above.  A negative target
- * gives 0, one >= vocab NaN.  -inf logits have probability 0: fewer than top_k
- * others leave ids -1 and -inf at the end.  A row of -inf only: entropy 0,
- * logprob -inf; a row with NaN or +inf: NaN and ids -1. */
+ * row_stride elements apart): logprob = log softmax at targets[row]; entropy =
+ * -sum p log p (in nats); the top_k <= 64 largest logits (ties: lowest id
+ * first) as top_ids [n_rows][top_k] and their log probabilities top_logprobs.
+ * logprob, entropy and the top pair may each be NULL.  Device pointers, as
+ * above.  A negative target gives 0, one >= vocab NaN.  -inf logits have
+ * probability 0: fewer than top_k others leave ids -1 and -inf at the end.  A
+ * row of -inf only: entropy 0, logprob -inf; a row with NaN or +inf: NaN and
+ * ids -1. */
 int cih_token_logprobs(int32_t dtype, const void *logits, int64_t row_stride, int32_t n_rows, int32_t vocab,
                        const int32_t *targets, float *logprob, float *entropy, int32_t top_k, int32_t *top_ids,
                        float *top_logprobs, void *workspace, size_t workspace_bytes, void *stream);

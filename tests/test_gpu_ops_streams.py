@@ -140,6 +140,19 @@ def test_two_streams_at_once(hip, streams, rows, lens, dtype):
         p.free()
 
 
+def test_the_threads_own_stream(hip):
+    a, b = (Program(hip, 7, PROMPT_ROWS, PROMPT_LENS) for _ in range(2))
+    for p in (a, b):
+        p.feed(PROMPT_LENS, 8)
+    hip.sync()
+    a.run(2)  # hipStreamPerThread
+    b.run()
+    hip.sync()
+    same(a.results(), b.results())
+    for p in (a, b):
+        p.free()
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
 @pytest.mark.parametrize("rows,lens", [(ROWS, LENS), (PROMPT_ROWS, PROMPT_LENS)], ids=["steps", "prompts"])
 def test_captured_and_replayed(hip, streams, rows, lens, dtype):
