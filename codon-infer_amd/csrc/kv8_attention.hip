@@ -26,10 +26,9 @@
 //
 // k_kv8_prompt (many columns).  V's codes become f16 and the weights f16 (FP32
 // rows: two f16, hi + lo), so that the matrix instruction adds to the running
-// output itself.  Bound by instruction issue, the exponentials, the weights'
-// conversions and V's (VALU 62% busy, matrix instructions 30%): 2047 rows of 16000 keys, 32
-// heads over 8 of 128, bfloat16, 655 us (767 TFLOP/s); 131 to 512 rows of 8
-// sequences, 20 heads of 64, FP32, 22 us.
+// output itself.  Bound by instruction issue, the exponentials and the weights'
+// conversions: 2047 rows of 16000 keys, 32 heads over 8 of 128, bfloat16, 567 us
+// (886 TFLOP/s); 131 to 512 rows of 8 sequences, 20 heads of 64, FP32, 22 us.
 #include <float.h>
 #include <stdlib.h>
 #include <string.h>
@@ -697,10 +696,16 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 // with PL f16 a weight.  The running maximum follows only when a score exceeds it by 2^8, and the output's
 // unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
 // 2^3 at the running maximum and have room for both.
+//
+// SHARE (heads of 128): a page's V becomes f16 once for the four waves, in LDS, a
+// page ahead.  Its conversion was a third of the instructions (2047 rows of 16000
+// keys 656 -> 570 us); at narrower heads, with fewer columns and less to convert, the waves' waiting for each
+// other costs as much (20 heads of 64: 2 x 512 rows 13.0, shared 14.8).
 template <int DP, int PL, class T, int CT>
 __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
+    constexpr bool SHARE = DP == 128;
     constexpr float SLACK = 8.0f, P0 = 3.0f, UNIT = 16.0f;
     // The last rows, which see most keys, go first, over all (sequence, kv head)
     // pairs (a pair after the other left the longest to a quarter of the CUs:
@@ -711,14 +716,24 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     const Kv8Seq q = kv8_seq(a.s, pair / a.c.hk);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g4 = lane >> 4;
-    const int f0 = (tile * 4 + wave) * CT * 16, f1 = min(f0 + CT * 16, q.n * g) - 1;  // columns of the wave
-    if (f0 > f1) return;
-    const Column c0 = column(a, q, kvh, g, f0), c1 = column(a, q, kvh, g, f1);
-    const int any0 = __builtin_amdgcn_readfirstlane(c0.begin), any1 = __builtin_amdgcn_readfirstlane(c1.end);
-    const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
-    const int pg0 = any0 / KV8_PAGE, np = (any1 + KV8_PAGE - 1) / KV8_PAGE - pg0;
-    const int first = pg0 + split * pps, last = pg0 + min(np, (split + 1) * pps);
+    // columns of the workgroup, and the pages of the split that they see
+    const int w0 = tile * 4 * CT * 16, w1 = min(w0 + 4 * CT * 16, q.n * g) - 1;
+    if (w0 > w1) return;
+    const int pg0 = column(a, q, kvh, g, w0).begin / KV8_PAGE;
+    const int np = (column(a, q, kvh, g, w1).end + KV8_PAGE - 1) / KV8_PAGE - pg0;
+    int first = __builtin_amdgcn_readfirstlane(pg0 + split * pps);
+    int last = __builtin_amdgcn_readfirstlane(pg0 + min(np, (split + 1) * pps));
     if (split > 0 && first >= last) return;  // the join knows
+    // columns of the wave (none: it only helps with V)
+    const int f0 = w0 + wave * CT * 16, f1 = min(f0 + CT * 16, q.n * g) - 1;
+    const Column c0 = column(a, q, kvh, g, f0), c1 = column(a, q, kvh, g, max(f0, f1));
+    const int any0 = __builtin_amdgcn_readfirstlane(c0.begin), any1 = __builtin_amdgcn_readfirstlane(f0 <= f1 ? c1.end : 0);
+    const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
+    if (!SHARE) {  // the wave's own pages
+        if (f0 > f1) return;
+        first = max(first, any0 / KV8_PAGE);
+        last = min(last, (any1 + KV8_PAGE - 1) / KV8_PAGE);
+    }
 
     constexpr int QB = PL + 1;  // bytes of a query
     i32x4 ql[CT][QB][KS];
@@ -740,7 +755,11 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     }
     float unit = 0.0f;  // o is in units of it (0: nothing added yet)
 
-    i32x4 kr[4][KS], vr[DT];
+    // SHARE: V's codes as f16, the operands of the page and of the next one; a wave converts a quarter
+    constexpr int VN = SHARE ? DT / 4 : DT;  // of the wave's loads of V
+    __shared__ f16x8 vs[SHARE ? 2 : 1][SHARE ? DT : 1][2][64];
+    const int dt0 = SHARE ? wave * VN : 0;
+    i32x4 kr[4][KS], vn[VN];
     float sk = 0.0f, sv = 0.0f, skn = 0.0f, svn = 0.0f;
     unsigned long long bad = 0, badn = 0;
     // the lane's offsets in a page: with the page's address in scalar registers a load takes one vector register
@@ -757,32 +776,62 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         svn = uniform(&a.c.scales[ph].y);
         badn = uniform(a.c.bad + ph);
     };
-    int id = first < last ? page_id(a.c, q, first) : -1;
-    if (first < last) load_k(id);
+    auto load_v = [&](int id) __attribute__((always_inline)) {
+        const page_ptr v = scalar_address(a.c.v + ((int64_t)max(id, 0) * a.c.hk + kvh) * (KV8_PAGE * DP));
+#pragma unroll
+        for (int n = 0; n < VN; n++) vn[n] = load16(v + voff + (dt0 + n) * 16 * KV8_PAGE);
+    };
+    auto operand = [&](int n, int h) __attribute__((always_inline)) {
+        return quants_f16<1>(qu32x2_t{(unsigned)vn[n][2 * h], (unsigned)vn[n][2 * h + 1]}, 0);
+    };
+    auto convert_v = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < VN; n++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) vs[at][dt0 + n][h][lane] = operand(n, h);
+    };
+    // LDS only: loads of K and V stay under way
+    auto barrier = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    // ids of the page and the next one, and the table's entry of the one after that
+    auto entry = [&](int pg) __attribute__((always_inline)) { return q.table && pg < last ? uniform(q.table + pg) : -1; };
+    auto valid = [&](int e) __attribute__((always_inline)) {
+        return __builtin_amdgcn_readfirstlane(e >= 0 && e < a.c.n_pages ? e : -1);
+    };
+    int id = valid(entry(first)), next = valid(entry(first + 1)), e2 = entry(first + 2);
+    if (first < last) {
+        load_k(id);
+        if (SHARE) {
+            load_v(id);
+            convert_v(0);
+            if (first + 1 < last) load_v(next);
+        }
+    }
+    if (SHARE) barrier();
     for (int pg = first; pg < last; pg++) {
+        const int at = SHARE ? (pg - first) & 1 : 0;
         sk = skn;
         sv = svn;
         bad = badn;
-        {
-            const page_ptr v = scalar_address(a.c.v + ((int64_t)max(id, 0) * a.c.hk + kvh) * (KV8_PAGE * DP));
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++) vr[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
+        const bool missing = id < 0;
+        const int j0 = pg * KV8_PAGE, next2 = valid(e2);
+        if (!SHARE) {
+            load_v(id);
+        } else if (pg + 1 < last) {
+            convert_v(at ^ 1);
+            if (pg + 2 < last) load_v(next2);
         }
+        e2 = entry(pg + 3);
+        if (!SHARE || (j0 + KV8_PAGE > any0 && j0 < any1)) {
         float s[CT][4][4];
 #pragma unroll
         for (int t = 0; t < CT; t++)
 #pragma unroll
             for (int kt = 0; kt < 4; kt++) score_tile<QB, KS>(kr[kt], ql[t], s[t][kt]);
-        const bool missing = id < 0;
-        if (pg + 1 < last) {
-            id = page_id(a.c, q, pg + 1);
-            load_k(id);
-        }
+        if (pg + 1 < last) load_k(next);
         if (!(sk >= 0.0f && sk <= FLT_MAX && sv >= 0.0f && sv <= FLT_MAX)) {
             bad = ~0ull;
             sk = sv = 0.0f;  // columns that do not see the page add nothing
         }
-        const int j0 = pg * KV8_PAGE;
         if (j0 < all0 || j0 + KV8_PAGE > all1 || bad || missing) {  // hidden keys
 #pragma unroll
             for (int t = 0; t < CT; t++) {
@@ -847,13 +896,19 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         for (int dt = 0; dt < DT; dt++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                const f16x8 v = quants_f16<1>(qu32x2_t{(unsigned)vr[dt][2 * h], (unsigned)vr[dt][2 * h + 1]}, 0);
+                const f16x8 v = SHARE ? vs[at][SHARE ? dt : 0][h][lane] : operand(SHARE ? 0 : dt, h);
 #pragma unroll
                 for (int t = 0; t < CT; t++)
 #pragma unroll
                     for (int n = 0; n < PL; n++)
                         o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[t][n][h], o[t][dt], 0, 0, 0);
             }
+        } else if (pg + 1 < last) {
+            load_k(next);
+        }
+        id = next;
+        next = next2;
+        if (SHARE && pg + 1 < last) barrier();
     }
 
 #pragma unroll
@@ -884,8 +939,8 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     }
 }
 
-// Columns of a prompt wave, / 16: heads of 128 share V's conversion over 32
-// (20 heads, 4096 rows: bfloat16 238 -> 147 us, FP32 245 -> 215), narrower
+// Columns of a prompt wave, / 16: heads of 128 share a wave's reads of V over 32
+// (20 heads, 4096 rows, before the waves shared its conversion: bfloat16 238 -> 147 us, FP32 245 -> 215), narrower
 // ones gain more from twice the waves (64 wide: 92 and 96, 20 -> 17; 32 wide 80
 // and 79, 17 -> 15).
 constexpr int prompt_tiles(int dp) { return dp == 128 ? 2 : 1; }
@@ -893,38 +948,35 @@ constexpr int prompt_tiles(int dp) { return dp == 128 ? 2 : 1; }
 // Which kernel, and how the pages of a sequence are split.
 struct Plan {
     bool prompt;
-    int g, tiles, splits, pps;  // tiles of cols columns (a workgroup of a prompt has four)
+    int g, tiles, splits, pps;  // tiles of cols columns, a workgroup's
     int cols;
     int64_t blocks;
 };
 // Prompts: k_kv8_prompt where the columns alone fill the GPU, or are more than
-// a workgroup's and the keys long enough to be split (us, FP32 rows, 20
-// heads of 64, the one kernel and the other: 2 sequences of 512 rows 18.8
-// and 13.1, 256 rows of 4096 keys 36.7 and 30.1, but 512 of 1024 16.9 and 19.8, 64 of
-// 1024 10.3 and 15.7).  Its pages are split until the workgroups are as many as
-// run at once (heads of 128: two a CU, and one does as well for 16-bit rows: bfloat16, 2
-// x 512 rows of 4096 keys, 32 over 8 heads, 98 unsplit, 117 in two; narrower heads four a
-// CU), not below 8 pages each (512 rows of 65536 keys, 32 over 8 heads of 128: FP32
-// 3082 unsplit, 1006; bfloat16 1420, 702), and only from 32 pages
-// on (1000 rows of 1000 keys: 18.1 unsplit, 29.8).
+// 64 and the keys long enough to be split (us, FP32 rows, 20 heads of 64, the one
+// kernel and the other: 2 sequences of 512 rows 18.7 and 13.4, 256 rows of 4096 keys
+// 36.7 and 30.4, but 512 of 1024 16.9 and 19.8, 64 of 1024 10.3 and 15.7).  Its
+// pages are split until the workgroups are as many as run at once (two a CU for heads of
+// 128, else four), not below 8 pages each (512 rows of 65536 keys, 32 over 8 heads
+// of 128: FP32 3082 unsplit, 867; bfloat16 1420, 608), and only from 32 pages on (1000
+// rows of 1000 keys: 18.1 unsplit, 29.8).
 //
 // Few columns: splits of 16 to 64 pages, a wave's 4 to 16, so that there are some
 // 2048 workgroups; shorter ones cost more in the join than they gain (8 single tokens of 700, 20
 // heads of 64: 8.4 us, with 8 pages 12.1), and from 4096 tiles on none is split.
-Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, bool full, int causal, int window, bool step, size_t ws_floats) {
+Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window, bool step, size_t ws_floats) {
     Plan p;
     p.g = heads / c.hk;
     const int64_t columns = (int64_t)s.max_rows * p.g, pairs = (int64_t)s.n_seq * c.hk;
     const bool fits = pairs * ((columns + 15) / 16) >= 1024, split = s.max_pages >= 32;
     const char *e = getenv("CIH_KV8_PROMPT");
     p.prompt = step ? false : e ? !strcmp(e, "1") : columns > 16 && (fits || (columns > 64 && split));
-    p.cols = p.prompt ? 16 * prompt_tiles(c.dp) : 16;
-    const int wg = p.prompt ? 4 * p.cols : p.cols;
-    p.tiles = (int)((columns + wg - 1) / wg);
+    p.cols = p.prompt ? 64 * prompt_tiles(c.dp) : 16;
+    p.tiles = (int)((columns + p.cols - 1) / p.cols);
     const int64_t tasks = pairs * p.tiles;
     int64_t pps = s.max_pages;
     if (p.prompt && split) {
-        const int64_t want = max((int64_t)1, (c.dp < 128 ? 1024 : full ? 512 : 256) / tasks);
+        const int64_t want = max((int64_t)1, (c.dp < 128 ? 1024 : 512) / tasks);
         pps = max((int64_t)8, (s.max_pages + want - 1) / want);
     } else if (!p.prompt && tasks < 4096) {
         pps = max((int64_t)16, min(s.max_pages * tasks / 2048, (int64_t)64));
@@ -946,7 +998,7 @@ template <int DP, class T>
 hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t ws_floats, hipStream_t st) {
     constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
     constexpr int CT = prompt_tiles(DP);
-    const Plan p = plan(a.c, a.s, a.heads, full, a.causal, a.window, step != nullptr, ws_floats);
+    const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, step != nullptr, ws_floats);
     const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;  // of the join
     if (!kv8_grid(p.blocks, 256) || (p.splits > 1 && !kv8_grid(rows, 64 * JOIN_WAVES))) return hipErrorInvalidValue;
     if constexpr (full)
@@ -987,8 +1039,8 @@ hipError_t launch_dims(const Kv8Attention &a, const Kv8Step *step, float *ws, si
 
 size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads) {
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return 0;
-    // a window leaves fewer pages at as many pages a split, and 16-bit rows are split less
-    const Plan p = plan(c, s, heads, true, 1, 0, false, SIZE_MAX);
+    // a window leaves fewer pages at as many pages a split: what is enough without one is enough
+    const Plan p = plan(c, s, heads, 1, 0, false, SIZE_MAX);
     return p.splits == 1 ? 0 : (size_t)s.n_rows * heads * p.splits * (c.dp + 2);
 }
 
