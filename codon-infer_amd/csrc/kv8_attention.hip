@@ -693,9 +693,12 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 }
 
 // Four waves of CT x 16 columns each, over the pages of a split that these see,
-// with PL f16 a weight.  The running maximum follows only when a score exceeds it by 2^8, and the output's
-// unit (a V scale) only when a page's differs by more than 2^4: f16 weights are
-// 2^3 at the running maximum and have room for both.
+// with PL f16 a weight.  A column's weights are 2^3 at its reference w, a score, and its
+// output is in units of 2^w 2^unit; w follows only when a score exceeds it by 2^8, unit (an
+// exponent) only when a page's V scale differs by more than 2^4: f16 weights have room for both.  unit
+// goes down as well as up, as far as what the column already holds leaves room in
+// FP32; V scales of the whole range of FP32 go together, and a
+// column is not touched by a page that it does not see.
 //
 // SHARE (heads of 128): a page's V becomes f16 once for the four waves, in LDS, a
 // page ahead.  Its conversion was a third of the instructions (2047 rows of 16000
@@ -706,7 +709,10 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr bool SHARE = DP == 128;
-    constexpr float SLACK = 8.0f, P0 = 3.0f, UNIT = 16.0f;
+    constexpr float SLACK = 8.0f, P0 = 3.0f;
+    constexpr int UNIT = 4;
+    constexpr float ROOM = 60.0f;  // of a column's sums above 2^w (2^w 2^unit): what adds less than 2^-60 of them may be lost
+    constexpr int NO_EXP = -4096;  // a page whose values are 0
     // The last rows, which see most keys, go first, over all (sequence, kv head)
     // pairs (a pair after the other left the longest to a quarter of the CUs:
     // prompts of 131 to 512 rows 28.4 -> 25.4 us; whole pairs to one XCD: no difference).
@@ -737,8 +743,9 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 
     constexpr int QB = PL + 1;  // bytes of a query
     i32x4 ql[CT][QB][KS];
-    float f[CT], m[CT], l[CT];
-    int begin[CT], end[CT];
+    float f[CT], w[CT], l[CT];
+    float top[CT], most[CT];  // the largest score, the largest score + exponent of its page's V scale
+    int begin[CT], end[CT], unit[CT];
     f32x4 o[CT][DT];
 #pragma unroll
     for (int t = 0; t < CT; t++) {
@@ -748,12 +755,13 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         f[t] = query_bytes<QB, KS>(x, a.scale, ql[t]);
         begin[t] = col.begin;
         end[t] = col.end;
-        m[t] = -INFINITY;
+        w[t] = -FLT_MAX;  // below every score
+        top[t] = most[t] = -INFINITY;
+        unit[t] = 0;
         l[t] = f[t] != f[t] ? NAN : 0.0f;  // a query that is not finite
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) o[t][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    float unit = 0.0f;  // o is in units of it (0: nothing added yet)
 
     // SHARE: V's codes as f16, the operands of the page and of the next one; a wave converts a quarter
     constexpr int VN = SHARE ? DT / 4 : DT;  // of the wave's loads of V
@@ -846,6 +854,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
             }
         }
         float fk[CT], x[CT];
+        const int ex = sv > 0.0f ? __builtin_amdgcn_frexp_expf(sv) : NO_EXP;
         bool move = false;
 #pragma unroll
         for (int t = 0; t < CT; t++) {
@@ -856,29 +865,34 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 #pragma unroll
                 for (int r = 0; r < 4; r++) x[t] = fmaxf(x[t], s[t][kt][r]);
             x[t] *= fk[t];
-            move |= x[t] > m[t] + SLACK;
+            move |= x[t] > w[t] + SLACK || (x[t] > -INFINITY && abs(ex - unit[t]) > UNIT);
         }
-        const float svu = sv > 0.0f ? sv : unit;  // a page of zeros fits any unit
-        move |= svu > unit * UNIT || svu * UNIT < unit;
         if (__any(move)) {
-            const float w = unit > 0.0f ? unit / svu : 0.0f;
-            unit = svu;
 #pragma unroll
             for (int t = 0; t < CT; t++) {
-                const float mn = fmaxf(m[t], groups_max(x[t]));
-                const float y = m[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[t] - mn), z = y * w;
-                m[t] = mn;
+                const float mp = groups_max(x[t]);
+                top[t] = fmaxf(top[t], mp);
+                most[t] = fmaxf(most[t], mp + (float)ex);
+                float wn = mp > w[t] + SLACK ? mp : w[t];
+                wn = fmaxf(wn, top[t] - ROOM);
+                const int un = max(ex, (int)fminf(fmaxf(most[t] - ROOM - wn, (float)NO_EXP), (float)-NO_EXP));
+                const bool seen = mp > -INFINITY;
+                const float d = seen ? w[t] - wn : 0.0f;
+                const float y = __builtin_amdgcn_exp2f(d), z = __builtin_amdgcn_exp2f(d + (float)(seen ? unit[t] - un : 0));
+                w[t] = seen ? wn : w[t];
+                unit[t] = seen ? un : unit[t];
                 l[t] *= y;
 #pragma unroll
                 for (int dt = 0; dt < DT; dt++) o[t][dt] *= z;
             }
         }
-        const float ratio = unit > 0.0f ? svu / unit : 1.0f;
-        const float up = P0 + __builtin_amdgcn_logf(ratio), down = __builtin_amdgcn_exp2f(-P0) / ratio;
+        const float up = P0 + (sv > 0.0f ? __builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(sv)) : 0.0f), down = __builtin_amdgcn_exp2f(-up);
         f16x8 p[CT][PL][2];
 #pragma unroll
         for (int t = 0; t < CT; t++) {
-            const float off = up - (m[t] == -INFINITY ? 0.0f : m[t]);
+            // (an exponent far below the unit: the weights are 0 in f16, their sum in FP32 is not)
+            const int rel = min(max(ex - unit[t], -40), UNIT);
+            const float off = up + (float)rel - w[t];
             float sum = 0.0f;
 #pragma unroll
             for (int kt = 0; kt < 4; kt++)
@@ -890,7 +904,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
                     p[t][0][kt / 2][kt % 2 * 4 + r] = hi;
                     if (PL == 2) p[t][PL - 1][kt / 2][kt % 2 * 4 + r] = (_Float16)(e - (float)hi);
                 }
-            l[t] = fmaf(sum, down, l[t]);
+            l[t] = fmaf(sum, ldexpf(down, -rel), l[t]);
         }
 #pragma unroll
         for (int dt = 0; dt < DT; dt++)
@@ -919,23 +933,27 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         if (col.row < 0) continue;
         if (splits > 1) {
             float *p = ws + (((int64_t)col.row * a.heads + col.head) * splits + split) * (DP + 2);
-            const float x = unit * __builtin_amdgcn_exp2f(-P0);
+            const float x = __builtin_amdgcn_exp2f(-P0);
 #pragma unroll
             for (int dt = 0; dt < DT; dt++)
 #pragma unroll
                 for (int r = 0; r < 4; r += 2)
-                    *reinterpret_cast<float2 *>(p + dt * 16 + g4 * 4 + r) = make_float2(o[t][dt][r] * x, o[t][dt][r + 1] * x);
-            if (g4 == 0) *reinterpret_cast<float2 *>(p + DP) = make_float2(m[t], sum);
+                    *reinterpret_cast<float2 *>(p + dt * 16 + g4 * 4 + r) =
+                        make_float2(ldexpf(o[t][dt][r] * x, unit[t]), ldexpf(o[t][dt][r + 1] * x, unit[t]));
+            if (g4 == 0) *reinterpret_cast<float2 *>(p + DP) = make_float2(w[t], sum);
             continue;
         }
-        const float x = unit / sum * __builtin_amdgcn_exp2f(-P0);
+        const float x = __builtin_amdgcn_exp2f(-P0) / sum;
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             const int i = dt * 16 + g4 * 4;
-            if (i < a.c.d) store_out4<T>(a, col.row, col.head, i, sum == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : o[t][dt] * x);
+            f32x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; r++) y[r] = sum == 0.0f ? 0.0f : ldexpf(o[t][dt][r] * x, unit[t]);
+            if (i < a.c.d) store_out4<T>(a, col.row, col.head, i, y);
         }
         if (g4 == 0 && a.lse)
-            a.lse[(int64_t)col.row * a.heads + col.head] = sum == 0.0f ? -INFINITY : (m[t] + log2f(sum)) * LN2;
+            a.lse[(int64_t)col.row * a.heads + col.head] = sum == 0.0f ? -INFINITY : (w[t] + log2f(sum)) * LN2;
     }
 }
 

@@ -1,0 +1,83 @@
+"""Attention over the 8-bit cache on the GPU, both kernels, within the bounds of
+tests/kv8_bounds.py: what the kernels' own roundings add to a row, and no more."""
+import numpy as np
+import pytest
+
+import codon_hip as ch
+import kv8_bounds as B
+import kv8_ref as R
+from codon_hip.devmem import DeviceArray, Hip
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    return Hip()
+
+
+def offsets(rows):
+    return np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
+
+
+def attend(hip, c, table, lens, rows, q, dtype, causal=True, window=0, scale=None):
+    """The call's out and lse as float64."""
+    n, h, d = q.shape
+    arr = [DeviceArray(hip, x) for x in (offsets(rows), np.asarray(lens, np.int32), table)]
+    qd, od = R.put(hip, q, dtype), R.put(hip, q * 0 + 7, dtype)
+    lse = DeviceArray(hip, np.full((n, h), 7, np.float32))
+    cache = c.upload()
+    b = ch.Kv8Batch(*arr, n, max(rows))
+    ws = DeviceArray(hip, np.full(cache.attend_workspace(b, h) + 16, 255, np.uint8))
+    kw = {} if scale is None else {"scale": scale}
+    cache.attend(b, qd, od, lse=lse, causal=causal, window=window, workspace=ws, **kw)
+    got = R.get(od), R.get(lse)
+    R.free(*arr, qd, od, lse, ws, *c.dev)
+    return got
+
+
+def check(hip, monkeypatch, kernel, c, table, lens, rows, q, dtype, causal=True, window=0, only=None, scale=None,
+          seqs=None, alike=False):
+    """One call against the bounds (only: rows of a sequence that are looked at; seqs: sequences)."""
+    monkeypatch.setenv("CIH_KV8_PROMPT", "1" if kernel == "prompt" else "0")
+    got, glse = attend(hip, c, table, lens, rows, q, dtype, causal, window, scale)
+    g = q.shape[1] // c.h
+    cu = offsets(rows)
+    for i, (n, r) in enumerate(zip(lens, rows)):
+        if seqs is not None and i not in seqs:
+            continue
+        at = np.arange(r) if only is None else np.unique(np.clip(only, 0, r - 1)) if r else np.arange(0)
+        ref, rlse, tol, ltol = B.attend(c, table[i], n, n - r + at, q[cu[i] + at], c.d ** -0.5 if scale is None else scale,
+                                        causal, window, g, dtype, kernel, alike)
+        mine, mlse = got[cu[i] + at], glse[cu[i] + at]
+        bad = ~(np.abs(mine - ref) <= tol)
+        assert not bad.any(), (i, np.argwhere(bad)[:4], mine[bad][:4], ref[bad][:4], tol[bad][:4], bad.mean())
+        fine = np.isfinite(rlse)
+        assert np.array_equal(mlse[~fine], rlse[~fine])
+        off = np.abs(mlse[fine] - rlse[fine])
+        assert (off <= ltol[fine]).all(), (i, (off - ltol[fine]).max())
+
+
+# ---- V scales of any size ----------------------------------------------------
+
+# three pages each: a fall, a rise, both, over most of what FP32 holds
+SCALES = [(1.0, 1e-36, 0.02), (1e34, 0.02, 1e-30), (1e-36, 1.0, 1e34), (0.02, 1e36, 1e-4), (1e-37, 1e-37, 1e36),
+          (2.6e36, 1e-37, 2.6e36)]
+
+
+def far_apart(hip, monkeypatch, kernel, g=1):
+    """Rows of which some see a page of other size and some do not: each keeps the precision of what it sees."""
+    rng = np.random.default_rng(31)
+    lens = [180] * len(SCALES)
+    c = R.Cache(hip, rng, 3 * len(SCALES), 1, 64)
+    table = R.tables(rng, lens, len(c.k))
+    for i, sv in enumerate(SCALES):
+        c.scales[table[i, :3], 0, 1] = sv
+    q = R.rounded(rng.standard_normal((180 * len(SCALES), g, 64)) * 0.5, "float32")
+    check(hip, monkeypatch, kernel, c, table, lens, lens, q, "float32",
+          only=[0, 1, 30, 62, 63, 64, 65, 66, 70, 90, 126, 127, 128, 129, 131, 150, 179])
+
+
+def test_prompts_over_v_scales_far_apart(hip, monkeypatch):
+    far_apart(hip, monkeypatch, "prompt")
+    far_apart(hip, monkeypatch, "prompt", g=3)
