@@ -25,8 +25,8 @@
 // One page of 20 heads of 16 takes 4 us, all latency.
 //
 // k_kv8_prompt (many columns).  V's codes become f16 and the weights f16 (FP32
-// rows: two f16, hi + lo), so that the matrix instruction adds to the running
-// output itself.  Bound by instruction issue, the exponentials and the weights'
+// rows: two f16, hi + lo); a page's sums join the running
+// output in FP32.  Bound by instruction issue, the exponentials and the weights'
 // conversions: 2047 rows of 16000 keys, 32 heads over 8 of 128, bfloat16, 567 us
 // (886 TFLOP/s); 131 to 512 rows of 8 sequences, 20 heads of 64, FP32, 22 us.
 #include <float.h>
@@ -906,17 +906,23 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
                 }
             l[t] = fmaf(sum, ldexpf(down, -rel), l[t]);
         }
+        // The page's sums by themselves, then added: as one chain over 60,000 keys the
+        // matrix instructions' roundings grow to 6e-5 of an output of one sign, this way to 1e-6.
 #pragma unroll
-        for (int dt = 0; dt < DT; dt++)
+        for (int dt = 0; dt < DT; dt++) {
+            const f16x8 v0 = SHARE ? vs[at][SHARE ? dt : 0][0][lane] : operand(SHARE ? 0 : dt, 0);
+            const f16x8 v1 = SHARE ? vs[at][SHARE ? dt : 0][1][lane] : operand(SHARE ? 0 : dt, 1);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const f16x8 v = SHARE ? vs[at][SHARE ? dt : 0][h][lane] : operand(SHARE ? 0 : dt, h);
+            for (int t = 0; t < CT; t++) {
+                f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int t = 0; t < CT; t++)
-#pragma unroll
-                    for (int n = 0; n < PL; n++)
-                        o[t][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[t][n][h], o[t][dt], 0, 0, 0);
+                for (int n = 0; n < PL; n++) {
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, p[t][n][0], d, 0, 0, 0);
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, p[t][n][1], d, 0, 0, 0);
+                }
+                o[t][dt] += d;
             }
+        }
         } else if (pg + 1 < last) {
             load_k(next);
         }

@@ -81,3 +81,19 @@ def far_apart(hip, monkeypatch, kernel, g=1):
 def test_prompts_over_v_scales_far_apart(hip, monkeypatch):
     far_apart(hip, monkeypatch, "prompt")
     far_apart(hip, monkeypatch, "prompt", g=3)
+
+
+# ---- long sums ---------------------------------------------------------------
+
+@pytest.mark.parametrize("kernel", ["few", "prompt"])
+@pytest.mark.parametrize("scale", [0.0, 0.05])
+def test_long_sums_of_one_sign(hip, monkeypatch, kernel, scale):
+    """Values of one sign under flat weights, the keys not split: roundings that all fall to one side add up."""
+    rng = np.random.default_rng(38)
+    n, d, hk, seqs = 30000, 16, 32, 32
+    c = R.Cache(hip, rng, 469, hk, d)
+    table = np.repeat(R.tables(rng, [n], 469), seqs, 0)
+    c.scales[:] = 0.02, 0.01
+    c.v[:] = rng.integers(60, 120, c.v.shape)
+    q = R.rounded(rng.standard_normal((17 * seqs, hk, d)), "float32")
+    check(hip, monkeypatch, kernel, c, table, [n] * seqs, [17] * seqs, q, "float32", scale=scale, only=[3], seqs=[0, 31])
