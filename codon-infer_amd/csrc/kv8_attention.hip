@@ -693,12 +693,14 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 }
 
 // Four waves of CT x 16 columns each, over the pages of a split that these see,
-// with PL f16 a weight.  A column's weights are 2^3 at its reference w, a score, and its
-// output is in units of 2^w 2^unit; w follows only when a score exceeds it by 2^8, unit (an
-// exponent) only when a page's V scale differs by more than 2^4: f16 weights have room for both.  unit
-// goes down as well as up, as far as what the column already holds leaves room in
-// FP32; V scales of the whole range of FP32 go together, and a
-// column is not touched by a page that it does not see.
+// with PL f16 a weight.  A column's weights are 2^8 at its reference w, a score, and its
+// output is in units of 2^w 2^unit.  w moves when a score exceeds it by 2^5, or when all of a page
+// that the column sees is more than 2^NEAR below it; unit (an exponent) when a page's V
+// scale is not within 2^2 of it: f16 weights have room for that, and what rounds to 0 among
+// them is below 2^(NEAR - 30) of the largest of its page (FP32 rows: 2^-26).  Both go down
+// as well as up, as far as what the column already holds leaves room in
+// FP32, so many small weights behind a large one keep their bits, V scales of the whole range of
+// FP32 go together, and a column is not touched by a page that it does not see.
 //
 // SHARE (heads of 128): a page's V becomes f16 once for the four waves, in LDS, a
 // page ahead.  Its conversion was a third of the instructions (2047 rows of 16000
@@ -709,8 +711,8 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr bool SHARE = DP == 128;
-    constexpr float SLACK = 8.0f, P0 = 3.0f;
-    constexpr int UNIT = 4;
+    constexpr float SLACK = 5.0f, P0 = 8.0f, NEAR = PL == 2 ? 4.0f : 8.0f;
+    constexpr int UNIT = 2;
     constexpr float ROOM = 60.0f;  // of a column's sums above 2^w (2^w 2^unit): what adds less than 2^-60 of them may be lost
     constexpr int NO_EXP = -4096;  // a page whose values are 0
     // The last rows, which see most keys, go first, over all (sequence, kv head)
@@ -798,6 +800,11 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 #pragma unroll
             for (int h = 0; h < 2; h++) vs[at][dt0 + n][h][lane] = operand(n, h);
     };
+    // of a ballot, which columns: column c is lanes c, c + 16, c + 32, c + 48
+    auto lanes = [](unsigned long long b) __attribute__((always_inline)) {
+        b |= b >> 32;
+        return (unsigned)(b | b >> 16) & 0xffff;
+    };
     // LDS only: loads of K and V stay under way
     auto barrier = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // ids of the page and the next one, and the table's entry of the one after that
@@ -855,7 +862,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         }
         float fk[CT], x[CT];
         const int ex = sv > 0.0f ? __builtin_amdgcn_frexp_expf(sv) : NO_EXP;
-        bool move = false;
+        unsigned over = 0, near[CT], all = 0xffff;  // columns above their reference, and those that the reference suits
 #pragma unroll
         for (int t = 0; t < CT; t++) {
             fk[t] = fmaxf(f[t] * sk, 0x1p-120f);  // above 0: what is hidden stays at -inf
@@ -865,15 +872,21 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
 #pragma unroll
                 for (int r = 0; r < 4; r++) x[t] = fmaxf(x[t], s[t][kt][r]);
             x[t] *= fk[t];
-            move |= x[t] > w[t] + SLACK || (x[t] > -INFINITY && abs(ex - unit[t]) > UNIT);
+            over |= lanes(__ballot(x[t] > w[t] + SLACK));
+            near[t] = lanes(__ballot(x[t] >= w[t] - NEAR && abs(ex - unit[t]) <= UNIT));
+            all &= near[t];
         }
-        if (__any(move)) {
+        unsigned move = over;
+        if (all != 0xffff)  // (columns that see nothing of the page need no other)
+#pragma unroll
+            for (int t = 0; t < CT; t++) move |= lanes(__ballot(x[t] > -INFINITY)) & ~near[t];
+        if (move) {
 #pragma unroll
             for (int t = 0; t < CT; t++) {
                 const float mp = groups_max(x[t]);
                 top[t] = fmaxf(top[t], mp);
                 most[t] = fmaxf(most[t], mp + (float)ex);
-                float wn = mp > w[t] + SLACK ? mp : w[t];
+                float wn = mp > w[t] + SLACK || mp < w[t] - NEAR ? mp : w[t];
                 wn = fmaxf(wn, top[t] - ROOM);
                 const int un = max(ex, (int)fminf(fmaxf(most[t] - ROOM - wn, (float)NO_EXP), (float)-NO_EXP));
                 const bool seen = mp > -INFINITY;

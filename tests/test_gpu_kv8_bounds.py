@@ -97,3 +97,40 @@ def test_long_sums_of_one_sign(hip, monkeypatch, kernel, scale):
     c.v[:] = rng.integers(60, 120, c.v.shape)
     q = R.rounded(rng.standard_normal((17 * seqs, hk, d)), "float32")
     check(hip, monkeypatch, kernel, c, table, [n] * seqs, [17] * seqs, q, "float32", scale=scale, only=[3], seqs=[0, 31])
+
+
+# ---- many small weights behind a large one -----------------------------------
+
+@pytest.mark.parametrize("behind", ["first", "middle"])
+def test_prompts_with_a_key_above_all_others(hip, monkeypatch, behind):
+    """A key of weight 1 and 16,000 of e^-19.5 to e^-21, whose values differ from its: together they move the output
+    by 4e-5, each by less than float16 can say beside 1.  So many sequences and heads that the keys are not split; they
+    share their pages."""
+    rng = np.random.default_rng(32)
+    n, d, hk, seqs = 16000, 16, 32, 32
+    c = R.Cache(hip, rng, 250, hk, d)
+    table = np.repeat(R.tables(rng, [n], 250), seqs, 0)
+    c.scales[:] = 25 / 127, 0.01
+    c.k[:] = 0
+    c.k[..., 0] = rng.integers(20, 28, (250, hk, 64))
+    c.v[:] = rng.integers(60, 120, c.v.shape)
+    one = 0 if behind == "first" else 7777
+    c.k[table[0, one // 64], :, one % 64, 0] = 127
+    c.v[table[0, one // 64], :, :, one % 64] = -100
+    q = np.zeros((17 * seqs, hk, d))
+    q[..., 0] = 1
+    for kernel in ("prompt", "few"):
+        check(hip, monkeypatch, kernel, c, table, [n] * seqs, [17] * seqs, q, "float32", scale=1.0, only=[0, 16], seqs=[0, 31],
+              alike=True)
+
+
+def test_prompts_of_uneven_scores(hip, monkeypatch):
+    """Scores that differ by some 30 from page to page, in both directions."""
+    rng = np.random.default_rng(33)
+    for dtype in ("float32", "bfloat16"):
+        for spread in (2.0, 8.0):
+            n = 700
+            c = R.Cache(hip, rng, 11, 1, 64)
+            table = R.tables(rng, [n], 11)
+            q = R.rounded(rng.standard_normal((n, 2, 64)) * spread, dtype)
+            check(hip, monkeypatch, "prompt", c, table, [n], [n], q, dtype, only=np.arange(0, n, 23))
