@@ -70,6 +70,12 @@ __device__ __forceinline__ float groups_sum(float v) {
     return groups(v, [](float a, float b) { return a + b; });
 }
 
+// A V scale as mant 2^exponent, the exponent NO_EXP for 0 (a page of zeros): outputs are kept
+// in units of 2^unit that follow the pages' exponents, so that no FP32 scale is too
+// large or too small for the sums.
+constexpr int NO_EXP = -4096;
+__device__ __forceinline__ int scale_exp(float s) { return s > 0.0f ? __builtin_amdgcn_frexp_expf(s) : NO_EXP; }
+
 // What a column sees, and where it is.
 struct Column {
     int row, head;   // row of the row tensors (-1: no such column)
@@ -384,7 +390,8 @@ __device__ __forceinline__ void patch_v(Tile<DP> &t, int lo, const unsigned char
 
 // One workgroup of W waves per (sequence, kv head, 16 columns, split of the
 // pages): with four waves a page's latency (1 us) is paid for four pages at once.  Its waves take the split's pages in turn and join their sums at the
-// end.  splits > 1: unnormalised results [row][head][split][DP + 2] in ws.
+// end.  splits > 1: results of the split's keys alone [row][head][split][DP + 2] in ws
+// (output, maximum score, sum of 2^(score - maximum)).
 //
 // STEP (a decoder's row a sequence, FP32, no shared heads): the rows come as
 // Q | K | V, or as the partial sums of their projection; the workgroup rotates its
@@ -399,7 +406,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
     constexpr float P = PL == 3 ? 127.0f * 65536 : 127.0f * 256;
     __shared__ __attribute__((aligned(16))) float so[W][16][DP + 4];
-    __shared__ float sml[W][2][16];
+    __shared__ float sml[W][3][16];  // maximum, sum, unit
     int b = blockIdx.x;
     const int split = b % splits;
     b /= splits;
@@ -463,6 +470,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     const float f = query_bytes<3, KS>(x, a.scale, ql);
 
     float m = -INFINITY, l = 0.0f;
+    int unit = NO_EXP;  // o is in units of 2^m 2^unit: at least what any page can have added, over 127
     float o[DT][4];
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -531,12 +539,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
                 pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
             }
         }
-        const float mn = fmaxf(m, base == mp ? mp : m);
-        const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-        const float add = mp == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mp - mn);
-        l = fmaf(l, keep, sum * add);
+        const float mn = fmaxf(m, base == mp ? mp : m), mb = mn == -INFINITY ? 0.0f : mn;
+        const float down = m - mb, below = mp - mb;  // -inf: nothing yet, nothing here
+        l = fmaf(l, __builtin_amdgcn_exp2f(down), sum * __builtin_amdgcn_exp2f(below));
         m = mn;
-        const float av = add * (1.0f / P) * sv;
+        const int ex = scale_exp(sv), from = unit;
+        unit = max(unit + (int)fmaxf(down, (float)NO_EXP), ex + (int)fmaxf(below, (float)NO_EXP));
+        const float keep = __builtin_amdgcn_exp2f(down + (float)(from - unit));
+        const float av = __builtin_amdgcn_exp2f(below + (float)(ex - unit)) * __builtin_amdgcn_frexp_mantf(sv) * (1.0f / P);
         if (STEP && pg == own.pg && own.patch && !missing) patch_v(t, own.lo, code[1], lane);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
@@ -574,6 +584,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     if (g4 == 0) {
         sml[wave][0][c] = m;
         sml[wave][1][c] = l;
+        sml[wave][2][c] = (float)unit;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < 16 * DP; e += 64 * W) {
@@ -584,23 +595,27 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
 #pragma unroll
         for (int w = 1; w < W; w++) mm = fmaxf(mm, sml[w][0][cc]);
         const float base = mm == -INFINITY ? 0.0f : mm;
+        float u = 2.0f * NO_EXP;  // whole numbers
+#pragma unroll
+        for (int w = 0; w < W; w++) u = fmaxf(u, sml[w][2][cc] + truncf(fmaxf(sml[w][0][cc] - base, (float)NO_EXP)));
         float ll = 0.0f, oo = 0.0f;
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            const float x = __builtin_amdgcn_exp2f(sml[w][0][cc] - base);
+            const float down = sml[w][0][cc] - base, x = __builtin_amdgcn_exp2f(down);
             ll += sml[w][1][cc] != sml[w][1][cc] ? NAN : sml[w][1][cc] * x;
-            oo = fmaf(so[w][cc][i], x, oo);
+            oo = fmaf(so[w][cc][i], __builtin_amdgcn_exp2f(down + (sml[w][2][cc] - u)), oo);
         }
+        const float out = ll == 0.0f ? 0.0f : ldexpf(oo / ll, (int)u);
         if (splits > 1) {
             float *p = ws + (((int64_t)k.row * a.heads + k.head) * splits + split) * (DP + 2);
-            p[i] = oo;
+            p[i] = out;
             if (i == 0) {
                 p[DP] = mm;
                 p[DP + 1] = ll;
             }
             continue;
         }
-        if (i < a.c.d) store_out<T>(a, k.row, k.head, i, ll == 0.0f ? 0.0f : oo / ll);
+        if (i < a.c.d) store_out<T>(a, k.row, k.head, i, out);
         if (i == 0 && a.lse) a.lse[(int64_t)k.row * a.heads + k.head] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
     }
 }
@@ -641,43 +656,47 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
                 for (int u = 0; u < DL; u++) o[s][u] = ps[(DP >= 64 ? lane : lane % DP) + 64 * u];
             }
             const float mn = fmaxf(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), mm);
-            const float base = mn == -INFINITY ? 0.0f : mn, y = __builtin_amdgcn_exp2f(mm - base);
+            const float base = mn == -INFINITY ? 0.0f : mn;
+            ll *= __builtin_amdgcn_exp2f(mm - base);
             mm = mn;
-            ll *= y;
-#pragma unroll
-            for (int u = 0; u < DL; u++) oo[u] *= y;
+            float x[4], sum = ll;
 #pragma unroll
             for (int s = 0; s < 4; s++) {
-                const float x = __builtin_amdgcn_exp2f(m[s] - base);
-                ll += s0 + s < used ? l[s] * x : 0.0f;  // (x may be 0: 0 NaN is NaN)
-#pragma unroll
-                for (int u = 0; u < DL; u++) oo[u] = s0 + s < used ? fmaf(o[s][u], x, oo[u]) : oo[u];
+                x[s] = s0 + s < used ? l[s] * __builtin_amdgcn_exp2f(m[s] - base) : 0.0f;  // (0 NaN is NaN)
+                sum += x[s];
             }
+            // oo is the mean so far, so that it is never larger than a value
+            const float each = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int u = 0; u < DL; u++) oo[u] *= ll * each;
+            ll = sum;
+#pragma unroll
+            for (int s = 0; s < 4; s++)
+#pragma unroll
+                for (int u = 0; u < DL; u++) oo[u] = s0 + s < used ? fmaf(o[s][u], x[s] * each, oo[u]) : oo[u];
         }
     } else {
         for (int s = lane; s < used; s += 64) mm = fmaxf(mm, p[s * (DP + 2) + DP]);
 #pragma unroll
         for (int x = 32; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor(mm, x));
         const float base = mm == -INFINITY ? 0.0f : mm;
+        for (int s = lane; s < used; s += 64) ll += p[s * (DP + 2) + DP + 1] * __builtin_amdgcn_exp2f(p[s * (DP + 2) + DP] - base);
+        ll = wave_butterfly(ll);
+        const float each = ll == 0.0f ? 0.0f : 1.0f / ll;
 #pragma unroll 4
         for (int s = wave; s < used; s += W) {
             const float *ps = p + s * (DP + 2);
-            const float x = __builtin_amdgcn_exp2f(ps[DP] - base);
-            ll += ps[DP + 1] * x;
+            const float x = ps[DP + 1] * __builtin_amdgcn_exp2f(ps[DP] - base) * each;
 #pragma unroll
             for (int u = 0; u < DL; u++)
                 if (DP >= 64 || lane < DP) oo[u] = fmaf(ps[lane + 64 * u], x, oo[u]);
         }
-        __shared__ float so[W][DP], sl[W];
+        __shared__ float so[W][DP];
 #pragma unroll
         for (int u = 0; u < DL; u++)
             if (DP >= 64 || lane < DP) so[wave][lane + 64 * u] = oo[u];
-        if (lane == 0) sl[wave] = ll;
         __syncthreads();
         if (wave > 0) return;  // (behind the last barrier)
-        ll = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; w++) ll += sl[w];
 #pragma unroll
         for (int u = 0; u < DL; u++) {
             oo[u] = 0.0f;
@@ -688,7 +707,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
     }
 #pragma unroll
     for (int u = 0; u < DL; u++)
-        if (lane + 64 * u < a.c.d) store_out<T>(a, row, h, lane + 64 * u, ll == 0.0f ? 0.0f : oo[u] / ll);
+        if (lane + 64 * u < a.c.d) store_out<T>(a, row, h, lane + 64 * u, oo[u]);
     if (a.lse && lane == 0) a.lse[(int64_t)row * a.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * LN2;
 }
 
@@ -714,7 +733,6 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     constexpr float SLACK = 5.0f, P0 = 8.0f, NEAR = PL == 2 ? 4.0f : 8.0f;
     constexpr int UNIT = 2;
     constexpr float ROOM = 60.0f;  // of a column's sums above 2^w (2^w 2^unit): what adds less than 2^-60 of them may be lost
-    constexpr int NO_EXP = -4096;  // a page whose values are 0
     // The last rows, which see most keys, go first, over all (sequence, kv head)
     // pairs (a pair after the other left the longest to a quarter of the CUs:
     // prompts of 131 to 512 rows 28.4 -> 25.4 us; whole pairs to one XCD: no difference).
@@ -861,7 +879,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
             }
         }
         float fk[CT], x[CT];
-        const int ex = sv > 0.0f ? __builtin_amdgcn_frexp_expf(sv) : NO_EXP;
+        const int ex = scale_exp(sv);
         unsigned over = 0, near[CT], all = 0xffff;  // columns above their reference, and those that the reference suits
 #pragma unroll
         for (int t = 0; t < CT; t++) {
@@ -950,26 +968,24 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         float sum = groups_sum(l[t]);
         if (begin[t] >= end[t]) sum = 0.0f;
         if (col.row < 0) continue;
-        if (splits > 1) {
-            float *p = ws + (((int64_t)col.row * a.heads + col.head) * splits + split) * (DP + 2);
-            const float x = __builtin_amdgcn_exp2f(-P0);
-#pragma unroll
-            for (int dt = 0; dt < DT; dt++)
-#pragma unroll
-                for (int r = 0; r < 4; r += 2)
-                    *reinterpret_cast<float2 *>(p + dt * 16 + g4 * 4 + r) =
-                        make_float2(ldexpf(o[t][dt][r] * x, unit[t]), ldexpf(o[t][dt][r + 1] * x, unit[t]));
-            if (g4 == 0) *reinterpret_cast<float2 *>(p + DP) = make_float2(w[t], sum);
-            continue;
-        }
         const float x = __builtin_amdgcn_exp2f(-P0) / sum;
+        float *p = ws + (((int64_t)col.row * a.heads + col.head) * splits + split) * (DP + 2);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
             const int i = dt * 16 + g4 * 4;
             f32x4 y;
 #pragma unroll
             for (int r = 0; r < 4; r++) y[r] = sum == 0.0f ? 0.0f : ldexpf(o[t][dt][r] * x, unit[t]);
-            if (i < a.c.d) store_out4<T>(a, col.row, col.head, i, y);
+            if (splits > 1) {
+                *reinterpret_cast<float2 *>(p + i) = make_float2(y[0], y[1]);
+                *reinterpret_cast<float2 *>(p + i + 2) = make_float2(y[2], y[3]);
+            } else if (i < a.c.d) {
+                store_out4<T>(a, col.row, col.head, i, y);
+            }
+        }
+        if (splits > 1) {
+            if (g4 == 0) *reinterpret_cast<float2 *>(p + DP) = make_float2(w[t], sum);
+            continue;
         }
         if (g4 == 0 && a.lse)
             a.lse[(int64_t)col.row * a.heads + col.head] = sum == 0.0f ? -INFINITY : (w[t] + log2f(sum)) * LN2;

@@ -83,6 +83,27 @@ def test_prompts_over_v_scales_far_apart(hip, monkeypatch):
     far_apart(hip, monkeypatch, "prompt", g=3)
 
 
+def test_rows_over_v_scales_far_apart(hip, monkeypatch):
+    far_apart(hip, monkeypatch, "few")
+    far_apart(hip, monkeypatch, "few", g=3)
+
+
+@pytest.mark.parametrize("kernel", ["few", "prompt"])
+@pytest.mark.parametrize("rows", [1, 100])
+def test_split_keys_over_v_scales_far_apart(hip, monkeypatch, kernel, rows):
+    """Splits joined: pages of 10^-37 to 10^36, and values near the largest that FP32 has, of one sign and of both."""
+    rng = np.random.default_rng(34)
+    for lo, hi, one_sign in ((-37, 36.4, False), (36.4, 36.42, True), (-37, -36, False)):
+        n = 4500
+        c = R.Cache(hip, rng, 71, 1, 64)
+        table = R.tables(rng, [n], 71)
+        c.scales[:, 0, 1] = 10.0 ** rng.uniform(lo, hi, 71)
+        if one_sign:
+            c.v = np.abs(c.v)
+        q = R.rounded(rng.standard_normal((rows, 1, 64)) * 0.3, "float32")
+        check(hip, monkeypatch, kernel, c, table, [n], [rows], q, "float32", only=[0, 1, 33, 64, 99])
+
+
 # ---- long sums ---------------------------------------------------------------
 
 @pytest.mark.parametrize("kernel", ["few", "prompt"])
