@@ -16,8 +16,8 @@
 // their lane.
 //
 // k_kv8_attend (few columns: single tokens).  Keys are split over waves and
-// workgroups.  The weights are bytes as well, three for FP32 rows and two for
-// 16-bit ones, P = 127 256^2 (127 256) at the largest of the page: p v is exact,
+// workgroups.  The weights are bytes as well, three of them, P = 127 256^2 at the largest of the page (two
+// would do for bfloat16 but not for float16, and the third costs nothing where the codes' bytes bound it): p v is exact,
 // and each page joins the running output with exp(max of the page - running max)
 // times its V scale in FP32.  Bound by reading the codes once: 64 sequences of
 // 1025 to 7500 tokens, 32 heads over 8 of 128, bfloat16, 143 us (4.2 TB/s); one
@@ -400,11 +400,11 @@ __device__ __forceinline__ void patch_v(Tile<DP> &t, int lo, const unsigned char
 // new codes into the tile that they requested before, else they read the page anew.  The
 // page has no other reader in the launch.  650M, one row at position 280: 11.4 us (append
 // 2 and the projection's sums 1.5 of it), the attention alone 5.5.
-template <int DP, int PL, class T, int W, bool STEP>
+template <int DP, class T, int W, bool STEP>
 __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws, StepArg<STEP> step) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
-    constexpr float P = PL == 3 ? 127.0f * 65536 : 127.0f * 256;
+    constexpr float P = 127.0f * 65536;
     __shared__ __attribute__((aligned(16))) float so[W][16][DP + 4];
     __shared__ float sml[W][3][16];  // maximum, sum, unit
     int b = blockIdx.x;
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         if (mp == INFINITY) l = NAN;
         const float base = mp == -INFINITY ? 0.0f : mp;
         // the page's weights as bytes; their sum before that rounding, which lse does not share
-        i32x4 pl[PL];
+        i32x4 pl[3];
         float sum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < 4; kt++) {
@@ -523,21 +523,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
                 const float e = __builtin_amdgcn_exp2f(s[kt][r] - base);
                 v[r] = (unsigned)rintf(e * P);
                 sum += e;
-                v[r] += PL == 3 ? 0x8080 : 0x80;
+                v[r] += 0x8080;
             }
-            if (PL == 3) {
-                const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010602u);  // bytes 2 | bytes 1
-                const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010602u);
-                const unsigned b01 = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), b23 = __builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u);
-                pl[0][kt] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
-                pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
-                pl[PL - 1][kt] = (int)(__builtin_amdgcn_perm(b23, b01, 0x05040100u) ^ 0x80808080u);
-            } else {
-                const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x04000501u);  // bytes 1 | bytes 0
-                const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x04000501u);
-                pl[0][kt] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
-                pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
-            }
+            const unsigned a01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010602u);  // bytes 2 | bytes 1
+            const unsigned a23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010602u);
+            const unsigned b01 = __builtin_amdgcn_perm(v[1], v[0], 0x0c0c0400u), b23 = __builtin_amdgcn_perm(v[3], v[2], 0x0c0c0400u);
+            pl[0][kt] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+            pl[1][kt] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302u) ^ 0x80808080u);
+            pl[2][kt] = (int)(__builtin_amdgcn_perm(b23, b01, 0x05040100u) ^ 0x80808080u);
         }
         const float mn = fmaxf(m, base == mp ? mp : m), mb = mn == -INFINITY ? 0.0f : mn;
         const float down = m - mb, below = mp - mb;  // -inf: nothing yet, nothing here
@@ -550,14 +543,14 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         if (STEP && pg == own.pg && own.patch && !missing) patch_v(t, own.lo, code[1], lane);
 #pragma unroll
         for (int dt = 0; dt < DT; dt++) {
-            i32x4 d[PL];
+            i32x4 d[3];
 #pragma unroll
-            for (int n = 0; n < PL; n++)
+            for (int n = 0; n < 3; n++)
                 d[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(t.v[dt], pl[n], i32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float hi = (float)(d[0][r] * 256 + d[1][r]);
-                o[dt][r] = fmaf(o[dt][r], keep, (PL == 3 ? fmaf(hi, 256.0f, (float)d[PL - 1][r]) : hi) * av);
+                o[dt][r] = fmaf(o[dt][r], keep, fmaf(hi, 256.0f, (float)d[2][r]) * av);
             }
         }
     };
@@ -1056,13 +1049,13 @@ hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t 
     if (!kv8_grid(p.blocks, 256) || (p.splits > 1 && !kv8_grid(rows, 64 * JOIN_WAVES))) return hipErrorInvalidValue;
     if constexpr (full)
         if (step)
-            hipLaunchKernelGGL((k_kv8_attend<DP, 3, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
+            hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                                p.splits, p.pps, ws, *step);
     if (!step && p.prompt)
         hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                            p.splits, p.pps, ws);
     else if (!step)
-        hipLaunchKernelGGL((k_kv8_attend<DP, full ? 3 : 2, T, 4, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g,
+        hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g,
                            p.tiles, p.splits, p.pps, ws, NoStep{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;

@@ -155,3 +155,31 @@ def test_prompts_of_uneven_scores(hip, monkeypatch):
             table = R.tables(rng, [n], 11)
             q = R.rounded(rng.standard_normal((n, 2, 64)) * spread, dtype)
             check(hip, monkeypatch, "prompt", c, table, [n], [n], q, dtype, only=np.arange(0, n, 23))
+
+
+# ---- ordinary rows -----------------------------------------------------------
+
+@pytest.mark.parametrize("kernel", ["few"])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("d,hk,g", [(16, 2, 1), (24, 2, 2), (32, 1, 3), (64, 1, 4), (64, 2, 1), (128, 1, 4)])
+def test_rows(hip, monkeypatch, kernel, dtype, d, hk, g):
+    """Flat and peaked softmaxes: single tokens, drafted rows, prompts, chunks, windows."""
+    rng = np.random.default_rng(35 + d)
+    lens, rows = [1, 65, 130, 333, 700, 700], [1, 65, 130, 40, 1, 5]
+    for causal, window, spread in ((True, 0, 0.5), (True, 100, 2.0), (False, 0, 0.5)):
+        c = R.Cache(hip, rng, 40, hk, d)
+        table = R.tables(rng, lens, 40)
+        q = R.rounded(rng.standard_normal((sum(rows), hk * g, d)) * spread, dtype)
+        check(hip, monkeypatch, kernel, c, table, lens, rows, q, dtype, causal, window, only=[0, 1, 17, 39, 63, 64, 100, 129])
+
+
+@pytest.mark.parametrize("kernel", ["few"])
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_rows_over_split_keys(hip, monkeypatch, kernel, dtype):
+    rng = np.random.default_rng(36)
+    lens, rows = [9001, 4100], [1, 80]
+    c = R.Cache(hip, rng, 210, 1, 64)
+    table = R.tables(rng, lens, 210)
+    for window in (0, 1500):
+        q = R.rounded(rng.standard_normal((81, 2, 64)) * 0.5, dtype)
+        check(hip, monkeypatch, kernel, c, table, lens, rows, q, dtype, window=window, only=[0, 1, 40, 79])
