@@ -25,7 +25,7 @@
 // One page of 20 heads of 16 takes 4 us, all latency.
 //
 // k_kv8_prompt (many columns).  V's codes become f16 and the weights f16 (FP32
-// rows: two f16, hi + lo); a page's sums join the running
+// and float16 rows: two f16, hi + lo; one has 11 bits, three more than a bfloat16 row keeps); a page's sums join the running
 // output in FP32.  Bound by instruction issue, the exponentials and the weights'
 // conversions: 2047 rows of 16000 keys, 32 heads over 8 of 128, bfloat16, 567 us
 // (886 TFLOP/s); 131 to 512 rows of 8 sequences, 20 heads of 64, FP32, 22 us.
@@ -718,7 +718,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 // page ahead.  Its conversion was a third of the instructions (2047 rows of 16000
 // keys 656 -> 570 us); at narrower heads, with fewer columns and less to convert, the waves' waiting for each
 // other costs as much (20 heads of 64: 2 x 512 rows 13.0, shared 14.8).
-template <int DP, int PL, class T, int CT>
+template <int DP, int QB, int PL, class T, int CT>
 __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
@@ -754,7 +754,6 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         last = min(last, (any1 + KV8_PAGE - 1) / KV8_PAGE);
     }
 
-    constexpr int QB = PL + 1;  // bytes of a query
     i32x4 ql[CT][QB][KS];
     float f[CT], w[CT], l[CT];
     float top[CT], most[CT];  // the largest score, the largest score + exponent of its page's V scale
@@ -1052,7 +1051,7 @@ hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t 
             hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                                p.splits, p.pps, ws, *step);
     if (!step && p.prompt)
-        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 2 : 1, T, CT>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
+        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 3 : 2, std::is_same<T, __bf16>::value ? 1 : 2, T, CT>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                            p.splits, p.pps, ws);
     else if (!step)
         hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g,

@@ -159,7 +159,7 @@ def test_prompts_of_uneven_scores(hip, monkeypatch):
 
 # ---- ordinary rows -----------------------------------------------------------
 
-@pytest.mark.parametrize("kernel", ["few"])
+@pytest.mark.parametrize("kernel", ["few", "prompt"])
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("d,hk,g", [(16, 2, 1), (24, 2, 2), (32, 1, 3), (64, 1, 4), (64, 2, 1), (128, 1, 4)])
 def test_rows(hip, monkeypatch, kernel, dtype, d, hk, g):
@@ -173,7 +173,7 @@ def test_rows(hip, monkeypatch, kernel, dtype, d, hk, g):
         check(hip, monkeypatch, kernel, c, table, lens, rows, q, dtype, causal, window, only=[0, 1, 17, 39, 63, 64, 100, 129])
 
 
-@pytest.mark.parametrize("kernel", ["few"])
+@pytest.mark.parametrize("kernel", ["few", "prompt"])
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 def test_rows_over_split_keys(hip, monkeypatch, kernel, dtype):
     rng = np.random.default_rng(36)
@@ -183,3 +183,25 @@ def test_rows_over_split_keys(hip, monkeypatch, kernel, dtype):
     for window in (0, 1500):
         q = R.rounded(rng.standard_normal((81, 2, 64)) * 0.5, dtype)
         check(hip, monkeypatch, kernel, c, table, lens, rows, q, dtype, window=window, only=[0, 1, 40, 79])
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n_seq,rows,hk,g,d,kernel", [(64, 17, 20, 1, 64, "prompt"), (8, 1, 20, 1, 64, "few"),
+                                                      (1, 100, 4, 1, 64, "few"), (1, 100, 4, 4, 128, "prompt")])
+def test_the_kernel_that_the_sizes_choose(hip, monkeypatch, dtype, n_seq, rows, hk, g, d, kernel):
+    """... is the one that is meant: bit by bit what it gives when it is asked for."""
+    rng = np.random.default_rng(37)
+    n = 2100 if kernel == "prompt" and n_seq == 1 else 150
+    lens, counts = [n] * n_seq, [rows] * n_seq
+    need = sum(-(-x // 64) for x in lens)
+    c = R.Cache(hip, rng, need, hk, d)
+    table = R.tables(rng, lens, need)
+    q = R.rounded(rng.standard_normal((sum(counts), hk * g, d)), dtype)
+    monkeypatch.delenv("CIH_KV8_PROMPT", raising=False)
+    chosen = attend(hip, c, table, lens, counts, q, dtype)
+    got = {}
+    for name, e in (("few", "0"), ("prompt", "1")):
+        monkeypatch.setenv("CIH_KV8_PROMPT", e)
+        got[name] = attend(hip, c, table, lens, counts, q, dtype)
+    assert all(np.array_equal(a, b) for a, b in zip(chosen, got[kernel]))
+    assert not all(np.array_equal(a, b) for a, b in zip(*got.values()))
