@@ -844,8 +844,9 @@ int cih_generate(cih_decoder *dc, int32_t n, const int32_t *slots, const int32_t
     // (chunks of max_rows positions), so a stream's cache does not depend on
     // which other streams run with it
     const auto t0 = std::chrono::steady_clock::now();
+    // (all of them start anew before the first takes pages)
+    for (int i = 0; i < n; i++) release_slot(dc, slots[i]);
     for (int i = 0; i < n; i++) {
-        release_slot(dc, slots[i]);
         for (int p0 = 0; p0 < pos[i]; p0 += dc->max_rows) {
             const int k = std::min(dc->max_rows, pos[i] - p0);
             std::vector<int32_t> sl(k, slots[i]), tk(prompts + offsets[i] + p0, prompts + offsets[i] + p0 + k), ps(k);

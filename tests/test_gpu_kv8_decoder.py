@@ -361,3 +361,26 @@ def test_refusals():
             dec.read_cache(*a)
     dec.close()
     m.close()
+
+
+def test_generate_again_over_a_tight_pool():
+    """The slots' pages of the call before go back before the first prompt takes any: 4 + 1 pages fit where 1 + 3 are held."""
+    cfg, w, m = make(32, "q8", heads=2, layers=1)
+    dec = ch.GpuDecoder(m, n_slots=3, max_len=300, max_rows=64, kv8=True, n_pages=6)
+    dec.generate([tokens(60, 1), tokens(180, 2)], 0.0, 2, [1, 2])
+    again = [tokens(250, 3), tokens(50, 4)]
+    got, _, _ = dec.generate(again, 0.0, 4, [1, 2])
+    fresh = ch.GpuDecoder(m, n_slots=2, max_len=300, max_rows=64, kv8=True)
+    want, _, _ = fresh.generate(again, 0.0, 4, [1, 2])
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+    # one that does not fit leaves no slot with what it held before
+    dec.decode([2], [0], [0])
+    dec.read_cache(0, 2, 0, 1)
+    with pytest.raises(ch.CihError) as e:
+        dec.generate([tokens(290, 5), tokens(128, 6), tokens(40, 7)], 0.0, 2, [1, 2, 3])
+    assert e.value.code == -3
+    with pytest.raises(ch.CihError):
+        dec.read_cache(0, 2, 0, 1)
+    for d in (dec, fresh):
+        d.close()
+    m.close()
