@@ -541,14 +541,14 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
     const size_t d = m->cfg.dim, F = m->cfg.hidden_dim, V = m->cfg.vocab_size, L = m->cfg.n_layers;
     const size_t R = max_rows;
     cih_rope plain{};
+    RopeArg turns;
     if (kv8) {
         // RoPE of the reference (apply_rope, lib.rs:3533-3552), with the angles in 64 bits
         if (!rope) {
             if (int rc = cih_rope_init(&plain, m->hd, 0, 10000.0, CIH_ROPE_NONE, 1.0, 1)) return rc;
             rope = &plain;
         }
-        if (rope->rot_dim < 2 || rope->rot_dim > m->hd || rope->rot_dim % 2)
-            return set_error(CIH_ERR_SHAPE, "%d rotary dims in a head of %d", rope->rot_dim, m->hd);
+        if (int rc = kv8_rope(rope, m->hd, turns)) return rc;
     }
     std::unique_ptr<cih_decoder, void (*)(cih_decoder *)> held(new cih_decoder(), destroy);
     cih_decoder *dc = held.get();
@@ -572,10 +572,7 @@ int create(cih_model *m, int32_t n_slots, int32_t max_len, int32_t max_rows, boo
         const size_t H = m->cfg.n_heads, dp = kv8_dims(m->hd), ph = L * kv.n_pages * H;
         cache = ph * KV8_PAGE * dp;
         kv.view = {nullptr, nullptr, nullptr, nullptr, kv.n_pages, (int)H, m->hd, (int)dp};
-        kv.rope.rot = rope->rot_dim;
-        kv.rope.inter = rope->interleaved != 0;
-        kv.rope.gain = rope->gain;
-        for (int j = 0; j < kv.rope.rot / 2; j++) kv.rope.turns[j] = rope->freq[j] / 6.283185307179586476925;
+        kv.rope = turns;
         // partial results of split keys: at most a split for every 16 pages, and no more than 64 MiB (fewer splits then)
         kv.ws_floats = std::min<size_t>((size_t)R * H * ((kv.max_pages + 15) / 16) * (dp + 2), (size_t)16 << 20);
         good = dalloc(kv.view.k, cache, al) == hipSuccess && dalloc(kv.view.v, cache, al) == hipSuccess &&

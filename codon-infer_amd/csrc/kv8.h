@@ -6,6 +6,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include "../../include/codon_hip.h"
+
 namespace cih {
 
 constexpr int KV8_PAGE = 64;
@@ -63,6 +65,9 @@ struct RopeArg {
     float gain = 1.0f;
     double turns[64] = {};
 };
+
+// r (NULL: no rotary positions) for heads of head_dim as the kernels take it; an error code and message if it is refused.
+int kv8_rope(const cih_rope *r, int head_dim, RopeArg &a);
 
 // Workgroups of `threads` that one launch may have: its threads are counted in 32 bits.
 inline bool kv8_grid(int64_t blocks, int threads) { return blocks > 0 && blocks <= INT32_MAX && blocks <= (int64_t)UINT32_MAX / threads; }

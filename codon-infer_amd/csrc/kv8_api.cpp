@@ -85,18 +85,6 @@ int check_float(int dtype) {
     return 0;
 }
 
-int check_rope(const cih_rope *r, int d, RopeArg &a) {
-    if (!r) return 0;
-    if (r->rot_dim < 2 || r->rot_dim > d || r->rot_dim % 2)
-        return set_error(CIH_ERR_SHAPE, "%d rotary dims in a head of %d", r->rot_dim, d);
-    a.rot = r->rot_dim;
-    a.inter = r->interleaved != 0;
-    a.gain = r->gain;
-    const double turn = 6.283185307179586476925;
-    for (int j = 0; j < a.rot / 2; j++) a.turns[j] = r->freq[j] / turn;
-    return 0;
-}
-
 int check_heads(int heads, int hk, const Kv8Seqs &s) {
     if (heads < 1 || heads > 65535 || heads % hk)
         return set_error(CIH_ERR_SHAPE, "%d query heads over %d key/value heads", heads, hk);
@@ -106,6 +94,22 @@ int check_heads(int heads, int hk, const Kv8Seqs &s) {
 }
 
 }  // namespace
+
+int cih::kv8_rope(const cih_rope *r, int head_dim, RopeArg &a) {
+    if (!r) return 0;
+    if (r->rot_dim < 2 || r->rot_dim > head_dim || r->rot_dim % 2)
+        return set_error(CIH_ERR_SHAPE, "%d rotary dims in a head of %d", r->rot_dim, head_dim);
+    a.rot = r->rot_dim;
+    a.inter = r->interleaved != 0;
+    a.gain = r->gain;
+    if (!std::isfinite(a.gain)) return set_error(CIH_ERR_ARG, "the rotary gain is not finite");
+    const double turn = 6.283185307179586476925;
+    for (int j = 0; j < a.rot / 2; j++) {
+        if (!std::isfinite(r->freq[j])) return set_error(CIH_ERR_ARG, "rotary frequency %d is not finite", j);
+        a.turns[j] = r->freq[j] / turn;
+    }
+    return 0;
+}
 
 #define CIH_TRY(expr)                    \
     do {                                 \
@@ -153,7 +157,7 @@ int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32
     CIH_TRY(check_float(dtype));
     CIH_TRY(check_cache(cache, c, true));
     CIH_TRY(check_batch(batch, s, true));
-    CIH_TRY(check_rope(rope, c.d, ra));
+    CIH_TRY(kv8_rope(rope, c.d, ra));
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return CIH_OK;
     CIH_TRY(check_rows(k, "k", dtype, kv));
     CIH_TRY(check_rows(v, "v", dtype, vv));

@@ -272,7 +272,8 @@ typedef struct cih_rows {
 
 /* Rotary positions: pair j < rot_dim / 2 of a head turns by position * freq[j]
  * radians, both values times gain.  The pair is (j, j + rot_dim / 2), or with
- * interleaved (2 j, 2 j + 1); dims from rot_dim on stay as they are. */
+ * interleaved (2 j, 2 j + 1); dims from rot_dim on stay as they are.  A gain or
+ * a freq[j] that is not finite is refused (CIH_ERR_ARG). */
 typedef struct cih_rope {
     int32_t rot_dim, interleaved;
     float gain;

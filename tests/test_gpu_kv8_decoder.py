@@ -384,3 +384,17 @@ def test_generate_again_over_a_tight_pool():
     for d in (dec, fresh):
         d.close()
     m.close()
+
+
+def test_rope_not_finite():
+    cfg, w, m = make(16)
+    for field in ("gain", "freq"):
+        r = ch.Rope(16)
+        if field == "gain":
+            r.struct.gain = np.inf
+        else:
+            r.struct.freq[7] = np.nan
+        with pytest.raises(ch.CihError) as e:
+            ch.GpuDecoder(m, n_slots=1, max_len=64, max_rows=8, kv8=True, rope=r)
+        assert e.value.code == -1
+    m.close()

@@ -189,3 +189,21 @@ def test_decoder_refusals_without_a_model():
     assert lib.cih_decoder_create_kv8(None, 1, 64, 8, 0, ctypes.addressof(r), None) == -1
     assert lib.cih_decoder_score(None, 1, None, None, None, 0, None, None, None, None) == -1
     assert lib.cih_decoder_read_cache(None, 0, 0, 0, 1, None, None) == -1
+
+
+@pytest.mark.parametrize("field", ["gain", 0, 31])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_rope_not_finite(field, value):
+    """Rotary positions that a caller filled: they would make every key NaN."""
+    c, b, r = cache(), batch(), ch.Rope(64)
+    row = Fake((3, 2, 64))
+    if field == "gain":
+        r.struct.gain = value
+    else:
+        r.struct.freq[field] = value
+    assert code(c.append, b, row, row, rope=r) == -1
+    # frequencies past the pairs that turn are not read
+    part = ch.Rope(32)
+    part.struct.freq[16] = value
+    assert code(c.append, b, Fake((3, 2, 64), at=0), row, rope=part) == -1
+    assert "rotary" not in C.lib().cih_last_error().decode()
