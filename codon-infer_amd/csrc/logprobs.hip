@@ -489,8 +489,7 @@ LpPlan lp_plan(int n, int vocab, int top) {
 
 template <class T> hipError_t launch_lp(const TokenLogprobs &a, float *ws, hipStream_t st) {
     if (a.vocab <= 64) {
-        hipLaunchKernelGGL(k_logprobs_narrow<T>, dim3(a.n / NARROW_ROWS + (a.n % NARROW_ROWS != 0)), dim3(64 * NARROW_ROWS), 0,
-                           st, a);
+        hipLaunchKernelGGL(k_logprobs_narrow<T>, dim3((a.n + NARROW_ROWS - 1) / NARROW_ROWS), dim3(64 * NARROW_ROWS), 0, st, a);
         return hipGetLastError();
     }
     const LpPlan p = lp_plan(a.n, a.vocab, a.top);
@@ -513,15 +512,32 @@ size_t token_logprobs_floats(int n, int vocab, int top) {
     return p.chunks > 1 ? (size_t)n * p.chunks * (4 + 2 * top) : 0;
 }
 
-hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, size_t ws_floats, hipStream_t st) {
-    if (a.n == 0) return hipSuccess;
-    if (token_logprobs_floats(a.n, a.vocab, a.top) > ws_floats) return hipErrorInvalidValue;
-    switch (a.dtype) {
-        case FT_F32: return launch_lp<float>(a, ws, st);
-        case FT_F16: return launch_lp<_Float16>(a, ws, st);
-        case FT_BF16: return launch_lp<__bf16>(a, ws, st);
+// A launch counts its threads in 32 bits: this many rows have at most 2^31, and
+// more of them go in several launches (rows are split into chunks only where they are few).
+constexpr int LAUNCH_ROWS = 1 << 22;
+
+hipError_t launch_token_logprobs(const TokenLogprobs &all, float *ws, size_t ws_floats, hipStream_t st) {
+    if (token_logprobs_floats(all.n, all.vocab, all.top) > ws_floats) return hipErrorInvalidValue;
+    for (int r0 = 0; r0 < all.n; r0 += LAUNCH_ROWS) {
+        TokenLogprobs a = all;
+        a.n = std::min(all.n - r0, LAUNCH_ROWS);
+        a.logits = static_cast<const char *>(all.logits) + r0 * all.stride * (all.dtype == FT_F32 ? 4 : 2);
+        if (all.targets) a.targets += r0;
+        if (all.logprob) a.logprob += r0;
+        if (all.entropy) a.entropy += r0;
+        if (all.top > 0) {
+            a.top_ids += (int64_t)r0 * all.top;
+            a.top_lp += (int64_t)r0 * all.top;
+        }
+        hipError_t e = hipErrorInvalidValue;
+        switch (a.dtype) {
+            case FT_F32: e = launch_lp<float>(a, ws, st); break;
+            case FT_F16: e = launch_lp<_Float16>(a, ws, st); break;
+            case FT_BF16: e = launch_lp<__bf16>(a, ws, st); break;
+        }
+        if (e != hipSuccess) return e;
     }
-    return hipErrorInvalidValue;
+    return hipSuccess;
 }
 
 }  // namespace cih

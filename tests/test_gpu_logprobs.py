@@ -126,3 +126,33 @@ def test_outputs_left_out_and_strides(hip):
         for want in (("logprob",), ("entropy",), ("top",), ("logprob", "top")):
             run(hip, x, rng.integers(0, vocab, 6) if "logprob" in want else None, 4, "bfloat16", stride=vocab + 7, want=want)
         run(hip, x, rng.integers(0, vocab, 6), 0, "float16", stride=vocab + 1, want=("logprob", "entropy"))
+
+
+@pytest.mark.parametrize("n,vocab,k", [((1 << 26) + 77, 2, 0), ((1 << 23) + 5, 3, 2), ((1 << 22) + 9, 70, 3)])
+def test_more_rows_than_a_launch_has_threads(hip, n, vocab, k):
+    """Rows past 2^22, which several launches share, and past 2^26, whose waves have more than 2^32 lanes: every row is
+    the one of its place in a block of rows that repeats."""
+    rng = np.random.default_rng(vocab)
+    period = 1009
+    x = R.rounded(rng.standard_normal((period, vocab)) * 3, "float16")
+    t = rng.integers(0, vocab, period).astype(np.int32)
+    want = R.logprobs(x, t, k)
+    reps = -(-n // period)
+    base = DeviceArray(hip, np.tile(x.astype(np.float16), (reps, 1))[:n])
+    targets = DeviceArray(hip, np.tile(t, reps)[:n])
+    lp, en = [DeviceArray(hip, np.full(n, 7, np.float32)) for _ in range(2)]
+    ids, top = DeviceArray(hip, np.full((n, k), 7, np.int32)), DeviceArray(hip, np.full((n, k), 7, np.float32))
+    assert ch.token_logprobs_workspace(n, vocab, k) == 0
+    ch.token_logprobs(base, targets, lp, en, *((ids, top) if k else (None, None)))
+    tol = 2.0 ** -18 * (1 + 2 * np.abs(x).max() + np.log(vocab))
+    for a, w in ((lp, want[0]), (en, want[1])) + (((top, want[3]),) if k else ()):
+        got = a.numpy()
+        first = got[:period]
+        assert np.abs(first - w).max() <= tol
+        whole = got[:n // period * period].reshape(-1, *first.shape)
+        assert (whole == first).all() and (got[whole.shape[0] * period:] == first[:n % period]).all()
+    if k:
+        got = ids.numpy()
+        assert np.array_equal(got[:period], want[2]) and np.array_equal(got[-(n % period):], want[2][:n % period])
+        assert (got[:n // period * period].reshape(-1, period, k) == want[2]).all()
+    R.free(base, targets, lp, en, ids, top)
