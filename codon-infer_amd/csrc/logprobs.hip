@@ -179,7 +179,7 @@ template <int K> __device__ __forceinline__ u64 top_bound(const u64 (&key)[K], i
             t |= (u64)(o & a) << (32 - 32 * h);
             if (o != a) {
                 b = 63 - 32 * h - __builtin_clz(o ^ a);
-                t = t >> (b + 1) << (b + 1);
+                t &= ~0ull << b << 1;  // (b may be 63)
             }
         }
     }

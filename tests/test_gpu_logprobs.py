@@ -156,3 +156,14 @@ def test_more_rows_than_a_launch_has_threads(hip, n, vocab, k):
         assert np.array_equal(got[:period], want[2]) and np.array_equal(got[-(n % period):], want[2][:n % period])
         assert (got[:n // period * period].reshape(-1, period, k) == want[2]).all()
     R.free(base, targets, lp, en, ids, top)
+
+
+@pytest.mark.parametrize("vocab,k", [(900, 1), (5000, 3), (70000, 20)])
+def test_alternatives_among_both_signs(hip, vocab, k):
+    """The threads' largest logits differ in their sign: few or many of them positive, all but one, none but one."""
+    rng = np.random.default_rng(k)
+    x = -np.abs(rng.standard_normal((6, vocab))) * 3 - 1
+    x[1] *= -1
+    for r, n in ((2, 1), (3, k), (4, 2 * k + 9), (5, vocab // 2)):
+        x[r, rng.permutation(vocab)[:n]] *= -1
+    run(hip, x, rng.integers(0, vocab, 6), k, "float32")
