@@ -459,8 +459,8 @@ int staged_row(const cih_decoder *dc, int i) { return dc->kv.on ? dc->kv.order[i
 int stage_rows(cih_decoder *dc, const int32_t *slots, const int32_t *tokens, const int32_t *pos, int n) {
     const int V = dc->m->cfg.vocab_size;
     if (n < 1 || n > dc->max_rows) return set_error(CIH_ERR_CAPACITY, "%d rows outside [1, %d]", n, dc->max_rows);
-    // a call before this one may still be copying the staged arrays
-    if (dc->kv.on) HIPCHK(hipStreamSynchronize(dc->m->stream));
+    // rows before these may still be on their way from the staged arrays (a prompt's chunks)
+    HIPCHK(hipStreamSynchronize(dc->m->stream));
     std::map<int, int> next;  // slot -> next position this call may write
     for (int i = 0; i < n; i++) {
         const int s = slots[i], p = pos[i], t = tokens[i];

@@ -382,3 +382,20 @@ def test_prefill_has_room_for_its_splits(d, F, rows, monkeypatch):
     assert np.abs(got[0] - got[1]).max() <= 1e-5 * max(1.0, np.abs(got[1]).max())
     dec.close()
     m.close()
+
+
+def test_prompt_in_many_chunks_fp32_weights():
+    """A prompt that goes through in chunks of few rows leaves the keys and values that one call leaves (FP32 rounding
+    of other kernels: 1e-4 of the largest)."""
+    cfg = ch.EsmConfig(128, 512, 2, 4)
+    m = ch.GpuModel(cfg, ch.EsmWeights.random(cfg, seed=8, std=0.06, bias_std=0.02), max_batch=1, max_len=16)
+    t = np.concatenate([[0], 4 + np.random.default_rng(8).integers(0, 20, 60)]).astype(np.int32)
+    a, b = (ch.GpuDecoder(m, n_slots=1, max_len=80, max_rows=r) for r in (4, 64))
+    for d in (a, b):
+        d.generate([t], 0.0, 0, [1])
+    for layer in range(2):
+        for x, y in zip(a.read_cache(layer, 0, 0, 61), b.read_cache(layer, 0, 0, 61)):
+            assert np.abs(x - y).max() <= 1e-4 * np.abs(y).max()
+    a.close()
+    b.close()
+    m.close()
