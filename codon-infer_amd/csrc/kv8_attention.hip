@@ -16,19 +16,21 @@
 // their lane.
 //
 // k_kv8_attend (few columns: single tokens).  Keys are split over waves and
-// workgroups.  The weights are bytes as well, three of them, P = 127 256^2 at the largest of the page (two
-// would do for bfloat16 but not for float16, and the third costs nothing where the codes' bytes bound it): p v is exact,
-// and each page joins the running output with exp(max of the page - running max)
-// times its V scale in FP32.  Bound by reading the codes once: 64 sequences of
-// 1025 to 7500 tokens, 32 heads over 8 of 128, bfloat16, 143 us (4.2 TB/s); one
-// of 65003, 40 heads of 64, float16, 70 us (4.75 TB/s, what a copy reaches).
-// One page of 20 heads of 16 takes 4 us, all latency.
+// workgroups.  The weights are bytes as well, three of them, P = 127 256^2 at the
+// largest of the page: p v is exact, and each page joins the running output with
+// exp(max of the page - running max) times its V scale in FP32.  (Two bytes would do for
+// bfloat16 rows, but what they round away shows in float16; the third costs 1% where the codes'
+// bytes are the bound.)  Bound by reading the codes once: 64 sequences of 1025 to
+// 8190 tokens, 32 heads over 8 of 128, bfloat16, 146 us (4.15 TB/s); one of 65003, 40 heads of
+// 64, float16, 70 us (4.75 TB/s, what a copy reaches).  One row of 131 tokens, 20 heads of 16, takes
+// 5.2 us, all latency.
 //
-// k_kv8_prompt (many columns).  V's codes become f16 and the weights f16 (FP32
-// and float16 rows: two f16, hi + lo; one has 11 bits, three more than a bfloat16 row keeps); a page's sums join the running
-// output in FP32.  Bound by instruction issue, the exponentials and the weights'
-// conversions: 2047 rows of 16000 keys, 32 heads over 8 of 128, bfloat16, 567 us
-// (886 TFLOP/s); 131 to 512 rows of 8 sequences, 20 heads of 64, FP32, 22 us.
+// k_kv8_prompt (many columns).  V's codes become f16 and the weights f16 (FP32 and
+// float16 rows: two f16, hi + lo; one has 11 bits, three more than a bfloat16 row
+// keeps); a page's sums join the running output in FP32.  Bound by instruction
+// issue, the exponentials and the weights' conversions: 2047 rows of 16000 keys, 32 heads over 8
+// of 128, bfloat16, 600 us (837 TFLOP/s), float16 776; 131 to 512 rows of 8
+// sequences, 20 heads of 64, FP32, 23 us.
 #include <float.h>
 #include <stdlib.h>
 #include <string.h>
@@ -999,16 +1001,16 @@ struct Plan {
 };
 // Prompts: k_kv8_prompt where the columns alone fill the GPU, or are more than
 // 64 and the keys long enough to be split (us, FP32 rows, 20 heads of 64, the one
-// kernel and the other: 2 sequences of 512 rows 18.7 and 13.4, 256 rows of 4096 keys
-// 36.7 and 30.4, but 512 of 1024 16.9 and 19.8, 64 of 1024 10.3 and 15.7).  Its
+// kernel and the other: 2 sequences of 512 rows 21.5 and 15.1, 256 rows of 4096 keys
+// 35.3 and 33.7, but 512 of 1024 19.7 and 23.6, 64 of 1024 10.8 and 22.7).  Its
 // pages are split until the workgroups are as many as run at once (two a CU for heads of
 // 128, else four), not below 8 pages each (512 rows of 65536 keys, 32 over 8 heads
-// of 128: FP32 3082 unsplit, 867; bfloat16 1420, 608), and only from 32 pages on (1000
-// rows of 1000 keys: 18.1 unsplit, 29.8).
+// of 128: FP32 2861 unsplit, 921; bfloat16 1945, 648), and only from 32 pages on (1000
+// rows of 1000 keys, when that was measured: 18.1 unsplit, 29.8; now 23.7 unsplit).
 //
 // Few columns: splits of 16 to 64 pages, a wave's 4 to 16, so that there are some
 // 2048 workgroups; shorter ones cost more in the join than they gain (8 single tokens of 700, 20
-// heads of 64: 8.4 us, with 8 pages 12.1), and from 4096 tiles on none is split.
+// heads of 64: 8.0 us, with 8 pages 12.1), and from 4096 tiles on none is split.
 Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window, bool step, size_t ws_floats) {
     Plan p;
     p.g = heads / c.hk;
@@ -1059,7 +1061,7 @@ hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t 
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     // A wave a row where the rows fill the GPU or the splits are few (20 heads of 64, 1024 rows
-    // in three splits: 76 us, by four waves 104), else four (128 rows of heads, 16 splits: 26.9, by one 28.6).
+    // of 6100 keys: 107 us, by four waves 137), else four (6 rows of 16000 keys, 16 splits: 17.7, by one 18.6).
     if (p.splits <= 8 || rows >= 8192)
         hipLaunchKernelGGL((k_kv8_join<DP, T, 1>), dim3((rows + JOIN_WAVES - 1) / JOIN_WAVES), dim3(64 * JOIN_WAVES), 0, st, a,
                            p.g, p.cols, p.splits, p.pps, ws);

@@ -5,7 +5,8 @@
 //   log p(i) = x_i - m - ln 2 log2 s,  entropy = ln 2 (log2 s - t / s).
 // A NaN or +inf anywhere makes s NaN.  Bound by reading the logits once, and close
 // to it by the seven operations a logit: 512 rows of 131072 bfloat16 logits 26 us without
-// alternatives, 31 with 20 (4.3 TB/s), 40 with 64; 8192 rows of 33, 7.6 us, mostly latency.
+// alternatives, 31 with 20 (4.3 TB/s), 40 with 64; 8192 rows of 33, 7.4 us: eight waves a SIMD,
+// each with as many steps of the count of better logits as there are logits.
 #include <limits.h>
 
 #include <algorithm>

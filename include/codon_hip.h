@@ -226,7 +226,9 @@ int cih_dms(cih_model *m, const int32_t *residues, int32_t n, int32_t window, in
  * the null stream), return without waiting, allocate nothing and keep nothing
  * between calls, so that they may be captured into a graph.  Sizes on the host
  * (n_seq, n_rows, max_rows, max_pages) fix the grids; row offsets, lengths and
- * tables are read on the device when the kernels run. */
+ * tables are read on the device when the kernels run.  A call whose grid would
+ * pass 2^24 workgroups (n_seq * kv_heads * the pages of 64, or the tiles of 16 rows
+ * times q_heads / kv_heads, that max_rows make) returns CIH_ERR_HIP. */
 
 enum cih_float { CIH_F32 = 0, CIH_F16 = 1, CIH_BF16 = 2 };
 
