@@ -895,10 +895,10 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         if (move) {
 #pragma unroll
             for (int t = 0; t < CT; t++) {
-                const float mp = groups_max(x[t]);
+                const float mp = ceilf(groups_max(x[t]));  // whole: sums are scaled by powers of two
                 top[t] = fmaxf(top[t], mp);
                 most[t] = fmaxf(most[t], mp + (float)ex);
-                float wn = mp > w[t] + SLACK || mp < w[t] - NEAR ? mp : w[t];
+                float wn = mp > w[t] + SLACK || mp <= w[t] - NEAR ? mp : w[t];
                 wn = fmaxf(wn, top[t] - ROOM);
                 const int un = max(ex, (int)fminf(fmaxf(most[t] - ROOM - wn, (float)NO_EXP), (float)-NO_EXP));
                 const bool seen = mp > -INFINITY;
