@@ -35,6 +35,8 @@ EXPORTED = [
     "cih_matmul_tiled_noalloc", "cih_rope_init", "cih_kv8_append", "cih_kv8_read", "cih_kv8_attention",
     "cih_kv8_attention_workspace", "cih_token_logprobs", "cih_token_logprobs_workspace",
     "cih_decoder_create_kv8", "cih_decoder_score", "cih_decoder_read_cache",
+    "cih_kv8_append_shifted", "cih_kv8_attention_sinks", "cih_kv8_weigh", "cih_kv8_evict", "cih_kv8_evict_workspace",
+    "cih_verify_drafts", "cih_verify_drafts_workspace",
 ]
 
 DMS_MASKED_MARGINAL, DMS_WILDTYPE_MARGINAL = 0, 1
@@ -134,6 +136,13 @@ def lib():
         "cih_kv8_read": [vp, vp, i32, vp, vp, vp],
         "cih_kv8_attention": [vp, vp, i32, i32, vp, vp, vp, f32, i32, i32, vp, ctypes.c_size_t, vp],
         "cih_kv8_attention_workspace": [vp, vp, i32, ctypes.POINTER(ctypes.c_size_t)],
+        "cih_kv8_append_shifted": [vp, vp, i32, vp, vp, i32, vp, vp, vp, vp, vp],
+        "cih_kv8_attention_sinks": [vp, vp, i32, i32, vp, vp, vp, f32, i32, i32, i32, vp, ctypes.c_size_t, vp],
+        "cih_kv8_weigh": [vp, vp, i32, i32, vp, vp, f32, i32, i32, i32, f32, vp, vp],
+        "cih_kv8_evict": [vp, vp, i32, i32, i32, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp],
+        "cih_kv8_evict_workspace": [vp, vp, i32, ctypes.POINTER(ctypes.c_size_t)],
+        "cih_verify_drafts": [i32, vp, i64, vp, i64, i32, i32, i32, vp, vp, vp, vp, f32, vp, vp, vp, ctypes.c_size_t, vp],
+        "cih_verify_drafts_workspace": [i32, i32, i32, ctypes.POINTER(ctypes.c_size_t)],
         "cih_token_logprobs": [i32, vp, i64, i32, i32, vp, vp, vp, i32, vp, vp, vp, ctypes.c_size_t, vp],
         "cih_token_logprobs_workspace": [i32, i32, i32, ctypes.POINTER(ctypes.c_size_t)],
         "cih_dequantize_device": [i32, vp, i64, vp],

@@ -1,7 +1,9 @@
 """The device operators of the C ABI on arrays in GPU memory: the 8-bit paged
 key/value cache with rotary positions (cih_kv8_append, cih_kv8_read), attention
-over it (cih_kv8_attention) and the log probabilities of given tokens
-(cih_token_logprobs).  None of them has a counterpart in the reference.
+over it (cih_kv8_attention), the attention weight that its tokens gather and
+eviction by it (cih_kv8_weigh, cih_kv8_evict), the log probabilities of given
+tokens (cih_token_logprobs) and the verification of drafted ones
+(cih_verify_drafts).  None of them has a counterpart in the reference.
 
 Arrays are anything with data_ptr(), shape, stride() in elements and dtype:
 torch tensors on the GPU, or devmem.DeviceArray.  Outputs are written into
@@ -161,8 +163,9 @@ class Kv8Batch:
         if _dtype(table) != "int32":
             raise TypeError(f"table is {_dtype(table)}: int32 is needed")
         stride = table.stride()[0] if table.shape[0] > 1 else table.shape[1]
+        self.lens = lens
         self._arrays = (cu_rows, lens, table) + (() if slots is None else (slots,))
-        self.n_rows = n_rows
+        self.n_rows, self.n_seq = n_rows, n
         self.struct = C.Kv8BatchStruct(_plain(cu_rows, "cu_rows", i32, (n + 1,)), _plain(lens, "lens", i32, (n,)),
                                        table.data_ptr(), None if slots is None else _plain(slots, "slots", i32, (n,)),
                                        n, n_rows, max_rows, table.shape[0], stride, table.shape[1])
@@ -188,16 +191,18 @@ class Kv8Cache:
         self._at = _at(self.struct)
         self._gpu = _where(self._arrays)
         self._scale = head_dim ** -0.5
+        self._weights = (n, h, page)
 
     @staticmethod
     def dims(head_dim):
         """Dims of a head as stored."""
         return 32 if head_dim == 24 else head_dim
 
-    def append(self, batch, k, v, q=None, q_out=None, rope=None, stream=None):
+    def append(self, batch, k, v, q=None, q_out=None, rope=None, stream=None, shifts=None):
         """Writes the batch's rows k and v [n_rows][kv_heads][head_dim] into the
         cache at their positions, k rotated by rope; q [n_rows][q_heads][head_dim]
-        rotated goes to q_out (default: q itself)."""
+        rotated goes to q_out (default: q itself).  shifts: int32 [n_seq], added to
+        a sequence's positions for their angles (what evict took)."""
         t, shape = _float(k, "k"), (batch.n_rows, self.kv_heads, self.head_dim)
         ks, vs = _rows(k, "k", shape), _rows(v, "v", shape)
         if _float(v, "v") != t:
@@ -211,10 +216,12 @@ class Kv8Cache:
             qs, qo = _rows(q, "q", shape), _rows(q_out, "q_out", shape)
             if _float(q, "q") != t or _float(q_out, "q_out") != t:
                 raise TypeError("q, q_out and k differ in type")
-        at = _same(_same(_where((k, v) if q is None else (k, v, q, q_out)), self._gpu), batch._gpu)
+        sh = None if shifts is None else _plain(shifts, "shifts", ("int32",), (batch.n_seq,))
+        at = _same(_same(_where((k, v, shifts) if q is None else (k, v, q, q_out, shifts)), self._gpu), batch._gpu)
         a = _at
-        C.check(_lib.cih_kv8_append(self._at, batch._at, t, a(ks), a(vs), heads, a(qs) if qs else None,
-                                       a(qo) if qo else None, a(rope.struct) if rope else None, _stream(at, stream)))
+        C.check(_lib.cih_kv8_append_shifted(self._at, batch._at, t, a(ks), a(vs), heads, a(qs) if qs else None,
+                                            a(qo) if qo else None, a(rope.struct) if rope else None, sh,
+                                            _stream(at, stream)))
 
     def read(self, batch, k, v, stream=None):
         """The batch's rows read back into k and v [n_rows][kv_heads][head_dim]."""
@@ -232,11 +239,11 @@ class Kv8Cache:
         C.check(_lib.cih_kv8_attention_workspace(self._at, batch._at, q_heads, ctypes.byref(n)))
         return n.value
 
-    def attend(self, batch, q, out, lse=None, scale=None, causal=True, window=0, workspace=None, stream=None):
+    def attend(self, batch, q, out, lse=None, scale=None, causal=True, window=0, workspace=None, stream=None, sinks=0):
         """Attention of the batch's rows q [n_rows][q_heads][head_dim] over the
         cache into out (q's shape and type) and lse float32 [n_rows][q_heads].
-        scale: default 1 / sqrt(head_dim).  workspace: uint8, of attend_workspace
-        bytes at least."""
+        scale: default 1 / sqrt(head_dim).  sinks: first tokens that a window
+        leaves visible.  workspace: uint8, of attend_workspace bytes at least."""
         t, heads = _float(q, "q"), q.shape[1]
         shape = (batch.n_rows, heads, self.head_dim)
         qs, os = _rows(q, "q", shape), _rows(out, "out", shape)
@@ -245,9 +252,52 @@ class Kv8Cache:
         ls = None if lse is None else _plain(lse, "lse", ("float32",), shape[:2])
         ws, size = _workspace(workspace)
         at = _same(_same(_where((q, out, lse, workspace)), self._gpu), batch._gpu)
-        C.check(_lib.cih_kv8_attention(self._at, batch._at, t, heads, _at(qs), _at(os), ls,
-                                          self._scale if scale is None else scale, 1 if causal else 0, window, ws, size,
-                                          _stream(at, stream)))
+        C.check(_lib.cih_kv8_attention_sinks(self._at, batch._at, t, heads, _at(qs), _at(os), ls,
+                                             self._scale if scale is None else scale, 1 if causal else 0, window, sinks,
+                                             ws, size, _stream(at, stream)))
+
+    def weigh(self, batch, q, lse, weights, scale=None, causal=True, window=0, sinks=0, keep=1.0, stream=None):
+        """Adds to weights (float32 [n_pages][kv_heads][64], beside the cache) what
+        the batch's rows q give each token they see: the sum of exp(scale q.k - lse)
+        over rows and the query heads of a kv head, with lse [n_rows][q_heads] from
+        attend with the same arguments.  keep: the share that earlier weights keep
+        (0: start anew)."""
+        t, heads = _float(q, "q"), q.shape[1]
+        shape = (batch.n_rows, heads, self.head_dim)
+        qs = _rows(q, "q", shape)
+        ls = _plain(lse, "lse", ("float32",), shape[:2])
+        wt = _plain(weights, "weights", ("float32",), self._weights)
+        at = _same(_same(_where((q, lse, weights)), self._gpu), batch._gpu)
+        C.check(_lib.cih_kv8_weigh(self._at, batch._at, t, heads, _at(qs), ls, self._scale if scale is None else scale,
+                                   1 if causal else 0, window, sinks, keep, wt, _stream(at, stream)))
+
+    def evict_workspace(self, batch, budget):
+        """Bytes of workspace that evict needs for a batch of these sizes."""
+        n = ctypes.c_size_t()
+        C.check(_lib.cih_kv8_evict_workspace(self._at, batch._at, budget, ctypes.byref(n)))
+        return n.value
+
+    def evict(self, batch, weights, budget, first=0, recent=0, weights_out=None, lens_out=None, shifts=None, kept=None,
+              workspace=None, stream=None):
+        """Cuts the batch's sequences to at most budget tokens: each kv head keeps its
+        first `first`, its last `recent` and of the others those with the largest
+        weights, in their order.  The kept tokens' weights go to weights_out
+        (default: weights itself), the new lengths to lens_out (default: the
+        batch's lens), how many tokens went is added to shifts (int32 [n_seq]), the
+        places that the kept ones had go to kept (int32 [n_seq][kv_heads][budget],
+        -1 behind them)."""
+        n, i32 = batch.n_seq, ("int32",)
+        weights_out = weights if weights_out is None else weights_out
+        lens_out = batch.lens if lens_out is None else lens_out
+        wt = _plain(weights, "weights", ("float32",), self._weights)
+        wo = _plain(weights_out, "weights_out", ("float32",), self._weights)
+        lo = _plain(lens_out, "lens_out", i32, (n,))
+        sh = None if shifts is None else _plain(shifts, "shifts", i32, (n,))
+        kp = None if kept is None else _plain(kept, "kept", i32, (n, self.kv_heads, budget))
+        ws, size = _workspace(workspace)
+        at = _same(_same(_where((weights, weights_out, lens_out, shifts, kept, workspace)), self._gpu), batch._gpu)
+        C.check(_lib.cih_kv8_evict(self._at, batch._at, budget, first, recent, wt, wo, lo, sh, kp, ws, size,
+                                   _stream(at, stream)))
 
 
 def _workspace(w):
@@ -287,3 +337,46 @@ def token_logprobs(logits, targets=None, logprob=None, entropy=None, top_ids=Non
     at = _where((logits, targets, logprob, entropy, top_ids, top_logprobs, workspace))
     C.check(_lib.cih_token_logprobs(_float(logits, "logits"), logits.data_ptr(), logits.stride()[0], n, vocab, tg, lp,
                                        en, k, ids, tl, ws, size, _stream(at, stream)))
+
+
+def verify_drafts_workspace(n_seq, n_drafts, vocab):
+    """Bytes of workspace that verify_drafts needs."""
+    n = ctypes.c_size_t()
+    C.check(_lib.cih_verify_drafts_workspace(n_seq, n_drafts, vocab, ctypes.byref(n)))
+    return n.value
+
+
+def verify_drafts(logits, drafts, cu_drafts, accepted, tokens, draft_logits=None, accept_at=None, sample_at=None,
+                  temperature=1.0, workspace=None, stream=None):
+    """Speculative sampling: of the drafts of sequence i (int32 [n_drafts], from
+    cu_drafts[i] to cu_drafts[i + 1]), how many are accepted (int32 [n_seq]) and the
+    token after them (int32 [n_seq]).  logits [n_drafts + n_seq][vocab]: the target's,
+    a row for each draft of a sequence and one after them; draft_logits
+    [n_drafts][vocab]: what the drafts were drawn from (None: they are certain).
+    accept_at float32 [n_drafts] and sample_at float32 [n_seq]: random numbers in
+    [0, 1), not needed at temperature 0."""
+    (n,), d, vocab = tokens.shape, drafts.shape[0], logits.shape[1]
+    f32, i32 = ("float32",), ("int32",)
+    t = _float(logits, "logits")
+    if logits.shape[0] != n + d:
+        raise ValueError(f"logits has {logits.shape[0]} rows: {n + d} are needed")
+    if vocab != 1 and logits.stride()[1] != 1:
+        raise ValueError("logits: the last axis must be contiguous")
+    dl, ds = None, 0
+    if draft_logits is not None:
+        if draft_logits.shape != (d, vocab):
+            raise ValueError(f"draft_logits has shape {tuple(draft_logits.shape)}: {(d, vocab)} is needed")
+        if vocab != 1 and draft_logits.stride()[1] != 1:
+            raise ValueError("draft_logits: the last axis must be contiguous")
+        if _float(draft_logits, "draft_logits") != t:
+            raise TypeError("logits and draft_logits differ in type")
+        dl, ds = draft_logits.data_ptr(), draft_logits.stride()[0]
+    dr = _plain(drafts, "drafts", i32, (d,))
+    cu = _plain(cu_drafts, "cu_drafts", i32, (n + 1,))
+    ac, tk = _plain(accepted, "accepted", i32, (n,)), _plain(tokens, "tokens", i32, (n,))
+    ua = None if accept_at is None else _plain(accept_at, "accept_at", f32, (d,))
+    us = None if sample_at is None else _plain(sample_at, "sample_at", f32, (n,))
+    ws, size = _workspace(workspace)
+    at = _where((logits, drafts, cu_drafts, accepted, tokens, draft_logits, accept_at, sample_at, workspace))
+    C.check(_lib.cih_verify_drafts(t, logits.data_ptr(), logits.stride()[0], dl, ds, n, d, vocab, cu, dr, ua, us,
+                                   temperature, ac, tk, ws, size, _stream(at, stream)))

@@ -64,6 +64,7 @@ struct RopeArg {
     int rot = 0, inter = 0;
     float gain = 1.0f;
     double turns[64] = {};
+    const int *shift = nullptr;  // [n_seq]: added to a sequence's positions
 };
 
 // r (NULL: no rotary positions) for heads of head_dim as the kernels take it; an error code and message if it is refused.
@@ -95,6 +96,12 @@ __device__ __forceinline__ int kv8_page(const Kv8View &c, const Kv8Seq &q, int p
     return id >= 0 && id < c.n_pages ? id : -1;
 }
 
+// The angle's position of token p of sequence i.
+__device__ __forceinline__ int rope_position(const RopeArg &r, int i, int p) {
+    if (!r.shift) return p;
+    const int64_t x = (int64_t)p + r.shift[i];
+    return (int)(x < INT32_MIN ? INT32_MIN : x > INT32_MAX - KV8_PAGE ? INT32_MAX - KV8_PAGE : x);
+}
 // cos and sin (times gain) of position p's angle at pair j.  The angle in
 // turns is reduced in 64 bits: at position 1e6 a 32-bit product is off by
 // 0.06 radians.
@@ -135,7 +142,7 @@ struct Kv8Attention {
     int dtype, heads, out_h2;
     float *lse;
     float scale;
-    int causal, window;
+    int causal, window, sinks;  // (sinks 0 without a window)
     int q16, out16;  // set by the launch: queries in 16-byte loads, output in stores of 4 dims
 };
 
@@ -157,6 +164,28 @@ hipError_t launch_kv8_read(const Kv8View &c, const Kv8Seqs &s, int dtype, const 
 hipError_t launch_kv8_attention(const Kv8Attention &a, float *ws, size_t ws_floats, hipStream_t st);
 size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads);
 
+// The attention weight of each cached token over the rows of `a` (out unused, lse
+// read) into weights [page][head][64]: a token before the rows keeps `keep` of what it had.
+struct Kv8Weigh {
+    Kv8Attention a;
+    float keep;
+    float *weights;
+};
+hipError_t launch_kv8_weigh(const Kv8Weigh &w, hipStream_t st);
+
+// Eviction to `budget` tokens a sequence and head: the first `first`, the last
+// `recent` and the best of the others by `weights`.
+struct Kv8Evict {
+    Kv8View c;
+    Kv8Seqs s;
+    int budget, first, recent;
+    const float *weights;
+    float *weights_out;
+    int *lens_out, *shifts, *kept;  // each may be nullptr
+};
+size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget);
+hipError_t launch_kv8_evict(const Kv8Evict &e, void *ws, hipStream_t st);
+
 constexpr int LOGPROBS_MAX_TOP = 64;
 struct TokenLogprobs {
     int dtype;
@@ -170,6 +199,21 @@ struct TokenLogprobs {
 };
 size_t token_logprobs_floats(int n, int vocab, int top);
 hipError_t launch_token_logprobs(const TokenLogprobs &a, float *ws, size_t ws_floats, hipStream_t st);
+
+// Verification of drafted tokens: sequence i has drafts [cu[i], cu[i + 1]) and the
+// target's rows from cu[i] + i on, one more.
+struct VerifyDrafts {
+    int dtype;
+    const void *logits, *draft;  // draft nullptr: the drafted token is certain
+    int64_t stride, draft_stride;
+    int n_seq, n_drafts, vocab;
+    const int *cu, *drafted;
+    const float *accept_at, *sample_at;
+    float temperature;
+    int *accepted, *tokens;
+};
+size_t verify_drafts_bytes(int n_seq, int n_drafts, int vocab);
+hipError_t launch_verify_drafts(const VerifyDrafts &v, void *ws, hipStream_t st);
 
 // Element types of the row tensors.
 enum { FT_F32 = 0, FT_F16 = 1, FT_BF16 = 2 };

@@ -37,12 +37,13 @@ __device__ __forceinline__ void pair_dims(const RopeArg &r, int j, int &i0, int 
 // [lo, hi) (in the page).  Pages a sequence's rows can touch: per_seq.
 struct PageTask {
     Kv8Seq q;
-    int h, pg, lo, hi;
+    int i, h, pg, lo, hi;
 };
 __device__ __forceinline__ bool page_task(const Kv8View &c, const Kv8Seqs &s, int per_seq, PageTask &t) {
     const int b = blockIdx.x, rest = b / c.hk;
     t.h = b - rest * c.hk;
     const int i = rest / per_seq;
+    t.i = i;
     t.q = kv8_seq(s, i);
     const int first = max(t.q.start, 0);
     if (first >= t.q.len) return false;
@@ -63,6 +64,7 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv8_append(Kv8View c, Kv8Seqs s,
     const int nt = t.hi - t.lo, d = c.d, tid = threadIdx.x, half = d / 2;
     const int p0 = t.pg * KV8_PAGE + t.lo;          // position of the first new token
     const int64_t row0 = t.q.r0 + (p0 - t.q.start);  // and its row
+    const int turn0 = rope_position(rope, t.i, p0);
     float *kf = sm;                                  // [nt][d]: K, rotated
     unsigned char *vq = reinterpret_cast<unsigned char *>(sm + nt * d);  // [d][VQ]: V's codes, by dim
     if (tid == 0) sbad = 0;
@@ -78,7 +80,7 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv8_append(Kv8View c, Kv8Seqs s,
         float cs = 1.0f, sn = 0.0f;
         const bool turn = 2 * j < rope.rot;
         if (turn) {
-            rope_cs(rope, p0 + n, j, cs, sn);
+            rope_cs(rope, turn0 + n, j, cs, sn);
             const float y0 = x0 * cs - x1 * sn;
             x1 = x1 * cs + x0 * sn;
             x0 = y0;
@@ -221,6 +223,7 @@ __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, Row
     const int nt = t.hi - t.lo, d = c.d, tid = threadIdx.x;
     const int p0 = t.pg * KV8_PAGE + t.lo;
     const int64_t row0 = t.q.r0 + (p0 - t.q.start);
+    const int turn0 = rope_position(rope, t.i, p0);
     const int id = kv8_page(c, t.q, t.pg);
     const int64_t ph = (int64_t)max(id, 0) * c.hk + t.h;
     float2 old = {0.0f, 0.0f};
@@ -297,7 +300,7 @@ __global__ __launch_bounds__(NT) void k_kv8_append_vec(Kv8View c, Kv8Seqs s, Row
             float cs[VL], sn[VL];
             if (turn) {
 #pragma unroll
-                for (int e = 0; e < VL; e++) rope_cs(rope, p0 + n, (rope.inter ? da / 2 : da) + e, cs[e], sn[e]);
+                for (int e = 0; e < VL; e++) rope_cs(rope, turn0 + n, (rope.inter ? da / 2 : da) + e, cs[e], sn[e]);
                 rotate(kx[it][0], kx[it][1], cs, sn);
             }
             if (q.p)

@@ -1,5 +1,5 @@
-// C entries of the 8-bit paged key/value cache and of the token log
-// probabilities: argument checks on the host, then the launches.
+// C entries of the 8-bit paged key/value cache, of the token log probabilities and
+// of the verification of drafts: argument checks on the host, then the launches.
 #include <cmath>
 
 #include "kv8.h"
@@ -93,6 +93,32 @@ int check_heads(int heads, int hk, const Kv8Seqs &s) {
     return 0;
 }
 
+// What attention and the weights that it leaves have in common.
+int check_call(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int dtype, int heads, float scale, int causal,
+               int window, int sinks, Kv8Attention &a) {
+    if (int rc = check_float(dtype)) return rc;
+    if (int rc = check_cache(cache, a.c, true)) return rc;
+    if (int rc = check_batch(batch, a.s, true)) return rc;
+    if (int rc = check_heads(heads, a.c.hk, a.s)) return rc;
+    if (window < 0) return set_error(CIH_ERR_ARG, "window %d", window);
+    if (sinks < 0) return set_error(CIH_ERR_ARG, "%d sinks", sinks);
+    if (!std::isfinite(scale)) return set_error(CIH_ERR_ARG, "the scale is not finite");
+    a.dtype = dtype;
+    a.heads = heads;
+    a.scale = scale;
+    a.causal = causal != 0;
+    a.window = window;
+    a.sinks = window > 0 ? sinks : 0;  // without a window all of them are visible anyway
+    return 0;
+}
+
+int check_budget(int budget, int first, int recent) {
+    if (budget < 1 || budget > 1 << 30) return set_error(CIH_ERR_SHAPE, "a budget of %d tokens", budget);
+    if (first < 0 || recent < 0 || (int64_t)first + recent > budget)
+        return set_error(CIH_ERR_ARG, "%d first and %d recent tokens in a budget of %d", first, recent, budget);
+    return 0;
+}
+
 }  // namespace
 
 int cih::kv8_rope(const cih_rope *r, int head_dim, RopeArg &a) {
@@ -147,9 +173,9 @@ int cih_rope_init(cih_rope *r, int32_t rot_dim, int32_t interleaved, double base
     return CIH_OK;
 }
 
-int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
-                   const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out, const cih_rope *rope,
-                   void *stream) {
+int cih_kv8_append_shifted(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
+                           const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out,
+                           const cih_rope *rope, const int32_t *shifts, void *stream) {
     Kv8View c;
     Kv8Seqs s;
     RowsView kv, vv, qv{}, qo{};
@@ -158,6 +184,8 @@ int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32
     CIH_TRY(check_cache(cache, c, true));
     CIH_TRY(check_batch(batch, s, true));
     CIH_TRY(kv8_rope(rope, c.d, ra));
+    if (!aligned(shifts, 4)) return set_error(CIH_ERR_ARG, "shifts must be 4-byte aligned");
+    ra.shift = shifts;
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return CIH_OK;
     CIH_TRY(check_rows(k, "k", dtype, kv));
     CIH_TRY(check_rows(v, "v", dtype, vv));
@@ -174,6 +202,12 @@ int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32
     const hipError_t e = launch_kv8_append(c, s, dtype, kv, vv, q ? q_heads : c.hk, qv, qo, ra, st);
     if (e != hipSuccess) return set_error(CIH_ERR_HIP, "cache append failed: %s", hipGetErrorString(e));
     return CIH_OK;
+}
+
+int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
+                   const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out, const cih_rope *rope,
+                   void *stream) {
+    return cih_kv8_append_shifted(cache, batch, dtype, k, v, q_heads, q, q_out, rope, nullptr, stream);
 }
 
 int cih_kv8_read(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
@@ -207,16 +241,11 @@ int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch 
     return CIH_OK;
 }
 
-int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
-                      const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal, int32_t window,
-                      void *workspace, size_t workspace_bytes, void *stream) {
+int cih_kv8_attention_sinks(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
+                            const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal,
+                            int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *stream) {
     Kv8Attention a{};
-    CIH_TRY(check_float(dtype));
-    CIH_TRY(check_cache(cache, a.c, true));
-    CIH_TRY(check_batch(batch, a.s, true));
-    CIH_TRY(check_heads(q_heads, a.c.hk, a.s));
-    if (window < 0) return set_error(CIH_ERR_ARG, "window %d", window);
-    if (!std::isfinite(scale)) return set_error(CIH_ERR_ARG, "the scale is not finite");
+    CIH_TRY(check_call(cache, batch, dtype, q_heads, scale, causal, window, sinks, a));
     if (a.s.n_rows == 0 || a.s.n_seq == 0 || a.s.max_rows == 0) return CIH_OK;
     CIH_TRY(check_rows(q, "q", dtype, a.q));
     CIH_TRY(check_rows(out, "out", dtype, a.out));
@@ -227,16 +256,78 @@ int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, in
     const size_t need = kv8_attention_floats(a.c, a.s, q_heads) * sizeof(float);
     if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
         return set_error(CIH_ERR_CAPACITY, "the call needs a 16-byte aligned workspace of %zu bytes", need);
-    a.dtype = dtype;
-    a.heads = q_heads;
     a.lse = lse;
-    a.scale = scale;
-    a.causal = causal != 0;
-    a.window = window;
     hipStream_t st = static_cast<hipStream_t>(stream);
     CIH_TRY(check_stream(st));
-    const hipError_t e = launch_kv8_attention(a, static_cast<float *>(workspace), workspace_bytes / sizeof(float), st);
+    const hipError_t e = launch_kv8_attention(a, static_cast<float *>(workspace), need > 0 ? workspace_bytes / sizeof(float) : 0, st);
     if (e != hipSuccess) return set_error(CIH_ERR_HIP, "attention over the cache failed: %s", hipGetErrorString(e));
+    return CIH_OK;
+}
+
+int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
+                      const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal, int32_t window,
+                      void *workspace, size_t workspace_bytes, void *stream) {
+    return cih_kv8_attention_sinks(cache, batch, dtype, q_heads, q, out, lse, scale, causal, window, 0, workspace,
+                                   workspace_bytes, stream);
+}
+
+int cih_kv8_weigh(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
+                  const cih_rows *q, const float *lse, float scale, int32_t causal, int32_t window, int32_t sinks,
+                  float keep, float *weights, void *stream) {
+    Kv8Weigh w{};
+    CIH_TRY(check_call(cache, batch, dtype, q_heads, scale, causal, window, sinks, w.a));
+    if (!(keep >= 0.0f && keep <= 1.0f)) return set_error(CIH_ERR_ARG, "keep is not within [0, 1]");
+    if (w.a.s.n_rows == 0 || w.a.s.n_seq == 0 || w.a.s.max_rows == 0) return CIH_OK;
+    CIH_TRY(check_rows(q, "q", dtype, w.a.q));
+    if (!lse || !weights) return set_error(CIH_ERR_ARG, "null %s", lse ? "weights" : "lse");
+    if (!aligned(lse, 4) || !aligned(weights, 4)) return set_error(CIH_ERR_ARG, "lse and weights must be 4-byte aligned");
+    w.a.lse = const_cast<float *>(lse);
+    w.keep = keep;
+    w.weights = weights;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    CIH_TRY(check_stream(st));
+    const hipError_t e = launch_kv8_weigh(w, st);
+    if (e != hipSuccess) return set_error(CIH_ERR_HIP, "weighing the cache failed: %s", hipGetErrorString(e));
+    return CIH_OK;
+}
+
+int cih_kv8_evict_workspace(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t budget, size_t *bytes) {
+    Kv8View c;
+    Kv8Seqs s;
+    if (!bytes) return set_error(CIH_ERR_ARG, "null bytes");
+    CIH_TRY(check_cache(cache, c, false));
+    CIH_TRY(check_batch(batch, s, false));
+    CIH_TRY(check_budget(budget, 0, 0));
+    *bytes = kv8_evict_bytes(c, s, budget);
+    return CIH_OK;
+}
+
+int cih_kv8_evict(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t budget, int32_t first, int32_t recent,
+                  const float *weights, float *weights_out, int32_t *lens_out, int32_t *shifts, int32_t *kept,
+                  void *workspace, size_t workspace_bytes, void *stream) {
+    Kv8Evict e{};
+    CIH_TRY(check_cache(cache, e.c, true));
+    CIH_TRY(check_batch(batch, e.s, true));
+    CIH_TRY(check_budget(budget, first, recent));
+    if (e.s.n_seq == 0) return CIH_OK;
+    if (!weights || !lens_out) return set_error(CIH_ERR_ARG, "null %s", weights ? "lens_out" : "weights");
+    if (!aligned(weights, 4) || !aligned(weights_out, 4) || !aligned(lens_out, 4) || !aligned(shifts, 4) || !aligned(kept, 4))
+        return set_error(CIH_ERR_ARG, "weights, lens_out, shifts and kept must be 4-byte aligned");
+    const size_t need = kv8_evict_bytes(e.c, e.s, budget);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return set_error(CIH_ERR_CAPACITY, "the call needs a 16-byte aligned workspace of %zu bytes", need);
+    e.budget = budget;
+    e.first = first;
+    e.recent = recent;
+    e.weights = weights;
+    e.weights_out = weights_out;
+    e.lens_out = lens_out;
+    e.shifts = shifts;
+    e.kept = kept;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    CIH_TRY(check_stream(st));
+    const hipError_t rc = launch_kv8_evict(e, workspace, st);
+    if (rc != hipSuccess) return set_error(CIH_ERR_HIP, "eviction from the cache failed: %s", hipGetErrorString(rc));
     return CIH_OK;
 }
 
@@ -269,6 +360,47 @@ int cih_token_logprobs(int32_t dtype, const void *logits, int64_t row_stride, in
     const TokenLogprobs a{dtype, logits, n_rows > 1 ? row_stride : 0, n_rows, vocab, top_k, targets, logprob, entropy, top_ids, top_logprobs};
     const hipError_t e = launch_token_logprobs(a, static_cast<float *>(workspace), workspace_bytes / sizeof(float), st);
     if (e != hipSuccess) return set_error(CIH_ERR_HIP, "token log probabilities failed: %s", hipGetErrorString(e));
+    return CIH_OK;
+}
+
+int cih_verify_drafts_workspace(int32_t n_seq, int32_t n_drafts, int32_t vocab, size_t *bytes) {
+    if (!bytes) return set_error(CIH_ERR_ARG, "null bytes");
+    if (n_seq < 0 || n_seq > 1 << 24 || n_drafts < 0 || n_drafts > 1 << 24 || vocab < 1 || vocab > 1 << 30)
+        return set_error(CIH_ERR_SHAPE, "%d drafts of %d sequences over %d tokens", n_drafts, n_seq, vocab);
+    *bytes = verify_drafts_bytes(n_seq, n_drafts, vocab);
+    return CIH_OK;
+}
+
+int cih_verify_drafts(int32_t dtype, const void *logits, int64_t row_stride, const void *draft_logits,
+                      int64_t draft_stride, int32_t n_seq, int32_t n_drafts, int32_t vocab, const int32_t *cu_drafts,
+                      const int32_t *drafts, const float *accept_at, const float *sample_at, float temperature,
+                      int32_t *accepted, int32_t *tokens, void *workspace, size_t workspace_bytes, void *stream) {
+    size_t need = 0;
+    CIH_TRY(check_float(dtype));
+    CIH_TRY(cih_verify_drafts_workspace(n_seq, n_drafts, vocab, &need));
+    if (!(temperature >= 0.0f) || !std::isfinite(temperature)) return set_error(CIH_ERR_ARG, "the temperature must be finite and not negative");
+    if (n_seq == 0) return CIH_OK;
+    const bool draws = temperature > 0.0f;
+    if (!draws) draft_logits = nullptr;
+    if (!logits || !cu_drafts || !accepted || !tokens || (n_drafts > 0 && !drafts) || (draws && !sample_at) ||
+        (draws && n_drafts > 0 && !accept_at))
+        return set_error(CIH_ERR_ARG, "null argument");
+    const int64_t most = (int64_t)1 << 31;
+    if ((row_stride < vocab && (int64_t)n_seq + n_drafts > 1) || row_stride > most)
+        return set_error(CIH_ERR_SHAPE, "rows of %d logits, %lld apart", vocab, (long long)row_stride);
+    if (draft_logits && n_drafts > 0 && ((draft_stride < vocab && n_drafts > 1) || draft_stride > most))
+        return set_error(CIH_ERR_SHAPE, "draft rows of %d logits, %lld apart", vocab, (long long)draft_stride);
+    if (!aligned(logits, float_size(dtype)) || !aligned(draft_logits, float_size(dtype)) || !aligned(cu_drafts, 4) ||
+        !aligned(drafts, 4) || !aligned(accept_at, 4) || !aligned(sample_at, 4) || !aligned(accepted, 4) || !aligned(tokens, 4))
+        return set_error(CIH_ERR_ARG, "an argument is not aligned to its type");
+    if (need > 0 && (!workspace || !aligned(workspace, 16) || workspace_bytes < need))
+        return set_error(CIH_ERR_CAPACITY, "the call needs a 16-byte aligned workspace of %zu bytes", need);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    CIH_TRY(check_stream(st));
+    const VerifyDrafts v{dtype, logits, draft_logits, row_stride, draft_stride, n_seq, n_drafts, vocab, cu_drafts,
+                         drafts, accept_at, sample_at, temperature, accepted, tokens};
+    const hipError_t e = launch_verify_drafts(v, workspace, st);
+    if (e != hipSuccess) return set_error(CIH_ERR_HIP, "the verification of drafts failed: %s", hipGetErrorString(e));
     return CIH_OK;
 }
 

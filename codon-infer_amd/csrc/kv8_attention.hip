@@ -39,62 +39,18 @@
 
 #include "kernels.h"
 #include "kv8.h"
+#include "kv8_tiles.h"
 #include "x3.h"
 
 namespace cih {
 
 namespace {
 
-typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
-
-// max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (the swaps exchange lane
-// halves between two registers: w is v in a register of its own)
-template <class OP> __device__ __forceinline__ float groups(float v, OP op) {
-    float w = v;
-    asm volatile("" : "+v"(w));
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(w), false, false);
-    const unsigned r0 = r[0], r1 = r[1];
-    v = op(__uint_as_float(r0), __uint_as_float(r1));
-    w = v;
-    asm volatile("" : "+v"(w));
-    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(w), false, false);
-    const unsigned t0 = t[0], t1 = t[1];
-    return op(__uint_as_float(t0), __uint_as_float(t1));
-}
-__device__ __forceinline__ float groups_max(float v) {
-    return groups(v, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float groups_sum(float v) {
-    return groups(v, [](float a, float b) { return a + b; });
-}
-
 // A V scale as mant 2^exponent, the exponent NO_EXP for 0 (a page of zeros): outputs are kept
 // in units of 2^unit that follow the pages' exponents, so that no FP32 scale is too
 // large or too small for the sums.
 constexpr int NO_EXP = -4096;
 __device__ __forceinline__ int scale_exp(float s) { return s > 0.0f ? __builtin_amdgcn_frexp_expf(s) : NO_EXP; }
-
-// What a column sees, and where it is.
-struct Column {
-    int row, head;   // row of the row tensors (-1: no such column)
-    int begin, end;  // keys [begin, end)
-};
-__device__ __forceinline__ Column column(const Kv8Attention &a, const Kv8Seq &q, int kvh, int g, int f) {
-    Column c;
-    const int r = f / g;
-    c.row = r < q.n ? q.r0 + r : -1;
-    c.head = kvh * g + (f - r * g);
-    const int pos = q.start + r;
-    c.end = a.causal ? min(q.len, pos + 1) : q.len;
-    c.begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    if (pos < 0 || c.row < 0) c.end = 0;
-    if (c.begin > c.end) c.begin = c.end;
-    return c;
-}
 
 // Four dims i .. of one row (i % 4 == 0).
 template <class T>
@@ -116,143 +72,6 @@ __device__ __forceinline__ void store_out(const Kv8Attention &a, int row, int he
         h2_store(static_cast<unsigned short *>(a.out.p), row, head * a.c.d + i, a.heads * a.c.d, x);
     else
         static_cast<T *>(a.out.p)[row * a.out.rs + head * a.out.hs + i] = (T)x;
-}
-
-// A value that all lanes read at the same address and nothing writes meanwhile: by a scalar load.
-template <class V> __device__ __forceinline__ V uniform(const V *p) {
-    return *(const __attribute__((address_space(4))) V *)(unsigned long long)p;
-}
-// A page's address, the same in all lanes, in scalar registers.
-typedef const __attribute__((address_space(1))) signed char *page_ptr;
-__device__ __forceinline__ page_ptr scalar_address(const signed char *p) {
-    const unsigned long long u = (unsigned long long)p;
-    const unsigned lo = __builtin_amdgcn_readfirstlane((int)u), hi = __builtin_amdgcn_readfirstlane((int)(u >> 32));
-    return (page_ptr)((unsigned long long)hi << 32 | lo);
-}
-__device__ __forceinline__ i32x4 load16(page_ptr p) { return *(const __attribute__((address_space(1))) i32x4 *)p; }
-__device__ __forceinline__ int page_id(const Kv8View &c, const Kv8Seq &q, int pg) {
-    const int id = q.table ? uniform(q.table + pg) : -1;
-    return __builtin_amdgcn_readfirstlane(id >= 0 && id < c.n_pages ? id : -1);
-}
-
-// Which of the 16 keys j0 .. are visible, as bits.
-__device__ __forceinline__ unsigned visible16(int begin, int end, int j0) {
-    const int lo = min(max(begin - j0, 0), 16), hi = min(max(end - j0, 0), 16);
-    return ((1u << hi) - 1) & ~((1u << lo) - 1);
-}
-
-// A page of one head in registers: the A operands of both products.
-template <int DP> struct Tile {
-    static constexpr int KS = DP > 64 ? DP / 64 : 1;  // k steps of q k
-    i32x4 k[4][KS], v[DP / 16];
-    float sk, sv;
-    unsigned long long bad;
-};
-// First of the 16 dims a lane reads of a key; dims past a narrow head's meet zeros of the query.
-template <int DP> __device__ __forceinline__ int k_dim(int g4) { return (DP >= 64 ? g4 : g4 % (DP / 16)) * 16; }
-template <int DP>
-__device__ __forceinline__ void load_k(Tile<DP> &t, const Kv8View &c, int id, int kvh, int lane) {
-    const int64_t ph = (int64_t)max(id, 0) * c.hk + kvh;
-    const page_ptr k = scalar_address(c.k + ph * (KV8_PAGE * DP));
-    const int i = lane & 15, g4 = lane >> 4;
-    // the page's address in scalar registers, the lane's offset in one vector register
-    const unsigned koff = ((i >> 2) * 16 + (i & 3)) * DP + k_dim<DP>(g4);
-#pragma unroll
-    for (int s = 0; s < Tile<DP>::KS; s++)
-#pragma unroll
-        for (int kt = 0; kt < 4; kt++) t.k[kt][s] = load16(k + koff + (kt * 4 * DP + s * 64));
-    t.sk = uniform(&c.scales[ph].x);
-    t.sv = uniform(&c.scales[ph].y);
-    t.bad = uniform(c.bad + ph);
-}
-template <int DP>
-__device__ __forceinline__ void load_v(Tile<DP> &t, const Kv8View &c, int id, int kvh, int lane) {
-    const int64_t ph = (int64_t)max(id, 0) * c.hk + kvh;
-    const page_ptr v = scalar_address(c.v + ph * (KV8_PAGE * DP));
-    const unsigned voff = (lane & 15) * KV8_PAGE + (lane >> 4) * 16;
-#pragma unroll
-    for (int dt = 0; dt < DP / 16; dt++) t.v[dt] = load16(v + voff + dt * 16 * KV8_PAGE);
-}
-
-// A column's query, the 16 values of a lane of each k step.
-template <int KS, class T>
-__device__ __forceinline__ void load_query(const Kv8Attention &a, const Column &col, int g4, float (&x)[KS][16]) {
-    constexpr int VL = 16 / sizeof(T);
-    typedef T vec __attribute__((ext_vector_type(VL)));
-    const T *qp = static_cast<const T *>(a.q.p) + (col.row >= 0 ? col.row * a.q.rs + col.head * a.q.hs : 0);
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int e = 0; e < 16; e += VL) {  // a head has whole groups of VL dims
-            const int i = s * 64 + g4 * 16 + e;
-            const T *p = qp + (i < a.c.d ? i : 0);
-            T w[VL];
-            if (a.q16) {
-                const vec y = *reinterpret_cast<const vec *>(p);
-#pragma unroll
-                for (int u = 0; u < VL; u++) w[u] = y[u];
-            } else {
-#pragma unroll
-                for (int u = 0; u < VL; u++) w[u] = p[u];
-            }
-#pragma unroll
-            for (int u = 0; u < VL; u++) {
-                x[s][e + u] = col.row >= 0 && i < a.c.d ? to_f32(w[u]) : 0.0f;
-            }
-        }
-}
-
-// A column's query as QB bytes a value, ready as the second operand, and the
-// factor that makes scores in units of log2 of its sums with a page's codes
-// (times the K scale); NaN if the query is not finite.
-template <int QB, int KS>
-__device__ __forceinline__ float query_bytes(const float (&x)[KS][16], float scale, i32x4 (&ql)[QB][KS]) {
-    constexpr int BITS = 8 * QB - 1, HALF = QB == 3 ? 0x8080 : 0x80;  // the lower bytes are + 128 at first
-    constexpr float MOST = (1 << BITS) - 1 - HALF;
-    unsigned top = 0;
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) top = max(top, __float_as_uint(x[s][e]) & 0x7fffffffu);  // NaN above infinity above the rest
-    float mx = __uint_as_float(top);
-    const bool lost = groups_max(mx <= FLT_MAX ? 0.0f : 1.0f) > 0.0f;
-    mx = groups_max(mx);
-    int e = BITS - __builtin_amdgcn_frexp_expf(mx);
-    if (ldexpf(mx, e) > MOST) e--;
-    // a negative scale turns the query, so that the factor is never negative
-    const float sign = lost ? 0.0f : scale < 0.0f ? -1.0f : 1.0f;
-#pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int w = 0; w < 4; w++) {
-            unsigned o[QB] = {};
-#pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int v = (int)rintf(ldexpf(lost ? 0.0f : x[s][4 * w + u] * sign, e)) + HALF;
-#pragma unroll
-                for (int n = 0; n < QB; n++) o[n] |= (unsigned)(v >> (8 * (QB - 1 - n)) & 255) << (8 * u);
-            }
-#pragma unroll
-            for (int n = 0; n < QB; n++) ql[n][s][w] = (int)(n == 0 ? o[n] : o[n] ^ 0x80808080u);
-        }
-    return lost ? NAN : ldexpf(fabsf(scale) * LOG2E, (QB == 3 ? 8 : 0) - e);
-}
-
-// Scores of 16 keys with one column, in the units of the last byte but (three bytes) one.
-template <int QB, int KS>
-__device__ __forceinline__ void score_tile(const i32x4 (&k)[KS], const i32x4 (&ql)[QB][KS], float (&s)[4]) {
-    i32x4 d = {0, 0, 0, 0}, h = {0, 0, 0, 0};
-    if (QB == 3) {
-#pragma unroll
-        for (int x = 0; x < KS; x++) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[QB - 1][x], d, 0, 0, 0);
-        d >>= 8;
-    }
-#pragma unroll
-    for (int x = 0; x < KS; x++) h = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[0][x], h, 0, 0, 0);
-#pragma unroll
-    for (int x = 0; x < KS; x++) d = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[x], ql[1][x], d, 0, 0, 0);
-#pragma unroll
-    for (int r = 0; r < 4; r++) s[r] = (float)(h[r] * 256 + d[r]);  // below 2^30
 }
 
 struct NoStep {};
@@ -402,7 +221,7 @@ __device__ __forceinline__ void patch_v(Tile<DP> &t, int lo, const unsigned char
 // new codes into the tile that they requested before, else they read the page anew.  The
 // page has no other reader in the launch.  650M, one row at position 280: 11.4 us (append
 // 2 and the projection's sums 1.5 of it), the attention alone 5.5.
-template <int DP, class T, int W, bool STEP>
+template <int DP, class T, int W, bool STEP, bool SINK>
 __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws, StepArg<STEP> step) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
@@ -424,12 +243,16 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
     const Column c0 = column(a, q, kvh, g, tile * 16), c1 = column(a, q, kvh, g, min(tile * 16 + 15, q.n * g - 1));
     const int any0 = __builtin_amdgcn_readfirstlane(c0.begin), any1 = __builtin_amdgcn_readfirstlane(c1.end);
     const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
-    const int pg0 = any0 / KV8_PAGE, np = (any1 + KV8_PAGE - 1) / KV8_PAGE - pg0;  // pages
-    const int first = pg0 + split * pps, last = pg0 + min(np, (split + 1) * pps);
+    // SINK: pages are counted without those between the sinks and the window
+    const int sinks = SINK ? a.sinks : 0;
+    const SeenPages seen(any0, any1, sinks);
+    const int base_pg = SINK ? 0 : seen.skip, np = seen.n;
+    const int first = base_pg + split * pps, last = base_pg + min(np, (split + 1) * pps);
     if (split > 0 && first >= last) return;  // the join knows
+    auto page_of = [&](int pg) __attribute__((always_inline)) { return SINK ? seen.at(pg) : pg; };
 
     // the split's pages, dealt out to the waves
-    auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? page_id(a.c, q, pg) : -1; };
+    auto id_of = [&](int pg) __attribute__((always_inline)) { return pg < last ? page_id(a.c, q, page_of(pg)) : -1; };
     Tile<DP> t;
     int pg = first + wave, id = id_of(pg);
     float x[KS][16];
@@ -497,9 +320,11 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
             sv = 0.0f;  // columns that do not see the page add nothing
         }
         if (pg + W < last) load_k(t, a.c, next, kvh, lane);
-        const int j0 = pg * KV8_PAGE;
-        if (j0 < all0 || j0 + KV8_PAGE > all1 || bad || missing) {
-            const unsigned see = missing ? 0 : visible16(col.begin, col.end, j0 + g4 * 16), lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
+        const int j0 = page_of(pg) * KV8_PAGE;
+        if ((j0 < all0 && !(SINK && j0 + KV8_PAGE <= sinks)) || j0 + KV8_PAGE > all1 || bad || missing) {
+            unsigned see = missing ? 0 : visible16(col.begin, col.end, j0 + g4 * 16);
+            if (SINK && !missing) see |= visible16(0, min(sinks, col.end), j0 + g4 * 16);
+            const unsigned lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
             if (see & lost) l = NAN;
 #pragma unroll
             for (int kt = 0; kt < 4; kt++)
@@ -570,8 +395,8 @@ __global__ __launch_bounds__(64 * W, 2) void k_kv8_attend(Kv8Attention a, int g,
         id = next;
     }
 
-    if (f != f && any1 > any0) l = NAN;  // a query that is not finite
-    if (col.begin >= col.end) l = 0.0f;
+    if (f != f && (any1 > any0 || (SINK && any1 > 0))) l = NAN;  // a query that is not finite
+    if (col.begin >= col.end && !(SINK && col.end > 0)) l = 0.0f;
     l = groups_sum(l);
 #pragma unroll
     for (int dt = 0; dt < DT; dt++)
@@ -632,7 +457,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
     // the splits of its columns that had pages
     const int kvh = h / g, f = r * g + (h - kvh * g), t0 = f / cols * cols;
     const Column c0 = column(a, q, kvh, g, t0), c1 = column(a, q, kvh, g, min(t0 + cols - 1, q.n * g - 1));
-    const int pg0 = c0.begin / KV8_PAGE, np = (c1.end + KV8_PAGE - 1) / KV8_PAGE - pg0;
+    const int np = SeenPages(c0.begin, c1.end, a.sinks).n;
     const int used = min(splits, max(1, (np + pps - 1) / pps));
     const int row = q.r0 + r;
     const float *p = ws + ((int64_t)row * a.heads + h) * splits * (DP + 2);
@@ -720,7 +545,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_kv8_join(Kv8Attention a, in
 // page ahead.  Its conversion was a third of the instructions (2047 rows of 16000
 // keys 656 -> 570 us); at narrower heads, with fewer columns and less to convert, the waves' waiting for each
 // other costs as much (20 heads of 64: 2 x 512 rows 13.0, shared 14.8).
-template <int DP, int QB, int PL, class T, int CT>
+template <int DP, int QB, int PL, class T, int CT, bool SINK>
 __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, int tiles, int splits, int pps,
                                                        float *__restrict__ ws) {
     constexpr int KS = Tile<DP>::KS, DT = DP / 16;
@@ -740,11 +565,16 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     // columns of the workgroup, and the pages of the split that they see
     const int w0 = tile * 4 * CT * 16, w1 = min(w0 + 4 * CT * 16, q.n * g) - 1;
     if (w0 > w1) return;
-    const int pg0 = column(a, q, kvh, g, w0).begin / KV8_PAGE;
-    const int np = (column(a, q, kvh, g, w1).end + KV8_PAGE - 1) / KV8_PAGE - pg0;
-    int first = __builtin_amdgcn_readfirstlane(pg0 + split * pps);
-    int last = __builtin_amdgcn_readfirstlane(pg0 + min(np, (split + 1) * pps));
+    // SINK: pages are counted without those between the sinks and the window
+    const int sinks = SINK ? a.sinks : 0;
+    SeenPages seen(column(a, q, kvh, g, w0).begin, column(a, q, kvh, g, w1).end, sinks);
+    seen.sink = __builtin_amdgcn_readfirstlane(seen.sink);
+    seen.skip = __builtin_amdgcn_readfirstlane(seen.skip);
+    const int base_pg = SINK ? 0 : seen.skip;
+    int first = __builtin_amdgcn_readfirstlane(base_pg + split * pps);
+    int last = __builtin_amdgcn_readfirstlane(base_pg + min(seen.n, (split + 1) * pps));
     if (split > 0 && first >= last) return;  // the join knows
+    auto page_of = [&](int pg) __attribute__((always_inline)) { return SINK ? seen.at(pg) : pg; };
     // columns of the wave (none: it only helps with V)
     const int f0 = w0 + wave * CT * 16, f1 = min(f0 + CT * 16, q.n * g) - 1;
     const Column c0 = column(a, q, kvh, g, f0), c1 = column(a, q, kvh, g, max(f0, f1));
@@ -752,8 +582,8 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     const int all0 = __builtin_amdgcn_readfirstlane(c1.begin), all1 = __builtin_amdgcn_readfirstlane(c0.end);
     if (!SHARE) {  // the wave's own pages
         if (f0 > f1) return;
-        first = max(first, any0 / KV8_PAGE);
-        last = min(last, (any1 + KV8_PAGE - 1) / KV8_PAGE);
+        if (!SINK) first = max(first, any0 / KV8_PAGE);
+        last = min(last, (any1 + KV8_PAGE - 1) / KV8_PAGE - (SINK ? seen.skip : 0));
     }
 
     i32x4 ql[CT][QB][KS];
@@ -820,7 +650,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     // LDS only: loads of K and V stay under way
     auto barrier = [&]() __attribute__((always_inline)) { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
     // ids of the page and the next one, and the table's entry of the one after that
-    auto entry = [&](int pg) __attribute__((always_inline)) { return q.table && pg < last ? uniform(q.table + pg) : -1; };
+    auto entry = [&](int pg) __attribute__((always_inline)) { return q.table && pg < last ? uniform(q.table + page_of(pg)) : -1; };
     auto valid = [&](int e) __attribute__((always_inline)) {
         return __builtin_amdgcn_readfirstlane(e >= 0 && e < a.c.n_pages ? e : -1);
     };
@@ -840,7 +670,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
         sv = svn;
         bad = badn;
         const bool missing = id < 0;
-        const int j0 = pg * KV8_PAGE, next2 = valid(e2);
+        const int j0 = page_of(pg) * KV8_PAGE, next2 = valid(e2);
         if (!SHARE) {
             load_v(id);
         } else if (pg + 1 < last) {
@@ -848,7 +678,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
             if (pg + 2 < last) load_v(next2);
         }
         e2 = entry(pg + 3);
-        if (!SHARE || (j0 + KV8_PAGE > any0 && j0 < any1)) {
+        if (!SHARE || ((j0 + KV8_PAGE > any0 || (SINK && j0 < sinks)) && j0 < any1)) {
         float s[CT][4][4];
 #pragma unroll
         for (int t = 0; t < CT; t++)
@@ -859,10 +689,11 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
             bad = ~0ull;
             sk = sv = 0.0f;  // columns that do not see the page add nothing
         }
-        if (j0 < all0 || j0 + KV8_PAGE > all1 || bad || missing) {  // hidden keys
+        if ((j0 < all0 && !(SINK && j0 + KV8_PAGE <= sinks)) || j0 + KV8_PAGE > all1 || bad || missing) {  // hidden keys
 #pragma unroll
             for (int t = 0; t < CT; t++) {
                 unsigned see = missing ? 0 : visible16(begin[t], end[t], j0 + g4 * 16);
+                if (SINK && !missing) see |= visible16(0, min(sinks, end[t]), j0 + g4 * 16);
                 const unsigned lost = (unsigned)(bad >> (g4 * 16)) & 0xffff;
                 l[t] = see & lost ? NAN : l[t];
                 see &= ~lost;
@@ -960,7 +791,7 @@ __global__ __launch_bounds__(256, 2) void k_kv8_prompt(Kv8Attention a, int g, in
     for (int t = 0; t < CT; t++) {
         const Column col = column(a, q, kvh, g, f0 + t * 16 + c);
         float sum = groups_sum(l[t]);
-        if (begin[t] >= end[t]) sum = 0.0f;
+        if (begin[t] >= end[t] && !(SINK && end[t] > 0)) sum = 0.0f;
         if (col.row < 0) continue;
         const float x = __builtin_amdgcn_exp2f(-P0) / sum;
         float *p = ws + (((int64_t)col.row * a.heads + col.head) * splits + split) * (DP + 2);
@@ -1011,7 +842,7 @@ struct Plan {
 // Few columns: splits of 16 to 64 pages, a wave's 4 to 16, so that there are some
 // 2048 workgroups; shorter ones cost more in the join than they gain (8 single tokens of 700, 20
 // heads of 64: 8.0 us, with 8 pages 12.1), and from 4096 tiles on none is split.
-Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window, bool step, size_t ws_floats) {
+Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window, int sinks, bool step, size_t ws_floats) {
     Plan p;
     p.g = heads / c.hk;
     const int64_t columns = (int64_t)s.max_rows * p.g, pairs = (int64_t)s.n_seq * c.hk;
@@ -1021,20 +852,25 @@ Plan plan(const Kv8View &c, const Kv8Seqs &s, int heads, int causal, int window,
     p.cols = p.prompt ? 64 * prompt_tiles(c.dp) : 16;
     p.tiles = (int)((columns + p.cols - 1) / p.cols);
     const int64_t tasks = pairs * p.tiles;
-    int64_t pps = s.max_pages;
-    if (p.prompt && split) {
-        const int64_t want = max((int64_t)1, (c.dp < 128 ? 1024 : 512) / tasks);
-        pps = max((int64_t)8, (s.max_pages + want - 1) / want);
-    } else if (!p.prompt && tasks < 4096) {
-        pps = max((int64_t)16, min(s.max_pages * tasks / 2048, (int64_t)64));
-    }
     // pages that the keys of a tile's columns touch at most
     int64_t pages = s.max_pages;
     if (window > 0)
-        pages = min(pages, ((int64_t)window + (causal ? p.cols / p.g + 1 : s.max_rows) + KV8_PAGE - 2) / KV8_PAGE + 1);
+        pages = min(pages, ((int64_t)window + (causal ? p.cols / p.g + 1 : s.max_rows) + KV8_PAGE - 2) / KV8_PAGE + 1 +
+                               ((int64_t)sinks + KV8_PAGE - 1) / KV8_PAGE);
+    const int64_t most = sinks > 0 ? pages : s.max_pages;
+    int64_t pps = most;
+    if (p.prompt && split) {
+        const int64_t want = max((int64_t)1, (c.dp < 128 ? 1024 : 512) / tasks);
+        pps = max((int64_t)8, (most + want - 1) / want);
+    } else if (!p.prompt && tasks < 4096) {
+        pps = max((int64_t)16, min(most * tasks / 2048, (int64_t)64));
+    }
+    const size_t each = (size_t)s.n_rows * heads * (c.dp + 2);  // floats of one split of all rows
+    if (sinks > 0)  // as few pages a split as the workspace of the whole table allows
+        pps = max(pps, (pages + (int64_t)(ws_floats / each) - 1) / max((int64_t)1, (int64_t)(ws_floats / each)));
     for (;; pps *= 2) {
         p.splits = (int)max((int64_t)1, (pages + pps - 1) / pps);
-        if (p.splits == 1 || (size_t)s.n_rows * heads * p.splits * (c.dp + 2) <= ws_floats) break;
+        if (p.splits == 1 || each * p.splits <= ws_floats) break;
     }
     p.pps = (int)(p.splits == 1 ? (int64_t)1 << 24 : pps);
     p.blocks = tasks * p.splits;
@@ -1045,19 +881,24 @@ template <int DP, class T>
 hipError_t launch(const Kv8Attention &a, const Kv8Step *step, float *ws, size_t ws_floats, hipStream_t st) {
     constexpr bool full = std::is_same<T, float>::value;  // FP32 rows
     constexpr int CT = prompt_tiles(DP);
-    const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, step != nullptr, ws_floats);
+    const Plan p = plan(a.c, a.s, a.heads, a.causal, a.window, a.sinks, step != nullptr, ws_floats);
     const int64_t rows = (int64_t)a.s.n_seq * a.s.max_rows * a.heads;  // of the join
     if (!kv8_grid(p.blocks, 256) || (p.splits > 1 && !kv8_grid(rows, 64 * JOIN_WAVES))) return hipErrorInvalidValue;
     if constexpr (full)
         if (step)
-            hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, true>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
+            hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, true, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                                p.splits, p.pps, ws, *step);
-    if (!step && p.prompt)
-        hipLaunchKernelGGL((k_kv8_prompt<DP, full ? 3 : 2, std::is_same<T, __bf16>::value ? 1 : 2, T, CT>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
+    constexpr int QB = full ? 3 : 2, PL = std::is_same<T, __bf16>::value ? 1 : 2;
+    auto prompt = [&](auto sink) {
+        hipLaunchKernelGGL((k_kv8_prompt<DP, QB, PL, T, CT, decltype(sink)::value>), dim3(p.blocks), dim3(256), 0, st, a, p.g, p.tiles,
                            p.splits, p.pps, ws);
-    else if (!step)
-        hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, false>), dim3(p.blocks), dim3(256), 0, st, a, p.g,
+    };
+    auto few = [&](auto sink) {
+        hipLaunchKernelGGL((k_kv8_attend<DP, T, 4, false, decltype(sink)::value>), dim3(p.blocks), dim3(256), 0, st, a, p.g,
                            p.tiles, p.splits, p.pps, ws, NoStep{});
+    };
+    if (!step && p.prompt) a.sinks > 0 ? prompt(std::true_type{}) : prompt(std::false_type{});
+    else if (!step) a.sinks > 0 ? few(std::true_type{}) : few(std::false_type{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.splits == 1) return e;
     // A wave a row where the rows fill the GPU or the splits are few (20 heads of 64, 1024 rows
@@ -1087,7 +928,7 @@ hipError_t launch_dims(const Kv8Attention &a, const Kv8Step *step, float *ws, si
 size_t kv8_attention_floats(const Kv8View &c, const Kv8Seqs &s, int heads) {
     if (s.n_rows == 0 || s.n_seq == 0 || s.max_rows == 0) return 0;
     // a window leaves fewer pages at as many pages a split: what is enough without one is enough
-    const Plan p = plan(c, s, heads, 1, 0, false, SIZE_MAX);
+    const Plan p = plan(c, s, heads, 1, 0, 0, false, SIZE_MAX);
     return p.splits == 1 ? 0 : (size_t)s.n_rows * heads * p.splits * (c.dp + 2);
 }
 

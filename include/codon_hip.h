@@ -307,6 +307,13 @@ int cih_kv8_append(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32
                    const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out, const cih_rope *rope,
                    void *stream);
 
+/* The same with angles of other positions: shifts[i] (device, [n_seq]; NULL: 0)
+ * is added to the positions of sequence i's rows, for K and q alike, as after
+ * cih_kv8_evict, which leaves a sequence fewer tokens than it has had. */
+int cih_kv8_append_shifted(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, const cih_rows *k,
+                           const cih_rows *v, int32_t q_heads, const cih_rows *q, const cih_rows *q_out,
+                           const cih_rope *rope, const int32_t *shifts, void *stream);
+
 /* The batch's rows read back from the cache as values of type dtype (K as
  * stored, rotated); a bad token's values are NaN.  Rows that are not there
  * are left untouched. */
@@ -329,6 +336,73 @@ int cih_kv8_attention(const cih_kv8_cache *cache, const cih_kv8_batch *batch, in
                       const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal, int32_t window,
                       void *workspace, size_t workspace_bytes, void *stream);
 int cih_kv8_attention_workspace(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t q_heads, size_t *bytes);
+
+/* The same with first tokens that stay visible: a row at position p sees tokens
+ * j < lens[i], with causal only j <= p, with window > 0 only j > p - window or
+ * j < sinks (without a window sinks change nothing).  Pages between the sinks and the
+ * window are not read, and may be missing from the table.  The workspace is
+ * cih_kv8_attention_workspace's. */
+int cih_kv8_attention_sinks(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
+                            const cih_rows *q, const cih_rows *out, float *lse, float scale, int32_t causal,
+                            int32_t window, int32_t sinks, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- a bounded cache -------------------------------------------------------- */
+
+/* The attention weight that cached tokens gather: weights [n_pages][kv_heads][64],
+ * beside the cache, gets for token j of a sequence, in each kv head,
+ *     keep * (what it had) + sum of exp(scale q.k_j - lse) over the batch's rows that
+ *     see it and the query heads that share the kv head,
+ * q, lse, scale, causal, window and sinks as in the attention of the same rows.
+ * Tokens at the rows' own positions start from 0, with keep = 0 all do: memory
+ * that no call has written is not read.  keep is within [0, 1].  Rows whose lse is
+ * not finite (they see nothing, or a bad token) add nothing.  Sequences without
+ * rows, missing pages and tokens from lens[i] on stay as they are.  No page may
+ * stand twice in the batch's tables. */
+int cih_kv8_weigh(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t dtype, int32_t q_heads,
+                  const cih_rows *q, const float *lse, float scale, int32_t causal, int32_t window, int32_t sinks,
+                  float keep, float *weights, void *stream);
+
+/* Cuts sequences to at most budget tokens: each kv head of a sequence that holds more
+ * keeps its first `first` tokens, its last `recent` ones (first + recent <=
+ * budget), and those of the others with the largest weights (ties: the earlier
+ * token; NaN below all), moved to the places 0 .. budget - 1 in their order; the pages
+ * behind them are the caller's again.  A page's scale becomes the largest of those that
+ * its tokens come from, and codes are rounded again where their scale grows.  cu_rows and the
+ * rows of the batch are not used; the heads of a sequence may keep different tokens.
+ *     weights_out (NULL: not wanted; may be weights): the kept tokens' weights at
+ *         their new places.
+ *     lens_out (may be lens): tokens that the sequence now holds.
+ *     shifts (NULL: none): how many tokens went is added, for cih_kv8_append_shifted.
+ *     kept (NULL: none) [n_seq][kv_heads][budget]: the places that the kept tokens
+ *         had, ascending, -1 behind them.
+ * A sequence within the budget keeps all its tokens.  One whose slot or one of whose pages
+ * is not there is left alone (kept -1, lens_out its length).  No page may stand twice in the tables
+ * of a call.  workspace: 16-byte aligned, of cih_kv8_evict_workspace's size. */
+int cih_kv8_evict(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t budget, int32_t first, int32_t recent,
+                  const float *weights, float *weights_out, int32_t *lens_out, int32_t *shifts, int32_t *kept,
+                  void *workspace, size_t workspace_bytes, void *stream);
+int cih_kv8_evict_workspace(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t budget, size_t *bytes);
+
+/* ---- verification of drafted tokens ----------------------------------------------
+ * Speculative sampling from given random numbers.  Sequence i has the drafts
+ * cu_drafts[i] .. cu_drafts[i + 1] (of n_drafts, none allowed), and the target's
+ * logits for them and the token after them: rows cu_drafts[i] + i .. cu_drafts[i + 1] + i
+ * of logits [n_drafts + n_seq][vocab].  draft_logits [n_drafts][vocab] are those the
+ * drafts were drawn from (NULL: they were certain, as looked-up ones are).  With
+ * p = softmax(logits / temperature), q the same of draft_logits (or 1 at the draft): draft x
+ * is accepted if accept_at[draft] * q(x) < p(x); accepted[i] counts those before the first
+ * that is not, and tokens[i] follows them: the first token whose running sum of max(p - q, 0)
+ * (after all drafts: of p) exceeds sample_at[i] times its total.  Both are in [0, 1).
+ * temperature 0: a draft is accepted if it is the row's largest logit (ties: the lowest
+ * id), and tokens[i] is the largest; draft_logits, accept_at and sample_at are not read.
+ * -inf logits have probability 0.  A row, of the target or the draft, with NaN or
+ * +inf or of -inf only ends its sequence: the drafts before it are accepted, tokens[i]
+ * is -1.  A draft outside [0, vocab) is not accepted.  Device pointers; workspace as above. */
+int cih_verify_drafts(int32_t dtype, const void *logits, int64_t row_stride, const void *draft_logits,
+                      int64_t draft_stride, int32_t n_seq, int32_t n_drafts, int32_t vocab, const int32_t *cu_drafts,
+                      const int32_t *drafts, const float *accept_at, const float *sample_at, float temperature,
+                      int32_t *accepted, int32_t *tokens, void *workspace, size_t workspace_bytes, void *stream);
+int cih_verify_drafts_workspace(int32_t n_seq, int32_t n_drafts, int32_t vocab, size_t *bytes);
 
 /* ---- log probabilities of given tokens ----------------------------------------
  * Beside log_softmax_canonical (lib.rs:4426-4441), over the whole vocabulary.

@@ -227,6 +227,29 @@ extern "C" {
                              stream: *mut c_void) -> c_int;
     pub fn cih_kv8_attention_workspace(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, q_heads: i32,
                                        bytes: *mut usize) -> c_int;
+    pub fn cih_kv8_append_shifted(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, dtype: i32,
+                                  k: *const cih_rows, v: *const cih_rows, q_heads: i32, q: *const cih_rows,
+                                  q_out: *const cih_rows, rope: *const cih_rope, shifts: *const i32,
+                                  stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_attention_sinks(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, dtype: i32, q_heads: i32,
+                                   q: *const cih_rows, out: *const cih_rows, lse: *mut f32, scale: f32, causal: i32,
+                                   window: i32, sinks: i32, workspace: *mut c_void, workspace_bytes: usize,
+                                   stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_weigh(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, dtype: i32, q_heads: i32,
+                         q: *const cih_rows, lse: *const f32, scale: f32, causal: i32, window: i32, sinks: i32,
+                         keep: f32, weights: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_evict(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, budget: i32, first: i32,
+                         recent: i32, weights: *const f32, weights_out: *mut f32, lens_out: *mut i32,
+                         shifts: *mut i32, kept: *mut i32, workspace: *mut c_void, workspace_bytes: usize,
+                         stream: *mut c_void) -> c_int;
+    pub fn cih_kv8_evict_workspace(cache: *const cih_kv8_cache, batch: *const cih_kv8_batch, budget: i32,
+                                   bytes: *mut usize) -> c_int;
+    pub fn cih_verify_drafts(dtype: i32, logits: *const c_void, row_stride: i64, draft_logits: *const c_void,
+                             draft_stride: i64, n_seq: i32, n_drafts: i32, vocab: i32, cu_drafts: *const i32,
+                             drafts: *const i32, accept_at: *const f32, sample_at: *const f32, temperature: f32,
+                             accepted: *mut i32, tokens: *mut i32, workspace: *mut c_void, workspace_bytes: usize,
+                             stream: *mut c_void) -> c_int;
+    pub fn cih_verify_drafts_workspace(n_seq: i32, n_drafts: i32, vocab: i32, bytes: *mut usize) -> c_int;
     pub fn cih_token_logprobs(dtype: i32, logits: *const c_void, row_stride: i64, n_rows: i32, vocab: i32,
                               targets: *const i32, logprob: *mut f32, entropy: *mut f32, top_k: i32,
                               top_ids: *mut i32, top_logprobs: *mut f32, workspace: *mut c_void,
