@@ -14,33 +14,38 @@ namespace cih {
 
 namespace {
 
-constexpr int CHOOSE_THREADS = 1024, MOVE_THREADS = 256;
+constexpr int MOVE_THREADS = 256;
 
 // Of each (sequence, head), in the workspace.
 struct Work {
-    int *list;                 // [budget]: the kept tokens
-    float2 *ratio;             // [budget]: by which their codes are scaled, K and V
-    float *weight;             // [budget]
+    int *state;                // tokens held, tokens kept, whether they move, the next page to move
+    int *list;                 // [tokens]: the kept ones
+    float2 *ratio;             // [tokens]: by which their codes are scaled, K and V
+    float *weight;             // [tokens]
     float2 *scales;            // [pages]
     unsigned long long *bad;   // [pages]
-    int *state;                // {tokens kept, 1 if they move}
-    int pages, tokens;
+    int *rank;                 // [pages + 1]: how many kept tokens come from pages before this one
+    int *read;                 // [pages]: whether this page's tokens have been read
+    int pages;
 };
 __host__ __device__ inline size_t work_size(int budget) {  // a multiple of 16 bytes
     const size_t pages = (budget + KV8_PAGE - 1) / KV8_PAGE, tokens = pages * KV8_PAGE;
-    return tokens * (sizeof(int) + sizeof(float2) + sizeof(float)) + pages * (sizeof(float2) + sizeof(unsigned long long)) + 16;
+    return 16 + tokens * (sizeof(int) + sizeof(float2) + sizeof(float)) +
+           (pages * (sizeof(float2) + sizeof(unsigned long long) + 2 * sizeof(int)) + sizeof(int) + 15) / 16 * 16;
 }
 __device__ __forceinline__ Work work_of(void *ws, int budget, int64_t pair) {
     char *p = static_cast<char *>(ws) + pair * work_size(budget);
     Work w;
     w.pages = (budget + KV8_PAGE - 1) / KV8_PAGE;
-    w.tokens = w.pages * KV8_PAGE;
+    const int tokens = w.pages * KV8_PAGE;
     w.state = reinterpret_cast<int *>(p);
     w.ratio = reinterpret_cast<float2 *>(p + 16);
-    w.scales = reinterpret_cast<float2 *>(w.ratio + w.tokens);
+    w.list = reinterpret_cast<int *>(w.ratio + tokens);
+    w.weight = reinterpret_cast<float *>(w.list + tokens);
+    w.scales = reinterpret_cast<float2 *>(w.weight + tokens);
     w.bad = reinterpret_cast<unsigned long long *>(w.scales + w.pages);
-    w.list = reinterpret_cast<int *>(w.bad + w.pages);
-    w.weight = reinterpret_cast<float *>(w.list + w.tokens);
+    w.read = reinterpret_cast<int *>(w.bad + w.pages);
+    w.rank = w.read + w.pages;
     return w;
 }
 
@@ -61,191 +66,334 @@ __device__ __forceinline__ Held held(const Kv8Seqs &s, int i) {
             slot >= 0 && slot < s.table_rows ? s.table + (int64_t)slot * s.table_stride : nullptr};
 }
 
-__global__ __launch_bounds__(CHOOSE_THREADS) void k_kv8_choose(Kv8Evict e, void *ws) {
-    __shared__ int total, part[CHOOSE_THREADS / 64][2];
+// Sum of v over the threads before this one, and over all.
+template <int NT> __device__ __forceinline__ int block_scan(int v, int *part, int &all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();  // part was read
+    if (lane == 63) part[wave] = x;
+    __syncthreads();
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) {
+        if (w < wave) before += part[w];
+        all += part[w];
+    }
+    return before + x - v;
+}
+
+// NT threads; a wave owns a run of pages, token `lane` of each in a lane.  The smallest key that
+// is kept is found by its digits from the highest on (12, 12 and 8 bits), each from a
+// histogram of the keys that have the digits before it.  NK pages a wave at most, their weights in
+// registers; NK = 0: any number, in runs of 8 pages, of which as many as fit are kept in LDS (every
+// stride-th) and the others read again for each digit.
+constexpr int RUN = 8, LDS_RUNS = 64;
+template <int NT, int NK> __global__ __launch_bounds__(NT) void k_kv8_choose(Kv8Evict e, void *ws) {
+    constexpr int BINS = 4096, PER = BINS / NT, NW = NT / 64;
+    __shared__ int hist[BINS], part[NW], found[2], count[2][NW];
+    __shared__ float kept_here[NK > 0 ? 1 : LDS_RUNS * RUN * KV8_PAGE];
     const int h = blockIdx.x % e.c.hk, i = blockIdx.x / e.c.hk;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Held q = held(e.s, i);
     const Work w = work_of(ws, e.budget, blockIdx.x);
     int *kept = e.kept ? e.kept + (int64_t)blockIdx.x * e.budget : nullptr;
-    const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE;
+    const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE, runs = (pages + RUN - 1) / RUN;
+    // the wave's pages: NK > 0 as even as they go, else whole runs
+    const int own = NK > 0 ? (pages + NW - 1) / NW : (runs + NW - 1) / NW * RUN;
+    const int first = min(wave * own, pages), last = min(first + own, pages);
+    const int stride = (runs + LDS_RUNS - 1) / LDS_RUNS;
+    auto id_of = [&](int p) __attribute__((always_inline)) { return p < pages ? (int)q.table[p] : 0; };
+    auto there = [&](int id) __attribute__((always_inline)) { return id >= 0 && id < e.c.n_pages; };
+    auto weight_at = [&](int id, int j) __attribute__((always_inline)) {
+        return j < q.n ? e.weights[((int64_t)id * e.c.hk + h) * KV8_PAGE + lane] : 0.0f;
+    };
     // every page has to be there
-    if (tid == 0) total = 0;
+    if (tid == 0) found[0] = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) hist[k * NT + tid] = 0;
     __syncthreads();
-    int gone = q.table == nullptr && q.n > 0;
-    for (int p = tid; !gone && p < pages; p += CHOOSE_THREADS) {
-        const int id = q.table[p];
-        gone |= id < 0 || id >= e.c.n_pages;
+    bool gone = q.table == nullptr;
+    float x[NK > 0 ? NK : RUN];
+    // NK pages from p on: weights (0 where none is), whether all are there
+    auto load = [&](int p0) __attribute__((always_inline)) {
+        int id[NK > 0 ? NK : RUN];
+        bool fine = true;
+#pragma unroll
+        for (int k = 0; k < (NK > 0 ? NK : RUN); k++) id[k] = p0 + k < last ? id_of(p0 + k) : 0;
+#pragma unroll
+        for (int k = 0; k < (NK > 0 ? NK : RUN); k++) {
+            fine &= there(id[k]);
+            x[k] = p0 + k < last && there(id[k]) ? weight_at(id[k], (p0 + k) * KV8_PAGE + lane) : 0.0f;
+        }
+        return fine;
+    };
+    // f(token, weight) for each token of the lane, in order
+    auto tokens = [&](auto f) __attribute__((always_inline)) {
+        if constexpr (NK > 0) {
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+                if (first + k < last) f((first + k) * KV8_PAGE + lane, x[k]);
+        } else {
+            for (int p = first; p < last; p += RUN) {
+                const int r = p / RUN;
+                if (r % stride == 0) {
+#pragma unroll
+                    for (int k = 0; k < RUN; k++) x[k] = kept_here[(r / stride * RUN + k) * KV8_PAGE + lane];
+                } else {
+                    load(p);
+                }
+#pragma unroll
+                for (int k = 0; k < RUN; k++)
+                    if (p + k < last) f((p + k) * KV8_PAGE + lane, x[k]);
+            }
+        }
+    };
+    const int lo = e.first, hi = q.n - e.recent, need = e.budget - e.first - e.recent;
+    auto top = [&](int j, float y) __attribute__((always_inline)) {  // the first digit
+        if (j >= lo && j < hi) atomicAdd(&hist[weight_key(y) >> 20], 1);
+    };
+    if (!gone) {
+        if constexpr (NK > 0) {
+            gone = !load(first);
+            tokens(top);
+        } else {
+            for (int p = first; p < last; p += RUN) {
+                gone |= !load(p);
+                const int r = p / RUN;
+#pragma unroll
+                for (int k = 0; k < RUN; k++) {
+                    if (r % stride == 0) kept_here[(r / stride * RUN + k) * KV8_PAGE + lane] = x[k];
+                    if (p + k < last) top((p + k) * KV8_PAGE + lane, x[k]);
+                }
+            }
+        }
     }
-    if (gone) atomicOr(&total, 1);
+    if (gone && q.n > 0) found[0] = 1;
     __syncthreads();
-    const bool lost = total != 0;
-    auto weight = [&](int j) { return e.weights[((int64_t)q.table[j / KV8_PAGE] * e.c.hk + h) * KV8_PAGE + j % KV8_PAGE]; };
-    if (lost || q.n <= e.budget) {  // stays as it is
-        const int n = lost ? 0 : q.n;
-        for (int m = tid; kept && m < e.budget; m += CHOOSE_THREADS) kept[m] = m < n ? m : -1;
-        for (int m = tid; m < n; m += CHOOSE_THREADS) {
-            w.list[m] = m;
-            w.weight[m] = weight(m);
-        }
-        if (tid == 0) {
-            w.state[0] = n;
-            w.state[1] = 0;
-        }
+    const bool lost = found[0] != 0;
+    const int n = lost ? 0 : q.n;
+    if (tid == 0) {
+        w.state[0] = q.n;
+        w.state[1] = min(n, e.budget);
+        w.state[2] = n > e.budget;
+        w.state[3] = 0;
+    }
+    if (n <= e.budget) {  // stays as it is
+        for (int m = tid; kept && m < e.budget; m += NT) kept[m] = m < n ? m : -1;
+        if (n > 0)
+            tokens([&](int j, float y) __attribute__((always_inline)) {
+                if (j < n) w.weight[j] = y;
+            });
         return;
     }
-    const int lo = e.first, hi = q.n - e.recent, need = e.budget - e.first - e.recent;  // of tokens [lo, hi), fewer than those
-    auto count = [&](unsigned least) {  // tokens with a key of at least that
-        __syncthreads();
-        if (tid == 0) total = 0;
-        __syncthreads();
-        int n = 0;
-        for (int j = lo + tid; j < hi; j += CHOOSE_THREADS) n += weight_key(weight(j)) >= least;
+    // of tokens [lo, hi) fewer are kept than there are
+    unsigned border = 0xffffffffu;  // (need 0: above all keys)
+    int equal = need;               // kept of those at the border
+    if (need > 0) {
+        border = 0;
+        for (int pass = 0; pass < 3; pass++) {
+            const int shift = pass == 0 ? 20 : pass == 1 ? 8 : 0, mask = pass < 2 ? 4095 : 255;
+            if (pass > 0) {
+                const int known = pass == 1 ? 20 : 8;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-        if (lane == 0) atomicAdd(&total, n);
-        __syncthreads();
-        return total;
-    };
-    // the smallest key that is kept, from its highest bit on
-    unsigned border = 0;
-    for (int bit = 31; bit >= 0; bit--)
-        if (count(border | 1u << bit) >= need) border |= 1u << bit;
-    int equal = need;
-    if (border != 0xffffffffu) equal -= count(border + 1);
-    // in order: all above the border, the first of those at it
-    int before = 0, ties = 0;
-    for (int j0 = 0; j0 < q.n; j0 += CHOOSE_THREADS) {
-        const int j = j0 + tid;
-        const unsigned key = j >= lo && j < hi ? weight_key(weight(j)) : 0;
-        const bool mid = j >= lo && j < hi, at = mid && key == border;
-        const bool sure = j < q.n && (!mid || key > border);
-        const unsigned long long below = (1ull << lane) - 1, a = __ballot(at), b = __ballot(sure);
-        __syncthreads();
-        if (lane == 0) {
-            part[wave][0] = __popcll(a);
-            part[wave][1] = __popcll(b);
-        }
-        __syncthreads();
-        int at_before = ties + __popcll(a & below), sure_before = before + __popcll(b & below), at_all = 0, sure_all = 0;
-        for (int x = 0; x < CHOOSE_THREADS / 64; x++) {
-            if (x < wave) {
-                at_before += part[x][0];
-                sure_before += part[x][1];
+                for (int k = 0; k < PER; k++) hist[k * NT + tid] = 0;
+                __syncthreads();
+                tokens([&](int j, float y) __attribute__((always_inline)) {
+                    const unsigned key = weight_key(y);
+                    if (j >= lo && j < hi && key >> known == border >> known) atomicAdd(&hist[key >> shift & mask], 1);
+                });
+                __syncthreads();
             }
-            at_all += part[x][0];
-            sure_all += part[x][1];
+            // the largest first: thread t has bins BINS - 1 - PER t and below
+            int mine[PER], sum = 0, all;
+#pragma unroll
+            for (int k = 0; k < PER; k++) sum += mine[k] = hist[BINS - 1 - PER * tid - k];
+            int before = block_scan<NT>(sum, part, all);
+            if (before < equal && before + sum >= equal)
+#pragma unroll
+                for (int k = 0; k < PER; k++) {
+                    if (before < equal && before + mine[k] >= equal) {
+                        found[0] = BINS - 1 - PER * tid - k;
+                        found[1] = equal - before;
+                    }
+                    before += mine[k];
+                }
+            __syncthreads();
+            border |= (unsigned)found[0] << shift;
+            equal = found[1];
+            __syncthreads();
         }
-        if (sure || (at && at_before < equal)) {
-            const int m = sure_before + min(at_before, equal);
-            w.list[m] = j;
-            w.weight[m] = weight(j);
-            if (kept) kept[m] = j;
-        }
-        ties += at_all;
-        before += sure_all;
+    }
+    auto sure_of = [&](int j, float y) __attribute__((always_inline)) { return j < n && (j < lo || j >= hi || weight_key(y) > border); };
+    auto at_of = [&](int j, float y) __attribute__((always_inline)) { return j >= lo && j < hi && weight_key(y) == border; };
+    // in order: all above the border, the first of those at it
+    int sure = 0, ties = 0;
+    tokens([&](int j, float y) __attribute__((always_inline)) {
+        sure += __popcll(__ballot(sure_of(j, y)));
+        ties += __popcll(__ballot(at_of(j, y)));
+    });
+    if (lane == 0) {
+        count[0][wave] = sure;
+        count[1][wave] = ties;
     }
     __syncthreads();
-    // the pages' records, a wave a page
-    for (int p = wave; p < w.pages; p += CHOOSE_THREADS / 64) {
-        const int m = p * KV8_PAGE + lane;
-        const bool there = m < e.budget;
-        const int j = there ? w.list[m] : 0;
-        const int64_t ph = (int64_t)q.table[j / KV8_PAGE] * e.c.hk + h;
-        const float2 old = there ? e.c.scales[ph] : float2{0.0f, 0.0f};
-        float2 now = old;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            now.x = fmaxf(now.x, __shfl_xor(now.x, o));
-            now.y = fmaxf(now.y, __shfl_xor(now.y, o));
+    sure = ties = 0;
+    for (int u = 0; u < wave; u++) {
+        sure += count[0][u];
+        ties += count[1][u];
+    }
+    tokens([&](int j, float y) __attribute__((always_inline)) {
+        const unsigned long long below = (1ull << lane) - 1, a = __ballot(at_of(j, y)), b = __ballot(sure_of(j, y));
+        const int t = ties + __popcll(a & below), m = sure + __popcll(b & below) + min(t, equal);
+        if (lane == 0 && j / KV8_PAGE <= w.pages) w.rank[j / KV8_PAGE] = m;
+        if (b >> lane & 1 || (a >> lane & 1 && t < equal)) {
+            w.list[m] = j;
+            w.weight[m] = y;
+            if (kept) kept[m] = j;
         }
-        const unsigned long long bits = __ballot(there && e.c.bad[ph] >> (j % KV8_PAGE) & 1);
+        sure += __popcll(b);
+        ties += __popcll(a);
+    });
+    if (tid == 0 && pages <= w.pages) w.rank[pages] = e.budget;
+    __syncthreads();
+    // the pages' records, a wave a page
+    for (int p = wave; p < w.pages; p += NW) {
+        const int m = p * KV8_PAGE + lane;
+        const bool used = m < e.budget;
+        const int j = used ? w.list[m] : 0;
+        const int64_t ph = (int64_t)q.table[j / KV8_PAGE] * e.c.hk + h;
+        const float2 old = used ? e.c.scales[ph] : float2{0.0f, 0.0f};
+        const unsigned long long bits = __ballot(used && e.c.bad[ph] >> (j % KV8_PAGE) & 1);
+        // (not negative: as bits they compare alike)
+        const float2 now = {__uint_as_float(wave_max_bits(__float_as_uint(old.x))), __uint_as_float(wave_max_bits(__float_as_uint(old.y)))};
         w.ratio[m] = {now.x > 0.0f ? old.x / now.x : 0.0f, now.y > 0.0f ? old.y / now.y : 0.0f};
         if (lane == 0) {
             w.scales[p] = now;
             w.bad[p] = bits;
+            w.read[p] = 0;
         }
+    }
+}
+
+// Four codes scaled by r <= 1: u - 128 is the code, the fused product is rounded
+// once, as code r is, and 1.5 2^23 rounds it to a whole number in the low bits.
+__device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
+    const unsigned u = w ^ 0x80808080u;
+    unsigned o[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const float x = fmaf((float)(u >> (8 * b) & 0xff), r, -128.0f * r);
+        o[b] = __float_as_uint(x + 12582912.0f);
+    }
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(o[3], o[2], 0x0c0c0400u), __builtin_amdgcn_perm(o[1], o[0], 0x0c0c0400u), 0x05040100u);
+}
+
+// One workgroup per (sequence, head, page that is filled).  Token m of the kept ones comes from
+// place m or a later one, so a page may be written once the pages before it that take tokens from it
+// have read them.  A workgroup draws its page's number when it starts: those that it waits for have
+// started before it, and say that they have read before they wait themselves.
+template <int DP> __global__ __launch_bounds__(MOVE_THREADS) void k_kv8_move(Kv8Evict e, void *ws, int pages) {
+    constexpr int KP = (DP / 16 * KV8_PAGE + MOVE_THREADS - 1) / MOVE_THREADS, VP = DP * 16 / MOVE_THREADS;
+    __shared__ int spage;
+    const int64_t pair = blockIdx.x / pages;
+    const int h = pair % e.c.hk, i = pair / e.c.hk, tid = threadIdx.x;
+    const Work w = work_of(ws, e.budget, pair);
+    const int held = w.state[0], n = w.state[1];
+    const bool moves = w.state[2] != 0;
+    int p = blockIdx.x % pages;
+    if (p == 0 && h == 0 && tid == 0) {
+        // (a sequence that is left alone keeps its length, also one that is not there)
+        if (moves) e.lens_out[i] = e.budget;
+        else if (e.lens_out != e.s.lens) e.lens_out[i] = e.s.lens[i];
+        if (moves && e.shifts) e.shifts[i] += held - e.budget;
+    }
+    if (moves) {
+        if (tid == 0) spage = atomicAdd(&w.state[3], 1);
+        __syncthreads();
+        p = spage;
+    }
+    const int m0 = p * KV8_PAGE, here = min(KV8_PAGE, n - m0);
+    if (here <= 0) return;
+    const int slot = e.s.slots ? e.s.slots[i] : i;
+    const int *table = e.s.table + (int64_t)slot * e.s.table_stride;
+    const int64_t to = (int64_t)table[p] * e.c.hk + h;
+    if (tid < here && e.weights_out) e.weights_out[to * KV8_PAGE + tid] = w.weight[m0 + tid];
+    if (!moves) return;
+    const bool stays = here == KV8_PAGE && w.list[m0 + KV8_PAGE - 1] == m0 + KV8_PAGE - 1;
+    uint4 k[KP];
+    unsigned v[VP];
+    if (!stays) {
+        // K: 16 dims of a token; V: four tokens of a dim
+#pragma unroll
+        for (int it = 0; it < KP; it++) {
+            const int at = tid + it * MOVE_THREADS, m = min(at / (DP / 16), here - 1), j = w.list[m0 + m];
+            k[it] = *reinterpret_cast<const uint4 *>(
+                e.c.k + (((int64_t)table[j / KV8_PAGE] * e.c.hk + h) * KV8_PAGE + j % KV8_PAGE) * DP + at % (DP / 16) * 16);
+        }
+        const int vm = tid % 16 * 4;
+        const signed char *src[4];
+        unsigned char b[VP][4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const int j = w.list[m0 + min(vm + u, here - 1)];
+            src[u] = e.c.v + (((int64_t)table[j / KV8_PAGE] * e.c.hk + h) * DP + tid / 16) * KV8_PAGE + j % KV8_PAGE;
+        }
+#pragma unroll
+        for (int it = 0; it < VP; it++)
+#pragma unroll
+            for (int u = 0; u < 4; u++) b[it][u] = (unsigned char)src[u][it * (MOVE_THREADS / 16) * KV8_PAGE];
+#pragma unroll
+        for (int it = 0; it < KP; it++) {
+            const float r = w.ratio[m0 + min((tid + it * MOVE_THREADS) / (DP / 16), here - 1)].x;
+            k[it] = make_uint4(shrink4(k[it].x, r), shrink4(k[it].y, r), shrink4(k[it].z, r), shrink4(k[it].w, r));
+        }
+        float r[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) r[u] = w.ratio[m0 + min(vm + u, here - 1)].y;
+#pragma unroll
+        for (int it = 0; it < VP; it++) {
+            unsigned o[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++)
+                o[u] = __float_as_uint(fmaf((float)(b[it][u] ^ 0x80), r[u], -128.0f * r[u]) + 12582912.0f);
+            v[it] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(o[3], o[2], 0x0c0c0400u), __builtin_amdgcn_perm(o[1], o[0], 0x0c0c0400u), 0x05040100u);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // every wave's loads have come back
+    __syncthreads();
+    if (tid == 0) __hip_atomic_store(&w.read[p], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (stays) return;  // (its scales are what they were)
+    // pages that take tokens from this one
+    const int r0 = w.rank[p], r1 = w.rank[p + 1];
+    if (r0 < r1) {
+        const int q = r0 / KV8_PAGE + tid;  // 64 tokens go to two pages at most
+        if (q <= (r1 - 1) / KV8_PAGE && q < p)
+            while (!__hip_atomic_load(&w.read[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) __builtin_amdgcn_s_sleep(1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < KP; it++) {
+        const int at = tid + it * MOVE_THREADS, m = at / (DP / 16);
+        if (m < here) *reinterpret_cast<uint4 *>(e.c.k + (to * KV8_PAGE + m) * DP + at % (DP / 16) * 16) = k[it];
+    }
+    const int vm = tid % 16 * 4;
+#pragma unroll
+    for (int it = 0; it < VP; it++) {
+        signed char *y = e.c.v + (to * DP + tid / 16 + it * (MOVE_THREADS / 16)) * KV8_PAGE + vm;
+        if (vm + 4 <= here) *reinterpret_cast<unsigned *>(y) = v[it];
+        else
+            for (int u = 0; vm + u < here; u++) y[u] = (signed char)(v[it] >> (8 * u));
     }
     if (tid == 0) {
-        w.state[0] = e.budget;
-        w.state[1] = 1;
+        e.c.scales[to] = w.scales[p];
+        e.c.bad[to] = w.bad[p];
     }
-}
-
-// One workgroup per (sequence, head) and K or V: page after page, its codes read before they
-// are written.  Token m of the kept ones comes from place m or a later one, so what is written has been read.
-__global__ __launch_bounds__(MOVE_THREADS) void k_kv8_move(Kv8Evict e, void *ws) {
-    const int which = blockIdx.x & 1, pair = blockIdx.x >> 1, h = pair % e.c.hk, i = pair / e.c.hk, tid = threadIdx.x;
-    const Held q = held(e.s, i);
-    const Work w = work_of(ws, e.budget, pair);
-    const int n = w.state[0], dp = e.c.dp;
-    if (which == 0 && h == 0 && tid == 0) {
-        const int len = w.state[1] ? e.budget : e.s.lens[i];
-        if (w.state[1] && e.shifts) e.shifts[i] += q.n - e.budget;
-        w.state[2] = len;
-    }
-    if (which == 0 && e.weights_out)
-        for (int m = tid; m < n; m += MOVE_THREADS)
-            e.weights_out[((int64_t)q.table[m / KV8_PAGE] * e.c.hk + h) * KV8_PAGE + m % KV8_PAGE] = w.weight[m];
-    if (!w.state[1]) return;
-    for (int p = 0; p < w.pages; p++) {
-        const int64_t to = (int64_t)q.table[p] * e.c.hk + h;
-        const int held_here = min(KV8_PAGE, n - p * KV8_PAGE);
-        unsigned x[8][4];
-#pragma unroll
-        for (int it = 0; it < 8; it++) {
-            const int at = tid + it * MOVE_THREADS;
-            if (which == 0) {  // 16 dims of a token
-                const int per = dp / 16, m = at / per, d = at % per * 16;
-                if (m >= held_here) continue;
-                const int j = w.list[p * KV8_PAGE + m];
-                const float r = w.ratio[p * KV8_PAGE + m].x;
-                const uint4 y = *reinterpret_cast<const uint4 *>(
-                    e.c.k + (((int64_t)q.table[j / KV8_PAGE] * e.c.hk + h) * KV8_PAGE + j % KV8_PAGE) * dp + d);
-                x[it][0] = recode4(y.x, r);
-                x[it][1] = recode4(y.y, r);
-                x[it][2] = recode4(y.z, r);
-                x[it][3] = recode4(y.w, r);
-            } else {  // four tokens of a dim
-                const int d = at / 16, m0 = at % 16 * 4;
-                if (d >= dp || m0 >= held_here) continue;
-                unsigned o = 0;
-                for (int u = 0; u < 4 && m0 + u < held_here; u++) {
-                    const int j = w.list[p * KV8_PAGE + m0 + u];
-                    const signed char y = e.c.v[(((int64_t)q.table[j / KV8_PAGE] * e.c.hk + h) * dp + d) * KV8_PAGE + j % KV8_PAGE];
-                    o |= (unsigned)code8((float)y, w.ratio[p * KV8_PAGE + m0 + u].y) << (8 * u);
-                }
-                x[it][0] = o;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int it = 0; it < 8; it++) {
-            const int at = tid + it * MOVE_THREADS;
-            if (which == 0) {
-                const int per = dp / 16, m = at / per, d = at % per * 16;
-                if (m < held_here)
-                    *reinterpret_cast<uint4 *>(e.c.k + (to * KV8_PAGE + m) * dp + d) = make_uint4(x[it][0], x[it][1], x[it][2], x[it][3]);
-            } else {
-                const int d = at / 16, m0 = at % 16 * 4;
-                signed char *y = e.c.v + (to * dp + d) * KV8_PAGE + m0;
-                if (d < dp && m0 + 4 <= held_here) *reinterpret_cast<unsigned *>(y) = x[it][0];
-                else if (d < dp)
-                    for (int u = 0; m0 + u < held_here; u++) y[u] = (signed char)(x[it][0] >> (8 * u));
-            }
-        }
-        if (which == 0 && tid == 0) {
-            e.c.scales[to] = w.scales[p];
-            e.c.bad[to] = w.bad[p];
-        }
-        __syncthreads();
-    }
-}
-
-// Last, for lens_out may be lens.
-__global__ void k_kv8_lens(Kv8Evict e, void *ws) {
-    const int i = blockIdx.x * 64 + threadIdx.x;
-    if (i < e.s.n_seq) e.lens_out[i] = work_of(ws, e.budget, (int64_t)i * e.c.hk).state[2];
 }
 
 }  // namespace
@@ -255,12 +403,21 @@ size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget) {
 }
 
 hipError_t launch_kv8_evict(const Kv8Evict &e, void *ws, hipStream_t st) {
-    const int64_t pairs = (int64_t)e.s.n_seq * e.c.hk;
+    const int64_t pairs = (int64_t)e.s.n_seq * e.c.hk, most = (int64_t)e.s.max_pages * KV8_PAGE;
     if (pairs == 0) return hipSuccess;
-    if (!kv8_grid(pairs, CHOOSE_THREADS) || !kv8_grid(2 * pairs, MOVE_THREADS)) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(k_kv8_choose, dim3(pairs), dim3(CHOOSE_THREADS), 0, st, e, ws);
-    hipLaunchKernelGGL(k_kv8_move, dim3(2 * pairs), dim3(MOVE_THREADS), 0, st, e, ws);
-    if (e.lens_out) hipLaunchKernelGGL(k_kv8_lens, dim3((e.s.n_seq + 63) / 64), dim3(64), 0, st, e, ws);
+    const int pages = (int)min((int64_t)(e.budget + KV8_PAGE - 1) / KV8_PAGE, (int64_t)e.s.max_pages);
+    if (!kv8_grid(pairs, 1024) || !kv8_grid(pairs * pages, MOVE_THREADS)) return hipErrorInvalidValue;
+    if (most <= 2048) hipLaunchKernelGGL((k_kv8_choose<256, 8>), dim3(pairs), dim3(256), 0, st, e, ws);
+    else if (most <= 8192) hipLaunchKernelGGL((k_kv8_choose<1024, 8>), dim3(pairs), dim3(1024), 0, st, e, ws);
+    else hipLaunchKernelGGL((k_kv8_choose<1024, 0>), dim3(pairs), dim3(1024), 0, st, e, ws);
+    const dim3 grid(pairs * pages), threads(MOVE_THREADS);
+    switch (e.c.dp) {
+        case 16: hipLaunchKernelGGL(k_kv8_move<16>, grid, threads, 0, st, e, ws, pages); break;
+        case 32: hipLaunchKernelGGL(k_kv8_move<32>, grid, threads, 0, st, e, ws, pages); break;
+        case 64: hipLaunchKernelGGL(k_kv8_move<64>, grid, threads, 0, st, e, ws, pages); break;
+        case 128: hipLaunchKernelGGL(k_kv8_move<128>, grid, threads, 0, st, e, ws, pages); break;
+        default: return hipErrorInvalidValue;
+    }
     return hipGetLastError();
 }
 

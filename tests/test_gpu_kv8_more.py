@@ -367,9 +367,31 @@ def test_evict_slots_missing_pages_and_table_ends(hip):
     run_evict(hip, np.random.default_rng(6), [300, 20, 300, 500], 128, 4, 30, slots=True, inplace=True)
 
 
-@pytest.mark.parametrize("n,budget", [(20000, 4000), (9000, 8999), (5000, 64)])
+@pytest.mark.parametrize("n,budget", [(20000, 4000), (9000, 8999), (5000, 64), (8192, 8191), (70000, 3001), (131, 7)])
 def test_evict_long(hip, n, budget):
-    run_evict(hip, np.random.default_rng(n), [n, 77], budget, 4, 32, hk=1, d=32)
+    run_evict(hip, np.random.default_rng(n), [n, 77, n // 2], budget, 4, budget // 3, hk=1, d=32)
+
+
+@pytest.mark.parametrize("max_pages", [32, 33, 128, 129, 1500])
+def test_evict_short_sequences_in_wide_tables(hip, max_pages):
+    rng = np.random.default_rng(max_pages)
+    run_evict(hip, rng, [300, 0, 1, 1999, 64], 64, 4, 16, max_pages=max_pages)
+    run_evict(hip, rng, [1999, 700], 650, 0, 0, max_pages=max_pages, weights=lambda s: rng.integers(0, 2, s).astype(np.float32), inplace=True)
+
+
+@pytest.mark.parametrize("pattern", ["last", "first", "even", "runs"])
+def test_evict_where_the_kept_tokens_lie(hip, pattern):
+    """Pages that all wait for one, that wait for none, and that take tokens from many."""
+    def weights(shape):
+        return np.zeros(shape, np.float32)
+
+    def edit(c, table, w):
+        for i, n in enumerate((2000, 4096)):
+            j = np.arange(n)
+            like = {"last": j, "first": -j, "even": j % 2, "runs": (j // 100) % 3}[pattern]
+            w[table[i, j // 64], :, j % 64] = like[:, None]
+
+    run_evict(hip, np.random.default_rng(1), [2000, 4096], 999, 1, 1, d=128, weights=weights, edit=edit)
 
 
 def test_evict_again_and_again(hip):
