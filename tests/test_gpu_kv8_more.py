@@ -188,7 +188,9 @@ def run_weigh(hip, rng, lens, rows, hk, g, d, dtype, window=0, sinks=0, causal=T
 
 @pytest.fixture(params=["0", "1"], ids=["few", "prompt"])
 def weigh_kernel(request, monkeypatch):
+    """The kernel that the sizes choose, and that of many columns for all."""
     monkeypatch.setenv("CIH_KV8_WEIGH", request.param)
+    return request.param
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -265,6 +267,34 @@ def test_weigh_query_sizes(hip, weigh_kernel):
             assert (np.abs(got - w[0]) <= tol[0] + 1e-37).all(), (dtype, size)
             R.free(q, wt, lv)
             x.free()
+
+
+@pytest.mark.parametrize("dtype,small,large", [("float16", 3e-7, 1.0), ("float16", 2e-5, 60000.0), ("bfloat16", 1e-3, 1e37),
+                                               ("bfloat16", 1e-37, 1.0), ("float32", 1e-3, 1e3)])
+def test_weigh_small_values_beside_large_ones(hip, weigh_kernel, dtype, small, large):
+    """A column's large value meets codes of 0, so that its small ones decide (FP32 rows: as far as 2^-22 of the large one holds them)."""
+    x = Case(hip, np.random.default_rng(8), [130], [33], 1, 1, 64, dtype)
+    R.free(*x.c.dev)
+    x.c.k[:, :, :, 0] = 0
+    x.cache = x.c.upload()
+    q = np.random.default_rng(9).standard_normal(x.q.shape) * small
+    q[..., 0] = large
+    q = R.rounded(q, dtype)
+    if weigh_kernel == "0" or dtype == "float32":
+        q[..., 0] = R.rounded(np.array([small * 4]), dtype)  # three bytes hold a row to 2^-22 of its largest value
+    scale = 0.25 / small
+    lse = M.attention(x.c, x.table[0], 130, np.arange(97, 130), q[:33], scale, True, 0, 0, 1)[1]
+    lse = np.concatenate([lse, np.zeros((x.n - 33, 1))]).astype(np.float32)
+    dev, wt, lv = R.put(hip, q, dtype), DeviceArray(hip, np.zeros(x.c.k.shape[:3], np.float32)), DeviceArray(hip, lse)
+    x.cache.weigh(x.batch, dev, lv, wt, scale=scale)
+    # the restatement's bound without the large value, which adds nothing to a score
+    q[..., 0] = 0
+    w, tol = M.gained(x.c, x.table[0], 130, np.arange(97, 130), q[:33], lse[:33].astype(np.float64), scale, True, 0, 0, 1)
+    got = wt.numpy()[x.table[0], 0].reshape(-1)[:130]
+    off = (np.abs(got - w[0]) / (4 * tol[0] + 1e-37)).max()
+    assert off <= 1, off
+    R.free(dev, wt, lv)
+    x.free()
 
 
 # ---- eviction -----------------------------------------------------------------------------
