@@ -130,9 +130,9 @@ __global__ __launch_bounds__(64 * WEIGH_WAVES) void k_kv8_weigh(Kv8Weigh w, int 
 }
 
 // Many columns.  The wave's page becomes f16 (bfloat16 rows: bfloat16) once, which holds the codes as
-// they are, and stays in registers; the queries go by in LDS, 64 columns at a time for the four waves, as they
+// they are, and stays in registers; the queries go by in LDS, 128 columns at a time for the eight waves, as they
 // are (FP32 rows: two f16, hi + lo, under a power of two of the column's own).  sp pages a workgroup: with less than
-// four, the waves of a page share the columns among them.
+// eight, the waves of a page share the columns among them.
 template <class T> struct Half {
     typedef _Float16 one;
     typedef _Float16 type __attribute__((ext_vector_type(8)));
@@ -165,17 +165,18 @@ struct RowOf {
     __device__ __forceinline__ int row(int f) const { return (int)((unsigned long long)(unsigned)f * m >> shift); }
 };
 
-constexpr int TILES = 4, COLS = 16 * TILES;  // of a turn
+constexpr int MANY_WAVES = 8, MANY = 64 * MANY_WAVES, TILES = 8, COLS = 16 * TILES;  // of a turn
 template <int DP, class T>
-__global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, int sp, RowOf of) {
+__global__ __launch_bounds__(MANY, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, int sp, RowOf of) {
     typedef Half<T> H;
     typedef typename H::type half8;
     constexpr int KS = DP >= 64 ? DP / 32 : 1, L = H::LIMBS, PIECES = DP / 8;
-    constexpr int IT = (COLS * PIECES + 255) / 256;  // pieces of 8 dims a thread stages
+    constexpr int IT = (COLS * PIECES + MANY - 1) / MANY;  // pieces of 8 dims a thread stages
     constexpr bool FULL = std::is_same<T, float>::value;
     const Kv8Attention &a = w.a;
     __shared__ half8 sq[2][L][TILES][KS][64];
-    __shared__ float soff[2][COLS], sfac[2][COLS], red[WEIGH_WAVES][64];
+    __shared__ float2 scol[2][COLS];  // of a column: lse in units of log2 (infinite: it adds nothing), the scores' factor
+    __shared__ float red[MANY_WAVES][64];
     const int pairs = a.c.hk * a.s.n_seq, pair = blockIdx.x % pairs, group = blockIdx.x / pairs;
     const int kvh = pair % a.c.hk, tid = threadIdx.x;
     const Kv8Seq q = kv8_seq(a.s, pair / a.c.hk);
@@ -206,40 +207,38 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
     const SeenBy by(a, q, group * sp * KV8_PAGE, sp * KV8_PAGE);
     const int c0 = (int64_t)by.r0 * g / COLS, c1 = by.r0 < by.r1 ? (int)(((int64_t)by.r1 * g + COLS - 1) / COLS) : c0;
     if (DP == 16)  // lanes whose dims there are none of
-        for (int e = tid; e < 2 * L * TILES * 64; e += 256)
+        for (int e = tid; e < 2 * L * TILES * 64; e += MANY)
             if (e % 64 >= 32) (&sq[0][0][0][0][0])[e] = half8{};
 
-    // Pieces of the thread: 8 dims of a column.  Its row and head follow from turn to turn without a division.
+    // Pieces of the thread: 8 dims of a column, whose row and head follow from turn to turn without a
+    // division.  Columns that are not there have a neighbour's query.
     constexpr int VL = 16 / sizeof(T), N = 8 / VL;
     typedef T vec __attribute__((ext_vector_type(VL)));
     vec held[IT][N];
     float held_lse = INFINITY;
-    int row[IT], head[IT], lse_row, lse_head;  // (row of the sequence)
+    int row[IT], head[IT], lse_row = 0, lse_head = 0;  // (row of the sequence)
+    const T *piece[IT];
 #pragma unroll
     for (int it = 0; it < IT; it++) {
-        const int f = c0 * COLS + (tid + it * 256) / PIECES;
+        const int e = tid + it * MANY, p = e % PIECES, f = c0 * COLS + e / PIECES;
         row[it] = of.row(f);
         head[it] = f - row[it] * g;
+        piece[it] = static_cast<const T *>(a.q.p) + q.r0 * a.q.rs + kvh * g * a.q.hs + (p * 8 < a.c.d ? p * 8 : 0);
     }
-    lse_row = of.row(c0 * COLS + tid % COLS);
-    lse_head = c0 * COLS + tid % COLS - lse_row * g;
+    if (tid < COLS) {
+        lse_row = of.row(c0 * COLS + tid);
+        lse_head = c0 * COLS + tid - lse_row * g;
+    }
     const int step_row = of.row(COLS), step_head = COLS - step_row * g;
-    auto there_is = [&](int r) __attribute__((always_inline)) { return r < q.n && q.start + r >= 0; };
     auto follow = [&](int &r, int &h) __attribute__((always_inline)) {
-        r += step_row;
-        h += step_head;
-        if (h >= g) {
-            h -= g;
-            r++;
-        }
+        const bool over = h + step_head >= g;
+        r += step_row + (over ? 1 : 0);
+        h += step_head - (over ? g : 0);
     };
     auto load = [&]() __attribute__((always_inline)) {  // and on to the next turn
 #pragma unroll
         for (int it = 0; it < IT; it++) {
-            const int p = (tid + it * 256) % PIECES;
-            const bool here = there_is(row[it]);
-            const T *x = static_cast<const T *>(a.q.p) + (here ? (q.r0 + row[it]) * a.q.rs + (kvh * g + head[it]) * a.q.hs : 0) +
-                         (p * 8 < a.c.d ? p * 8 : 0);
+            const T *x = piece[it] + min(row[it], q.n - 1) * a.q.rs + head[it] * a.q.hs;
             if (a.q16) {
 #pragma unroll
                 for (int u = 0; u < N; u++) held[it][u] = *reinterpret_cast<const vec *>(x + u * VL);
@@ -247,13 +246,14 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
 #pragma unroll
                 for (int u = 0; u < 8; u++) held[it][u / VL][u % VL] = x[u];
             }
-            if (!here || p * 8 >= a.c.d)
+            if (DP == 32 && (tid + it * MANY) % PIECES * 8 >= a.c.d)
 #pragma unroll
                 for (int u = 0; u < N; u++) held[it][u] = vec{};
             follow(row[it], head[it]);
         }
         if (tid < COLS) {
-            held_lse = there_is(lse_row) ? a.lse[(int64_t)(q.r0 + lse_row) * a.heads + kvh * g + lse_head] : INFINITY;
+            held_lse = lse_row < q.n && q.start + lse_row >= 0
+                           ? a.lse[(int64_t)(q.r0 + lse_row) * a.heads + kvh * g + lse_head] : INFINITY;
             follow(lse_row, lse_head);
         }
     };
@@ -265,8 +265,8 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
         constexpr unsigned MOST = FULL ? 0 : F16 ? 0x7c00u - 1 : 0x7800u, LEAST = F16 ? 0x0400u : 0x2000u;  // 2^113; 2^-14, 2^-63
 #pragma unroll
         for (int it = 0; it < IT; it++) {
-            const int e = tid + it * 256, p = e % PIECES, col = e / PIECES;
-            if (COLS * PIECES % 256 != 0 && col >= COLS) continue;  // (whole waves)
+            const int e = tid + it * MANY, p = e % PIECES, col = e / PIECES;
+            if (COLS * PIECES % MANY != 0 && col >= COLS) continue;  // (whole waves)
             // which k step and lanes have dims p * 8 ..; columns turned by p, so that the stores of a column meet no bank twice
             const int s = DP >= 64 ? p / 8 * 2 + (p & 1) : 0;
             const int gg = DP >= 64 ? p % 8 / 2 : DP == 32 ? (p & 1) * 2 + (p >> 1) : p;
@@ -274,11 +274,12 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
             float fac = a.scale * LOG2E;
             unsigned top = 0;
             if constexpr (!FULL) {
-                typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
-                const u16x8 bits = __builtin_bit_cast(u16x8, held[it][0]) & (unsigned short)0x7fff;
-                const auto m4 = __builtin_elementwise_max(bits.lo, bits.hi);
-                const auto m2 = __builtin_elementwise_max(m4.lo, m4.hi);
-                top = max((unsigned)m2.x, (unsigned)m2.y);
+                typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+                const i32x4 bits = __builtin_bit_cast(i32x4, held[it][0]) & 0x7fff7fff;
+                const u16x2 m = __builtin_elementwise_max(
+                    __builtin_elementwise_max(__builtin_bit_cast(u16x2, (int)bits[0]), __builtin_bit_cast(u16x2, (int)bits[1])),
+                    __builtin_elementwise_max(__builtin_bit_cast(u16x2, (int)bits[2]), __builtin_bit_cast(u16x2, (int)bits[3])));
+                top = max((unsigned)m.x, (unsigned)m.y);
                 *to = __builtin_bit_cast(half8, held[it][0]);
             }
             if (FULL || __ballot(top > MOST || (top > 0 && top < LEAST))) {
@@ -309,13 +310,13 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
                 if (L == 2) *(to + (&sq[0][L - 1][0][0][0] - &sq[0][0][0][0][0])) = lo;
                 fac = lost ? NAN : ldexpf(fac, -up);
             }
-            if (p == 0) sfac[at][col] = fac;
+            if (p == 0) scol[at][col].y = fac;
         }
-        if (tid < COLS) soff[at][tid] = fabsf(held_lse) <= FLT_MAX ? held_lse * LOG2E : INFINITY;
+        if (tid < COLS) scol[at][tid].x = fabsf(held_lse) <= FLT_MAX ? held_lse * LOG2E : INFINITY;
     };
     float sum[16] = {};
     auto turn_of = [&](int turn, int at) __attribute__((always_inline)) {
-        for (int tile = wave / sp; tile < TILES; tile += WEIGH_WAVES / sp) {
+        for (int tile = wave / sp; tile < TILES; tile += MANY_WAVES / sp) {
             // positions of the tile's first and last column
             const int f = turn * COLS + tile * 16, p0 = q.start + of.row(f), p1 = q.start + of.row(f + 15);
             const bool sink = j0 < a.sinks;
@@ -333,25 +334,23 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
 #pragma unroll
                     for (int kt = 0; kt < 4; kt++) s[kt] = H::mfma(k[kt][u], x, s[kt]);
                 }
-            float off = soff[at][tile * 16 + c];
-            const float fac = sfac[at][tile * 16 + c];
-            const float fk = fminf(fmaxf(fac * sk, -FLT_MAX), FLT_MAX);
-            if (fac != fac) off = INFINITY;  // a query that is not finite
+            const float2 of_col = scol[at][tile * 16 + c];
+            float fk = of_col.y * sk, off = of_col.x;
+            fk = fminf(fmaxf(fk, -FLT_MAX), FLT_MAX);
+            if (of_col.y != of_col.y) off = INFINITY;  // a query that is not finite
+            if (fk == 0.0f) fk = 0x1p-149f;            // so that what is hidden stays at -inf
             const bool all = (!a.causal || j0 + KV8_PAGE - 1 <= p0) &&
                              (a.window == 0 || j0 > (int64_t)p1 - a.window || j0 + KV8_PAGE <= a.sinks);
-            if (all) {
-#pragma unroll
-                for (int u = 0; u < 16; u++) sum[u] += __builtin_amdgcn_exp2f(fmaf(s[u / 4][u % 4], fk, -off));
-            } else {
+            if (!all) {
                 const Column col = column(a, q, kvh, g, f + c);
                 unsigned see = visible16(col.begin, col.end, j0 + g4 * 16);
                 if (a.sinks > 0) see |= visible16(0, min(a.sinks, col.end), j0 + g4 * 16);
+                const float never = fk > 0.0f ? -INFINITY : INFINITY;
 #pragma unroll
-                for (int u = 0; u < 16; u++) {
-                    const float e = __builtin_amdgcn_exp2f(fmaf(s[u / 4][u % 4], fk, -off));
-                    sum[u] += see >> u & 1 ? e : 0.0f;
-                }
+                for (int u = 0; u < 16; u++) s[u / 4][u % 4] = see >> u & 1 ? s[u / 4][u % 4] : never;
             }
+#pragma unroll
+            for (int u = 0; u < 16; u++) sum[u] += __builtin_amdgcn_exp2f(fmaf(s[u / 4][u % 4], fk, -off));
         }
     };
     if (c0 < c1) {
@@ -367,11 +366,11 @@ __global__ __launch_bounds__(256, 2) void k_kv8_weigh_prompt(Kv8Weigh w, int g, 
         }
     }
     float x = lanes_reduce(sum, c);
-    if (sp < WEIGH_WAVES) {
+    if (sp < MANY_WAVES) {
         red[wave][lane] = x;
         __syncthreads();
         if (wave >= sp) return;
-        for (int v = wave + sp; v < WEIGH_WAVES; v += sp) x += red[v][lane];
+        for (int v = wave + sp; v < MANY_WAVES; v += sp) x += red[v][lane];
     }
     if (pg < np) gain(w, q, id, kvh, pg, lane, x);
 }
@@ -382,11 +381,11 @@ template <int DP, class T> hipError_t launch(const Kv8Weigh &w, hipStream_t st) 
     const char *e = getenv("CIH_KV8_WEIGH");
     const bool many = (int64_t)w.a.s.max_rows * g > 16;
     if (many || (e && !strcmp(e, "1"))) {
-        int sp = WEIGH_WAVES;
-        while (sp > 1 && pairs * ((mp + sp - 1) / sp) < 512) sp /= 2;
+        int sp = MANY_WAVES;
+        while (sp > 1 && pairs * ((mp + sp - 1) / sp) < 256) sp /= 2;
         const int64_t blocks = pairs * ((mp + sp - 1) / sp);
-        if (!kv8_grid(blocks, 256)) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((k_kv8_weigh_prompt<DP, T>), dim3(blocks), dim3(256), 0, st, w, g, sp, RowOf(g));
+        if (!kv8_grid(blocks, MANY)) return hipErrorInvalidValue;
+        hipLaunchKernelGGL((k_kv8_weigh_prompt<DP, T>), dim3(blocks), dim3(MANY), 0, st, w, g, sp, RowOf(g));
     } else {
         const int pps = (int)max((int64_t)16, min(mp * pairs / 2048, (int64_t)64)), groups = (int)((mp + pps - 1) / pps);
         if (!kv8_grid(pairs * groups, 64 * WEIGH_WAVES)) return hipErrorInvalidValue;
