@@ -2,8 +2,18 @@
 // softmax(logits / T) and q = softmax(draft logits / T), draft x is taken if u q(x) < p(x).
 // The token after the taken ones comes from max(p - q, 0) at the first refusal, from p
 // after all drafts: the first whose running sum passes v times the whole.  T = 0: the largest logit.
-// Sums and borders in 64 bits: in 32 a border moves across tokens.
+//
+// Whether a draft is taken asks for two sums of a row, whose FP32 exponentials' errors (10^-7) decide
+// as rarely as the random numbers' own 24 bits do.  A drawn token lies between two running sums of
+// as many terms as there are tokens, and errors of 10^-7 of the whole would move it to a neighbour in one
+// draw of a hundred (131,072 tokens): what is drawn from is summed in 64 bits, and only that row.
+//
+// k_verify_rows: (largest, sum) of parts of all rows.  k_verify_take, k_verify_left: a workgroup a part of
+// the drawn row of a sequence: the 64-bit sums of p and q, then those of what is drawn from.  k_verify_draw: the
+// token.  k_verify_narrow does it all for vocabularies of up to 256 tokens, a workgroup a sequence.
 #include <float.h>
+
+#include <type_traits>
 
 #include "kernels.h"
 #include "kv8.h"
@@ -12,148 +22,594 @@ namespace cih {
 
 namespace {
 
-constexpr int VERIFY_THREADS = 256;
+constexpr float LOG2E = 1.44269504088896340736f;
+constexpr int NONE = 0x7fffffff;
+constexpr int VERIFY_THREADS = 256, VERIFY_WAVES = VERIFY_THREADS / 64;
+constexpr int NARROW = 256;  // tokens
+constexpr int FINE = 1024;   // tokens of a piece of a part, of which the sums are kept
 
-template <class V, class OP> __device__ __forceinline__ V block_all(V v, OP op, V *red) {
+template <class V, class OP> __device__ __forceinline__ V wave_all(V v, OP op) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
+    return v;
+}
+template <class V, class OP> __device__ __forceinline__ V block_all(V v, OP op, V *red) {
+    v = wave_all(v, op);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int w = 1; w < VERIFY_THREADS / 64; w++) v = op(v, red[w]);
+    for (int w = 1; w < VERIFY_WAVES; w++) v = op(v, red[w]);
     return v;
 }
-
-// A row's largest logit and the sum of exp((x - largest) / T); lost: no distribution.
-struct Dist {
-    double m, z;
-    bool lost;
-    int best;
+struct Plus {
+    template <class V> __device__ __forceinline__ V operator()(V a, V b) const { return a + b; }
 };
-template <class T> __device__ Dist dist(const T *x, int vocab, double heat, double *red, int *ired) {
-    Dist d;
-    float m = -INFINITY;
-    int best = 0x7fffffff;
-    bool bad = false;
-    for (int j = threadIdx.x; j < vocab; j += VERIFY_THREADS) {
-        const float y = to_f32(x[j]);
-        bad |= !(y < INFINITY);
-        if (y > m) {
-            m = y;
-            best = j;
-        }
-    }
-    const float all = (float)block_all((double)m, [](double a, double b) { return a > b ? a : b; }, red);
-    d.best = block_all(m == all ? best : 0x7fffffff, [](int a, int b) { return min(a, b); }, ired);
-    d.lost = block_all((int)bad, [](int a, int b) { return a | b; }, ired) || all == -INFINITY;
-    d.m = all;
-    d.z = 0.0;
-    if (heat > 0.0 && !d.lost) {
-        double z = 0.0;
-        for (int j = threadIdx.x; j < vocab; j += VERIFY_THREADS) z += exp(((double)to_f32(x[j]) - d.m) / heat);
-        d.z = block_all(z, [](double a, double b) { return a + b; }, red);
-    }
-    return d;
-}
-__device__ __forceinline__ double prob(const Dist &d, float x, double heat) { return exp(((double)x - d.m) / heat) / d.z; }
+struct Less {
+    template <class V> __device__ __forceinline__ V operator()(V a, V b) const { return b < a ? b : a; }
+};
+struct More {
+    template <class V> __device__ __forceinline__ V operator()(V a, V b) const { return b > a ? b : a; }
+};
 
-template <class T> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify(VerifyDrafts v) {
-    __shared__ double red[VERIFY_THREADS / 64], scan[VERIFY_THREADS];
-    __shared__ int ired[VERIFY_THREADS / 64];
-    const int i = blockIdx.x, tid = threadIdx.x;
-    const int c0 = min(max(v.cu[i], 0), v.n_drafts), c1 = min(max(v.cu[i + 1], c0), v.n_drafts);
-    const double heat = v.temperature;
-    int taken = 0, token = -1;
-    Dist p{}, q{};
-    bool refused = false, lost = false;
-    const T *pr = nullptr, *qr = nullptr;
-    for (;; taken++) {
-        pr = static_cast<const T *>(v.logits) + (int64_t)(c0 + i + taken) * v.stride;
-        p = dist(pr, v.vocab, heat, red, ired);
-        lost = p.lost;
-        if (lost || c0 + taken >= c1) break;
-        const int x = v.drafted[c0 + taken];
-        const bool known = x >= 0 && x < v.vocab;
-        if (heat == 0.0) {
-            if (x != p.best) break;
-            continue;
-        }
-        double qx = 1.0;
-        if (v.draft) {
-            qr = static_cast<const T *>(v.draft) + (int64_t)(c0 + taken) * v.draft_stride;
-            q = dist(qr, v.vocab, heat, red, ired);
-            lost = q.lost;
-            if (lost) break;
-            if (known) qx = prob(q, to_f32(qr[x]), heat);
-        }
-        refused = !(known && (double)v.accept_at[c0 + taken] * qx < prob(p, to_f32(pr[x]), heat));
-        if (refused) break;
+// A row's largest logit (NaN: one is NaN or +inf), where it first stands, sum of exp((x - largest) / T).
+struct Stats {
+    float m, s;
+    int at;
+};
+__device__ __forceinline__ bool no_dist(float m) { return !(m <= FLT_MAX && m > -INFINITY); }
+
+// exp((x - m) / T) as FP32 and in 64 bits (for x <= m).
+struct Heat {
+    float scale;  // log2 e / T
+    double over;  // 1 / T
+    // (a finite scale above 0: at the edges of FP32 0 and -inf differences keep their exponentials)
+    __device__ __forceinline__ explicit Heat(float t)
+        : scale(t > 0.0f ? fminf(fmaxf(LOG2E / t, FLT_MIN), FLT_MAX) : 0.0f), over(t > 0.0f ? 1.0 / (double)t : 0.0) {}
+    __device__ __forceinline__ float e32(float x, float m) const { return __builtin_amdgcn_exp2f((x - m) * scale); }
+    __device__ __forceinline__ double e64(float x, float m) const {
+        return exp(((double)x - (double)m) * over);
     }
-    if (!lost && heat == 0.0) token = p.best;
-    if (!lost && heat > 0.0) {
-        const int x = refused ? v.drafted[c0 + taken] : -1;
-        bool left = refused;
-        auto weight = [&](int j) {
-            double w = prob(p, to_f32(pr[j]), heat);
-            if (left) w = v.draft ? fmax(w - prob(q, to_f32(qr[j]), heat), 0.0) : j == x ? 0.0 : w;
-            return w;
-        };
-        double all = 0.0;
-        for (int round = 0; round < 2; round++) {  // nothing left: from p itself
-            all = 0.0;
-            for (int j = tid; j < v.vocab; j += VERIFY_THREADS) all += weight(j);
-            all = block_all(all, [](double a, double b) { return a + b; }, red);
-            if (all > 0.0 || !left) break;
-            left = false;
+};
+
+// What a sequence's drafts are.
+struct Drafts {
+    int c0, c1;
+    __device__ __forceinline__ Drafts(const VerifyDrafts &v, int i) {
+        c0 = min(max(v.cu[i], 0), v.n_drafts);
+        c1 = min(max(v.cu[i + 1], c0), v.n_drafts);
+    }
+};
+template <class T> __device__ __forceinline__ const T *target_row(const VerifyDrafts &v, int64_t r) { return static_cast<const T *>(v.logits) + r * v.stride; }
+template <class T> __device__ __forceinline__ const T *draft_row(const VerifyDrafts &v, int64_t r) { return static_cast<const T *>(v.draft) + r * v.draft_stride; }
+
+// Whether draft d of the target's row with p, q (its stats; not used without draft logits) is taken.
+template <class T>
+__device__ __forceinline__ bool takes(const VerifyDrafts &v, const Heat &h, int d, const T *prow, const T *qrow, const Stats &p, const Stats &q) {
+    const int x = v.drafted[d];
+    if (x < 0 || x >= v.vocab) return false;
+    if (h.over == 0.0) return x == p.at;
+    const double px = h.e64(to_f32(prow[x]), p.m) / (double)p.s;
+    const double qx = qrow ? h.e64(to_f32(qrow[x]), q.m) / (double)q.s : 1.0;
+    return (double)v.accept_at[d] * qx < px;
+}
+
+// ---- narrow vocabularies: a workgroup a sequence, its waves take the rows in turn -----------------
+
+// A row of at most 64 NK tokens: token 64 k + lane.
+template <class T, int NK> struct NarrowRow {
+    float x[NK];
+    __device__ __forceinline__ void load(const T *row, int vocab, int lane) {
+#pragma unroll
+        for (int k = 0; k < NK; k++) x[k] = 64 * k + lane < vocab ? to_f32(row[64 * k + lane]) : -INFINITY;
+    }
+    __device__ __forceinline__ Stats stats(const Heat &h, int vocab, int lane) const {
+        float m = -INFINITY;
+        int at = NONE;
+        bool bad = false;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            bad |= !(x[k] < INFINITY);
+            if (x[k] > m) {
+                m = x[k];
+                at = 64 * k + lane;
+            }
         }
+        const float all = wave_all(m, More());
+        Stats s{all, 0.0f, wave_all(m == all ? at : NONE, Less())};
+        if (__ballot(bad)) s.m = NAN;
+        if (no_dist(s.m)) return s;
+        if (h.over > 0.0) {
+#pragma unroll
+            for (int k = 0; k < NK; k++)
+                if (64 * k < vocab) s.s += h.e32(x[k], all);
+            s.s = wave_all(s.s, Plus());
+        }
+        return s;
+    }
+};
+
+template <class T, int NK> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_narrow(VerifyDrafts v) {
+    __shared__ int stops[VERIFY_WAVES];
+    const int i = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Drafts d(v, i);
+    const Heat h(v.temperature);
+    const int n = d.c1 - d.c0;
+    // rows 0 .. n, a wave each, until one is not taken (row n never is)
+    int stop = NONE;
+    Stats p{}, q{};
+    NarrowRow<T, NK> pr, qr;
+    bool lost = false;
+    for (int r0 = 0;; r0 += VERIFY_WAVES) {
+        const int r = r0 + wave;
+        stop = NONE;
+        if (r <= n) {
+            const T *prow = target_row<T>(v, d.c0 + i + r), *qrow = v.draft && r < n ? draft_row<T>(v, d.c0 + r) : nullptr;
+            pr.load(prow, v.vocab, lane);
+            if (qrow) qr.load(qrow, v.vocab, lane);
+            p = pr.stats(h, v.vocab, lane);
+            lost = no_dist(p.m);
+            if (qrow) {
+                q = qr.stats(h, v.vocab, lane);
+                lost |= no_dist(q.m);
+            }
+            if (lost || r == n || !takes(v, h, d.c0 + r, prow, qrow, p, q)) stop = r;
+        }
+        if (lane == 0) stops[wave] = stop;
+        __syncthreads();
+        int first = stops[0];
+#pragma unroll
+        for (int w = 1; w < VERIFY_WAVES; w++) first = min(first, stops[w]);
+        if (first != NONE) {
+            if (stop != first) return;  // (another wave's row, behind the last barrier)
+            break;
+        }
+        __syncthreads();
+    }
+    int token = -1;
+    if (!lost && h.over == 0.0) token = p.at;
+    if (!lost && h.over > 0.0) {
+        const bool refused = stop < n;
+        const int x = refused ? v.drafted[d.c0 + stop] : -1;
+        // the sums of both in 64 bits, then what is drawn from
+        double w[NK], zp = 0.0, zq = 0.0, all = 0.0;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            w[k] = 0.0;
+            if (64 * k < v.vocab) {
+                w[k] = h.e64(pr.x[k], p.m);
+                zp += w[k];
+                if (refused && v.draft) zq += h.e64(qr.x[k], q.m);
+            }
+        }
+        zp = wave_all(zp, Plus());
+        if (refused) {
+            double left[NK];
+            const double rq = v.draft ? zp / wave_all(zq, Plus()) : 0.0;
+#pragma unroll
+            for (int k = 0; k < NK; k++) {
+                left[k] = 0.0;
+                if (64 * k < v.vocab) left[k] = v.draft ? fmax(w[k] - h.e64(qr.x[k], q.m) * rq, 0.0) : 64 * k + lane == x ? 0.0 : w[k];
+                all += left[k];
+            }
+            all = wave_all(all, Plus());
+            if (all > 0.0) {
+#pragma unroll
+                for (int k = 0; k < NK; k++) w[k] = left[k];
+            }
+        }
+        if (!(all > 0.0)) all = zp;
         const double border = (double)v.sample_at[i] * all;
         double sum = 0.0;
-        int last = -1, found = 0x7fffffff;
-        for (int j0 = 0; j0 < v.vocab; j0 += VERIFY_THREADS) {
-            const int j = j0 + tid;
-            const double w = j < v.vocab ? weight(j) : 0.0;
-            if (w > 0.0) last = j;
-            __syncthreads();
-            scan[tid] = w;
-            __syncthreads();
-            for (int o = 1; o < VERIFY_THREADS; o <<= 1) {
-                const double y = tid >= o ? scan[tid - o] : 0.0;
-                __syncthreads();
-                scan[tid] += y;
-                __syncthreads();
+        int found = NONE, last = -1;
+#pragma unroll
+        for (int k = 0; k < NK; k++) {
+            if (64 * k >= v.vocab || found != NONE) continue;
+            double c = w[k];
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const double y = __shfl_up(c, o);
+                if (lane >= o) c += y;
             }
-            const int at = block_all(w > 0.0 && sum + scan[tid] > border ? j : 0x7fffffff, [](int a, int b) { return min(a, b); }, ired);
-            if (at != 0x7fffffff) {
-                found = at;
-                break;
-            }
-            sum += scan[VERIFY_THREADS - 1];
+            const unsigned long long past = __ballot(w[k] > 0.0 && sum + c > border), some = __ballot(w[k] > 0.0);
+            if (past) found = 64 * k + __builtin_ctzll(past);
+            if (some) last = 64 * k + 63 - __builtin_clzll(some);
+            sum += __shfl(c, 63);
         }
-        last = block_all(last, [](int a, int b) { return max(a, b); }, ired);
-        token = found != 0x7fffffff ? found : last;
+        token = found != NONE ? found : last;
     }
-    if (tid == 0) {
-        v.accepted[i] = taken;
+    if (lane == 0) {
+        v.accepted[i] = stop;
         v.tokens[i] = token;
     }
 }
 
+// ---- wide vocabularies ------------------------------------------------------------------------
+
+// Parts of a row, of whole pieces: 4 to 16 pieces, so that all rows make some 2048 workgroups, and at most
+// 256 parts.
+struct Cut {
+    int parts, size;
+    __host__ __device__ Cut(int n_seq, int n_drafts, int vocab) {
+        const int64_t rows = (int64_t)n_seq + 2 * (int64_t)n_drafts, pieces = ((int64_t)vocab + FINE - 1) / FINE;
+        const int64_t want = pieces * rows / 2048, least = (pieces + 255) / 256;
+        const int64_t each = want < 4 ? 4 : want > 16 ? 16 : want;
+        size = (int)(each > least ? each : least) * FINE;
+        parts = (int)(((int64_t)vocab + size - 1) / size);
+    }
+};
+// A sequence's state between the kernels.
+struct Turn {
+    int taken, lost, refused, at;  // at: arg max of the row it stands at
+    float pm, qm;
+};
+struct Space {
+    Stats *stats;  // [rows of the target, then the draft][parts]
+    Turn *turn;    // [n_seq]
+    double *z;     // [n_seq][parts][2]: of p, of q
+    double *sums;  // [n_seq][parts][2][size / FINE]: of what is left, of p
+    int rows, parts, fine;
+};
+__host__ __device__ inline size_t up16(size_t n) { return (n + 15) / 16 * 16; }
+struct Layout {
+    size_t stats, turn, z, sums, bytes;
+    __host__ __device__ Layout(int n_seq, int n_drafts, int vocab) {
+        const Cut c(n_seq, n_drafts, vocab);
+        stats = 0;
+        turn = up16(((size_t)n_seq + 2 * (size_t)n_drafts) * c.parts * sizeof(Stats));
+        z = turn + up16(n_seq * sizeof(Turn));
+        sums = z + (size_t)n_seq * c.parts * 2 * sizeof(double);
+        bytes = sums + (size_t)n_seq * c.parts * 2 * (c.size / FINE) * sizeof(double);
+    }
+};
+__device__ __forceinline__ Space space_of(const VerifyDrafts &v, void *ws) {
+    const Cut c(v.n_seq, v.n_drafts, v.vocab);
+    const Layout l(v.n_seq, v.n_drafts, v.vocab);
+    char *p = static_cast<char *>(ws);
+    return {reinterpret_cast<Stats *>(p + l.stats), reinterpret_cast<Turn *>(p + l.turn), reinterpret_cast<double *>(p + l.z),
+            reinterpret_cast<double *>(p + l.sums), v.n_seq + v.n_drafts, c.parts, c.size / FINE};
+}
+
+// 16 bytes of a row's tokens j .. as FP32, -inf from `end` on.
+template <class T, bool VEC> __device__ __forceinline__ void load16(const T *row, int j, int end, float (&x)[16 / sizeof(T)]) {
+    constexpr int VL = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(VL)));
+    if (VEC && j + VL <= end) {
+        const vec y = *reinterpret_cast<const vec *>(row + j);
+#pragma unroll
+        for (int u = 0; u < VL; u++) x[u] = to_f32(y[u]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < VL; u++) x[u] = j + u < end ? to_f32(row[j + u]) : -INFINITY;
+    }
+}
+
+// A part of a row: one pass with the largest logit so far.
+template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_rows(VerifyDrafts v, void *ws) {
+    constexpr int VL = 16 / sizeof(T), RUN = 4, STEP = VERIFY_THREADS * VL;
+    __shared__ float fred[VERIFY_WAVES];
+    __shared__ int ired[VERIFY_WAVES];
+    const Space s = space_of(v, ws);
+    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+    const int part = blockIdx.x % s.parts, r = blockIdx.x / s.parts;
+    const T *row = r < s.rows ? target_row<T>(v, r) : draft_row<T>(v, r - s.rows);
+    const Heat h(v.temperature);
+    const int first = part * cut.size, end = (int)min((int64_t)first + cut.size, (int64_t)v.vocab);
+    float m = -INFINITY, sum = 0.0f;
+    int at = NONE;
+    bool bad = false;
+    for (int j0 = first + threadIdx.x * VL; j0 < end; j0 += RUN * STEP) {
+        float x[RUN][VL];
+#pragma unroll
+        for (int k = 0; k < RUN; k++) {
+            if (j0 + k * STEP < end) load16<T, VEC>(row, j0 + k * STEP, end, x[k]);
+            else
+#pragma unroll
+                for (int u = 0; u < VL; u++) x[k][u] = -INFINITY;
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < RUN; k++)
+#pragma unroll
+            for (int u = 0; u < VL; u++) {
+                bad |= !(x[k][u] < INFINITY);
+                top = fmaxf(top, x[k][u]);
+            }
+        if (top > m) {
+            if (h.over == 0.0) {  // where it stands
+#pragma unroll
+                for (int k = RUN - 1; k >= 0; k--)
+#pragma unroll
+                    for (int u = VL - 1; u >= 0; u--)
+                        if (x[k][u] == top) at = j0 + k * STEP + u;
+            }
+            sum *= h.e32(m, top);  // (0 at first)
+            m = top;
+        }
+        if (h.over > 0.0 && m > -INFINITY)
+#pragma unroll
+            for (int k = 0; k < RUN; k++)
+#pragma unroll
+                for (int u = 0; u < VL; u++) sum += h.e32(x[k][u], m);
+    }
+    const float all = block_all(m, More(), fred);
+    if (m > -INFINITY) sum *= h.e32(m, all);
+    sum = block_all(sum, Plus(), fred);
+    if (h.over == 0.0) at = block_all(m == all ? at : NONE, Less(), ired);
+    const bool lost = __syncthreads_or(bad);
+    if (threadIdx.x == 0) s.stats[blockIdx.x] = {lost ? NAN : all, sum, at};
+}
+
+// The parts of a row joined, by a wave.
+__device__ __forceinline__ Stats join(const Stats *s, int parts, const Heat &h, int lane) {
+    Stats o{-INFINITY, 0.0f, NONE};
+    bool bad = false;
+    for (int k = lane; k < parts; k += 64) {
+        const Stats x = s[k];
+        bad |= x.m != x.m;
+        const float m = fmaxf(o.m, x.m);
+        if (m > -INFINITY) {
+            o.s = o.s * (o.m > -INFINITY ? h.e32(o.m, m) : 0.0f) + x.s * (x.m > -INFINITY ? h.e32(x.m, m) : 0.0f);
+            if (x.m > o.m) o.at = x.at;
+            o.m = m;
+        }
+    }
+    const float m = wave_all(o.m, More());
+    o.s = wave_all(o.m > -INFINITY ? o.s * h.e32(o.m, m) : 0.0f, Plus());
+    o.at = wave_all(o.m == m ? o.at : NONE, Less());
+    o.m = __ballot(bad) ? NAN : m;
+    return o;
+}
+
+// Where a sequence's drafts end, found by every workgroup of it; then a part's 64-bit sums of the row that is drawn from.
+template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_take(VerifyDrafts v, void *ws) {
+    constexpr int VL = 16 / sizeof(T), STEP = VERIFY_THREADS * VL;
+    __shared__ double dred[VERIFY_WAVES];
+    __shared__ Turn turns[VERIFY_WAVES];
+    const Space s = space_of(v, ws);
+    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+    const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Drafts d(v, i);
+    const Heat h(v.temperature);
+    const int n = d.c1 - d.c0;
+    Turn t{};
+    for (int r0 = 0;; r0 += VERIFY_WAVES) {
+        const int r = r0 + wave;
+        t.taken = NONE;
+        if (r <= n) {
+            const bool drafted = v.draft && r < n;
+            const Stats p = join(s.stats + (int64_t)(d.c0 + i + r) * s.parts, s.parts, h, lane);
+            const Stats q = drafted ? join(s.stats + (int64_t)(s.rows + d.c0 + r) * s.parts, s.parts, h, lane) : Stats{};
+            const bool lost = no_dist(p.m) || (drafted && no_dist(q.m));
+            if (lost || r == n ||
+                !takes(v, h, d.c0 + r, target_row<T>(v, d.c0 + i + r), drafted ? draft_row<T>(v, d.c0 + r) : nullptr, p, q))
+                t = {r, lost, r < n, p.at, p.m, q.m};
+        }
+        if (lane == 0) turns[wave] = t;
+        __syncthreads();
+        t = turns[0];
+#pragma unroll
+        for (int w = 1; w < VERIFY_WAVES; w++)
+            if (turns[w].taken < t.taken) t = turns[w];
+        if (t.taken != NONE) break;
+        __syncthreads();
+    }
+    if (part == 0 && threadIdx.x == 0) {
+        s.turn[i] = t;
+        if (t.lost || h.over == 0.0) {
+            v.accepted[i] = t.taken;
+            v.tokens[i] = t.lost ? -1 : t.at;
+        }
+    }
+    if (t.lost || h.over == 0.0) return;
+    const T *prow = target_row<T>(v, d.c0 + i + t.taken), *qrow = t.refused && v.draft ? draft_row<T>(v, d.c0 + t.taken) : nullptr;
+    const int first = part * cut.size, end = (int)min((int64_t)first + cut.size, (int64_t)v.vocab);
+    double zp = 0.0, zq = 0.0;
+    for (int j = first + threadIdx.x * VL; j < end; j += STEP) {
+        float x[VL], y[VL];
+        load16<T, VEC>(prow, j, end, x);
+        if (qrow) load16<T, VEC>(qrow, j, end, y);
+#pragma unroll
+        for (int u = 0; u < VL; u++) zp += h.e64(x[u], t.pm);
+        if (qrow)
+#pragma unroll
+            for (int u = 0; u < VL; u++) zq += h.e64(y[u], t.qm);
+    }
+    zp = block_all(zp, Plus(), dred);
+    zq = block_all(zq, Plus(), dred);
+    if (threadIdx.x == 0) {
+        double *z = s.z + ((int64_t)i * s.parts + part) * 2;
+        z[0] = zp;
+        z[1] = zq;
+    }
+}
+
+// A row's sums of p and q over the parts, the same in all lanes of all waves.
+__device__ __forceinline__ void whole(const double *z, int parts, int lane, double &zp, double &zq) {
+    zp = zq = 0.0;
+    for (int k = lane; k < parts; k += 64) {
+        zp += z[2 * k];
+        zq += z[2 * k + 1];
+    }
+    zp = wave_all(zp, Plus());
+    zq = wave_all(zq, Plus());
+}
+
+// What is drawn from, in units of 1 / zp: max(p - q, 0) (left) and p.
+template <class T> struct Weights {
+    const T *prow, *qrow;
+    Heat h;
+    float pm, qm;
+    double rq;  // zp / zq
+    int x;      // a certain draft that was refused, else -1
+    bool refused;
+    __device__ __forceinline__ void of(float p, float q, int j, double &left, double &all) const {
+        all = h.e64(p, pm);
+        left = qrow ? fmax(all - h.e64(q, qm) * rq, 0.0) : j == x ? 0.0 : all;
+    }
+};
+template <class T> __device__ __forceinline__ Weights<T> weights_of(const VerifyDrafts &v, const Space &s, int i, const Drafts &d, const Turn &t, int lane) {
+    double zp, zq;
+    whole(s.z + (int64_t)i * s.parts * 2, s.parts, lane, zp, zq);
+    Weights<T> w{target_row<T>(v, d.c0 + i + t.taken), t.refused && v.draft ? draft_row<T>(v, d.c0 + t.taken) : nullptr, Heat(v.temperature),
+                 t.pm, t.qm, zp / zq, t.refused && !v.draft ? v.drafted[d.c0 + t.taken] : -1, t.refused != 0};
+    return w;
+}
+
+// The sums of each piece of FINE tokens of a part: a wave a piece.
+template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_left(VerifyDrafts v, void *ws) {
+    constexpr int VL = 16 / sizeof(T);
+    const Space s = space_of(v, ws);
+    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+    const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Turn t = s.turn[i];
+    if (t.lost) return;
+    const Drafts d(v, i);
+    const Weights<T> w = weights_of<T>(v, s, i, d, t, lane);
+    const int end = (int)min((int64_t)(part + 1) * cut.size, (int64_t)v.vocab);
+    double *out = s.sums + ((int64_t)i * s.parts + part) * 2 * s.fine;
+    for (int f = wave; f < s.fine; f += VERIFY_WAVES) {
+        const int first = part * cut.size + f * FINE, last = min(first + FINE, end);
+        double a = 0.0, b = 0.0;
+        for (int j = first + lane * VL; j < last; j += 64 * VL) {
+            float x[VL], y[VL] = {};
+            load16<T, VEC>(w.prow, j, last, x);
+            if (w.qrow) load16<T, VEC>(w.qrow, j, last, y);
+#pragma unroll
+            for (int u = 0; u < VL; u++) {
+                if (j + u >= last) continue;
+                double left, all;
+                w.of(x[u], y[u], j + u, left, all);
+                a += left;
+                b += all;
+            }
+        }
+        a = wave_all(a, Plus());
+        b = wave_all(b, Plus());
+        if (lane == 0) {
+            out[f] = a;
+            out[s.fine + f] = b;
+        }
+    }
+}
+
+// The piece in which the border lies, then the token: a wave a sequence.
+template <class T> __global__ __launch_bounds__(64) void k_verify_draw(VerifyDrafts v, void *ws) {
+    const Space s = space_of(v, ws);
+    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+    const int i = blockIdx.x, lane = threadIdx.x;
+    const Turn t = s.turn[i];
+    if (t.lost) return;
+    const Drafts d(v, i);
+    const Weights<T> w = weights_of<T>(v, s, i, d, t, lane);
+    const double *sums = s.sums + (int64_t)i * s.parts * 2 * s.fine;
+    const int pieces = (v.vocab + FINE - 1) / FINE;
+    auto sum_of = [&](int f, int which) { return sums[((int64_t)(f / s.fine) * 2 + which) * s.fine + f % s.fine]; };
+    // (nothing left: from p itself)
+    double all = 0.0;
+    int which = w.refused ? 0 : 1;
+    for (; which < 2; which++) {
+        all = 0.0;
+        for (int f = lane; f < pieces; f += 64) all += sum_of(f, which);
+        all = wave_all(all, Plus());
+        if (all > 0.0) break;
+    }
+    if (which > 1) which = 1;
+    const double border = (double)v.sample_at[i] * all;
+    auto before = [&](double c) {  // running sum over the lanes
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double y = __shfl_up(c, o);
+            if (lane >= o) c += y;
+        }
+        return c;
+    };
+    // the first piece whose running sum passes the border; else the last one with a weight
+    double sum = 0.0, start = 0.0, last_start = 0.0;
+    int piece = NONE, last = 0;
+    for (int f0 = 0; f0 < pieces && piece == NONE; f0 += 64) {
+        const double x = f0 + lane < pieces ? sum_of(f0 + lane, which) : 0.0, c = before(x);
+        const unsigned long long past = __ballot(x > 0.0 && sum + c > border), some = __ballot(x > 0.0);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            piece = f0 + at;
+            start = sum + __shfl(c - x, at);
+        }
+        if (some) {
+            const int at = 63 - __builtin_clzll(some);
+            last = f0 + at;
+            last_start = sum + __shfl(c - x, at);
+        }
+        sum += __shfl(c, 63);
+    }
+    if (piece == NONE) {
+        piece = last;
+        start = last_start;
+    }
+    // its tokens, 64 at a time
+    const int end = min((piece + 1) * FINE, v.vocab);
+    int found = NONE, behind = -1;
+    for (int j0 = piece * FINE; j0 < end && found == NONE; j0 += 64) {
+        const int j = j0 + lane;
+        double x = 0.0, whole_x = 0.0;
+        if (j < end) {
+            w.of(to_f32(w.prow[j]), w.qrow ? to_f32(w.qrow[j]) : 0.0f, j, x, whole_x);
+            if (which == 1) x = whole_x;
+        }
+        const double c = before(x);
+        const unsigned long long past = __ballot(x > 0.0 && start + c > border), some = __ballot(x > 0.0);
+        if (past) found = j0 + __builtin_ctzll(past);
+        if (some) behind = j0 + 63 - __builtin_clzll(some);
+        start += __shfl(c, 63);
+    }
+    if (lane == 0) {
+        v.accepted[i] = t.taken;
+        v.tokens[i] = found != NONE ? found : behind;
+    }
+}
+
+template <class T> hipError_t launch(const VerifyDrafts &v, void *ws, hipStream_t st) {
+    if (v.vocab <= NARROW) {
+        if (!kv8_grid(v.n_seq, VERIFY_THREADS)) return hipErrorInvalidValue;
+        if (v.vocab <= 64) hipLaunchKernelGGL((k_verify_narrow<T, 1>), dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v);
+        else hipLaunchKernelGGL((k_verify_narrow<T, NARROW / 64>), dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v);
+        return hipGetLastError();
+    }
+    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+    const bool draws = v.temperature > 0.0f;
+    const int64_t rows = (int64_t)v.n_seq + v.n_drafts + (v.draft ? v.n_drafts : 0), own = (int64_t)v.n_seq * cut.parts;
+    if (!kv8_grid(rows * cut.parts, VERIFY_THREADS) || !kv8_grid(own, VERIFY_THREADS)) return hipErrorInvalidValue;
+    auto aligned = [](const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T))) % 16 == 0; };
+    auto go = [&](auto vec) {
+        constexpr bool VEC = decltype(vec)::value;
+        hipLaunchKernelGGL((k_verify_rows<T, VEC>), dim3(rows * cut.parts), dim3(VERIFY_THREADS), 0, st, v, ws);
+        hipLaunchKernelGGL((k_verify_take<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, ws);
+        if (!draws) return;
+        hipLaunchKernelGGL((k_verify_left<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, ws);
+        hipLaunchKernelGGL(k_verify_draw<T>, dim3(v.n_seq), dim3(64), 0, st, v, ws);
+    };
+    if (aligned(v.logits, v.stride) && (!v.draft || aligned(v.draft, v.draft_stride))) go(std::true_type{});
+    else go(std::false_type{});
+    return hipGetLastError();
+}
+
 }  // namespace
 
-size_t verify_drafts_bytes(int n_seq, int n_drafts, int vocab) { return 0; }
+size_t verify_drafts_bytes(int n_seq, int n_drafts, int vocab) {
+    return vocab <= NARROW || n_seq == 0 ? 0 : Layout(n_seq, n_drafts, vocab).bytes;
+}
 
 hipError_t launch_verify_drafts(const VerifyDrafts &v, void *ws, hipStream_t st) {
     if (v.n_seq == 0) return hipSuccess;
-    if (!kv8_grid(v.n_seq, VERIFY_THREADS)) return hipErrorInvalidValue;
     switch (v.dtype) {
-        case FT_F32: hipLaunchKernelGGL(k_verify<float>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v); break;
-        case FT_F16: hipLaunchKernelGGL(k_verify<_Float16>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v); break;
-        case FT_BF16: hipLaunchKernelGGL(k_verify<__bf16>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v); break;
-        default: return hipErrorInvalidValue;
+        case FT_F32: return launch<float>(v, ws, st);
+        case FT_F16: return launch<_Float16>(v, ws, st);
+        case FT_BF16: return launch<__bf16>(v, ws, st);
     }
-    return hipGetLastError();
+    return hipErrorInvalidValue;
 }
 
 }  // namespace cih
