@@ -60,17 +60,36 @@ struct Stats {
 };
 __device__ __forceinline__ bool no_dist(float m) { return !(m <= FLT_MAX && m > -INFINITY); }
 
+// 2^t for t <= 0, to 10^-16 of itself: t = k + f with |f| <= 1/2, 2^f = e^y as its series in y = f ln 2 <= 0.35, whose
+// 14th term is 4 10^-18.  (The library's exp takes three times as many instructions.)
+__device__ __forceinline__ double pow2(double t) {
+    t = fmax(t, -2000.0);  // (2^-2000 is 0; -inf too)
+    const double k = rint(t), y = (t - k) * 0.69314718055994530942;
+    double e = 1.0 / 6227020800.0;  // 1 / 13!
+    e = fma(e, y, 1.0 / 479001600.0);
+    e = fma(e, y, 1.0 / 39916800.0);
+    e = fma(e, y, 1.0 / 3628800.0);
+    e = fma(e, y, 1.0 / 362880.0);
+    e = fma(e, y, 1.0 / 40320.0);
+    e = fma(e, y, 1.0 / 5040.0);
+    e = fma(e, y, 1.0 / 720.0);
+    e = fma(e, y, 1.0 / 120.0);
+    e = fma(e, y, 1.0 / 24.0);
+    e = fma(e, y, 1.0 / 6.0);
+    e = fma(e, y, 0.5);
+    e = fma(e, y, 1.0);
+    return ldexp(fma(e, y, 1.0), (int)k);
+}
+
 // exp((x - m) / T) as FP32 and in 64 bits (for x <= m).
 struct Heat {
     float scale;  // log2 e / T
-    double over;  // 1 / T
+    double over;  // the same
     // (a finite scale above 0: at the edges of FP32 0 and -inf differences keep their exponentials)
     __device__ __forceinline__ explicit Heat(float t)
-        : scale(t > 0.0f ? fminf(fmaxf(LOG2E / t, FLT_MIN), FLT_MAX) : 0.0f), over(t > 0.0f ? 1.0 / (double)t : 0.0) {}
+        : scale(t > 0.0f ? fminf(fmaxf(LOG2E / t, FLT_MIN), FLT_MAX) : 0.0f), over(t > 0.0f ? 1.4426950408889634074 / (double)t : 0.0) {}
     __device__ __forceinline__ float e32(float x, float m) const { return __builtin_amdgcn_exp2f((x - m) * scale); }
-    __device__ __forceinline__ double e64(float x, float m) const {
-        return exp(((double)x - (double)m) * over);
-    }
+    __device__ __forceinline__ double e64(float x, float m) const { return pow2(((double)x - (double)m) * over); }
 };
 
 // What a sequence's drafts are.
@@ -496,11 +515,13 @@ template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k
     }
 }
 
-// The piece in which the border lies, then the token: a wave a sequence.
-template <class T> __global__ __launch_bounds__(64) void k_verify_draw(VerifyDrafts v, void *ws) {
+// The piece in which the border lies, by every wave; then the token, a thread four of the piece's.
+template <class T> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_draw(VerifyDrafts v, void *ws) {
+    constexpr int OWN = FINE / VERIFY_THREADS;
+    __shared__ double part[VERIFY_WAVES];
+    __shared__ int ired[VERIFY_WAVES];
     const Space s = space_of(v, ws);
-    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
-    const int i = blockIdx.x, lane = threadIdx.x;
+    const int i = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Turn t = s.turn[i];
     if (t.lost) return;
     const Drafts d(v, i);
@@ -549,23 +570,35 @@ template <class T> __global__ __launch_bounds__(64) void k_verify_draw(VerifyDra
         piece = last;
         start = last_start;
     }
-    // its tokens, 64 at a time
-    const int end = min((piece + 1) * FINE, v.vocab);
-    int found = NONE, behind = -1;
-    for (int j0 = piece * FINE; j0 < end && found == NONE; j0 += 64) {
-        const int j = j0 + lane;
-        double x = 0.0, whole_x = 0.0;
-        if (j < end) {
-            w.of(to_f32(w.prow[j]), w.qrow ? to_f32(w.qrow[j]) : 0.0f, j, x, whole_x);
-            if (which == 1) x = whole_x;
+    const int first = piece * FINE + threadIdx.x * OWN;
+    double x[OWN], mine = 0.0;
+#pragma unroll
+    for (int u = 0; u < OWN; u++) {
+        x[u] = 0.0;
+        if (first + u < v.vocab) {
+            double left, p;
+            w.of(to_f32(w.prow[first + u]), w.qrow ? to_f32(w.qrow[first + u]) : 0.0f, first + u, left, p);
+            x[u] = which == 1 ? p : left;
         }
-        const double c = before(x);
-        const unsigned long long past = __ballot(x > 0.0 && start + c > border), some = __ballot(x > 0.0);
-        if (past) found = j0 + __builtin_ctzll(past);
-        if (some) behind = j0 + 63 - __builtin_clzll(some);
-        start += __shfl(c, 63);
+        mine += x[u];
     }
-    if (lane == 0) {
+    double c = before(mine);
+    if (lane == 63) part[wave] = c;
+    __syncthreads();
+    c = start + (c - mine);
+    for (int u = 0; u < wave; u++) c += part[u];
+    int found = NONE, behind = -1;
+#pragma unroll
+    for (int u = 0; u < OWN; u++) {
+        c += x[u];
+        if (x[u] > 0.0) {
+            behind = first + u;
+            if (c > border && found == NONE) found = first + u;
+        }
+    }
+    found = block_all(found, Less(), ired);
+    behind = block_all(behind, More(), ired);
+    if (threadIdx.x == 0) {
         v.accepted[i] = t.taken;
         v.tokens[i] = found != NONE ? found : behind;
     }
@@ -589,7 +622,7 @@ template <class T> hipError_t launch(const VerifyDrafts &v, void *ws, hipStream_
         hipLaunchKernelGGL((k_verify_take<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, ws);
         if (!draws) return;
         hipLaunchKernelGGL((k_verify_left<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, ws);
-        hipLaunchKernelGGL(k_verify_draw<T>, dim3(v.n_seq), dim3(64), 0, st, v, ws);
+        hipLaunchKernelGGL(k_verify_draw<T>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v, ws);
     };
     if (aligned(v.logits, v.stride) && (!v.draft || aligned(v.draft, v.draft_stride))) go(std::true_type{});
     else go(std::false_type{});
