@@ -33,14 +33,14 @@ template <class V, class OP> __device__ __forceinline__ V wave_all(V v, OP op) {
     for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
     return v;
 }
-template <class V, class OP> __device__ __forceinline__ V block_all(V v, OP op, V *red) {
+template <int W = VERIFY_WAVES, class V, class OP> __device__ __forceinline__ V block_all(V v, OP op, V *red) {
     v = wave_all(v, op);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = red[0];
 #pragma unroll
-    for (int w = 1; w < VERIFY_WAVES; w++) v = op(v, red[w]);
+    for (int w = 1; w < W; w++) v = op(v, red[w]);
     return v;
 }
 struct Plus {
@@ -60,25 +60,25 @@ struct Stats {
 };
 __device__ __forceinline__ bool no_dist(float m) { return !(m <= FLT_MAX && m > -INFINITY); }
 
-// 2^t for t <= 0, to 10^-16 of itself: t = k + f with |f| <= 1/2, 2^f = e^y as its series in y = f ln 2 <= 0.35, whose
-// 14th term is 4 10^-18.  (The library's exp takes three times as many instructions.)
+// 2^t for t <= 0, to 4 10^-16 of itself (0 from t = -1000 on): t = k + f with |f| <= 1/2, 2^f by the polynomial
+// of degree 10 that meets it at the 11 Chebyshev nodes, k into the exponent.  Half the clocks of the library's
+// exp, which the sums of a drawn row wait for.
 __device__ __forceinline__ double pow2(double t) {
-    t = fmax(t, -2000.0);  // (2^-2000 is 0; -inf too)
-    const double k = rint(t), y = (t - k) * 0.69314718055994530942;
-    double e = 1.0 / 6227020800.0;  // 1 / 13!
-    e = fma(e, y, 1.0 / 479001600.0);
-    e = fma(e, y, 1.0 / 39916800.0);
-    e = fma(e, y, 1.0 / 3628800.0);
-    e = fma(e, y, 1.0 / 362880.0);
-    e = fma(e, y, 1.0 / 40320.0);
-    e = fma(e, y, 1.0 / 5040.0);
-    e = fma(e, y, 1.0 / 720.0);
-    e = fma(e, y, 1.0 / 120.0);
-    e = fma(e, y, 1.0 / 24.0);
-    e = fma(e, y, 1.0 / 6.0);
-    e = fma(e, y, 0.5);
-    e = fma(e, y, 1.0);
-    return ldexp(fma(e, y, 1.0), (int)k);
+    constexpr double WHOLE = 6755399441055744.0;  // 1.5 2^52: its sum with a number has that rounded in its low bits
+    const double near = fmax(t, -1000.0), kd = near + WHOLE, f = near - (kd - WHOLE);
+    double e = 7.072585949269223e-09;
+    e = fma(e, f, 1.0208690299958306e-07);
+    e = fma(e, f, 1.321544258792169e-06);
+    e = fma(e, f, 1.5252657260200837e-05);
+    e = fma(e, f, 0.0001540353044173605);
+    e = fma(e, f, 0.0013333558230164974);
+    e = fma(e, f, 0.009618129107606888);
+    e = fma(e, f, 0.05550410866444772);
+    e = fma(e, f, 0.24022650695910097);
+    e = fma(e, f, 0.69314718055995);
+    e = fma(e, f, 1.0);
+    const double o = __hiloint2double(__double2hiint(e) + (__double2loint(kd) << 20), __double2loint(e));
+    return t > -1000.0 ? o : 0.0;
 }
 
 // exp((x - m) / T) as FP32 and in 64 bits (for x <= m).
@@ -103,16 +103,29 @@ struct Drafts {
 template <class T> __device__ __forceinline__ const T *target_row(const VerifyDrafts &v, int64_t r) { return static_cast<const T *>(v.logits) + r * v.stride; }
 template <class T> __device__ __forceinline__ const T *draft_row(const VerifyDrafts &v, int64_t r) { return static_cast<const T *>(v.draft) + r * v.draft_stride; }
 
-// Whether draft d of the target's row with p, q (its stats; not used without draft logits) is taken.
-template <class T>
-__device__ __forceinline__ bool takes(const VerifyDrafts &v, const Heat &h, int d, const T *prow, const T *qrow, const Stats &p, const Stats &q) {
-    const int x = v.drafted[d];
-    if (x < 0 || x >= v.vocab) return false;
-    if (h.over == 0.0) return x == p.at;
-    const double px = h.e64(to_f32(prow[x]), p.m) / (double)p.s;
-    const double qx = qrow ? h.e64(to_f32(qrow[x]), q.m) / (double)q.s : 1.0;
-    return (double)v.accept_at[d] * qx < px;
-}
+// A draft of the target's row, with its logits (qrow nullptr: it is certain).
+struct Draft {
+    int x;
+    float at, lp, lq;
+    bool certain, known;
+    Draft() = default;
+    template <class T>
+    __device__ __forceinline__ Draft(const VerifyDrafts &v, const Heat &h, int d, const T *prow, const T *qrow) : x(v.drafted[d]), at(0.0f), lp(0.0f), lq(0.0f) {
+        known = x >= 0 && x < v.vocab;
+        certain = qrow == nullptr;
+        if (h.over > 0.0) {
+            at = v.accept_at[d];
+            lp = to_f32(prow[known ? x : 0]);
+            lq = certain ? 0.0f : to_f32(qrow[known ? x : 0]);
+        }
+    }
+    // whether it is taken, p and q the rows' stats
+    __device__ __forceinline__ bool taken(const Heat &h, const Stats &p, const Stats &q) const {
+        if (h.over == 0.0) return x == p.at;
+        const double px = h.e64(lp, p.m) / (double)p.s, qx = certain ? 1.0 : h.e64(lq, q.m) / (double)q.s;
+        return known && (double)at * qx < px;
+    }
+};
 
 // ---- narrow vocabularies: a workgroup a sequence, its waves take the rows in turn -----------------
 
@@ -167,13 +180,15 @@ template <class T, int NK> __global__ __launch_bounds__(VERIFY_THREADS) void k_v
             const T *prow = target_row<T>(v, d.c0 + i + r), *qrow = v.draft && r < n ? draft_row<T>(v, d.c0 + r) : nullptr;
             pr.load(prow, v.vocab, lane);
             if (qrow) qr.load(qrow, v.vocab, lane);
+            Draft draft;
+            if (r < n) draft = Draft(v, h, d.c0 + r, prow, qrow);
             p = pr.stats(h, v.vocab, lane);
             lost = no_dist(p.m);
             if (qrow) {
                 q = qr.stats(h, v.vocab, lane);
                 lost |= no_dist(q.m);
             }
-            if (lost || r == n || !takes(v, h, d.c0 + r, prow, qrow, p, q)) stop = r;
+            if (lost || r == n || !draft.taken(h, p, q)) stop = r;
         }
         if (lane == 0) stops[wave] = stop;
         __syncthreads();
@@ -250,7 +265,7 @@ template <class T, int NK> __global__ __launch_bounds__(VERIFY_THREADS) void k_v
 // 256 parts.
 struct Cut {
     int parts, size;
-    __host__ __device__ Cut(int n_seq, int n_drafts, int vocab) {
+    Cut(int n_seq, int n_drafts, int vocab) {
         const int64_t rows = (int64_t)n_seq + 2 * (int64_t)n_drafts, pieces = ((int64_t)vocab + FINE - 1) / FINE;
         const int64_t want = pieces * rows / 2048, least = (pieces + 255) / 256;
         const int64_t each = want < 4 ? 4 : want > 16 ? 16 : want;
@@ -267,28 +282,25 @@ struct Space {
     Stats *stats;  // [rows of the target, then the draft][parts]
     Turn *turn;    // [n_seq]
     double *z;     // [n_seq][parts][2]: of p, of q
-    double *sums;  // [n_seq][parts][2][size / FINE]: of what is left, of p
-    int rows, parts, fine;
-};
-__host__ __device__ inline size_t up16(size_t n) { return (n + 15) / 16 * 16; }
-struct Layout {
-    size_t stats, turn, z, sums, bytes;
-    __host__ __device__ Layout(int n_seq, int n_drafts, int vocab) {
+    double *sums;  // [n_seq][parts][2][fine]: of what is left, of p
+    int rows, parts, size, fine;
+    size_t bytes;
+    Space(int n_seq, int n_drafts, int vocab, void *ws) {
+        auto up16 = [](size_t n) { return (n + 15) / 16 * 16; };
         const Cut c(n_seq, n_drafts, vocab);
-        stats = 0;
-        turn = up16(((size_t)n_seq + 2 * (size_t)n_drafts) * c.parts * sizeof(Stats));
-        z = turn + up16(n_seq * sizeof(Turn));
-        sums = z + (size_t)n_seq * c.parts * 2 * sizeof(double);
-        bytes = sums + (size_t)n_seq * c.parts * 2 * (c.size / FINE) * sizeof(double);
+        rows = n_seq + n_drafts;
+        parts = c.parts;
+        size = c.size;
+        fine = size / FINE;
+        const size_t all = ((size_t)rows + n_drafts) * parts * sizeof(Stats), cut = (size_t)n_seq * parts;
+        char *p = static_cast<char *>(ws);
+        stats = reinterpret_cast<Stats *>(p);
+        turn = reinterpret_cast<Turn *>(p + up16(all));
+        z = reinterpret_cast<double *>(p + up16(all) + up16(n_seq * sizeof(Turn)));
+        sums = z + cut * 2;
+        bytes = up16(all) + up16(n_seq * sizeof(Turn)) + cut * 2 * (1 + fine) * sizeof(double);
     }
 };
-__device__ __forceinline__ Space space_of(const VerifyDrafts &v, void *ws) {
-    const Cut c(v.n_seq, v.n_drafts, v.vocab);
-    const Layout l(v.n_seq, v.n_drafts, v.vocab);
-    char *p = static_cast<char *>(ws);
-    return {reinterpret_cast<Stats *>(p + l.stats), reinterpret_cast<Turn *>(p + l.turn), reinterpret_cast<double *>(p + l.z),
-            reinterpret_cast<double *>(p + l.sums), v.n_seq + v.n_drafts, c.parts, c.size / FINE};
-}
 
 // 16 bytes of a row's tokens j .. as FP32, -inf from `end` on.
 template <class T, bool VEC> __device__ __forceinline__ void load16(const T *row, int j, int end, float (&x)[16 / sizeof(T)]) {
@@ -305,16 +317,14 @@ template <class T, bool VEC> __device__ __forceinline__ void load16(const T *row
 }
 
 // A part of a row: one pass with the largest logit so far.
-template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_rows(VerifyDrafts v, void *ws) {
+template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_rows(VerifyDrafts v, Space s) {
     constexpr int VL = 16 / sizeof(T), RUN = 4, STEP = VERIFY_THREADS * VL;
     __shared__ float fred[VERIFY_WAVES];
     __shared__ int ired[VERIFY_WAVES];
-    const Space s = space_of(v, ws);
-    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
     const int part = blockIdx.x % s.parts, r = blockIdx.x / s.parts;
     const T *row = r < s.rows ? target_row<T>(v, r) : draft_row<T>(v, r - s.rows);
     const Heat h(v.temperature);
-    const int first = part * cut.size, end = (int)min((int64_t)first + cut.size, (int64_t)v.vocab);
+    const int first = part * s.size, end = (int)min((int64_t)first + s.size, (int64_t)v.vocab);
     float m = -INFINITY, sum = 0.0f;
     int at = NONE;
     bool bad = false;
@@ -381,36 +391,37 @@ __device__ __forceinline__ Stats join(const Stats *s, int parts, const Heat &h, 
     return o;
 }
 
-// Where a sequence's drafts end, found by every workgroup of it; then a part's 64-bit sums of the row that is drawn from.
-template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_take(VerifyDrafts v, void *ws) {
-    constexpr int VL = 16 / sizeof(T), STEP = VERIFY_THREADS * VL;
-    __shared__ double dred[VERIFY_WAVES];
-    __shared__ Turn turns[VERIFY_WAVES];
-    const Space s = space_of(v, ws);
-    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+// Where a sequence's drafts end, found by every workgroup of it (a wave a row: eight, so that up to seven drafts take one
+// round); then a part's 64-bit sums of the row that is drawn from.
+constexpr int TAKE_THREADS = 512, TAKE_WAVES = TAKE_THREADS / 64;
+template <class T, bool VEC> __global__ __launch_bounds__(TAKE_THREADS) void k_verify_take(VerifyDrafts v, Space s) {
+    constexpr int VL = 16 / sizeof(T), STEP = TAKE_THREADS * VL;
+    __shared__ double dred[TAKE_WAVES];
+    __shared__ Turn turns[TAKE_WAVES];
     const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Drafts d(v, i);
     const Heat h(v.temperature);
     const int n = d.c1 - d.c0;
     Turn t{};
-    for (int r0 = 0;; r0 += VERIFY_WAVES) {
+    for (int r0 = 0;; r0 += TAKE_WAVES) {
         const int r = r0 + wave;
         t.taken = NONE;
         if (r <= n) {
             const bool drafted = v.draft && r < n;
+            Draft draft;
+            if (r < n)
+                draft = Draft(v, h, d.c0 + r, target_row<T>(v, d.c0 + i + r), drafted ? draft_row<T>(v, d.c0 + r) : nullptr);
             const Stats p = join(s.stats + (int64_t)(d.c0 + i + r) * s.parts, s.parts, h, lane);
             const Stats q = drafted ? join(s.stats + (int64_t)(s.rows + d.c0 + r) * s.parts, s.parts, h, lane) : Stats{};
             const bool lost = no_dist(p.m) || (drafted && no_dist(q.m));
-            if (lost || r == n ||
-                !takes(v, h, d.c0 + r, target_row<T>(v, d.c0 + i + r), drafted ? draft_row<T>(v, d.c0 + r) : nullptr, p, q))
-                t = {r, lost, r < n, p.at, p.m, q.m};
+            if (lost || r == n || !draft.taken(h, p, q)) t = {r, lost, r < n, p.at, p.m, q.m};
         }
         if (lane == 0) turns[wave] = t;
         __syncthreads();
         t = turns[0];
 #pragma unroll
-        for (int w = 1; w < VERIFY_WAVES; w++)
+        for (int w = 1; w < TAKE_WAVES; w++)
             if (turns[w].taken < t.taken) t = turns[w];
         if (t.taken != NONE) break;
         __syncthreads();
@@ -424,7 +435,7 @@ template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k
     }
     if (t.lost || h.over == 0.0) return;
     const T *prow = target_row<T>(v, d.c0 + i + t.taken), *qrow = t.refused && v.draft ? draft_row<T>(v, d.c0 + t.taken) : nullptr;
-    const int first = part * cut.size, end = (int)min((int64_t)first + cut.size, (int64_t)v.vocab);
+    const int first = part * s.size, end = (int)min((int64_t)first + s.size, (int64_t)v.vocab);
     double zp = 0.0, zq = 0.0;
     for (int j = first + threadIdx.x * VL; j < end; j += STEP) {
         float x[VL], y[VL];
@@ -436,8 +447,8 @@ template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k
 #pragma unroll
             for (int u = 0; u < VL; u++) zq += h.e64(y[u], t.qm);
     }
-    zp = block_all(zp, Plus(), dred);
-    zq = block_all(zq, Plus(), dred);
+    zp = block_all<TAKE_WAVES>(zp, Plus(), dred);
+    zq = block_all<TAKE_WAVES>(zq, Plus(), dred);
     if (threadIdx.x == 0) {
         double *z = s.z + ((int64_t)i * s.parts + part) * 2;
         z[0] = zp;
@@ -478,20 +489,18 @@ template <class T> __device__ __forceinline__ Weights<T> weights_of(const Verify
 }
 
 // The sums of each piece of FINE tokens of a part: a wave a piece.
-template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_left(VerifyDrafts v, void *ws) {
+template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_left(VerifyDrafts v, Space s) {
     constexpr int VL = 16 / sizeof(T);
-    const Space s = space_of(v, ws);
-    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
     const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Turn t = s.turn[i];
     if (t.lost) return;
     const Drafts d(v, i);
     const Weights<T> w = weights_of<T>(v, s, i, d, t, lane);
-    const int end = (int)min((int64_t)(part + 1) * cut.size, (int64_t)v.vocab);
+    const int end = (int)min((int64_t)(part + 1) * s.size, (int64_t)v.vocab);
     double *out = s.sums + ((int64_t)i * s.parts + part) * 2 * s.fine;
     for (int f = wave; f < s.fine; f += VERIFY_WAVES) {
-        const int first = part * cut.size + f * FINE, last = min(first + FINE, end);
+        const int first = part * s.size + f * FINE, last = min(first + FINE, end);
         double a = 0.0, b = 0.0;
         for (int j = first + lane * VL; j < last; j += 64 * VL) {
             float x[VL], y[VL] = {};
@@ -516,11 +525,10 @@ template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k
 }
 
 // The piece in which the border lies, by every wave; then the token, a thread four of the piece's.
-template <class T> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_draw(VerifyDrafts v, void *ws) {
+template <class T> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_draw(VerifyDrafts v, Space s) {
     constexpr int OWN = FINE / VERIFY_THREADS;
     __shared__ double part[VERIFY_WAVES];
     __shared__ int ired[VERIFY_WAVES];
-    const Space s = space_of(v, ws);
     const int i = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Turn t = s.turn[i];
     if (t.lost) return;
@@ -611,18 +619,19 @@ template <class T> hipError_t launch(const VerifyDrafts &v, void *ws, hipStream_
         else hipLaunchKernelGGL((k_verify_narrow<T, NARROW / 64>), dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v);
         return hipGetLastError();
     }
-    const Cut cut(v.n_seq, v.n_drafts, v.vocab);
+    const Space s(v.n_seq, v.n_drafts, v.vocab, ws);
     const bool draws = v.temperature > 0.0f;
-    const int64_t rows = (int64_t)v.n_seq + v.n_drafts + (v.draft ? v.n_drafts : 0), own = (int64_t)v.n_seq * cut.parts;
-    if (!kv8_grid(rows * cut.parts, VERIFY_THREADS) || !kv8_grid(own, VERIFY_THREADS)) return hipErrorInvalidValue;
+    const int64_t rows = (int64_t)v.n_seq + v.n_drafts + (v.draft ? v.n_drafts : 0), own = (int64_t)v.n_seq * s.parts;
+    if (!kv8_grid(rows * s.parts, VERIFY_THREADS) || !kv8_grid(own, VERIFY_THREADS)) return hipErrorInvalidValue;
+    if (!kv8_grid(own, TAKE_THREADS)) return hipErrorInvalidValue;
     auto aligned = [](const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T))) % 16 == 0; };
     auto go = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
-        hipLaunchKernelGGL((k_verify_rows<T, VEC>), dim3(rows * cut.parts), dim3(VERIFY_THREADS), 0, st, v, ws);
-        hipLaunchKernelGGL((k_verify_take<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, ws);
+        hipLaunchKernelGGL((k_verify_rows<T, VEC>), dim3(rows * s.parts), dim3(VERIFY_THREADS), 0, st, v, s);
+        hipLaunchKernelGGL((k_verify_take<T, VEC>), dim3(own), dim3(TAKE_THREADS), 0, st, v, s);
         if (!draws) return;
-        hipLaunchKernelGGL((k_verify_left<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, ws);
-        hipLaunchKernelGGL(k_verify_draw<T>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v, ws);
+        hipLaunchKernelGGL((k_verify_left<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, s);
+        hipLaunchKernelGGL(k_verify_draw<T>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v, s);
     };
     if (aligned(v.logits, v.stride) && (!v.draft || aligned(v.draft, v.draft_stride))) go(std::true_type{});
     else go(std::false_type{});
@@ -632,7 +641,7 @@ template <class T> hipError_t launch(const VerifyDrafts &v, void *ws, hipStream_
 }  // namespace
 
 size_t verify_drafts_bytes(int n_seq, int n_drafts, int vocab) {
-    return vocab <= NARROW || n_seq == 0 ? 0 : Layout(n_seq, n_drafts, vocab).bytes;
+    return vocab <= NARROW || n_seq == 0 ? 0 : Space(n_seq, n_drafts, vocab, nullptr).bytes;
 }
 
 hipError_t launch_verify_drafts(const VerifyDrafts &v, void *ws, hipStream_t st) {
