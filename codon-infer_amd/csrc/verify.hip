@@ -8,9 +8,15 @@
 // as many terms as there are tokens, and errors of 10^-7 of the whole would move it to a neighbour in one
 // draw of a hundred (131,072 tokens): what is drawn from is summed in 64 bits, and only that row.
 //
-// k_verify_rows: (largest, sum) of parts of all rows.  k_verify_take, k_verify_left: a workgroup a part of
-// the drawn row of a sequence: the 64-bit sums of p and q, then those of what is drawn from.  k_verify_draw: the
-// token.  k_verify_narrow does it all for vocabularies of up to 256 tokens, a workgroup a sequence.
+// k_verify_rows: (largest, sum) of parts of all rows.  k_verify_finish, a workgroup a part of the
+// drawn row of a sequence: where its drafts end, then 64-bit sums of pieces of the part; the last workgroup of a sequence
+// draws.  k_verify_narrow does it all for vocabularies of up to 256 tokens, a workgroup a sequence.
+//
+// One pass sums what is left of p, max(e_p - r e_q, 0) with r = Z_p / Z_q, before r is known in 64 bits: the tokens that count
+// are those with e_p / e_q > r, and with r from the FP32 sums they are the same ones unless a token's ratio lies
+// between the two.  The pass keeps the sums of e_p and e_q over them, and how near to r the nearest ratio is; where the 64-bit r
+// turns out to be further away than that (one row of a hundred, or where p and q differ in a few tokens
+// only), the last workgroup sums the row again.
 #include <float.h>
 
 #include <type_traits>
@@ -26,7 +32,7 @@ constexpr float LOG2E = 1.44269504088896340736f;
 constexpr int NONE = 0x7fffffff;
 constexpr int VERIFY_THREADS = 256, VERIFY_WAVES = VERIFY_THREADS / 64;
 constexpr int NARROW = 256;  // tokens
-constexpr int FINE = 1024;   // tokens of a piece of a part, of which the sums are kept
+constexpr int FINE = 512;    // tokens of a piece of a part, of which the sums are kept
 
 template <class V, class OP> __device__ __forceinline__ V wave_all(V v, OP op) {
 #pragma unroll
@@ -261,44 +267,44 @@ template <class T, int NK> __global__ __launch_bounds__(VERIFY_THREADS) void k_v
 
 // ---- wide vocabularies ------------------------------------------------------------------------
 
-// Parts of a row, of whole pieces: 4 to 16 pieces, so that all rows make some 2048 workgroups, and at most
+// Parts of a row, of whole pieces: 8 to 32 pieces, so that all rows make some 2048 workgroups, and at most
 // 256 parts.
 struct Cut {
     int parts, size;
     Cut(int n_seq, int n_drafts, int vocab) {
         const int64_t rows = (int64_t)n_seq + 2 * (int64_t)n_drafts, pieces = ((int64_t)vocab + FINE - 1) / FINE;
         const int64_t want = pieces * rows / 2048, least = (pieces + 255) / 256;
-        const int64_t each = want < 4 ? 4 : want > 16 ? 16 : want;
+        const int64_t each = want < 8 ? 8 : want > 32 ? 32 : want;
         size = (int)(each > least ? each : least) * FINE;
         parts = (int)(((int64_t)vocab + size - 1) / size);
     }
 };
-// A sequence's state between the kernels.
-struct Turn {
-    int taken, lost, refused, at;  // at: arg max of the row it stands at
-    float pm, qm;
+// Sums over a piece: e_p and e_q of the tokens that are left, and of all.
+struct Piece {
+    double left_p, left_q, p, q;
 };
 struct Space {
-    Stats *stats;  // [rows of the target, then the draft][parts]
-    Turn *turn;    // [n_seq]
-    double *z;     // [n_seq][parts][2]: of p, of q
-    double *sums;  // [n_seq][parts][2][fine]: of what is left, of p
+    Stats *stats;   // [rows of the target, then the draft][parts]
+    int *done;      // [n_seq]: parts that have their sums
+    double *near;   // [n_seq][parts]: of the ratios that decide what is left, how near the nearest is (log2)
+    Piece *pieces;  // [n_seq][parts][fine]
     int rows, parts, size, fine;
     size_t bytes;
     Space(int n_seq, int n_drafts, int vocab, void *ws) {
-        auto up16 = [](size_t n) { return (n + 15) / 16 * 16; };
+        auto up32 = [](size_t n) { return (n + 31) / 32 * 32; };
         const Cut c(n_seq, n_drafts, vocab);
         rows = n_seq + n_drafts;
         parts = c.parts;
         size = c.size;
         fine = size / FINE;
-        const size_t all = ((size_t)rows + n_drafts) * parts * sizeof(Stats), cut = (size_t)n_seq * parts;
+        const size_t all = up32(((size_t)rows + n_drafts) * parts * sizeof(Stats)), own = up32((size_t)n_seq * sizeof(int));
+        const size_t cut = (size_t)n_seq * parts;
         char *p = static_cast<char *>(ws);
         stats = reinterpret_cast<Stats *>(p);
-        turn = reinterpret_cast<Turn *>(p + up16(all));
-        z = reinterpret_cast<double *>(p + up16(all) + up16(n_seq * sizeof(Turn)));
-        sums = z + cut * 2;
-        bytes = up16(all) + up16(n_seq * sizeof(Turn)) + cut * 2 * (1 + fine) * sizeof(double);
+        done = reinterpret_cast<int *>(p + all);
+        near = reinterpret_cast<double *>(p + all + own);
+        pieces = reinterpret_cast<Piece *>(p + all + own + up32(cut * sizeof(double)));
+        bytes = all + own + up32(cut * sizeof(double)) + cut * fine * sizeof(Piece);
     }
 };
 
@@ -367,7 +373,10 @@ template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k
     sum = block_all(sum, Plus(), fred);
     if (h.over == 0.0) at = block_all(m == all ? at : NONE, Less(), ired);
     const bool lost = __syncthreads_or(bad);
-    if (threadIdx.x == 0) s.stats[blockIdx.x] = {lost ? NAN : all, sum, at};
+    if (threadIdx.x == 0) {
+        s.stats[blockIdx.x] = {lost ? NAN : all, sum, at};
+        if (part == 0 && r < v.n_seq) s.done[r] = 0;
+    }
 }
 
 // The parts of a row joined, by a wave.
@@ -391,88 +400,12 @@ __device__ __forceinline__ Stats join(const Stats *s, int parts, const Heat &h, 
     return o;
 }
 
-// Where a sequence's drafts end, found by every workgroup of it (a wave a row: eight, so that up to seven drafts take one
-// round); then a part's 64-bit sums of the row that is drawn from.
-constexpr int TAKE_THREADS = 512, TAKE_WAVES = TAKE_THREADS / 64;
-template <class T, bool VEC> __global__ __launch_bounds__(TAKE_THREADS) void k_verify_take(VerifyDrafts v, Space s) {
-    constexpr int VL = 16 / sizeof(T), STEP = TAKE_THREADS * VL;
-    __shared__ double dred[TAKE_WAVES];
-    __shared__ Turn turns[TAKE_WAVES];
-    const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Drafts d(v, i);
-    const Heat h(v.temperature);
-    const int n = d.c1 - d.c0;
-    Turn t{};
-    for (int r0 = 0;; r0 += TAKE_WAVES) {
-        const int r = r0 + wave;
-        t.taken = NONE;
-        if (r <= n) {
-            const bool drafted = v.draft && r < n;
-            Draft draft;
-            if (r < n)
-                draft = Draft(v, h, d.c0 + r, target_row<T>(v, d.c0 + i + r), drafted ? draft_row<T>(v, d.c0 + r) : nullptr);
-            const Stats p = join(s.stats + (int64_t)(d.c0 + i + r) * s.parts, s.parts, h, lane);
-            const Stats q = drafted ? join(s.stats + (int64_t)(s.rows + d.c0 + r) * s.parts, s.parts, h, lane) : Stats{};
-            const bool lost = no_dist(p.m) || (drafted && no_dist(q.m));
-            if (lost || r == n || !draft.taken(h, p, q)) t = {r, lost, r < n, p.at, p.m, q.m};
-        }
-        if (lane == 0) turns[wave] = t;
-        __syncthreads();
-        t = turns[0];
-#pragma unroll
-        for (int w = 1; w < TAKE_WAVES; w++)
-            if (turns[w].taken < t.taken) t = turns[w];
-        if (t.taken != NONE) break;
-        __syncthreads();
-    }
-    if (part == 0 && threadIdx.x == 0) {
-        s.turn[i] = t;
-        if (t.lost || h.over == 0.0) {
-            v.accepted[i] = t.taken;
-            v.tokens[i] = t.lost ? -1 : t.at;
-        }
-    }
-    if (t.lost || h.over == 0.0) return;
-    const T *prow = target_row<T>(v, d.c0 + i + t.taken), *qrow = t.refused && v.draft ? draft_row<T>(v, d.c0 + t.taken) : nullptr;
-    const int first = part * s.size, end = (int)min((int64_t)first + s.size, (int64_t)v.vocab);
-    double zp = 0.0, zq = 0.0;
-    for (int j = first + threadIdx.x * VL; j < end; j += STEP) {
-        float x[VL], y[VL];
-        load16<T, VEC>(prow, j, end, x);
-        if (qrow) load16<T, VEC>(qrow, j, end, y);
-#pragma unroll
-        for (int u = 0; u < VL; u++) zp += h.e64(x[u], t.pm);
-        if (qrow)
-#pragma unroll
-            for (int u = 0; u < VL; u++) zq += h.e64(y[u], t.qm);
-    }
-    zp = block_all<TAKE_WAVES>(zp, Plus(), dred);
-    zq = block_all<TAKE_WAVES>(zq, Plus(), dred);
-    if (threadIdx.x == 0) {
-        double *z = s.z + ((int64_t)i * s.parts + part) * 2;
-        z[0] = zp;
-        z[1] = zq;
-    }
-}
-
-// A row's sums of p and q over the parts, the same in all lanes of all waves.
-__device__ __forceinline__ void whole(const double *z, int parts, int lane, double &zp, double &zq) {
-    zp = zq = 0.0;
-    for (int k = lane; k < parts; k += 64) {
-        zp += z[2 * k];
-        zq += z[2 * k + 1];
-    }
-    zp = wave_all(zp, Plus());
-    zq = wave_all(zq, Plus());
-}
-
-// What is drawn from, in units of 1 / zp: max(p - q, 0) (left) and p.
+// What is drawn from, in units of 1 / Z_p: max(p - q, 0) (left) and p.
 template <class T> struct Weights {
     const T *prow, *qrow;
     Heat h;
     float pm, qm;
-    double rq;  // zp / zq
+    double rq;  // Z_p / Z_q
     int x;      // a certain draft that was refused, else -1
     bool refused;
     __device__ __forceinline__ void of(float p, float q, int j, double &left, double &all) const {
@@ -480,87 +413,43 @@ template <class T> struct Weights {
         left = qrow ? fmax(all - h.e64(q, qm) * rq, 0.0) : j == x ? 0.0 : all;
     }
 };
-template <class T> __device__ __forceinline__ Weights<T> weights_of(const VerifyDrafts &v, const Space &s, int i, const Drafts &d, const Turn &t, int lane) {
-    double zp, zq;
-    whole(s.z + (int64_t)i * s.parts * 2, s.parts, lane, zp, zq);
-    Weights<T> w{target_row<T>(v, d.c0 + i + t.taken), t.refused && v.draft ? draft_row<T>(v, d.c0 + t.taken) : nullptr, Heat(v.temperature),
-                 t.pm, t.qm, zp / zq, t.refused && !v.draft ? v.drafted[d.c0 + t.taken] : -1, t.refused != 0};
-    return w;
-}
 
-// The sums of each piece of FINE tokens of a part: a wave a piece.
-template <class T, bool VEC> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_left(VerifyDrafts v, Space s) {
-    constexpr int VL = 16 / sizeof(T);
-    const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Turn t = s.turn[i];
-    if (t.lost) return;
-    const Drafts d(v, i);
-    const Weights<T> w = weights_of<T>(v, s, i, d, t, lane);
-    const int end = (int)min((int64_t)(part + 1) * s.size, (int64_t)v.vocab);
-    double *out = s.sums + ((int64_t)i * s.parts + part) * 2 * s.fine;
-    for (int f = wave; f < s.fine; f += VERIFY_WAVES) {
-        const int first = part * s.size + f * FINE, last = min(first + FINE, end);
-        double a = 0.0, b = 0.0;
-        for (int j = first + lane * VL; j < last; j += 64 * VL) {
-            float x[VL], y[VL] = {};
-            load16<T, VEC>(w.prow, j, last, x);
-            if (w.qrow) load16<T, VEC>(w.qrow, j, last, y);
+// Running sum over the wave's lanes.
+__device__ __forceinline__ double running(double c, int lane) {
 #pragma unroll
-            for (int u = 0; u < VL; u++) {
-                if (j + u >= last) continue;
-                double left, all;
-                w.of(x[u], y[u], j + u, left, all);
-                a += left;
-                b += all;
-            }
-        }
-        a = wave_all(a, Plus());
-        b = wave_all(b, Plus());
-        if (lane == 0) {
-            out[f] = a;
-            out[s.fine + f] = b;
-        }
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(c, o);
+        if (lane >= o) c += y;
     }
+    return c;
 }
 
-// The piece in which the border lies, by every wave; then the token, a thread four of the piece's.
-template <class T> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_draw(VerifyDrafts v, Space s) {
-    constexpr int OWN = FINE / VERIFY_THREADS;
-    __shared__ double part[VERIFY_WAVES];
-    __shared__ int ired[VERIFY_WAVES];
-    const int i = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Turn t = s.turn[i];
-    if (t.lost) return;
-    const Drafts d(v, i);
-    const Weights<T> w = weights_of<T>(v, s, i, d, t, lane);
-    const double *sums = s.sums + (int64_t)i * s.parts * 2 * s.fine;
+// Numbers that another workgroup of the launch reads: past the XCDs' caches, without writing those back, as a fence would
+// (64 sequences of 8 workgroups: 120 us, so 39).
+__device__ __forceinline__ void share(double *p, double x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ double shared(const double *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+constexpr int FINISH_THREADS = 512, FINISH_WAVES = FINISH_THREADS / 64;  // (a token of a piece a thread)
+
+// The token, by the last workgroup of sequence i: the piece in which the border lies, by every wave, then a thread a token.
+template <class T, class SUM> __device__ __forceinline__ int drawn(const VerifyDrafts &v, const Weights<T> &w, int i, int which, SUM sum_of, double *part, int *ired) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int pieces = (v.vocab + FINE - 1) / FINE;
-    auto sum_of = [&](int f, int which) { return sums[((int64_t)(f / s.fine) * 2 + which) * s.fine + f % s.fine]; };
-    // (nothing left: from p itself)
     double all = 0.0;
-    int which = w.refused ? 0 : 1;
-    for (; which < 2; which++) {
+    for (int f = lane; f < pieces; f += 64) all += sum_of(f, which);
+    all = wave_all(all, Plus());
+    if (which == 0 && !(all > 0.0)) {  // nothing left: from p itself
+        which = 1;
         all = 0.0;
         for (int f = lane; f < pieces; f += 64) all += sum_of(f, which);
         all = wave_all(all, Plus());
-        if (all > 0.0) break;
     }
-    if (which > 1) which = 1;
     const double border = (double)v.sample_at[i] * all;
-    auto before = [&](double c) {  // running sum over the lanes
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(c, o);
-            if (lane >= o) c += y;
-        }
-        return c;
-    };
     // the first piece whose running sum passes the border; else the last one with a weight
     double sum = 0.0, start = 0.0, last_start = 0.0;
     int piece = NONE, last = 0;
     for (int f0 = 0; f0 < pieces && piece == NONE; f0 += 64) {
-        const double x = f0 + lane < pieces ? sum_of(f0 + lane, which) : 0.0, c = before(x);
+        const double x = f0 + lane < pieces ? sum_of(f0 + lane, which) : 0.0, c = running(x, lane);
         const unsigned long long past = __ballot(x > 0.0 && sum + c > border), some = __ballot(x > 0.0);
         if (past) {
             const int at = __builtin_ctzll(past);
@@ -578,37 +467,169 @@ template <class T> __global__ __launch_bounds__(VERIFY_THREADS) void k_verify_dr
         piece = last;
         start = last_start;
     }
-    const int first = piece * FINE + threadIdx.x * OWN;
-    double x[OWN], mine = 0.0;
-#pragma unroll
-    for (int u = 0; u < OWN; u++) {
-        x[u] = 0.0;
-        if (first + u < v.vocab) {
-            double left, p;
-            w.of(to_f32(w.prow[first + u]), w.qrow ? to_f32(w.qrow[first + u]) : 0.0f, first + u, left, p);
-            x[u] = which == 1 ? p : left;
-        }
-        mine += x[u];
+    const int j = piece * FINE + threadIdx.x;
+    double x = 0.0;
+    if (j < v.vocab) {
+        double left, p;
+        w.of(to_f32(w.prow[j]), w.qrow ? to_f32(w.qrow[j]) : 0.0f, j, left, p);
+        x = which == 1 ? p : left;
     }
-    double c = before(mine);
+    double c = running(x, lane);
+    __syncthreads();  // part was read
     if (lane == 63) part[wave] = c;
     __syncthreads();
-    c = start + (c - mine);
+    c += start;
     for (int u = 0; u < wave; u++) c += part[u];
-    int found = NONE, behind = -1;
+    const int found = block_all<FINISH_WAVES>(x > 0.0 && c > border ? j : NONE, Less(), ired);
+    const int behind = block_all<FINISH_WAVES>(x > 0.0 ? j : -1, More(), ired);
+    return found != NONE ? found : behind;
+}
+
+// Where a sequence's drafts end, found by every workgroup of it (a wave a row: eight, so that up to seven drafts take one
+// round); then a part's sums, a wave a piece; the last workgroup draws.
+template <class T, bool VEC> __global__ __launch_bounds__(FINISH_THREADS) void k_verify_finish(VerifyDrafts v, Space s) {
+    constexpr int VL = 16 / sizeof(T);
+    struct Turn {
+        int taken, lost, refused, at;
+        Stats p, q;
+    };
+    __shared__ Turn turns[FINISH_WAVES];
+    __shared__ double dred[FINISH_WAVES];
+    __shared__ int ired[FINISH_WAVES];
+    const int part = blockIdx.x % s.parts, i = blockIdx.x / s.parts;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Drafts d(v, i);
+    const Heat h(v.temperature);
+    const int n = d.c1 - d.c0;
+    Turn t{};
+    for (int r0 = 0;; r0 += FINISH_WAVES) {
+        const int r = r0 + wave;
+        t.taken = NONE;
+        if (r <= n) {
+            const bool drafted = v.draft && r < n;
+            Draft draft;
+            if (r < n)
+                draft = Draft(v, h, d.c0 + r, target_row<T>(v, d.c0 + i + r), drafted ? draft_row<T>(v, d.c0 + r) : nullptr);
+            const Stats p = join(s.stats + (int64_t)(d.c0 + i + r) * s.parts, s.parts, h, lane);
+            const Stats q = drafted ? join(s.stats + (int64_t)(s.rows + d.c0 + r) * s.parts, s.parts, h, lane) : Stats{};
+            const bool lost = no_dist(p.m) || (drafted && no_dist(q.m));
+            if (lost || r == n || !draft.taken(h, p, q)) t = {r, lost, r < n, p.at, p, q};
+        }
+        if (lane == 0) turns[wave] = t;
+        __syncthreads();
+        int first = 0;
 #pragma unroll
-    for (int u = 0; u < OWN; u++) {
-        c += x[u];
-        if (x[u] > 0.0) {
-            behind = first + u;
-            if (c > border && found == NONE) found = first + u;
+        for (int w = 1; w < FINISH_WAVES; w++)
+            if (turns[w].taken < turns[first].taken) first = w;
+        t = turns[first];
+        if (t.taken != NONE) break;
+        __syncthreads();
+    }
+    if (t.lost || h.over == 0.0) {
+        if (part == 0 && threadIdx.x == 0) {
+            v.accepted[i] = t.taken;
+            v.tokens[i] = t.lost ? -1 : t.at;
+        }
+        return;
+    }
+    const bool draft = t.refused && v.draft;
+    Weights<T> w{target_row<T>(v, d.c0 + i + t.taken), draft ? draft_row<T>(v, d.c0 + t.taken) : nullptr, h, t.p.m, t.q.m, 0.0,
+                 t.refused && !v.draft ? v.drafted[d.c0 + t.taken] : -1, t.refused != 0};
+    // log2 of the ratio that decides what is left, from the FP32 sums
+    const double about = draft ? log2((double)t.p.s / (double)t.q.s) : 0.0;
+    const int end = (int)min((int64_t)(part + 1) * s.size, (int64_t)v.vocab);
+    double near = INFINITY;
+    for (int f = wave; f < s.fine; f += FINISH_WAVES) {
+        const int first = part * s.size + f * FINE, last = min(first + FINE, end);
+        Piece o{0.0, 0.0, 0.0, 0.0};
+        for (int j = first + lane * VL; j < last; j += 64 * VL) {
+            float x[VL], y[VL];
+            load16<T, VEC>(w.prow, j, last, x);
+            if (draft) {
+                load16<T, VEC>(w.qrow, j, last, y);
+#pragma unroll
+                for (int u = 0; u < VL; u++) {
+                    const double tp = ((double)x[u] - (double)w.pm) * h.over, tq = ((double)y[u] - (double)w.qm) * h.over;
+                    const double ep = pow2(tp), eq = pow2(tq), over = tp - tq - about;  // (NaN where both are -inf)
+                    near = fmin(near, fabs(over));
+                    o.p += ep;
+                    o.q += eq;
+                    o.left_p += over > 0.0 ? ep : 0.0;
+                    o.left_q += over > 0.0 ? eq : 0.0;
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < VL; u++) {
+                    const double ep = h.e64(x[u], w.pm);
+                    o.p += ep;
+                    o.left_p += j + u == w.x ? 0.0 : ep;
+                }
+            }
+        }
+        o.p = wave_all(o.p, Plus());
+        o.left_p = wave_all(o.left_p, Plus());
+        if (draft) {
+            o.q = wave_all(o.q, Plus());
+            o.left_q = wave_all(o.left_q, Plus());
+        }
+        if (lane == 0) {
+            Piece *to = s.pieces + ((int64_t)i * s.parts + part) * s.fine + f;
+            share(&to->left_p, o.left_p);
+            share(&to->left_q, o.left_q);
+            share(&to->p, o.p);
+            share(&to->q, o.q);
         }
     }
-    found = block_all(found, Less(), ired);
-    behind = block_all(behind, More(), ired);
+    near = block_all<FINISH_WAVES>(near, Less(), dred);
+    if (threadIdx.x == 0) share(&s.near[(int64_t)i * s.parts + part], near);
+    // the last workgroup of the sequence sees the others' sums: they are written before it is counted
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) ired[0] = atomicAdd(&s.done[i], 1);
+    __syncthreads();
+    if (ired[0] != s.parts - 1) return;
+    Piece *own = s.pieces + (int64_t)i * s.parts * s.fine;
+    const int pieces = (v.vocab + FINE - 1) / FINE;  // (parts are whole pieces: piece f of the row is own[f])
+    int which = t.refused ? 0 : 1;
+    if (draft) {
+        double zp = 0.0, zq = 0.0;
+        near = INFINITY;
+        for (int f = lane; f < pieces; f += 64) {
+            zp += shared(&own[f].p);
+            zq += shared(&own[f].q);
+        }
+        for (int k = lane; k < s.parts; k += 64) near = fmin(near, shared(&s.near[(int64_t)i * s.parts + k]));
+        zp = wave_all(zp, Plus());
+        zq = wave_all(zq, Plus());
+        near = wave_all(near, Less());
+        w.rq = zp / zq;
+        // (1e-10: the exponents' roundings, 1000 2^-53)
+        if (!(fabs(log2(w.rq) - about) < near - 1e-10)) {
+            __syncthreads();  // every wave has its sums
+            for (int f = wave; f < pieces; f += FINISH_WAVES) {
+                double sum = 0.0;
+                for (int j = f * FINE + lane; j < min((f + 1) * FINE, v.vocab); j += 64) {
+                    double left, p;
+                    w.of(to_f32(w.prow[j]), to_f32(w.qrow[j]), j, left, p);
+                    sum += left;
+                }
+                sum = wave_all(sum, Plus());
+                if (lane == 0) {
+                    share(&own[f].left_p, sum);
+                    share(&own[f].left_q, 0.0);
+                }
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+    }
+    auto sum_of = [&](int f, int which) __attribute__((always_inline)) {
+        return which == 1 ? shared(&own[f].p) : draft ? fmax(shared(&own[f].left_p) - w.rq * shared(&own[f].left_q), 0.0) : shared(&own[f].left_p);
+    };
+    const int token = drawn<T>(v, w, i, which, sum_of, dred, ired);
     if (threadIdx.x == 0) {
         v.accepted[i] = t.taken;
-        v.tokens[i] = found != NONE ? found : behind;
+        v.tokens[i] = token;
     }
 }
 
@@ -620,18 +641,14 @@ template <class T> hipError_t launch(const VerifyDrafts &v, void *ws, hipStream_
         return hipGetLastError();
     }
     const Space s(v.n_seq, v.n_drafts, v.vocab, ws);
-    const bool draws = v.temperature > 0.0f;
     const int64_t rows = (int64_t)v.n_seq + v.n_drafts + (v.draft ? v.n_drafts : 0), own = (int64_t)v.n_seq * s.parts;
     if (!kv8_grid(rows * s.parts, VERIFY_THREADS) || !kv8_grid(own, VERIFY_THREADS)) return hipErrorInvalidValue;
-    if (!kv8_grid(own, TAKE_THREADS)) return hipErrorInvalidValue;
+    if (!kv8_grid(own, FINISH_THREADS)) return hipErrorInvalidValue;
     auto aligned = [](const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T))) % 16 == 0; };
     auto go = [&](auto vec) {
         constexpr bool VEC = decltype(vec)::value;
         hipLaunchKernelGGL((k_verify_rows<T, VEC>), dim3(rows * s.parts), dim3(VERIFY_THREADS), 0, st, v, s);
-        hipLaunchKernelGGL((k_verify_take<T, VEC>), dim3(own), dim3(TAKE_THREADS), 0, st, v, s);
-        if (!draws) return;
-        hipLaunchKernelGGL((k_verify_left<T, VEC>), dim3(own), dim3(VERIFY_THREADS), 0, st, v, s);
-        hipLaunchKernelGGL(k_verify_draw<T>, dim3(v.n_seq), dim3(VERIFY_THREADS), 0, st, v, s);
+        hipLaunchKernelGGL((k_verify_finish<T, VEC>), dim3(own), dim3(FINISH_THREADS), 0, st, v, s);
     };
     if (aligned(v.logits, v.stride) && (!v.draft || aligned(v.draft, v.draft_stride))) go(std::true_type{});
     else go(std::false_type{});

@@ -152,6 +152,26 @@ def test_verify_ties_and_borders(hip, vocab):
     call(hip, two, two[:1], np.array([0, 1], np.int32), [3], [1.5], [0.4], 1.0, "float32")
 
 
+@pytest.mark.parametrize("vocab", [33, 200, 3000, 40000])
+@pytest.mark.parametrize("change", [0.5, -0.5, 0.01])
+def test_verify_drafts_that_differ_in_few_tokens(hip, vocab, change):
+    """What is left of p hangs on the last bits of the sums' ratio: all other tokens have the same p / q."""
+    rng = np.random.default_rng(vocab)
+    n = 24
+    logits = R.rounded(rng.standard_normal((2 * n, vocab)) * 2, "float32")
+    about = logits[::2].copy()
+    at = rng.integers(0, vocab, (n, 3))
+    for i in range(n):
+        about[i, at[i]] += change
+    about = R.rounded(about, "float32")
+    # accept_at beyond 1 refuses whatever was drafted
+    v = rng.random(n).astype(np.float32)
+    acc, tok = call(hip, logits, about, np.arange(n + 1), rng.integers(0, vocab, n), np.full(n, 3e38), v, 1.0, "float32")
+    assert (acc == 0).all()
+    if change < 0:  # the draft is below the target at three tokens only
+        assert all(t in a for t, a in zip(tok, at))
+
+
 def test_verify_temperatures(hip):
     rng = np.random.default_rng(9)
     for temperature in (1e-3, 0.05, 10.0, 1e30):
