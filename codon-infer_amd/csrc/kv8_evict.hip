@@ -63,6 +63,9 @@ __device__ __forceinline__ Held held(const Kv8Seqs &s, int i) {
             slot >= 0 && slot < s.table_rows ? s.table + (int64_t)slot * s.table_stride : nullptr};
 }
 
+// Where bin i of the histogram stands, so that threads that read runs of 4 or 16 bins meet no bank twice.
+__device__ __forceinline__ int bin(int i) { return i ^ (i >> 5 & 31); }
+
 // Running sum over the wave's lanes (shifts within rows of 16 lanes, then their last lanes' sums to the rows behind).
 template <int C, int ROWS> __device__ __forceinline__ int dpp_or_0(int v) { return __builtin_amdgcn_update_dpp(0, v, C, ROWS, 0xf, false); }
 __device__ __forceinline__ int wave_scan(int v) {
@@ -122,7 +125,7 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     };
     auto chosen = [](unsigned key) __attribute__((always_inline)) { return key - 1 < SURE - 1; };  // by its weight
     auto top = [&](unsigned key) __attribute__((always_inline)) {  // the first digit
-        if (chosen(key)) atomicAdd(&hist[key >> 20], 1);
+        if (chosen(key)) atomicAdd(&hist[bin(key >> 20)], 1);
     };
     // Every page has to be there: a wave's first pages, then runs of those behind.
     unsigned x[NK];
@@ -205,7 +208,7 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
             if (pass > 0) {
                 const int known = pass == 1 ? 20 : 8;
                 tokens([&](int, unsigned key, int) __attribute__((always_inline)) {
-                    if (key >> known == border >> known && chosen(key)) atomicAdd(&hist[key >> shift & mask], 1);
+                    if (key >> known == border >> known && chosen(key)) atomicAdd(&hist[bin(key >> shift & mask)], 1);
                 });
                 __syncthreads();
             }
@@ -213,8 +216,8 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
             int mine[PER], sum = 0;
 #pragma unroll
             for (int k = 0; k < PER; k++) {
-                sum += mine[k] = hist[BINS - 1 - PER * tid - k];
-                hist[BINS - 1 - PER * tid - k] = 0;
+                sum += mine[k] = hist[bin(BINS - 1 - PER * tid - k)];
+                hist[bin(BINS - 1 - PER * tid - k)] = 0;
             }
             int before = block_scan<NT>(sum, part);
             if (before < equal && before + sum >= equal)
