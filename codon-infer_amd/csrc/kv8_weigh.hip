@@ -62,14 +62,15 @@ constexpr int WEIGH_WAVES = 4;
 // At most 16 columns: one workgroup per (sequence, kv head, pps pages), its waves take the pages
 // in turn, the next page's keys under way; the query is an integer in three bytes, as in attention.
 template <int DP, class T>
-__global__ __launch_bounds__(64 * WEIGH_WAVES) void k_kv8_weigh(Kv8Weigh w, int g, int groups, int pps) {
+__global__ __launch_bounds__(64 * WEIGH_WAVES) void k_kv8_weigh(Kv8Weigh w, int g, int pps) {
     constexpr int KS = Tile<DP>::KS;
     const Kv8Attention &a = w.a;
-    int b = blockIdx.x;
-    const int group = b % groups;
-    b /= groups;
-    const int kvh = b % a.c.hk;
-    const Kv8Seq q = kv8_seq(a.s, b / a.c.hk);
+    // the same pages of all (sequence, kv head) pairs after each other: blocks go to the XCDs in turn, and
+    // where a pair's own followed each other the XCDs of the last pages had none of the shorter sequences'
+    // (64 sequences of 1025 to 8190 tokens 99 -> 74 us)
+    const int pairs = a.c.hk * a.s.n_seq, group = blockIdx.x / pairs, pair = blockIdx.x % pairs;
+    const int kvh = pair % a.c.hk;
+    const Kv8Seq q = kv8_seq(a.s, pair / a.c.hk);
     if (q.n == 0) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, g4 = lane >> 4;
@@ -387,9 +388,10 @@ template <int DP, class T> hipError_t launch(const Kv8Weigh &w, hipStream_t st) 
         if (!kv8_grid(blocks, MANY)) return hipErrorInvalidValue;
         hipLaunchKernelGGL((k_kv8_weigh_prompt<DP, T>), dim3(blocks), dim3(MANY), 0, st, w, g, sp, RowOf(g));
     } else {
-        const int pps = (int)max((int64_t)16, min(mp * pairs / 2048, (int64_t)64)), groups = (int)((mp + pps - 1) / pps);
+        // a page a wave at least (8 single tokens of 700, 20 heads of 64: 6.2 us, four pages 7.0)
+        const int pps = (int)max((int64_t)4, min(mp * pairs / 2048, (int64_t)64)), groups = (int)((mp + pps - 1) / pps);
         if (!kv8_grid(pairs * groups, 64 * WEIGH_WAVES)) return hipErrorInvalidValue;
-        hipLaunchKernelGGL((k_kv8_weigh<DP, T>), dim3(pairs * groups), dim3(64 * WEIGH_WAVES), 0, st, w, g, groups, pps);
+        hipLaunchKernelGGL((k_kv8_weigh<DP, T>), dim3(pairs * groups), dim3(64 * WEIGH_WAVES), 0, st, w, g, pps);
     }
     return hipGetLastError();
 }

@@ -34,10 +34,46 @@ constexpr int VERIFY_THREADS = 256, VERIFY_WAVES = VERIFY_THREADS / 64;
 constexpr int NARROW = 256;  // tokens
 constexpr int FINE = 512;    // tokens of a piece of a part, of which the sums are kept
 
-template <class V, class OP> __device__ __forceinline__ V wave_all(V v, OP op) {
+// Values of other lanes without LDS trips, word by word: f(word) gives each word's.
+template <class V, class F> __device__ __forceinline__ V words(V v, F f) {
+    constexpr int N = sizeof(V) / 4;
+    struct {
+        unsigned w[N];
+    } x = __builtin_bit_cast(decltype(x), v);
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = op(v, __shfl_xor(v, o));
-    return v;
+    for (int k = 0; k < N; k++) x.w[k] = f(x.w[k]);
+    return __builtin_bit_cast(V, x);
+}
+template <int C, int ROWS, class V> __device__ __forceinline__ V dpp_of(V v) {  // 0 where there is no such lane
+    return words(v, [](unsigned x) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, C, ROWS, 0xf, false); });
+}
+template <class V> __device__ __forceinline__ V across(V v, bool far) {  // lane ^ 32, or ^ 16
+    return words(v, [&](unsigned x) {
+        unsigned y = x;
+        asm volatile("" : "+v"(y));  // a register of its own
+        const auto r = far ? __builtin_amdgcn_permlane32_swap(x, y, false, false) : __builtin_amdgcn_permlane16_swap(x, y, false, false);
+        const unsigned r0 = r[0], r1 = r[1];
+        return threadIdx.x & (far ? 32 : 16) ? r0 : r1;
+    });
+}
+// op over the wave, the same in all lanes: neighbours, quads, halves of a row's 16 lanes, rows.
+template <class V, class OP> __device__ __forceinline__ V wave_all(V v, OP op) {
+    v = op(v, dpp_of<0xB1, 0xf>(v));
+    v = op(v, dpp_of<0x4E, 0xf>(v));
+    v = op(v, dpp_of<0x141, 0xf>(v));
+    v = op(v, dpp_of<0x140, 0xf>(v));
+    v = op(v, across(v, false));
+    return op(v, across(v, true));
+}
+// Running sum over the wave's lanes: within rows of 16, then the rows before.
+__device__ __forceinline__ double running(double c) {
+    c += dpp_of<0x111, 0xf>(c);
+    c += dpp_of<0x112, 0xf>(c);
+    c += dpp_of<0x114, 0xf>(c);
+    c += dpp_of<0x118, 0xf>(c);
+    c += dpp_of<0x142, 0xa>(c);
+    c += dpp_of<0x143, 0xc>(c);
+    return c;
 }
 template <int W = VERIFY_WAVES, class V, class OP> __device__ __forceinline__ V block_all(V v, OP op, V *red) {
     v = wave_all(v, op);
@@ -246,12 +282,7 @@ template <class T, int NK> __global__ __launch_bounds__(VERIFY_THREADS) void k_v
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             if (64 * k >= v.vocab || found != NONE) continue;
-            double c = w[k];
-#pragma unroll
-            for (int o = 1; o < 64; o <<= 1) {
-                const double y = __shfl_up(c, o);
-                if (lane >= o) c += y;
-            }
+            const double c = running(w[k]);
             const unsigned long long past = __ballot(w[k] > 0.0 && sum + c > border), some = __ballot(w[k] > 0.0);
             if (past) found = 64 * k + __builtin_ctzll(past);
             if (some) last = 64 * k + 63 - __builtin_clzll(some);
@@ -414,15 +445,6 @@ template <class T> struct Weights {
     }
 };
 
-// Running sum over the wave's lanes.
-__device__ __forceinline__ double running(double c, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(c, o);
-        if (lane >= o) c += y;
-    }
-    return c;
-}
 
 // Numbers that another workgroup of the launch reads: past the XCDs' caches, without writing those back, as a fence would
 // (64 sequences of 8 workgroups: 120 us, so 39).
@@ -449,7 +471,7 @@ template <class T, class SUM> __device__ __forceinline__ int drawn(const VerifyD
     double sum = 0.0, start = 0.0, last_start = 0.0;
     int piece = NONE, last = 0;
     for (int f0 = 0; f0 < pieces && piece == NONE; f0 += 64) {
-        const double x = f0 + lane < pieces ? sum_of(f0 + lane, which) : 0.0, c = running(x, lane);
+        const double x = f0 + lane < pieces ? sum_of(f0 + lane, which) : 0.0, c = running(x);
         const unsigned long long past = __ballot(x > 0.0 && sum + c > border), some = __ballot(x > 0.0);
         if (past) {
             const int at = __builtin_ctzll(past);
@@ -474,7 +496,7 @@ template <class T, class SUM> __device__ __forceinline__ int drawn(const VerifyD
         w.of(to_f32(w.prow[j]), w.qrow ? to_f32(w.qrow[j]) : 0.0f, j, left, p);
         x = which == 1 ? p : left;
     }
-    double c = running(x, lane);
+    double c = running(x);
     __syncthreads();  // part was read
     if (lane == 63) part[wave] = c;
     __syncthreads();
