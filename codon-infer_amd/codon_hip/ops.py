@@ -88,10 +88,6 @@ def _same(at, kept):
 
 
 def _dense(a):
-    try:
-        return a.is_contiguous()
-    except AttributeError:
-        pass
     n = 1
     for d, st in zip(reversed(a.shape), reversed(a.stride())):
         if d != 1 and st != n:
@@ -102,11 +98,19 @@ def _dense(a):
 
 def _plain(a, what, dtype, shape=None):
     """The address of an array without gaps, of this type (and shape)."""
-    if _dtype(a) not in dtype:
-        raise TypeError(f"{what} is {_dtype(a)}: {' or '.join(dtype)} is needed")
+    try:
+        name = _names[a.dtype]
+    except KeyError:
+        name = _dtype(a)
+    if name not in dtype:
+        raise TypeError(f"{what} is {name}: {' or '.join(dtype)} is needed")
     if shape is not None and a.shape != shape:
         raise ValueError(f"{what} has shape {tuple(a.shape)}: {tuple(shape)} is needed")
-    if not _dense(a):
+    try:
+        dense = a.is_contiguous()
+    except AttributeError:
+        dense = _dense(a)
+    if not dense:
         raise ValueError(f"{what} must be contiguous")
     return a.data_ptr()
 
@@ -355,22 +359,23 @@ def verify_drafts(logits, drafts, cu_drafts, accepted, tokens, draft_logits=None
     [n_drafts][vocab]: what the drafts were drawn from (None: they are certain).
     accept_at float32 [n_drafts] and sample_at float32 [n_seq]: random numbers in
     [0, 1), not needed at temperature 0."""
-    (n,), d, vocab = tokens.shape, drafts.shape[0], logits.shape[1]
+    (n,), (d,), (rows, vocab) = tokens.shape, drafts.shape, logits.shape
     f32, i32 = ("float32",), ("int32",)
-    t = _float(logits, "logits")
-    if logits.shape[0] != n + d:
-        raise ValueError(f"logits has {logits.shape[0]} rows: {n + d} are needed")
-    if vocab != 1 and logits.stride()[1] != 1:
+    t, (stride, one) = _float(logits, "logits"), logits.stride()
+    if rows != n + d:
+        raise ValueError(f"logits has {rows} rows: {n + d} are needed")
+    if vocab != 1 and one != 1:
         raise ValueError("logits: the last axis must be contiguous")
     dl, ds = None, 0
     if draft_logits is not None:
         if draft_logits.shape != (d, vocab):
             raise ValueError(f"draft_logits has shape {tuple(draft_logits.shape)}: {(d, vocab)} is needed")
-        if vocab != 1 and draft_logits.stride()[1] != 1:
+        ds, one = draft_logits.stride()
+        if vocab != 1 and one != 1:
             raise ValueError("draft_logits: the last axis must be contiguous")
         if _float(draft_logits, "draft_logits") != t:
             raise TypeError("logits and draft_logits differ in type")
-        dl, ds = draft_logits.data_ptr(), draft_logits.stride()[0]
+        dl = draft_logits.data_ptr()
     dr = _plain(drafts, "drafts", i32, (d,))
     cu = _plain(cu_drafts, "cu_drafts", i32, (n + 1,))
     ac, tk = _plain(accepted, "accepted", i32, (n,)), _plain(tokens, "tokens", i32, (n,))
@@ -378,5 +383,5 @@ def verify_drafts(logits, drafts, cu_drafts, accepted, tokens, draft_logits=None
     us = None if sample_at is None else _plain(sample_at, "sample_at", f32, (n,))
     ws, size = _workspace(workspace)
     at = _where((logits, drafts, cu_drafts, accepted, tokens, draft_logits, accept_at, sample_at, workspace))
-    C.check(_lib.cih_verify_drafts(t, logits.data_ptr(), logits.stride()[0], dl, ds, n, d, vocab, cu, dr, ua, us,
+    C.check(_lib.cih_verify_drafts(t, logits.data_ptr(), stride, dl, ds, n, d, vocab, cu, dr, ua, us,
                                    temperature, ac, tk, ws, size, _stream(at, stream)))
