@@ -667,14 +667,14 @@ template <class T> hipError_t launch(const VerifyDrafts &v, void *ws, hipStream_
     if (!kv8_grid(rows * s.parts, VERIFY_THREADS) || !kv8_grid(own, VERIFY_THREADS)) return hipErrorInvalidValue;
     if (!kv8_grid(own, FINISH_THREADS)) return hipErrorInvalidValue;
     auto aligned = [](const void *p, int64_t stride) { return (reinterpret_cast<uintptr_t>(p) | (uintptr_t)(stride * sizeof(T))) % 16 == 0; };
-    auto go = [&](auto vec) {
+    auto go = [&](auto vec) -> hipError_t {
         constexpr bool VEC = decltype(vec)::value;
         hipLaunchKernelGGL((k_verify_rows<T, VEC>), dim3(rows * s.parts), dim3(VERIFY_THREADS), 0, st, v, s);
+        if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
         hipLaunchKernelGGL((k_verify_finish<T, VEC>), dim3(own), dim3(FINISH_THREADS), 0, st, v, s);
+        return hipGetLastError();
     };
-    if (aligned(v.logits, v.stride) && (!v.draft || aligned(v.draft, v.draft_stride))) go(std::true_type{});
-    else go(std::false_type{});
-    return hipGetLastError();
+    return aligned(v.logits, v.stride) && (!v.draft || aligned(v.draft, v.draft_stride)) ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace
