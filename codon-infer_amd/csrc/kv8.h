@@ -181,7 +181,8 @@ struct Kv8Evict {
     int budget, first, recent;
     const float *weights;
     float *weights_out;
-    int *lens_out, *shifts, *kept;  // each may be nullptr
+    int *lens_out, *shifts, *kept;  // shifts, kept: may be nullptr
+    int room = 0;                   // set by the launch: tokens of the budget that a table has room for
 };
 size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget);
 hipError_t launch_kv8_evict(const Kv8Evict &e, void *ws, hipStream_t st);

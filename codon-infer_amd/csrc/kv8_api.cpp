@@ -307,7 +307,10 @@ int cih_kv8_evict(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_
                   void *workspace, size_t workspace_bytes, void *stream) {
     Kv8Evict e{};
     CIH_TRY(check_cache(cache, e.c, true));
-    CIH_TRY(check_batch(batch, e.s, true));
+    if (!batch) return set_error(CIH_ERR_ARG, "null batch");
+    cih_kv8_batch b = *batch;
+    if (!b.cu_rows) b.cu_rows = b.lens;  // not read
+    CIH_TRY(check_batch(&b, e.s, true));
     CIH_TRY(check_budget(budget, first, recent));
     if (e.s.n_seq == 0) return CIH_OK;
     if (!weights || !lens_out) return set_error(CIH_ERR_ARG, "null %s", weights ? "lens_out" : "weights");

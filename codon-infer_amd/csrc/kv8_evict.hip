@@ -16,28 +16,28 @@ namespace cih {
 
 namespace {
 
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
 // Of each (sequence, head), in the workspace.
 struct Work {
-    int4 *state;               // tokens held, tokens kept, whether they move, the next page to move
-    unsigned long long *mask;  // [pages of the table]: which tokens of a page are kept
-    int2 *list;                // [tokens]: the kept ones, place and page
-    float *weight;             // [tokens]
-    int *read;                 // [pages]: whether this page's tokens have been read
-    int *rank;                 // [pages + 1]: how many kept tokens come from pages before this one
+    int4 *state;    // tokens held, tokens kept, whether they move, the next run of pages to move
+    int2 *list;     // [tokens]: the kept ones, place and page
+    float *weight;  // [tokens]
+    int *read;      // [pages]: whether this page's tokens have been read
+    int *rank;      // [pages + 1]: how many kept tokens come from pages before this one
     int pages;
 };
-__host__ __device__ inline size_t work_size(int budget, int table_pages) {  // a multiple of 16 bytes
-    const size_t pages = (budget + KV8_PAGE - 1) / KV8_PAGE, tokens = pages * KV8_PAGE;
-    return sizeof(int4) + ((size_t)table_pages + 1) / 2 * 16 + tokens * (sizeof(int2) + sizeof(float)) +
+__host__ __device__ inline size_t work_size(int room) {  // a multiple of 16 bytes
+    const size_t pages = ((size_t)room + KV8_PAGE - 1) / KV8_PAGE, tokens = pages * KV8_PAGE;
+    return sizeof(int4) + tokens * (sizeof(int2) + sizeof(float)) +
            ((2 * pages + 1) * sizeof(int) + 15) / 16 * 16;
 }
 __device__ __forceinline__ Work work_of(const Kv8Evict &e, void *ws, int64_t pair) {
-    char *p = static_cast<char *>(ws) + pair * work_size(e.budget, e.s.max_pages);
+    char *p = static_cast<char *>(ws) + pair * work_size(e.room);
     Work w;
-    w.pages = (e.budget + KV8_PAGE - 1) / KV8_PAGE;
+    w.pages = (e.room + KV8_PAGE - 1) / KV8_PAGE;
     w.state = reinterpret_cast<int4 *>(p);
-    w.mask = reinterpret_cast<unsigned long long *>(w.state + 1);
-    w.list = reinterpret_cast<int2 *>(w.mask + ((int64_t)e.s.max_pages + 1) / 2 * 2);
+    w.list = reinterpret_cast<int2 *>(w.state + 1);
     w.weight = reinterpret_cast<float *>(w.list + (int64_t)w.pages * KV8_PAGE);
     w.read = reinterpret_cast<int *>(w.weight + (int64_t)w.pages * KV8_PAGE);
     w.rank = w.read + w.pages;
@@ -254,13 +254,8 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     tokens([&](int p, unsigned key, int id) __attribute__((always_inline)) {
         const unsigned long long below = (1ull << lane) - 1, a = __ballot(key == border), b = __ballot(key > border);
         const int t = ties + __popcll(a & below), m = sure + __popcll(b & below) + min(t, equal);
-        const bool keep = key > border || (key == border && t < equal);
-        const unsigned long long mask = __ballot(keep);
-        if (lane == 0) {
-            w.mask[p] = mask;
-            if (p <= w.pages) w.rank[p] = m;
-        }
-        if (keep) {
+        if (lane == 0 && p <= w.pages) w.rank[p] = m;
+        if (key > border || (key == border && t < equal)) {
             w.list[m] = make_int2(p * KV8_PAGE + lane, id);
             w.weight[m] = key == SURE || key == NAN_KEY || key == ZERO_KEY ? weight_at(id, p) : key_weight(key);
             if (kept) kept[m] = p * KV8_PAGE + lane;
@@ -271,15 +266,21 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     if (tid == 0 && pages <= w.pages) w.rank[pages] = e.budget;
 }
 
-// A code scaled by r <= 1, in the low byte: byte - 128 is the code (u its word ^ 0x80808080), the fused product is
-// rounded once, as code r is, and 1.5 2^23 rounds it to a whole number.
-template <int B> __device__ __forceinline__ unsigned shrink(unsigned u, float r) {
+// A code scaled by r <= 1, in the low byte: the product is rounded to FP32, as code r is, and 1.5 2^23 rounds it to a
+// whole number (not fused: that would round once).
+__device__ __forceinline__ unsigned shrink(int code, float r) {
+#pragma clang fp contract(off)
+    const float z = (float)code * r;
+    return __float_as_uint(z + 12582912.0f);
+}
+// Four codes of a word: byte - 128 is the code (of the word ^ 0x80808080), and the fused product is code r, rounded.
+template <int B> __device__ __forceinline__ unsigned shrink_byte(unsigned u, float r) {
     return __float_as_uint(fmaf((float)(u >> (8 * B) & 0xff), r, -128.0f * r) + 12582912.0f);
 }
 __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
     const unsigned u = w ^ 0x80808080u;
-    const unsigned lo = __builtin_amdgcn_perm(shrink<1>(u, r), shrink<0>(u, r), 0x0c0c0400u);
-    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(shrink<3>(u, r), shrink<2>(u, r), 0x0c0c0400u), lo, 0x05040100u);
+    const unsigned lo = __builtin_amdgcn_perm(shrink_byte<1>(u, r), shrink_byte<0>(u, r), 0x0c0c0400u);
+    return __builtin_amdgcn_perm(__builtin_amdgcn_perm(shrink_byte<3>(u, r), shrink_byte<2>(u, r), 0x0c0c0400u), lo, 0x05040100u);
 }
 
 // One workgroup per (sequence, head, run of pages that are filled).  Token m of the kept ones comes from
@@ -288,20 +289,21 @@ __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
 // started before it, and say that they have read before they wait themselves.  (Draws of one sequence and head follow
 // each other in memory, so a run is as long as a workgroup's waves allow.)
 //
-// V: a wave takes 64 dims.  A source page's rows go through LDS in 16-byte loads; then a lane is a dim and the
-// token, read as a byte and written behind the last one, is the same in all lanes, so that rows an odd number of words
-// apart meet no bank twice.  (A load from memory for each byte keeps the address unit busy for 64 clocks: 32 sequences
-// to 2,048 tokens, 8 heads of 128, 107 us.)  K: the other waves, 16 dims of a token a lane.
+// V: the codes of a dim's kept tokens are a product with a matrix that has one 1 in each column, exact on the int8
+// matrix instruction: A has a row for each of 16 places of the new page (its token's place in the source page, or none), B
+// the source page's codes as they lie there, 16 tokens of a dim a lane; what comes out, four places of a dim a
+// lane, is a word of the new page but for its scale.  Source pages add up.  (Other ways for 32 sequences to 2,048 tokens, 8 heads
+// of 128: a load from memory for each byte keeps the address unit busy, 107 us; rows through LDS and bytes there, a dim a
+// lane, 103.)  K: 16 dims of a token a lane.
+constexpr int MOST_POLLS = 1 << 20;
 template <int DP> struct Move {
-    static constexpr int VW = DP > 64 ? DP / 64 : 1, KW = DP > 64 ? 2 : 1, WAVES = VW + KW;  // of a page
-    static constexpr int RUN = 8 / WAVES, THREADS = 64 * WAVES * RUN;
-    static constexpr int KP = DP / 16 / KW;  // pieces of K a lane
+    static constexpr int WAVES = DP > 32 ? DP / 32 : 1;    // of a page
+    static constexpr int TILES = DP / 16 / WAVES;          // of 16 dims, a wave's; pieces of K, a lane's
+    static constexpr int RUN = 8 / WAVES, THREADS = 512;
 };
 template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_move(Kv8Evict e, void *ws, int runs) {
-    constexpr int VW = Move<DP>::VW, KW = Move<DP>::KW, KP = Move<DP>::KP, RUN = Move<DP>::RUN, UNIT = 64 * Move<DP>::WAVES;
-    constexpr int DL = DP > 64 ? 64 : DP, ROW = KV8_PAGE / 4 + 1;
+    constexpr int TILES = Move<DP>::TILES, RUN = Move<DP>::RUN, UNIT = 64 * Move<DP>::WAVES;
     __shared__ int srun;
-    __shared__ unsigned sv[RUN][VW][DL * ROW], sx[RUN][VW][DL * ROW];  // rows to be written, of a source page
     const int64_t pair = blockIdx.x / runs;
     const int h = pair % e.c.hk, i = pair / e.c.hk;
     const int unit = __builtin_amdgcn_readfirstlane(threadIdx.x / UNIT), tid = threadIdx.x % UNIT, lane = tid & 63;
@@ -327,7 +329,8 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
     if (tid < here && e.weights_out) e.weights_out[to * KV8_PAGE + tid] = w.weight[m0 + tid];
     if (!moves) return;
     int r0 = 0, r1 = 0;
-    uint4 k[KP];
+    const int g4 = lane >> 4;
+    uint4 k[TILES], v[TILES];
     float2 now = {0.0f, 0.0f};
     unsigned long long bad = 0;
     bool stays = true;
@@ -335,86 +338,91 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
         const int2 mine = w.list[m0 + min(lane, here - 1)];  // token `lane` of the page
         r0 = w.rank[p];
         r1 = w.rank[p + 1];
-        const int j0 = __builtin_amdgcn_readfirstlane(mine.x), j1 = __builtin_amdgcn_readlane(mine.x, 63);  // the first and last
         // (the last token in its own place: so are all, and the record is what it was)
-        stays = here == KV8_PAGE && j1 == m0 + KV8_PAGE - 1;
+        stays = here == KV8_PAGE && __builtin_amdgcn_readlane(mine.x, KV8_PAGE - 1) == m0 + KV8_PAGE - 1;
         if (!stays) {
+#pragma unroll
+            for (int it = 0; it < TILES; it++) {
+                const int at = tid + it * UNIT;
+                const int2 s = w.list[m0 + min(at / (DP / 16), here - 1)];
+                k[it] = *reinterpret_cast<const uint4 *>(
+                    e.c.k + (((int64_t)s.y * e.c.hk + h) * KV8_PAGE + s.x % KV8_PAGE) * DP + at % (DP / 16) * 16);
+            }
+            // the tokens of source pages in turn; the next page's codes under way
+            i32x4 x[TILES], y[TILES];
+            int from = 0, next = 0;  // the first token of the page in x, in y
+            auto load = [&](i32x4 (&o)[TILES], int first) __attribute__((always_inline)) {
+                const int64_t ph = (int64_t)__builtin_amdgcn_readlane(mine.y, first) * e.c.hk + h;
+#pragma unroll
+                for (int t = 0; t < TILES; t++)
+                    o[t] = *reinterpret_cast<const i32x4 *>(e.c.v + (ph * DP + (wave * TILES + t) * 16 + (lane & 15)) * KV8_PAGE + g4 * 16);
+                // behind the last of its tokens
+                return first + __popcll(__ballot(lane >= first && lane < here && mine.x / KV8_PAGE == __builtin_amdgcn_readlane(mine.x, first) / KV8_PAGE));
+            };
+            next = load(x, 0);
             // the new record: the largest scales (not negative: as bits they compare alike), the tokens' bad bits
             const int64_t ph = (int64_t)mine.y * e.c.hk + h;
-            if (wave >= VW) {
+            const float2 old = e.c.scales[ph];
+            bad = __ballot(lane < here && e.c.bad[ph] >> (mine.x % KV8_PAGE) & 1);
+            i32x4 sum[TILES][4];
+            int place[4];  // in its source page, of token 16 m + lane % 16
 #pragma unroll
-                for (int it = 0; it < KP; it++) {
-                    const int at = tid - 64 * VW + it * 64 * KW, m = at / (DP / 16);
-                    const int2 s = w.list[m0 + min(m, here - 1)];
-                    k[it] = *reinterpret_cast<const uint4 *>(
-                        e.c.k + (((int64_t)s.y * e.c.hk + h) * KV8_PAGE + s.x % KV8_PAGE) * DP + at % (DP / 16) * 16);
+            for (int m = 0; m < 4; m++) {
+                place[m] = __shfl(mine.x, m * 16 + (lane & 15)) % KV8_PAGE;
+#pragma unroll
+                for (int t = 0; t < TILES; t++) sum[t][m] = i32x4{0, 0, 0, 0};
+            }
+            for (;;) {
+                int behind = next;
+                if (next < here) behind = load(y, next);
+#pragma unroll
+                for (int m = 0; m < 4; m++) {
+                    if (next <= m * 16 || from >= m * 16 + 16) continue;
+                    const int at = m * 16 + (lane & 15), q = place[m] - g4 * 16;
+                    const int one = at >= from && at < next && q >= 0 && q < 16 ? 1 << 8 * (q & 3) : 0;
+                    i32x4 a;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) a[u] = q >> 2 == u ? one : 0;
+#pragma unroll
+                    for (int t = 0; t < TILES; t++) sum[t][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, x[t], sum[t][m], 0, 0, 0);
                 }
-                const float2 old = e.c.scales[ph];
-                bad = __ballot(lane < here && e.c.bad[ph] >> (mine.x % KV8_PAGE) & 1);
-                now = {__uint_as_float(wave_max_bits(__float_as_uint(old.x))), __uint_as_float(wave_max_bits(__float_as_uint(old.y)))};
-                const float ratio = now.x > 0.0f ? old.x / now.x : 0.0f;
+                if (next >= here) break;
+                from = next;
+                next = behind;
 #pragma unroll
-                for (int it = 0; it < KP; it++) {
-                    const float r = __shfl(ratio, (tid - 64 * VW + it * 64 * KW) / (DP / 16) % KV8_PAGE);
-                    k[it] = make_uint4(shrink4(k[it].x, r), shrink4(k[it].y, r), shrink4(k[it].z, r), shrink4(k[it].w, r));
+                for (int t = 0; t < TILES; t++) x[t] = y[t];
+            }
+            now = {__uint_as_float(wave_max_bits(__float_as_uint(old.x))), __uint_as_float(wave_max_bits(__float_as_uint(old.y)))};
+            const float rk = now.x > 0.0f ? old.x / now.x : 0.0f, rv = now.y > 0.0f ? old.y / now.y : 0.0f;
+#pragma unroll
+            for (int it = 0; it < TILES; it++) {
+                const float r = __shfl(rk, (tid + it * UNIT) / (DP / 16) % KV8_PAGE);
+                k[it] = make_uint4(shrink4(k[it].x, r), shrink4(k[it].y, r), shrink4(k[it].z, r), shrink4(k[it].w, r));
+            }
+            unsigned o[TILES][4];  // tokens 16 m + 4 g4 ..
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                float r[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) r[u] = __shfl(rv, m * 16 + g4 * 4 + u);
+#pragma unroll
+                for (int t = 0; t < TILES; t++) {
+                    unsigned c[4];
+#pragma unroll
+                    for (int u = 0; u < 4; u++) c[u] = shrink(sum[t][m][u], r[u]);
+                    o[t][m] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u),
+                                                    __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), 0x05040100u);
                 }
-            } else {
-                const float old = e.c.scales[ph].y, most = __uint_as_float(wave_max_bits(__float_as_uint(old)));
-                const int d = min(wave * 64 + lane, DP - 1);
-                unsigned *row = &sx[unit][wave][min(lane, DL - 1) * ROW];
-                const unsigned char *in = reinterpret_cast<const unsigned char *>(row);
-                unsigned char *out = reinterpret_cast<unsigned char *>(&sv[unit][wave][min(lane, DL - 1) * ROW]);
-                int got = 0;
-                const int s0 = j0 / KV8_PAGE, s1 = j1 / KV8_PAGE;
-                // the kept tokens of source page s that come here
-                auto mask_of = [&](int s) __attribute__((always_inline)) {
-                    unsigned long long m = w.mask[s];
-                    if (s == s0) m &= ~0ull << (j0 % KV8_PAGE);
-                    if (s == s1) m &= ~0ull >> (KV8_PAGE - 1 - j1 % KV8_PAGE);
-                    return m;
-                };
-                uint4 x[4];
-                float r = 0.0f;
-                auto load = [&](int s) __attribute__((always_inline)) {
-                    const int64_t from = (int64_t)__builtin_amdgcn_readfirstlane(table[s]) * e.c.hk + h;
-                    const uint4 *v = reinterpret_cast<const uint4 *>(e.c.v + (from * DP + d) * KV8_PAGE);
+            }
+            // word m of lanes 16 g .. to word g of lanes 16 m ..: tokens 16 g4 .. in a lane
 #pragma unroll
-                    for (int u = 0; u < 4; u++) x[u] = v[u];
-                    r = most > 0.0f ? e.c.scales[from].y / most : 0.0f;
-                };
-                int s = s0;
-                unsigned long long m = mask_of(s);
-                load(s);
-                for (;;) {
-#pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        row[4 * u] = x[u].x ^ 0x80808080u;
-                        row[4 * u + 1] = x[u].y ^ 0x80808080u;
-                        row[4 * u + 2] = x[u].z ^ 0x80808080u;
-                        row[4 * u + 3] = x[u].w ^ 0x80808080u;
-                    }
-                    const float ry = r, off = -128.0f * r;
-                    unsigned long long my = m;
-                    const int count = __popcll(my);
-                    // the next page with a kept token
-                    m = 0;
-                    while (s < s1 && m == 0) m = mask_of(++s);
-                    if (m) load(s);
-                    for (int t = 0; t < count; t += 8) {
-                        unsigned c[8];
-#pragma unroll
-                        for (int u = 0; u < 8; u++) {
-                            c[u] = in[my ? __builtin_ctzll(my) : 0];
-                            my &= my - 1;
-                        }
-#pragma unroll
-                        for (int u = 0; u < 8; u++)  // (what is past the last goes behind the row)
-                            out[t + u < count ? got + t + u : KV8_PAGE] =
-                                (unsigned char)__float_as_uint(fmaf((float)c[u], ry, off) + 12582912.0f);
-                    }
-                    got += count;
-                    if (!m) break;
-                }
+            for (int t = 0; t < TILES; t++) {
+                auto a = __builtin_amdgcn_permlane32_swap(o[t][0], o[t][2], false, false);
+                auto b = __builtin_amdgcn_permlane32_swap(o[t][1], o[t][3], false, false);
+                const unsigned a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];
+                a = __builtin_amdgcn_permlane16_swap(a0, b0, false, false);
+                b = __builtin_amdgcn_permlane16_swap(a1, b1, false, false);
+                v[t] = make_uint4(a[0], a[1], b[0], b[1]);
             }
         }
     }
@@ -425,50 +433,54 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
     if (!stays && r0 < r1) {
         const int q = r0 / KV8_PAGE + tid;
         if (q <= (r1 - 1) / KV8_PAGE && q < run * RUN)
-            while (!__hip_atomic_load(&w.read[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) __builtin_amdgcn_s_sleep(1);
+            // (microseconds; bounded for calls at the same time that share a workspace against the rule)
+            for (int n = 0; n < MOST_POLLS && !__hip_atomic_load(&w.read[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); n++)
+                __builtin_amdgcn_s_sleep(1);
     }
     __syncthreads();
     if (stays) return;
-    if (wave >= VW) {
 #pragma unroll
-        for (int it = 0; it < KP; it++) {
-            const int at = tid - 64 * VW + it * 64 * KW, m = at / (DP / 16);
-            if (m < here) *reinterpret_cast<uint4 *>(e.c.k + (to * KV8_PAGE + m) * DP + at % (DP / 16) * 16) = k[it];
-        }
-        if (tid == 64 * VW) {
-            e.c.scales[to] = now;
-            e.c.bad[to] = bad;
-        }
-        return;
+    for (int it = 0; it < TILES; it++) {
+        const int at = tid + it * UNIT, m = at / (DP / 16);
+        if (m < here) *reinterpret_cast<uint4 *>(e.c.k + (to * KV8_PAGE + m) * DP + at % (DP / 16) * 16) = k[it];
     }
-    // V: 16 tokens of a dim a lane
+    if (tid == 0) {
+        e.c.scales[to] = now;
+        e.c.bad[to] = bad;
+    }
 #pragma unroll
-    for (int it = 0; it < DL * 4 / 64; it++) {
-        const int at = it * 64 + lane, d = at / 4, c = at % 4;
-        const unsigned *row = &sv[unit][wave][d * ROW + c * 4];
-        signed char *y = e.c.v + (to * DP + wave * 64 + d) * KV8_PAGE + c * 16;
-        if (c * 16 + 16 <= here) {
-            *reinterpret_cast<uint4 *>(y) = make_uint4(row[0], row[1], row[2], row[3]);
-        } else {
-            for (int u = 0; c * 16 + u < here; u++) y[u] = (signed char)(row[u / 4] >> (8 * (u & 3)));
-        }
+    for (int t = 0; t < TILES; t++) {
+        signed char *z = e.c.v + (to * DP + (wave * TILES + t) * 16 + (lane & 15)) * KV8_PAGE + g4 * 16;
+        const unsigned word[4] = {v[t].x, v[t].y, v[t].z, v[t].w};
+        if (g4 * 16 + 16 <= here) *reinterpret_cast<uint4 *>(z) = v[t];
+        else
+#pragma unroll
+            for (int u = 0; u < 16; u++)
+                if (g4 * 16 + u < here) z[u] = (signed char)(word[u / 4] >> (8 * (u & 3)));
     }
 }
 
 }  // namespace
 
+// (a table holds no more)
+static int room_of(const Kv8Seqs &s, int budget) { return (int)min((int64_t)budget, (int64_t)s.max_pages * KV8_PAGE); }
+
 size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget) {
-    return (size_t)s.n_seq * c.hk * work_size(budget, s.max_pages);
+    return (size_t)s.n_seq * c.hk * work_size(room_of(s, budget));
 }
 
-hipError_t launch_kv8_evict(const Kv8Evict &e, void *ws, hipStream_t st) {
+hipError_t launch_kv8_evict(const Kv8Evict &call, void *ws, hipStream_t st) {
+    Kv8Evict e = call;
+    e.room = room_of(e.s, e.budget);
     const int64_t pairs = (int64_t)e.s.n_seq * e.c.hk, most = (int64_t)e.s.max_pages * KV8_PAGE;
     if (pairs == 0) return hipSuccess;
-    const int pages = (int)min((int64_t)(e.budget + KV8_PAGE - 1) / KV8_PAGE, (int64_t)e.s.max_pages);
+    const int pages = (e.room + KV8_PAGE - 1) / KV8_PAGE;
     if (!kv8_grid(pairs, 1024) || !kv8_grid(pairs * pages, 1024)) return hipErrorInvalidValue;
     if (most <= 2048) hipLaunchKernelGGL((k_kv8_choose<256, 8, 0>), dim3(pairs), dim3(256), 0, st, e, ws);
     else if (most <= 8192) hipLaunchKernelGGL((k_kv8_choose<1024, 8, 0>), dim3(pairs), dim3(1024), 0, st, e, ws);
     else hipLaunchKernelGGL((k_kv8_choose<1024, 32, 32>), dim3(pairs), dim3(1024), 0, st, e, ws);
+    // (the moves wait for one another by what the choice has cleared)
+    if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
     auto move = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
         const int runs = (pages + Move<DP>::RUN - 1) / Move<DP>::RUN;

@@ -64,6 +64,11 @@ def test_evict_refusals():
     assert code(c.evict, b, Fake((4, 2, 64), at=0), 100, workspace=ws) == -1
     assert code(c.evict, b, w, 100, shifts=Fake((2,), "int32", at=2), workspace=ws) == -1
     assert code(c.evict_workspace, b, 0) == -2
+    # a table's room bounds what the largest budgets need
+    assert c.evict_workspace(b, 1 << 30) == c.evict_workspace(b, 5 * 64)
+    # the rows' offsets are not read
+    b.struct.cu_rows = None
+    assert code(c.evict, b, w, 100) == -3
     lib = C.lib()
     assert lib.cih_kv8_evict_workspace(c._at, b._at, 4, None) == -1
     assert lib.cih_kv8_evict(None, b._at, 4, 0, 0, None, None, None, None, None, None, 0, None) == -1
