@@ -63,6 +63,27 @@ __device__ __forceinline__ Held held(const Kv8Seqs &s, int i) {
             slot >= 0 && slot < s.table_rows ? s.table + (int64_t)slot * s.table_stride : nullptr};
 }
 
+// Tokens of a sequence and head as a wave sees them: a page's token `lane` in a lane.
+struct Tokens {
+    const Kv8Evict &e;
+    Held q;
+    int h, lane;
+    __device__ __forceinline__ bool there(int id) const { return id >= 0 && id < e.c.n_pages; }
+    __device__ __forceinline__ int id(int p, int last) const { return p < last ? __builtin_amdgcn_readfirstlane(q.table[p]) : 0; }
+    __device__ __forceinline__ float weight(int id, int p, int last) const {
+        return p < last && there(id) && p * KV8_PAGE + lane < q.n ? e.weights[((int64_t)id * e.c.hk + h) * KV8_PAGE + lane] : 0.0f;
+    }
+    // kept for sure, not there, or by its weight
+    __device__ __forceinline__ unsigned key(int p, float y) const {
+        const int j = p * KV8_PAGE + lane;
+        const unsigned k = j < e.first || j >= q.n - e.recent ? SURE : weight_key(y);
+        return j < q.n ? k : NO_KEY;
+    }
+};
+__device__ __forceinline__ bool chosen(unsigned key) { return key - 1 < SURE - 1; }  // by its weight
+// A kept token's weight (a key of 0 or NaN does not have all of it).
+__device__ __forceinline__ bool has_weight(unsigned key) { return key != SURE && key != NAN_KEY && key != ZERO_KEY; }
+
 // Where bin i of the histogram stands, so that threads that read runs of 4 or 16 bins meet no bank twice.
 __device__ __forceinline__ int bin(int i) { return i ^ (i >> 5 & 31); }
 
@@ -90,13 +111,47 @@ template <int NT> __device__ __forceinline__ int block_scan(int v, int *part) {
     return before + x - v;
 }
 
+// The bin in which the `want` largest end, and how many of it are among them, of a histogram whose bins BINS - 1 - PER
+// t and below thread t has in `mine`.
+constexpr int BINS = 4096;
+template <int NT> __device__ __forceinline__ int2 bin_of(const int (&mine)[BINS / NT], int want, int *part, int *found) {
+    constexpr int PER = BINS / NT;
+    int sum = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) sum += mine[k];
+    int before = block_scan<NT>(sum, part);
+    if (before < want && before + sum >= want)
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            if (before < want && before + mine[k] >= want) {
+                found[0] = BINS - 1 - PER * (int)threadIdx.x - k;
+                found[1] = want - before;
+            }
+            before += mine[k];
+        }
+    __syncthreads();
+    return make_int2(found[0], found[1]);  // (next written behind block_scan's barrier)
+}
+// The same of a histogram in LDS, which is cleared.
+template <int NT> __device__ __forceinline__ int2 bin_of_hist(int *hist, int want, int *part, int *found) {
+    constexpr int PER = BINS / NT;
+    int mine[PER];
+#pragma unroll
+    for (int k = 0; k < PER; k++) {
+        int &c = hist[bin(BINS - 1 - PER * (int)threadIdx.x - k)];
+        mine[k] = c;
+        c = 0;
+    }
+    return bin_of<NT>(mine, want, part, found);
+}
+
 // NT threads; a wave owns a run of pages, token `lane` of each in a lane.  The smallest key that
 // is kept is found by its digits from the highest on (12, 12 and 8 bits), each from a
 // histogram of the keys that have the digits before it.  A wave keeps the keys of its first NK pages in
 // registers and of the next NL in LDS; those behind are read again for each digit.
 constexpr int RUN = 8;
 template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_choose(Kv8Evict e, void *ws) {
-    constexpr int BINS = 4096, PER = BINS / NT, NW = NT / 64;
+    constexpr int PER = BINS / NT, NW = NT / 64;
     __shared__ int hist[BINS], part[NW], found[2], count[2][NW];
     __shared__ unsigned in_lds[NL > 0 ? NW * NL * KV8_PAGE : 1];
     const int h = blockIdx.x % e.c.hk, i = blockIdx.x / e.c.hk;
@@ -107,23 +162,12 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE;
     const int own = (pages + NW - 1) / NW;  // pages of a wave
     const int first = min(wave * own, pages), last = min(first + own, pages);
-    auto there = [&](int id) __attribute__((always_inline)) { return id >= 0 && id < e.c.n_pages; };
-    // (0: no such page of the wave)
-    auto id_of = [&](int p) __attribute__((always_inline)) { return p < last ? __builtin_amdgcn_readfirstlane(q.table[p]) : 0; };
-    auto weight_at = [&](int id, int p) __attribute__((always_inline)) {
-        return p < last && there(id) && p * KV8_PAGE + lane < q.n ? e.weights[((int64_t)id * e.c.hk + h) * KV8_PAGE + lane] : 0.0f;
-    };
+    const Tokens z{e, q, h, lane};
     if (tid == 0) found[0] = 0;
 #pragma unroll
     for (int k = 0; k < PER; k++) hist[k * NT + tid] = 0;
     __syncthreads();
-    const int lo = e.first, hi = q.n - e.recent, need = e.budget - e.first - e.recent;
-    // a token's key: kept for sure, not there, or by its weight
-    auto key_of = [&](int j, float y) __attribute__((always_inline)) {
-        const unsigned k = j < lo || j >= hi ? SURE : weight_key(y);
-        return j < q.n ? k : NO_KEY;
-    };
-    auto chosen = [](unsigned key) __attribute__((always_inline)) { return key - 1 < SURE - 1; };  // by its weight
+    const int need = e.budget - e.first - e.recent;
     auto top = [&](unsigned key) __attribute__((always_inline)) {  // the first digit
         if (chosen(key)) atomicAdd(&hist[bin(key >> 20)], 1);
     };
@@ -133,32 +177,32 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     bool gone = q.table == nullptr;
     if (!gone) {
 #pragma unroll
-        for (int k = 0; k < NK; k++) id[k] = id_of(first + k);
+        for (int k = 0; k < NK; k++) id[k] = z.id(first + k, last);
         float y[NK];
 #pragma unroll
         for (int k = 0; k < NK; k++) {
-            gone |= !there(id[k]);
-            y[k] = weight_at(id[k], first + k);
+            gone |= !z.there(id[k]);
+            y[k] = z.weight(id[k], first + k, last);
         }
 #pragma unroll
         for (int k = 0; k < NK; k++) {
-            x[k] = first + k < last ? key_of((first + k) * KV8_PAGE + lane, y[k]) : NO_KEY;
+            x[k] = first + k < last ? z.key(first + k, y[k]) : NO_KEY;
             top(x[k]);
         }
         for (int p = first + NK; p < last; p += RUN) {
             int is[RUN];
             float y[RUN];
 #pragma unroll
-            for (int k = 0; k < RUN; k++) is[k] = id_of(p + k);
+            for (int k = 0; k < RUN; k++) is[k] = z.id(p + k, last);
 #pragma unroll
             for (int k = 0; k < RUN; k++) {
-                gone |= !there(is[k]);
-                y[k] = weight_at(is[k], p + k);
+                gone |= !z.there(is[k]);
+                y[k] = z.weight(is[k], p + k, last);
             }
 #pragma unroll
             for (int k = 0; k < RUN; k++)
                 if (p + k < last) {
-                    const unsigned key = key_of((p + k) * KV8_PAGE + lane, y[k]);
+                    const unsigned key = z.key(p + k, y[k]);
                     top(key);
                     const int at = p + k - first - NK;
                     if (at < NL) in_lds[(wave * NL + at) * KV8_PAGE + lane] = key;
@@ -178,11 +222,11 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
             unsigned y[RUN];
             const bool near = p + RUN <= first + NK + NL;
 #pragma unroll
-            for (int k = 0; k < RUN; k++) is[k] = id_of(p + k);
+            for (int k = 0; k < RUN; k++) is[k] = z.id(p + k, last);
 #pragma unroll
             for (int k = 0; k < RUN; k++)
                 y[k] = near ? in_lds[(wave * NL + p + k - first - NK) * KV8_PAGE + lane]
-                            : key_of((p + k) * KV8_PAGE + lane, weight_at(is[k], p + k));
+                            : z.key(p + k, z.weight(is[k], p + k, last));
 #pragma unroll
             for (int k = 0; k < RUN; k++)
                 if (p + k < last) f(p + k, y[k], is[k]);
@@ -193,7 +237,7 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
         for (int m = tid; kept && m < e.budget; m += NT) kept[m] = m < n ? m : -1;
         if (n > 0)
             tokens([&](int p, unsigned, int id) __attribute__((always_inline)) {
-                if (p * KV8_PAGE + lane < n) w.weight[p * KV8_PAGE + lane] = weight_at(id, p);
+                if (p * KV8_PAGE + lane < n) w.weight[p * KV8_PAGE + lane] = z.weight(id, p, last);
             });
         return;
     }
@@ -212,27 +256,9 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
                 });
                 __syncthreads();
             }
-            // the largest first: thread t has bins BINS - 1 - PER t and below, and clears them for the next digit
-            int mine[PER], sum = 0;
-#pragma unroll
-            for (int k = 0; k < PER; k++) {
-                sum += mine[k] = hist[bin(BINS - 1 - PER * tid - k)];
-                hist[bin(BINS - 1 - PER * tid - k)] = 0;
-            }
-            int before = block_scan<NT>(sum, part);
-            if (before < equal && before + sum >= equal)
-#pragma unroll
-                for (int k = 0; k < PER; k++) {
-                    if (before < equal && before + mine[k] >= equal) {
-                        found[0] = BINS - 1 - PER * tid - k;
-                        found[1] = equal - before;
-                    }
-                    before += mine[k];
-                }
-            __syncthreads();
-            border |= (unsigned)found[0] << shift;
-            equal = found[1];
-            // (found is next written behind a barrier)
+            const int2 bin = bin_of_hist<NT>(hist, equal, part, found);
+            border |= (unsigned)bin.x << shift;
+            equal = bin.y;
         }
     }
     // in order: all above the border, the first of those at it
@@ -257,13 +283,242 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
         if (lane == 0 && p <= w.pages) w.rank[p] = m;
         if (key > border || (key == border && t < equal)) {
             w.list[m] = make_int2(p * KV8_PAGE + lane, id);
-            w.weight[m] = key == SURE || key == NAN_KEY || key == ZERO_KEY ? weight_at(id, p) : key_weight(key);
+            w.weight[m] = has_weight(key) ? key_weight(key) : z.weight(id, p, last);
             if (kept) kept[m] = p * KV8_PAGE + lane;
         }
         sure += __popcll(b);
         ties += __popcll(a);
     });
     if (tid == 0 && pages <= w.pages) w.rank[pages] = e.budget;
+}
+
+// The same for a long table and few heads, by several workgroups (parts) of each sequence and head in three launches: each
+// part's histogram of the first digit; its tokens of the border's bin, when all parts' histograms are summed; the list, when all those
+// tokens' other digits are looked at.  40 heads of 65,003 tokens: 8 + 13 + 17 us, one workgroup of each 84 (it is bound by the instructions
+// of one CU), a launch for each of four digits of 8 bits and one for the list 74, 12 parts in two turns 9 + 24 + 23.  Each launch waits
+// for what others wrote: loads that do not depend on each other are all under way together.
+constexpr int PART_THREADS = 1024, PART_WAVES = PART_THREADS / 64, MOST_PARTS = 8;  // (one for a wave of the list's workgroups at most)
+struct Parts {
+    int2 *top;       // the border's first digit, and how many are kept of those that have it
+    int *above;      // [MOST_PARTS]: a part's tokens chosen for a larger first digit
+    int *near;       // [MOST_PARTS]: those with the border's
+    int *gone;       // [MOST_PARTS]: whether a page of the part is not there
+    int *hist;       // [parts][BINS]
+    unsigned *keys;  // [tokens of the table]: from a part's first token on, the keys of those with the border's first digit
+};
+inline size_t parts_size(int n, int max_pages) {
+    return (4 + 3 * MOST_PARTS + (size_t)n * BINS + (size_t)max_pages * KV8_PAGE) * sizeof(int);  // a multiple of 16 bytes
+}
+struct Part {
+    int64_t pair;
+    int own, first, last, begin;  // part; pages of this wave; the part's first page
+    int *hist;
+    Parts t;
+};
+__device__ __forceinline__ Part part_of(const Kv8Evict &e, char *ws, int parts, int64_t size, const Held &q, int64_t pair) {
+    Part a;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE, each = (pages + parts * PART_WAVES - 1) / (parts * PART_WAVES);
+    a.pair = pair;
+    a.own = blockIdx.x % parts;
+    a.begin = min(a.own * PART_WAVES * each, pages);
+    a.first = min(a.begin + wave * each, pages);
+    a.last = min(a.first + each, pages);
+    a.t.top = reinterpret_cast<int2 *>(ws + pair * size);
+    a.t.above = reinterpret_cast<int *>(a.t.top + 2);
+    a.t.near = a.t.above + MOST_PARTS;
+    a.t.gone = a.t.near + MOST_PARTS;
+    a.t.hist = a.t.gone + MOST_PARTS;
+    a.t.keys = reinterpret_cast<unsigned *>(a.t.hist + parts * BINS);
+    return a;
+}
+// f(page, key, page id, weight) for a wave's pages, in order.
+template <class F> __device__ __forceinline__ void each_page(const Tokens &z, const Part &a, F f) {
+    for (int p = a.first; p < a.last; p += RUN) {
+        int id[RUN];
+        float y[RUN];
+#pragma unroll
+        for (int k = 0; k < RUN; k++) id[k] = z.id(p + k, a.last);
+#pragma unroll
+        for (int k = 0; k < RUN; k++) y[k] = z.weight(id[k], p + k, a.last);
+#pragma unroll
+        for (int k = 0; k < RUN; k++)
+            if (p + k < a.last) f(p + k, z.key(p + k, y[k]), id[k], y[k]);
+    }
+}
+__global__ __launch_bounds__(PART_THREADS) void k_kv8_part(Kv8Evict e, char *ws, int parts, int64_t size) {
+    constexpr int PER = BINS / PART_THREADS;
+    __shared__ int hist[BINS], gone;
+    const int64_t pair = blockIdx.x / parts;
+    const int tid = threadIdx.x;
+    const Held q = held(e.s, pair / e.c.hk);
+    const Tokens z{e, q, (int)(pair % e.c.hk), tid & 63};
+    const Part a = part_of(e, ws, parts, size, q, pair);
+    if (tid == 0) gone = 0;
+#pragma unroll
+    for (int k = 0; k < PER; k++) hist[k * PART_THREADS + tid] = 0;
+    __syncthreads();
+    bool missing = q.table == nullptr;
+    if (!missing)
+        each_page(z, a, [&](int, unsigned key, int id, float) __attribute__((always_inline)) {
+            missing |= !z.there(id);
+            if (chosen(key)) atomicAdd(&hist[bin(key >> 20)], 1);
+        });
+    if (missing && q.n > 0) gone = 1;
+    __syncthreads();
+    int4 c;
+    c.x = hist[bin(PER * tid)];
+    c.y = hist[bin(PER * tid + 1)];
+    c.z = hist[bin(PER * tid + 2)];
+    c.w = hist[bin(PER * tid + 3)];
+    reinterpret_cast<int4 *>(a.t.hist + a.own * BINS)[tid] = c;
+    if (tid == 0) a.t.gone[a.own] = gone;
+}
+__global__ __launch_bounds__(PART_THREADS) void k_kv8_near(Kv8Evict e, char *ws, int parts, int64_t size) {
+    constexpr int PER = BINS / PART_THREADS;
+    __shared__ int part[PART_WAVES], found[2], above, near;
+    const int64_t pair = blockIdx.x / parts;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const Held q = held(e.s, pair / e.c.hk);
+    const Tokens z{e, q, (int)(pair % e.c.hk), lane};
+    const Part a = part_of(e, ws, parts, size, q, pair);
+    const int need = e.budget - e.first - e.recent;
+    if (q.table == nullptr || q.n <= e.budget || need == 0) return;
+    if (tid < 2) found[tid] = 0;
+    if (tid == 0) above = near = 0;
+    int4 c[MOST_PARTS];
+#pragma unroll
+    for (int k = 0; k < MOST_PARTS; k++)
+        c[k] = reinterpret_cast<const int4 *>(a.t.hist + min(k, parts - 1) * BINS)[BINS / PER - 1 - tid];
+    int sum[PER] = {}, mine[PER] = {};
+#pragma unroll
+    for (int k = 0; k < MOST_PARTS; k++) {
+        const int v[PER] = {c[k].w, c[k].z, c[k].y, c[k].x};
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            sum[u] += k < parts ? v[u] : 0;
+            mine[u] = k == a.own ? v[u] : mine[u];
+        }
+    }
+    const int2 top = bin_of<PART_THREADS>(sum, need, part, found);
+    int larger = 0;
+#pragma unroll
+    for (int u = 0; u < PER; u++) larger += BINS - 1 - PER * tid - u > top.x ? mine[u] : 0;
+    if (larger > 0) atomicAdd(&above, larger);
+    if (a.own == 0 && tid == 0) *a.t.top = top;
+    // (in any order)
+    unsigned *keys = a.t.keys + (int64_t)a.begin * KV8_PAGE;
+    each_page(z, a, [&](int, unsigned key, int, float) __attribute__((always_inline)) {
+        if (chosen(key) && (int)(key >> 20) == top.x) keys[atomicAdd(&near, 1)] = key;
+    });
+    __syncthreads();
+    if (tid == 0) {
+        a.t.above[a.own] = above;
+        a.t.near[a.own] = near;
+    }
+}
+__global__ __launch_bounds__(PART_THREADS) void k_kv8_list(Kv8Evict e, void *ws, char *parts_ws, int parts, int64_t size) {
+    constexpr int NK = 8;
+    __shared__ int hist[BINS], part[PART_WAVES], found[2], count[2][PART_WAVES], before[2];
+    const int64_t pair = blockIdx.x / parts;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Held q = held(e.s, pair / e.c.hk);
+    const Tokens z{e, q, (int)(pair % e.c.hk), lane};
+    const Work w = work_of(e, ws, pair);
+    const Part a = part_of(e, parts_ws, parts, size, q, pair);
+    int *kept = e.kept ? e.kept + pair * e.budget : nullptr;
+    const int need = e.budget - e.first - e.recent;
+    const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE;
+    const int n = __ballot(lane < parts && a.t.gone[min(lane, parts - 1)] != 0) ? 0 : q.n;
+    if (a.own == 0 && tid == 0) *w.state = make_int4(q.n, min(n, e.budget), n > e.budget, 0);
+    if (n <= e.budget) {  // stays as it is
+        for (int m = a.own * PART_THREADS + tid; kept && m < e.budget; m += parts * PART_THREADS) kept[m] = m < n ? m : -1;
+        if (n > 0)
+            each_page(z, a, [&](int p, unsigned, int, float y) __attribute__((always_inline)) {
+                if (p * KV8_PAGE + lane < n) w.weight[p * KV8_PAGE + lane] = y;
+            });
+        return;
+    }
+    for (int p = a.own * PART_THREADS + tid; p < w.pages; p += parts * PART_THREADS) w.read[p] = 0;
+    unsigned border = SURE - 1;  // (need 0: above all keys)
+    int equal = 0;
+    if (tid < 2) before[tid] = 0;
+    if (need > 0) {
+        // wave k has part k's keys of the border's bin: the first NK of a lane in registers
+        const int near = wave < parts ? a.t.near[wave] : 0, over = wave < a.own ? a.t.above[wave] : 0;
+        const int each = (pages + parts * PART_WAVES - 1) / (parts * PART_WAVES);
+        const unsigned *keys = a.t.keys + (int64_t)min(wave * PART_WAVES * each, pages) * KV8_PAGE;
+        const int2 top = *a.t.top;
+        unsigned x[NK];
+#pragma unroll
+        for (int k = 0; k < NK; k++) x[k] = k * 64 + lane < near ? keys[k * 64 + lane] : NO_KEY;
+        auto others = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+            for (int k = 0; k < NK; k++) f(x[k]);
+            for (int k = NK * 64; k < near; k += 64) f(k + lane < near ? keys[k + lane] : NO_KEY);
+        };
+#pragma unroll
+        for (int k = 0; k < BINS / PART_THREADS; k++) hist[k * PART_THREADS + tid] = 0;
+        if (tid < 2) found[tid] = 0;
+        __syncthreads();
+        others([&](unsigned key) __attribute__((always_inline)) {
+            if (key != NO_KEY) atomicAdd(&hist[bin(key >> 8 & 4095)], 1);
+        });
+        __syncthreads();
+        int2 b = bin_of_hist<PART_THREADS>(hist, top.y, part, found);
+        border = (unsigned)top.x << 20 | (unsigned)b.x << 8;
+        others([&](unsigned key) __attribute__((always_inline)) {
+            if (key != NO_KEY && key >> 8 == border >> 8) atomicAdd(&hist[bin(key & 255)], 1);
+        });
+        __syncthreads();
+        b = bin_of_hist<PART_THREADS>(hist, b.y, part, found);
+        border |= b.x;
+        equal = b.y;
+        // of the parts before this one
+        if (wave < a.own) {
+            int sure = 0, ties = 0;
+            others([&](unsigned key) __attribute__((always_inline)) {
+                sure += __popcll(__ballot(key > border));
+                ties += __popcll(__ballot(key == border));
+            });
+            if (lane == 0) {
+                atomicAdd(&before[0], sure + over);
+                atomicAdd(&before[1], ties);
+            }
+        }
+    }
+    // (those that are kept for sure: the first, and the recent if this part begins among them)
+    const int start = a.begin * KV8_PAGE;
+    const int fixed = min(start, e.first) + max(min(start, q.n) - (q.n - e.recent), 0);
+    int sure = 0, ties = 0;
+    each_page(z, a, [&](int, unsigned key, int, float) __attribute__((always_inline)) {
+        sure += __popcll(__ballot(key > border));
+        ties += __popcll(__ballot(key == border));
+    });
+    if (lane == 0) {
+        count[0][wave] = sure;
+        count[1][wave] = ties;
+    }
+    __syncthreads();
+    sure = before[0] + fixed;
+    ties = before[1];
+    for (int u = 0; u < wave; u++) {
+        sure += count[0][u];
+        ties += count[1][u];
+    }
+    each_page(z, a, [&](int p, unsigned key, int id, float y) __attribute__((always_inline)) {
+        const unsigned long long below = (1ull << lane) - 1, at = __ballot(key == border), over = __ballot(key > border);
+        const int tie = ties + __popcll(at & below), m = sure + __popcll(over & below) + min(tie, equal);
+        if (lane == 0 && p <= w.pages) w.rank[p] = m;
+        if (key > border || (key == border && tie < equal)) {
+            w.list[m] = make_int2(p * KV8_PAGE + lane, id);
+            w.weight[m] = y;
+            if (kept) kept[m] = p * KV8_PAGE + lane;
+        }
+        sure += __popcll(over);
+        ties += __popcll(at);
+    });
+    if (a.own == 0 && tid == 0 && pages <= w.pages) w.rank[pages] = e.budget;
 }
 
 // A code scaled by r <= 1, in the low byte: the product is rounded to FP32, as code r is, and 1.5 2^23 rounds it to a
@@ -462,11 +717,19 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
 
 }  // namespace
 
+// How many workgroups choose for a sequence and head (0: one, in one launch), so that one of 1,024 threads is on each CU.  Whole
+// evictions of one sequence to 4,000 tokens, one workgroup / several: 8 heads of 9,000 tokens 34 / 30 us, of 65,000 95 / 42; 40 heads 102 /
+// 57; 128 heads 130 / 122, 192 heads 156 / 195 (in two turns).
+static int choose_parts(const Kv8Seqs &s, int hk) {
+    const int64_t pairs = (int64_t)s.n_seq * hk, most = (int64_t)s.max_pages * KV8_PAGE;
+    return most <= 8192 || pairs > 128 ? 0 : (int)min((int64_t)MOST_PARTS, 256 / pairs);
+}
 // (a table holds no more)
 static int room_of(const Kv8Seqs &s, int budget) { return (int)min((int64_t)budget, (int64_t)s.max_pages * KV8_PAGE); }
 
 size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget) {
-    return (size_t)s.n_seq * c.hk * work_size(room_of(s, budget));
+    const int parts = choose_parts(s, c.hk);
+    return (size_t)s.n_seq * c.hk * (work_size(room_of(s, budget)) + (parts ? parts_size(parts, s.max_pages) : 0));
 }
 
 hipError_t launch_kv8_evict(const Kv8Evict &call, void *ws, hipStream_t st) {
@@ -478,7 +741,17 @@ hipError_t launch_kv8_evict(const Kv8Evict &call, void *ws, hipStream_t st) {
     if (!kv8_grid(pairs, 1024) || !kv8_grid(pairs * pages, 1024)) return hipErrorInvalidValue;
     if (most <= 2048) hipLaunchKernelGGL((k_kv8_choose<256, 8, 0>), dim3(pairs), dim3(256), 0, st, e, ws);
     else if (most <= 8192) hipLaunchKernelGGL((k_kv8_choose<1024, 8, 0>), dim3(pairs), dim3(1024), 0, st, e, ws);
-    else hipLaunchKernelGGL((k_kv8_choose<1024, 32, 32>), dim3(pairs), dim3(1024), 0, st, e, ws);
+    else if (const int parts = choose_parts(e.s, e.c.hk); !parts)
+        hipLaunchKernelGGL((k_kv8_choose<1024, 32, 32>), dim3(pairs), dim3(1024), 0, st, e, ws);
+    else {
+        char *more = static_cast<char *>(ws) + pairs * work_size(e.room);
+        const int64_t size = parts_size(parts, e.s.max_pages);
+        hipLaunchKernelGGL(k_kv8_part, dim3(pairs * parts), dim3(PART_THREADS), 0, st, e, more, parts, size);
+        if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+        hipLaunchKernelGGL(k_kv8_near, dim3(pairs * parts), dim3(PART_THREADS), 0, st, e, more, parts, size);
+        if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+        hipLaunchKernelGGL(k_kv8_list, dim3(pairs * parts), dim3(PART_THREADS), 0, st, e, ws, more, parts, size);
+    }
     // (the moves wait for one another by what the choice has cleared)
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
     auto move = [&](auto dp) {

@@ -409,6 +409,20 @@ def test_evict_short_sequences_in_wide_tables(hip, max_pages):
     run_evict(hip, rng, [1999, 700], 650, 0, 0, max_pages=max_pages, weights=lambda s: rng.integers(0, 2, s).astype(np.float32), inplace=True)
 
 
+@pytest.mark.parametrize("extra", [0, 63])
+@pytest.mark.parametrize("budget,first,recent", [(700, 3, 40), (130, 64, 66), (4000, 0, 3000), (8900, 1, 0)])
+def test_evict_long_tables_of_few_and_many_heads(hip, extra, budget, first, recent):
+    """Several workgroups choose for a head of few, one for each of many: ties, edges and pages that are not there."""
+    def missing(c, table, w):
+        table[2, 70] = -1
+
+    rng = np.random.default_rng(budget + extra)
+    values = np.array([0.0, -0.0, np.inf, -np.inf, np.nan, -1.0, 1e-40, -1e-40, 3e38, 1.0, 1.0000001], np.float32)
+    lens = [9001, 300, 5000, 8900] + [140] * extra
+    run_evict(hip, rng, lens, budget, first, recent, d=16, weights=lambda s: rng.choice(values, s), edit=missing)
+    run_evict(hip, rng, lens, budget, first, recent, d=16, weights=lambda s: rng.integers(0, 2, s).astype(np.float32), slots=True)
+
+
 @pytest.mark.parametrize("pattern", ["last", "first", "even", "runs"])
 def test_evict_where_the_kept_tokens_lie(hip, pattern):
     """Pages that all wait for one, that wait for none, and that take tokens from many."""
