@@ -148,7 +148,8 @@ template <int NT> __device__ __forceinline__ int2 bin_of_hist(int *hist, int wan
 // NT threads; a wave owns a run of pages, token `lane` of each in a lane.  The smallest key that
 // is kept is found by its digits from the highest on (12, 12 and 8 bits), each from a
 // histogram of the keys that have the digits before it.  A wave keeps the keys of its first NK pages in
-// registers and of the next NL in LDS; those behind are read again for each digit.
+// registers and of the next NL in LDS; those behind are read again for each digit.  Bound by its chain of loads, scans
+// and barriers: 8 sequences of 577 tokens, 20 heads, 10 us (bins that share a bank 13), 32 of 1,900 to 6,000, 8 heads, 16.
 constexpr int RUN = 8;
 template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_choose(Kv8Evict e, void *ws) {
     constexpr int PER = BINS / NT, NW = NT / 64;
@@ -549,7 +550,8 @@ __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
 // the source page's codes as they lie there, 16 tokens of a dim a lane; what comes out, four places of a dim a
 // lane, is a word of the new page but for its scale.  Source pages add up.  (Other ways for 32 sequences to 2,048 tokens, 8 heads
 // of 128: a load from memory for each byte keeps the address unit busy, 107 us; rows through LDS and bytes there, a dim a
-// lane, 103.)  K: 16 dims of a token a lane.
+// lane, 103; this way 99: the 252 MB that it cannot do without at 2.5 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
+// ticket, list, codes and flag, which two workgroups of 88 registers on a CU do not hide; 80 registers spill (115), 16 dims a wave (52 registers) double the workgroups and draws (118), 1,024 threads are no better (104).
 constexpr int MOST_POLLS = 1 << 20;
 template <int DP> struct Move {
     static constexpr int WAVES = DP > 32 ? DP / 32 : 1;    // of a page
@@ -559,12 +561,14 @@ template <int DP> struct Move {
 template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_move(Kv8Evict e, void *ws, int runs) {
     constexpr int TILES = Move<DP>::TILES, RUN = Move<DP>::RUN, UNIT = 64 * Move<DP>::WAVES;
     __shared__ int srun;
-    const int64_t pair = blockIdx.x / runs;
+    // runs of a pair start apart, on XCDs in turn (one after the other: 107 us for 99, all on one XCD 148)
+    const int pairs = e.s.n_seq * e.c.hk;
+    const int64_t pair = (blockIdx.x % pairs + blockIdx.x / pairs) % pairs;
     const int h = pair % e.c.hk, i = pair / e.c.hk;
     const int unit = __builtin_amdgcn_readfirstlane(threadIdx.x / UNIT), tid = threadIdx.x % UNIT, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Work w = work_of(e, ws, pair);
-    int run = blockIdx.x % runs;
+    int run = blockIdx.x / pairs;
     if (threadIdx.x == 0) srun = atomicAdd(&w.state->w, 1);
     const int slot = e.s.slots ? e.s.slots[i] : i;  // (sequences of slots that are not there have nothing to move)
     const int *table = e.s.table + (int64_t)slot * e.s.table_stride;
