@@ -17,6 +17,10 @@
 // between the two.  The pass keeps the sums of e_p and e_q over them, and how near to r the nearest ratio is; where the 64-bit r
 // turns out to be further away than that (one row of a hundred, or where p and q differ in a few tokens
 // only), the last workgroup sums the row again.
+//
+// 64 sequences of 3 to 7 drafts over 131,072 tokens (bfloat16): rows 30 us, bound by bytes (168 MB at 5.6 TB/s, a part from the
+// last-level cache), finish 37, bound by the 64-bit exponentials of 64 rows of p and q and three turns of dependent
+// loads; 8 drafted streams over 33 tokens (narrow) 4.5, a chain of loads and sums.
 #include <float.h>
 
 #include <type_traits>
