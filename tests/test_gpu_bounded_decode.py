@@ -250,6 +250,13 @@ def test_captured_and_replayed(hip, streams, args, dtype):  # noqa: F811
         p.free()
 
 
+def test_long_tables_at_once_and_replayed(hip, streams):  # noqa: F811
+    """Tables of more than 8,192 tokens, where several workgroups choose for a head."""
+    args = ([130, 7, 1], 8800, 250, 0, 0)
+    test_two_streams_at_once(hip, streams, args, "float16")
+    test_captured_and_replayed(hip, streams, args, "float16")
+
+
 def test_offsets_past_32_bits(hip):
     """Codes and weights at byte offsets beyond 2^31 and 2^32: as in a pool of five pages."""
     d, hk, g, n, budget, dtype = 128, 4, 2, 300, 130, "bfloat16"
