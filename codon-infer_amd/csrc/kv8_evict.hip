@@ -52,6 +52,9 @@ __device__ __forceinline__ unsigned weight_key(float x) {
 }
 __device__ __forceinline__ float key_weight(unsigned k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
+// Whether weights of sequences that stay as they are go anywhere.
+__device__ __forceinline__ bool copies(const Kv8Evict &e) { return e.weights_out && e.weights_out != e.weights; }
+
 // Tokens a sequence holds and its row of the table.
 struct Held {
     int n;
@@ -80,6 +83,8 @@ struct Tokens {
         return j < q.n ? k : NO_KEY;
     }
 };
+// A sequence that stays as it is has no weights looked at, only whether its pages are there.
+__device__ __forceinline__ Held looked_at(const Kv8Evict &e, const Held &q) { return {q.n > e.budget ? q.n : 0, q.table}; }
 __device__ __forceinline__ bool chosen(unsigned key) { return key - 1 < SURE - 1; }  // by its weight
 // A kept token's weight (a key of 0 or NaN does not have all of it).
 __device__ __forceinline__ bool has_weight(unsigned key) { return key != SURE && key != NAN_KEY && key != ZERO_KEY; }
@@ -163,7 +168,7 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE;
     const int own = (pages + NW - 1) / NW;  // pages of a wave
     const int first = min(wave * own, pages), last = min(first + own, pages);
-    const Tokens z{e, q, h, lane};
+    const Tokens z{e, q, h, lane}, look{e, looked_at(e, q), h, lane};
     if (tid == 0) found[0] = 0;
 #pragma unroll
     for (int k = 0; k < PER; k++) hist[k * NT + tid] = 0;
@@ -183,11 +188,11 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
 #pragma unroll
         for (int k = 0; k < NK; k++) {
             gone |= !z.there(id[k]);
-            y[k] = z.weight(id[k], first + k, last);
+            y[k] = look.weight(id[k], first + k, last);
         }
 #pragma unroll
         for (int k = 0; k < NK; k++) {
-            x[k] = first + k < last ? z.key(first + k, y[k]) : NO_KEY;
+            x[k] = first + k < last ? look.key(first + k, y[k]) : NO_KEY;
             top(x[k]);
         }
         for (int p = first + NK; p < last; p += RUN) {
@@ -198,12 +203,12 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
 #pragma unroll
             for (int k = 0; k < RUN; k++) {
                 gone |= !z.there(is[k]);
-                y[k] = z.weight(is[k], p + k, last);
+                y[k] = look.weight(is[k], p + k, last);
             }
 #pragma unroll
             for (int k = 0; k < RUN; k++)
                 if (p + k < last) {
-                    const unsigned key = z.key(p + k, y[k]);
+                    const unsigned key = look.key(p + k, y[k]);
                     top(key);
                     const int at = p + k - first - NK;
                     if (at < NL) in_lds[(wave * NL + at) * KV8_PAGE + lane] = key;
@@ -236,7 +241,7 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
     if (tid == 0) *w.state = make_int4(q.n, min(n, e.budget), n > e.budget, 0);
     if (n <= e.budget) {  // stays as it is
         for (int m = tid; kept && m < e.budget; m += NT) kept[m] = m < n ? m : -1;
-        if (n > 0)
+        if (n > 0 && copies(e))
             tokens([&](int p, unsigned, int id) __attribute__((always_inline)) {
                 if (p * KV8_PAGE + lane < n) w.weight[p * KV8_PAGE + lane] = z.weight(id, p, last);
             });
@@ -353,7 +358,7 @@ __global__ __launch_bounds__(PART_THREADS) void k_kv8_part(Kv8Evict e, char *ws,
     const int64_t pair = blockIdx.x / parts;
     const int tid = threadIdx.x;
     const Held q = held(e.s, pair / e.c.hk);
-    const Tokens z{e, q, (int)(pair % e.c.hk), tid & 63};
+    const Tokens z{e, looked_at(e, q), (int)(pair % e.c.hk), tid & 63};
     const Part a = part_of(e, ws, parts, size, q, pair);
     if (tid == 0) gone = 0;
 #pragma unroll
@@ -434,7 +439,7 @@ __global__ __launch_bounds__(PART_THREADS) void k_kv8_list(Kv8Evict e, void *ws,
     if (a.own == 0 && tid == 0) *w.state = make_int4(q.n, min(n, e.budget), n > e.budget, 0);
     if (n <= e.budget) {  // stays as it is
         for (int m = a.own * PART_THREADS + tid; kept && m < e.budget; m += parts * PART_THREADS) kept[m] = m < n ? m : -1;
-        if (n > 0)
+        if (n > 0 && copies(e))
             each_page(z, a, [&](int p, unsigned, int, float y) __attribute__((always_inline)) {
                 if (p * KV8_PAGE + lane < n) w.weight[p * KV8_PAGE + lane] = y;
             });
@@ -550,7 +555,7 @@ __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
 // the source page's codes as they lie there, 16 tokens of a dim a lane; what comes out, four places of a dim a
 // lane, is a word of the new page but for its scale.  Source pages add up.  (Other ways for 32 sequences to 2,048 tokens, 8 heads
 // of 128: a load from memory for each byte keeps the address unit busy, 107 us; rows through LDS and bytes there, a dim a
-// lane, 103; this way 99: the 252 MB that it cannot do without at 2.5 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
+// lane, 103; this way 92: the 252 MB that it cannot do without at 2.7 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
 // ticket, list, codes and flag, which two workgroups of 88 registers on a CU do not hide; 80 registers spill (115), 16 dims a wave (52 registers) double the workgroups and draws (118), 1,024 threads are no better (104).
 constexpr int MOST_POLLS = 1 << 20;
 template <int DP> struct Move {
@@ -569,17 +574,20 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const Work w = work_of(e, ws, pair);
     int run = blockIdx.x / pairs;
-    if (threadIdx.x == 0) srun = atomicAdd(&w.state->w, 1);
     const int slot = e.s.slots ? e.s.slots[i] : i;  // (sequences of slots that are not there have nothing to move)
     const int *table = e.s.table + (int64_t)slot * e.s.table_stride;
     const int held = w.state->x, n = w.state->y;
     const bool moves = w.state->z != 0;
+    // (behind the state, so that those of sequences that stay draw nothing: 64 sequences of 4,000 tokens within a budget of
+    // 4,096, 8 heads, 39 -> 23 us in all, and the moves 99 -> 92)
+    if (moves && threadIdx.x == 0) srun = atomicAdd(&w.state->w, 1);
     if (run == 0 && h == 0 && threadIdx.x == 0) {
         // (a sequence that is left alone keeps its length, also one that is not there)
         if (moves) e.lens_out[i] = e.budget;
         else if (e.lens_out != e.s.lens) e.lens_out[i] = e.s.lens[i];
         if (moves && e.shifts) e.shifts[i] += held - e.budget;
     }
+    if (!moves && !copies(e)) return;
     __syncthreads();
     if (moves) run = __builtin_amdgcn_readfirstlane(srun);
     const int p = run * RUN + unit, m0 = p * KV8_PAGE, here = min(KV8_PAGE, n - m0);
