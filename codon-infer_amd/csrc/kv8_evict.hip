@@ -556,7 +556,7 @@ __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
 // lane, is a word of the new page but for its scale.  Source pages add up.  (Other ways for 32 sequences to 2,048 tokens, 8 heads
 // of 128: a load from memory for each byte keeps the address unit busy, 107 us; rows through LDS and bytes there, a dim a
 // lane, 103; this way 92: the 252 MB that it cannot do without at 2.7 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
-// ticket, list, codes and flag, which two workgroups of 88 registers on a CU do not hide; 80 registers spill (115), 16 dims a wave (52 registers) double the workgroups and draws (118), 1,024 threads are no better (104).
+// ticket, list, codes and flag, which two workgroups of 88 registers on a CU do not hide; 80 registers spill (115), 16 dims a wave (52 registers) double the workgroups and draws (118), 1,024 threads are no better (101).
 constexpr int MOST_POLLS = 1 << 20;
 template <int DP> struct Move {
     static constexpr int WAVES = DP > 32 ? DP / 32 : 1;    // of a page
