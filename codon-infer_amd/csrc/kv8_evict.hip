@@ -20,7 +20,7 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // Of each (sequence, head), in the workspace.
 struct Work {
-    int4 *state;    // tokens held, tokens kept, whether they move, the next run of pages to move
+    int4 *state;    // the sequence's length, tokens kept, whether they move, the next run of pages to move
     int2 *list;     // [tokens]: the kept ones, place and page
     float *weight;  // [tokens]
     int *read;      // [pages]: whether this page's tokens have been read
@@ -55,15 +55,16 @@ __device__ __forceinline__ float key_weight(unsigned k) { return __uint_as_float
 // Whether weights of sequences that stay as they are go anywhere.
 __device__ __forceinline__ bool copies(const Kv8Evict &e) { return e.weights_out && e.weights_out != e.weights; }
 
-// Tokens a sequence holds and its row of the table.
+// Tokens a sequence holds (of its length those that the table has room for), its row of the table, its length.
 struct Held {
     int n;
     const int *table;
+    int len;
 };
 __device__ __forceinline__ Held held(const Kv8Seqs &s, int i) {
     const int slot = s.slots ? s.slots[i] : i;
     return {(int)min((int64_t)max(s.lens[i], 0), (int64_t)s.max_pages * KV8_PAGE),
-            slot >= 0 && slot < s.table_rows ? s.table + (int64_t)slot * s.table_stride : nullptr};
+            slot >= 0 && slot < s.table_rows ? s.table + (int64_t)slot * s.table_stride : nullptr, s.lens[i]};
 }
 
 // Tokens of a sequence and head as a wave sees them: a page's token `lane` in a lane.
@@ -84,7 +85,7 @@ struct Tokens {
     }
 };
 // A sequence that stays as it is has no weights looked at, only whether its pages are there.
-__device__ __forceinline__ Held looked_at(const Kv8Evict &e, const Held &q) { return {q.n > e.budget ? q.n : 0, q.table}; }
+__device__ __forceinline__ Held looked_at(const Kv8Evict &e, const Held &q) { return {q.n > e.budget ? q.n : 0, q.table, q.len}; }
 __device__ __forceinline__ bool chosen(unsigned key) { return key - 1 < SURE - 1; }  // by its weight
 // A kept token's weight (a key of 0 or NaN does not have all of it).
 __device__ __forceinline__ bool has_weight(unsigned key) { return key != SURE && key != NAN_KEY && key != ZERO_KEY; }
@@ -238,7 +239,7 @@ template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_ch
                 if (p + k < last) f(p + k, y[k], is[k]);
         }
     };
-    if (tid == 0) *w.state = make_int4(q.n, min(n, e.budget), n > e.budget, 0);
+    if (tid == 0) *w.state = make_int4(q.len, min(n, e.budget), n > e.budget, 0);
     if (n <= e.budget) {  // stays as it is
         for (int m = tid; kept && m < e.budget; m += NT) kept[m] = m < n ? m : -1;
         if (n > 0 && copies(e))
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(PART_THREADS) void k_kv8_list(Kv8Evict e, void *ws,
     const int need = e.budget - e.first - e.recent;
     const int pages = (q.n + KV8_PAGE - 1) / KV8_PAGE;
     const int n = __ballot(lane < parts && a.t.gone[min(lane, parts - 1)] != 0) ? 0 : q.n;
-    if (a.own == 0 && tid == 0) *w.state = make_int4(q.n, min(n, e.budget), n > e.budget, 0);
+    if (a.own == 0 && tid == 0) *w.state = make_int4(q.len, min(n, e.budget), n > e.budget, 0);
     if (n <= e.budget) {  // stays as it is
         for (int m = a.own * PART_THREADS + tid; kept && m < e.budget; m += parts * PART_THREADS) kept[m] = m < n ? m : -1;
         if (n > 0 && copies(e))
@@ -576,7 +577,7 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
     int run = blockIdx.x / pairs;
     const int slot = e.s.slots ? e.s.slots[i] : i;  // (sequences of slots that are not there have nothing to move)
     const int *table = e.s.table + (int64_t)slot * e.s.table_stride;
-    const int held = w.state->x, n = w.state->y;
+    const int len = w.state->x, n = w.state->y;
     const bool moves = w.state->z != 0;
     // (behind the state, so that those of sequences that stay draw nothing: 64 sequences of 4,000 tokens within a budget of
     // 4,096, 8 heads, 39 -> 23 us in all, and the moves 99 -> 92)
@@ -585,7 +586,7 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
         // (a sequence that is left alone keeps its length, also one that is not there)
         if (moves) e.lens_out[i] = e.budget;
         else if (e.lens_out != e.s.lens) e.lens_out[i] = e.s.lens[i];
-        if (moves && e.shifts) e.shifts[i] += held - e.budget;
+        if (moves && e.shifts) e.shifts[i] += len - e.budget;  // (positions go on behind it)
     }
     if (!moves && !copies(e)) return;
     __syncthreads();

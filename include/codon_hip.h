@@ -375,7 +375,9 @@ int cih_kv8_weigh(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_
  *     shifts (NULL: none): how many tokens went is added, for cih_kv8_append_shifted.
  *     kept (NULL: none) [n_seq][kv_heads][budget]: the places that the kept tokens
  *         had, ascending, -1 behind them.
- * A sequence within the budget keeps all its tokens.  One whose slot or one of whose pages
+ * A sequence within the budget keeps all its tokens.  Of one that is longer than its table has room for
+ * the table's tokens are held, and cut like others'; shifts grow by its length less the budget, so that
+ * positions go on behind its length.  One whose slot or one of whose pages
  * is not there is left alone (kept -1, lens_out its length).  No page may stand twice in the tables
  * of a call.  workspace: 16-byte aligned, of cih_kv8_evict_workspace's size. */
 int cih_kv8_evict(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t budget, int32_t first, int32_t recent,

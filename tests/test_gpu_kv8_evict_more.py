@@ -1,11 +1,14 @@
 """Eviction where the smaller tests do not reach: tables whose keys fill registers, LDS
-and more.
+and more, sequences longer than their tables.
 """
 import numpy as np
 import pytest
 
-from codon_hip.devmem import Hip
-from test_gpu_kv8_more import run_evict
+import codon_hip as ch
+import kv8_more_ref as M
+import kv8_ref as R
+from codon_hip.devmem import DeviceArray, Hip
+from test_gpu_kv8_more import Case, run_evict
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +37,38 @@ def test_many_heads_pages_behind_that_are_not_there(hip):
         table[1, 1090] = 1 << 30  # behind it
 
     run_evict(hip, np.random.default_rng(2), [40000, 70000, 45000] + [140] * 62, 3001, 4, 100, d=16, edit=missing)
+
+
+def test_lengths_past_the_table(hip):
+    """A sequence that is longer than its table holds the table's tokens: those are cut, and positions go on behind its length."""
+    rng, d, budget, lens = np.random.default_rng(3), 64, 100, [1000, 300, 321, 90, 1 << 30]
+    x = Case(hip, rng, [320, 300, 320, 90, 320], [1] * 5, 2, 1, d, "float32")
+    w = rng.uniform(0, 1, x.c.k.shape[:3]).astype(np.float32)
+    want = M.evict(x.c, w, x.table, lens, range(5), budget, 4, 30)
+    dev = [DeviceArray(hip, a) for a in (np.array(lens, np.int32), w, np.arange(5).astype(np.int32), np.zeros((5, 2, budget), np.int32))]
+    batch = ch.Kv8Batch(x.arr[0], dev[0], x.arr[2], 5, 1)
+    ws = DeviceArray(hip, np.zeros(x.cache.evict_workspace(batch, budget), np.uint8))
+    x.cache.evict(batch, dev[1], budget, first=4, recent=30, shifts=dev[2], kept=dev[3], workspace=ws)
+    assert np.array_equal(dev[3].numpy(), want[5])
+    held = dev[0].numpy()
+    assert list(held) == [100, 100, 100, 90, 100]
+    shifts = dev[2].numpy()
+    assert np.array_equal(shifts, np.arange(5) + lens - held)
+    # the next row of each: its place follows what is held, its angle the length there was
+    k, v = rng.standard_normal((5, 2, d)), rng.standard_normal((5, 2, d))
+    rows = [R.put(hip, a, "float32") for a in (k, v)]
+    grown, cu = DeviceArray(hip, held + 1), DeviceArray(hip, np.arange(6, dtype=np.int32))
+    rope = ch.Rope(d)
+    x.cache.append(ch.Kv8Batch(cu, grown, x.arr[2], 5, 1), *rows, rope=rope, shifts=dev[2])
+    gk, _, gs, _ = x.c.download()
+    for i in range(5):
+        page, at = x.table[i, held[i] // 64], held[i] % 64
+        turned = R.rope(R.rounded(k[i:i + 1], "float32"), np.array([lens[i] + i]), rope)[0]
+        assert (np.abs(gk[page, :, at] - turned / gs[page, :, :1].astype(np.float64)) <= 0.5 + 1e-3).all()
+    # a budget that is more than the table holds: the sequence stays as it is, its length too
+    hip.h2d(dev[0].data_ptr(), np.array(lens, np.int32))
+    ws2 = DeviceArray(hip, np.zeros(x.cache.evict_workspace(batch, 350), np.uint8))
+    x.cache.evict(batch, dev[1], 350, first=4, recent=30, shifts=dev[2], workspace=ws2)
+    assert list(dev[0].numpy()) == lens and np.array_equal(dev[2].numpy(), shifts)
+    R.free(ws, ws2, grown, cu, *rows, *dev)
+    x.free()
