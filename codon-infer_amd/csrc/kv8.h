@@ -184,6 +184,7 @@ struct Kv8Evict {
     int *lens_out, *shifts, *kept;  // shifts, kept: may be nullptr
     int room = 0;                   // set by the launch: tokens of the budget that a table has room for
 };
+bool kv8_evict_fits(const Kv8View &c, const Kv8Seqs &s, int budget);  // whether one launch may have that many workgroups
 size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget);
 hipError_t launch_kv8_evict(const Kv8Evict &e, void *ws, hipStream_t st);
 

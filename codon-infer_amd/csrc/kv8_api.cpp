@@ -119,6 +119,12 @@ int check_budget(int budget, int first, int recent) {
     return 0;
 }
 
+int check_evict_size(const Kv8View &c, const Kv8Seqs &s, int budget) {
+    if (!kv8_evict_fits(c, s, budget))
+        return set_error(CIH_ERR_SHAPE, "%d sequences of %d heads to %d tokens: more than one launch may have", s.n_seq, c.hk, budget);
+    return 0;
+}
+
 }  // namespace
 
 int cih::kv8_rope(const cih_rope *r, int head_dim, RopeArg &a) {
@@ -298,6 +304,7 @@ int cih_kv8_evict_workspace(const cih_kv8_cache *cache, const cih_kv8_batch *bat
     CIH_TRY(check_cache(cache, c, false));
     CIH_TRY(check_batch(batch, s, false));
     CIH_TRY(check_budget(budget, 0, 0));
+    CIH_TRY(check_evict_size(c, s, budget));
     *bytes = kv8_evict_bytes(c, s, budget);
     return CIH_OK;
 }
@@ -312,6 +319,7 @@ int cih_kv8_evict(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_
     if (!b.cu_rows) b.cu_rows = b.lens;  // not read
     CIH_TRY(check_batch(&b, e.s, true));
     CIH_TRY(check_budget(budget, first, recent));
+    CIH_TRY(check_evict_size(e.c, e.s, budget));
     if (e.s.n_seq == 0) return CIH_OK;
     if (!weights || !lens_out) return set_error(CIH_ERR_ARG, "null %s", weights ? "lens_out" : "weights");
     if (!aligned(weights, 4) || !aligned(weights_out, 4) || !aligned(lens_out, 4) || !aligned(shifts, 4) || !aligned(kept, 4))

@@ -559,11 +559,17 @@ __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
 // lane, 103; this way 92: the 252 MB that it cannot do without at 2.7 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
 // ticket, list, codes and flag, which two workgroups of 88 registers on a CU do not hide; 80 registers spill (115), 16 dims a wave (52 registers) double the workgroups and draws (118), 1,024 threads are no better (101).
 constexpr int MOST_POLLS = 1 << 20;
+constexpr int MOVE_THREADS = 512;
+constexpr int move_waves(int dp) { return dp > 32 ? dp / 32 : 1; }  // of a page
 template <int DP> struct Move {
-    static constexpr int WAVES = DP > 32 ? DP / 32 : 1;    // of a page
+    static constexpr int WAVES = move_waves(DP);
     static constexpr int TILES = DP / 16 / WAVES;          // of 16 dims, a wave's; pieces of K, a lane's
-    static constexpr int RUN = 8 / WAVES, THREADS = 512;
+    static constexpr int RUN = 8 / WAVES, THREADS = MOVE_THREADS;
 };
+inline int64_t move_runs(int pages, int dp) {  // of a sequence and head
+    const int run = 8 / move_waves(dp);
+    return (pages + run - 1) / run;
+}
 template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_move(Kv8Evict e, void *ws, int runs) {
     constexpr int TILES = Move<DP>::TILES, RUN = Move<DP>::RUN, UNIT = 64 * Move<DP>::WAVES;
     __shared__ int srun;
@@ -740,6 +746,14 @@ static int choose_parts(const Kv8Seqs &s, int hk) {
 // (a table holds no more)
 static int room_of(const Kv8Seqs &s, int budget) { return (int)min((int64_t)budget, (int64_t)s.max_pages * KV8_PAGE); }
 
+// Threads of the workgroups that choose in one launch.
+static int choose_threads(const Kv8Seqs &s) { return (int64_t)s.max_pages * KV8_PAGE <= 2048 ? 256 : 1024; }
+static int pages_of(int room) { return (room + KV8_PAGE - 1) / KV8_PAGE; }
+
+bool kv8_evict_fits(const Kv8View &c, const Kv8Seqs &s, int budget) {
+    const int64_t pairs = (int64_t)s.n_seq * c.hk;  // (with several parts each, 1,024 workgroups at most)
+    return pairs == 0 || (kv8_grid(pairs, choose_threads(s)) && kv8_grid(pairs * move_runs(pages_of(room_of(s, budget)), c.dp), MOVE_THREADS));
+}
 size_t kv8_evict_bytes(const Kv8View &c, const Kv8Seqs &s, int budget) {
     const int parts = choose_parts(s, c.hk);
     return (size_t)s.n_seq * c.hk * (work_size(room_of(s, budget)) + (parts ? parts_size(parts, s.max_pages) : 0));
@@ -750,9 +764,8 @@ hipError_t launch_kv8_evict(const Kv8Evict &call, void *ws, hipStream_t st) {
     e.room = room_of(e.s, e.budget);
     const int64_t pairs = (int64_t)e.s.n_seq * e.c.hk, most = (int64_t)e.s.max_pages * KV8_PAGE;
     if (pairs == 0) return hipSuccess;
-    const int pages = (e.room + KV8_PAGE - 1) / KV8_PAGE;
-    if (!kv8_grid(pairs, 1024) || !kv8_grid(pairs * pages, 1024)) return hipErrorInvalidValue;
-    if (most <= 2048) hipLaunchKernelGGL((k_kv8_choose<256, 8, 0>), dim3(pairs), dim3(256), 0, st, e, ws);
+    if (!kv8_evict_fits(e.c, e.s, e.budget)) return hipErrorInvalidValue;
+    if (choose_threads(e.s) == 256) hipLaunchKernelGGL((k_kv8_choose<256, 8, 0>), dim3(pairs), dim3(256), 0, st, e, ws);
     else if (most <= 8192) hipLaunchKernelGGL((k_kv8_choose<1024, 8, 0>), dim3(pairs), dim3(1024), 0, st, e, ws);
     else if (const int parts = choose_parts(e.s, e.c.hk); !parts)
         hipLaunchKernelGGL((k_kv8_choose<1024, 32, 32>), dim3(pairs), dim3(1024), 0, st, e, ws);
@@ -769,7 +782,7 @@ hipError_t launch_kv8_evict(const Kv8Evict &call, void *ws, hipStream_t st) {
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
     auto move = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
-        const int runs = (pages + Move<DP>::RUN - 1) / Move<DP>::RUN;
+        const int runs = (int)move_runs(pages_of(e.room), DP);
         hipLaunchKernelGGL(k_kv8_move<DP>, dim3(pairs * runs), dim3(Move<DP>::THREADS), 0, st, e, ws, runs);
     };
     switch (e.c.dp) {

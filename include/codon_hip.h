@@ -379,7 +379,10 @@ int cih_kv8_weigh(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_
  * the table's tokens are held, and cut like others'; shifts grow by its length less the budget, so that
  * positions go on behind its length.  One whose slot or one of whose pages
  * is not there is left alone (kept -1, lens_out its length).  No page may stand twice in the tables
- * of a call.  workspace: 16-byte aligned, of cih_kv8_evict_workspace's size. */
+ * of a call.  workspace: 16-byte aligned, of cih_kv8_evict_workspace's size.
+ * Refused, as more than one launch may have: n_seq kv_heads above 2^22 - 1 (tables of up to 32 pages: 2^23 - 1),
+ * and n_seq kv_heads ceil(pages / p) above 2^23 - 1, with the pages of the budget (or the table's, if fewer) and
+ * p = 2 for heads of 128, 4 of 64, 8 of 16 to 32. */
 int cih_kv8_evict(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_t budget, int32_t first, int32_t recent,
                   const float *weights, float *weights_out, int32_t *lens_out, int32_t *shifts, int32_t *kept,
                   void *workspace, size_t workspace_bytes, void *stream);

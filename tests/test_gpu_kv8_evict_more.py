@@ -1,5 +1,5 @@
 """Eviction where the smaller tests do not reach: tables whose keys fill registers, LDS
-and more, sequences longer than their tables.
+and more, grids of many pages, sequences longer than their tables.
 """
 import numpy as np
 import pytest
@@ -9,6 +9,7 @@ import kv8_more_ref as M
 import kv8_ref as R
 from codon_hip.devmem import DeviceArray, Hip
 from test_gpu_kv8_more import Case, run_evict
+from test_gpu_ops_streams import Raw
 
 pytestmark = pytest.mark.gpu
 
@@ -37,6 +38,34 @@ def test_many_heads_pages_behind_that_are_not_there(hip):
         table[1, 1090] = 1 << 30  # behind it
 
     run_evict(hip, np.random.default_rng(2), [40000, 70000, 45000] + [140] * 62, 3001, 4, 100, d=16, edit=missing)
+
+
+def test_grids_of_many_pages(hip):
+    """65,600 heads with room for 64 pages each (they launch 2^28 threads), most of them of sequences without tokens."""
+    rng = np.random.default_rng(5)
+    n, budget, at, held = 65600, 4096, [0, 37, 40000, 65599], [4130, 4097, 4096, 4160]
+    x = Case(hip, rng, held, [1] * 4, 1, 1, 16, "float32", max_pages=65)
+    w = np.exp(rng.standard_normal(x.c.k.shape[:3])).astype(np.float32)
+    want = M.evict(x.c, w, x.table, held, range(4), budget, 4, 100)
+    lens, table = np.zeros(n, np.int32), np.full((n, 65), -1, np.int32)
+    lens[at], table[at] = held, x.table
+    dev = [DeviceArray(hip, a) for a in (np.zeros(n + 1, np.int32), lens, table, w, np.zeros(n, np.int32))]
+    batch = ch.Kv8Batch(*dev[:3], 1, 1)
+    ws = Raw(hip, (x.cache.evict_workspace(batch, budget),), "uint8")
+    x.cache.evict(batch, dev[3], budget, first=4, recent=100, shifts=dev[4], workspace=ws)
+    lens[at], shifts = want[6], np.zeros(n, np.int32)
+    shifts[at] = np.array(held) - want[6]
+    assert np.array_equal(dev[1].numpy(), lens) and np.array_equal(dev[4].numpy(), shifts)
+    gk, gv, gs, _ = x.c.download()
+    gw = dev[3].numpy()
+    for i, m in enumerate(want[6]):
+        j = np.arange(m)
+        page = x.table[i, j // 64]
+        assert np.array_equal(gk[page, 0, j % 64], want[0][page, 0, j % 64])
+        assert np.array_equal(gv[page, 0, :, j % 64], want[1][page, 0, :, j % 64])
+        assert np.array_equal(gs[page], want[2][page]) and np.array_equal(gw[page, 0, j % 64], want[4][page, 0, j % 64])
+    R.free(ws, *dev)
+    x.free()
 
 
 def test_lengths_past_the_table(hip):
