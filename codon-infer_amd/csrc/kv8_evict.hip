@@ -7,6 +7,8 @@
 // codes and makes the new pages' records.  A page's new scale is the largest of the
 // pages that its tokens come from, so codes are rounded again only where their page's scale
 // grows: a token that moves many times is not rounded each time.
+#include <stdlib.h>
+
 #include <type_traits>
 
 #include "kernels.h"
@@ -570,9 +572,9 @@ inline int64_t move_runs(int pages, int dp) {  // of a sequence and head
     const int run = 8 / move_waves(dp);
     return (pages + run - 1) / run;
 }
-template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_move(Kv8Evict e, void *ws, int runs) {
+template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_move(Kv8Evict e, void *ws, int polls) {
     constexpr int TILES = Move<DP>::TILES, RUN = Move<DP>::RUN, UNIT = 64 * Move<DP>::WAVES;
-    __shared__ int srun;
+    __shared__ int srun, late[RUN];
     // runs of a pair start apart, on XCDs in turn (one after the other: 107 us for 99, all on one XCD 148)
     const int pairs = e.s.n_seq * e.c.hk;
     const int64_t pair = (blockIdx.x % pairs + blockIdx.x / pairs) % pairs;
@@ -588,6 +590,7 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
     // (behind the state, so that those of sequences that stay draw nothing: 64 sequences of 4,000 tokens within a budget of
     // 4,096, 8 heads, 39 -> 23 us in all, and the moves 99 -> 92)
     if (moves && threadIdx.x == 0) srun = atomicAdd(&w.state->w, 1);
+    if (threadIdx.x < RUN) late[threadIdx.x] = 0;
     if (run == 0 && h == 0 && threadIdx.x == 0) {
         // (a sequence that is left alone keeps its length, also one that is not there)
         if (moves) e.lens_out[i] = e.budget;
@@ -706,13 +709,20 @@ template <int DP> __global__ __launch_bounds__(Move<DP>::THREADS) void k_kv8_mov
     // pages of runs before this one that take tokens from a page: 64 tokens go to two at most
     if (!stays && r0 < r1) {
         const int q = r0 / KV8_PAGE + tid;
-        if (q <= (r1 - 1) / KV8_PAGE && q < run * RUN)
+        if (q <= (r1 - 1) / KV8_PAGE && q < run * RUN) {
             // (microseconds; bounded for calls at the same time that share a workspace against the rule)
-            for (int n = 0; n < MOST_POLLS && !__hip_atomic_load(&w.read[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); n++)
-                __builtin_amdgcn_s_sleep(1);
+            int n = polls;
+            for (; n > 0 && !__hip_atomic_load(&w.read[q], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); n--) __builtin_amdgcn_s_sleep(1);
+            if (n == 0) late[unit] = 1;
+        }
     }
     __syncthreads();
     if (stays) return;
+    // not read by all in time: left as it is, for them, and all its tokens bad, for everyone else
+    if (late[unit]) {
+        if (tid == 0) e.c.bad[to] = ~0ull;
+        return;
+    }
 #pragma unroll
     for (int it = 0; it < TILES; it++) {
         const int at = tid + it * UNIT, m = at / (DP / 16);
@@ -780,10 +790,12 @@ hipError_t launch_kv8_evict(const Kv8Evict &call, void *ws, hipStream_t st) {
     }
     // (the moves wait for one another by what the choice has cleared)
     if (const hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+    const char *p = getenv("CIH_KV8_EVICT_POLLS");
+    const int polls = p ? (int)min(max(strtol(p, nullptr, 10), 0l), (long)MOST_POLLS) : MOST_POLLS;
     auto move = [&](auto dp) {
         constexpr int DP = decltype(dp)::value;
         const int runs = (int)move_runs(pages_of(e.room), DP);
-        hipLaunchKernelGGL(k_kv8_move<DP>, dim3(pairs * runs), dim3(Move<DP>::THREADS), 0, st, e, ws, runs);
+        hipLaunchKernelGGL(k_kv8_move<DP>, dim3(pairs * runs), dim3(Move<DP>::THREADS), 0, st, e, ws, polls);
     };
     switch (e.c.dp) {
         case 16: move(std::integral_constant<int, 16>{}); break;

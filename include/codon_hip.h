@@ -379,7 +379,9 @@ int cih_kv8_weigh(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_
  * the table's tokens are held, and cut like others'; shifts grow by its length less the budget, so that
  * positions go on behind its length.  One whose slot or one of whose pages
  * is not there is left alone (kept -1, lens_out its length).  No page may stand twice in the tables
- * of a call.  workspace: 16-byte aligned, of cih_kv8_evict_workspace's size.
+ * of a call.  workspace: 16-byte aligned, of cih_kv8_evict_workspace's size, not shared by calls that run at the
+ * same time: a page that such a call would overwrite before all its tokens are read is left where it is and marked
+ * bad, so that reads and attention give NaN for it.
  * Refused, as more than one launch may have: n_seq kv_heads above 2^22 - 1 (tables of up to 32 pages: 2^23 - 1),
  * and n_seq kv_heads ceil(pages / p) above 2^23 - 1, with the pages of the budget (or the table's, if fewer) and
  * p = 2 for heads of 128, 4 of 64, 8 of 16 to 32. */

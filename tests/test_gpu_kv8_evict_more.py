@@ -1,5 +1,5 @@
 """Eviction where the smaller tests do not reach: tables whose keys fill registers, LDS
-and more, grids of many pages, sequences longer than their tables.
+and more, grids of many pages, sequences longer than their tables, waits that end.
 """
 import numpy as np
 import pytest
@@ -100,4 +100,47 @@ def test_lengths_past_the_table(hip):
     x.cache.evict(batch, dev[1], 350, first=4, recent=30, shifts=dev[2], workspace=ws2)
     assert list(dev[0].numpy()) == lens and np.array_equal(dev[2].numpy(), shifts)
     R.free(ws, ws2, grown, cu, *rows, *dev)
+    x.free()
+
+
+@pytest.mark.parametrize("d", [16, 24, 64, 128])
+def test_a_wait_that_ends_shows(hip, monkeypatch, d):
+    """Pages that do not hear in time (here: that do not listen) that their tokens were read are left as they
+    are, with all tokens bad; the others move."""
+    monkeypatch.setenv("CIH_KV8_EVICT_POLLS", "0")
+    rng, hk, budget, lens = np.random.default_rng(d), 2, 1500, [4000, 1400, 1700]
+    x = Case(hip, rng, lens, [1] * 3, hk, 1, d, "float32")
+    w = rng.uniform(0, 1, x.c.k.shape[:3]).astype(np.float32)
+    k, v, scales, bad, wout, kept, out = M.evict(x.c, w, x.table, lens, range(3), budget, 70, 200)
+    dev = [DeviceArray(hip, a) for a in (w, np.zeros((3, hk, budget), np.int32))]
+    ws = DeviceArray(hip, np.zeros(x.cache.evict_workspace(x.batch, budget), np.uint8))
+    x.cache.evict(x.batch, dev[0], budget, first=70, recent=200, kept=dev[1], workspace=ws)
+    assert np.array_equal(dev[1].numpy(), kept) and np.array_equal(x.arr[1].numpy(), out)
+    got, gw = x.c.download(), dev[0].numpy()
+    run = {16: 8, 24: 8, 64: 4, 128: 2}[d]
+    left = 0
+    for i, h in np.ndindex(3, hk):
+        tok = kept[i, h, :out[i]]
+        for p in range(-(-out[i] // 64)):
+            m, page = min(64, out[i] - p * 64), x.table[i, p]
+            r0, r1 = np.searchsorted(tok, [p * 64, p * 64 + 64])  # its tokens' new places
+            stays = m == 64 and tok[p * 64 + 63] == p * 64 + 63
+            waits = lens[i] > budget and not stays and r0 < r1 and r0 // 64 < p // run * run
+            assert np.array_equal(gw[page, h, :m], wout[page, h, :m])
+            want = (x.c.k, x.c.v, x.c.scales) if waits else (k, v, scales)
+            n = 64 if waits else m
+            assert np.array_equal(got[0][page, h, :n], want[0][page, h, :n])
+            assert np.array_equal(got[1][page, h, :, :n], want[1][page, h, :, :n])
+            assert np.array_equal(got[2][page, h], want[2][page, h])
+            if waits:
+                assert int(got[3][page, h]) == 2 ** 64 - 1
+            left += waits
+    assert 20 < left < hk * 2 * -(-budget // 64)
+    # such pages read as NaN
+    cu, back = DeviceArray(hip, np.array([0, budget], np.int32)), [R.put(hip, np.zeros((budget, hk, d)), "float32") for _ in range(2)]
+    one = DeviceArray(hip, np.array([budget], np.int32))
+    x.cache.read(ch.Kv8Batch(cu, one, x.arr[2], budget, budget), *back)
+    lost = np.isnan(R.get(back[0])).all(2).sum()
+    assert lost >= 64 and lost == np.isnan(R.get(back[1])).any(2).sum()
+    R.free(cu, one, ws, *back, *dev)
     x.free()
