@@ -367,7 +367,8 @@ int cih_kv8_weigh(const cih_kv8_cache *cache, const cih_kv8_batch *batch, int32_
  * budget), and those of the others with the largest weights (ties: the earlier
  * token; NaN below all), moved to the places 0 .. budget - 1 in their order; the pages
  * behind them are the caller's again.  A page's scale becomes the largest of those that
- * its tokens come from, and codes are rounded again where their scale grows.  The batch's rows
+ * its tokens come from, and codes are rounded again where their scale grows (a scale does not fall when the token that
+ * set it goes: a cache that has held outliers keeps their step).  The batch's rows
  * are not used (cu_rows may be NULL); the heads of a sequence may keep different tokens.
  *     weights_out (NULL: not wanted; may be weights): the kept tokens' weights at
  *         their new places.

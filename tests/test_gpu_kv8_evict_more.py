@@ -1,5 +1,6 @@
 """Eviction where the smaller tests do not reach: tables whose keys fill registers, LDS
-and more, grids of many pages, sequences longer than their tables, waits that end.
+and more, grids of many pages, sequences longer than their tables, waits that end,
+and the error that a cache gathers over many steps.
 """
 import numpy as np
 import pytest
@@ -143,4 +144,58 @@ def test_a_wait_that_ends_shows(hip, monkeypatch, d):
     lost = np.isnan(R.get(back[0])).all(2).sum()
     assert lost >= 64 and lost == np.isnan(R.get(back[1])).any(2).sum()
     R.free(cu, one, ws, *back, *dev)
+    x.free()
+
+
+@pytest.mark.parametrize("d", [16, 64, 128])
+def test_cut_again_and_again_keeps_the_values(hip, d):
+    """A sequence at its budget takes rows and is cut, 60 times, with an outlier now and then: what the cache holds of a
+    token is its own K (turned) and V, off by half a step of each scale that its code was rounded to."""
+    rng, hk, budget, new = np.random.default_rng(d), 2, 150, 13
+    x = Case(hip, rng, [budget + new], [1], hk, 1, d, "float32")
+    x.c.k[:], x.c.v[:], x.c.scales[:], x.c.bad[:] = 0, 0, 0, 0
+    for a, b in zip(x.c.dev, (x.c.k, x.c.v, x.c.scales, x.c.bad)):
+        hip.h2d(a.data_ptr(), b)
+    table, rope = x.table[0], ch.Rope(d)
+    wt, shifts = DeviceArray(hip, np.zeros(x.c.k.shape[:3], np.float32)), DeviceArray(hip, np.zeros(1, np.int32))
+    held, kept = DeviceArray(hip, np.zeros(1, np.int32)), DeviceArray(hip, np.zeros((1, hk, budget), np.int32))
+    ws = DeviceArray(hip, np.zeros(x.cache.evict_workspace(x.batch, budget), np.uint8))
+    own = np.zeros((hk, 0, 2, d))    # what each place's token was
+    off = np.zeros((hk, 0, 2))       # how far the cache may be from it
+    scale = np.zeros((hk, 0, 2))     # of the code that it has
+
+    def follow(own, off, scale, fresh):
+        """Half a step where a code was made or made again; what the cache holds is within that."""
+        gk, gv, gs, _ = x.c.download()
+        j = np.arange(own.shape[1])
+        page = table[j // 64]
+        now = gs[page].astype(np.float64).transpose(1, 0, 2)
+        again = (now != scale) | (j >= fresh)[None, :, None]
+        off = off + again * now * (0.5 + 1e-3)
+        got = np.stack((gk[page, :, j % 64, :d], gv[page, :, :d, j % 64]), 2).transpose(1, 0, 2, 3) * now[..., None]
+        assert (np.abs(got - own) <= off[..., None]).all()
+        return off, now
+
+    for step in range(60):
+        n0 = own.shape[1]
+        m = budget + new - n0
+        k, v = (rng.standard_normal((m, hk, d)) * np.where(rng.random((m, hk, 1)) < 0.05, 6.0, 1.0) for _ in range(2))
+        k, v = R.rounded(k, "float32"), R.rounded(v, "float32")
+        rows, cu = [R.put(hip, a, "float32") for a in (k, v)], DeviceArray(hip, np.array([0, m], np.int32))
+        lens = DeviceArray(hip, np.array([budget + new], np.int32))
+        batch = ch.Kv8Batch(cu, lens, x.arr[2], m, m)
+        x.cache.append(batch, *rows, rope=rope, shifts=shifts)
+        pos = np.arange(n0, budget + new) + int(shifts.numpy()[0])
+        both = np.stack((R.rope(k, pos, rope), v), 2).transpose(1, 0, 2, 3)
+        own, off = np.concatenate([own, both], 1), np.concatenate([off, np.zeros((hk, m, 2))], 1)
+        scale = np.concatenate([scale, np.zeros((hk, m, 2))], 1)
+        off, scale = follow(own, off, scale, n0)
+        hip.h2d(wt.data_ptr(), rng.random(x.c.k.shape[:3]).astype(np.float32))
+        x.cache.evict(batch, wt, budget, first=2, recent=20, lens_out=held, shifts=shifts, kept=kept, workspace=ws)
+        tok = kept.numpy()[0]
+        own, off, scale = (np.stack([a[h, tok[h]] for h in range(hk)]) for a in (own, off, scale))
+        off, scale = follow(own, off, scale, budget)
+        R.free(cu, lens, *rows)
+    assert shifts.numpy()[0] == 60 * new
+    R.free(wt, shifts, held, kept, ws)
     x.free()
