@@ -287,8 +287,8 @@ class Kv8Cache:
         first `first`, its last `recent` and of the others those with the largest
         weights, in their order.  The kept tokens' weights go to weights_out
         (default: weights itself), the new lengths to lens_out (default: the
-        batch's lens), how many tokens went is added to shifts (int32 [n_seq]), the
-        places that the kept ones had go to kept (int32 [n_seq][kv_heads][budget],
+        batch's lens), how many tokens went (its length less the budget) is added to
+        shifts (int32 [n_seq]), the places that the kept ones had go to kept (int32 [n_seq][kv_heads][budget],
         -1 behind them)."""
         n, i32 = batch.n_seq, ("int32",)
         weights_out = weights if weights_out is None else weights_out

@@ -157,7 +157,7 @@ template <int NT> __device__ __forceinline__ int2 bin_of_hist(int *hist, int wan
 // is kept is found by its digits from the highest on (12, 12 and 8 bits), each from a
 // histogram of the keys that have the digits before it.  A wave keeps the keys of its first NK pages in
 // registers and of the next NL in LDS; those behind are read again for each digit.  Bound by its chain of loads, scans
-// and barriers: 8 sequences of 577 tokens, 20 heads, 10 us (bins that share a bank 13), 32 of 1,900 to 6,000, 8 heads, 16.
+// and barriers: 8 sequences of 577 tokens, 20 heads, 9 us (bins that share a bank 13), 32 of 1,900 to 6,000, 8 heads, 15.
 constexpr int RUN = 8;
 template <int NT, int NK, int NL> __global__ __launch_bounds__(NT) void k_kv8_choose(Kv8Evict e, void *ws) {
     constexpr int PER = BINS / NT, NW = NT / 64;
@@ -558,7 +558,7 @@ __device__ __forceinline__ unsigned shrink4(unsigned w, float r) {
 // the source page's codes as they lie there, 16 tokens of a dim a lane; what comes out, four places of a dim a
 // lane, is a word of the new page but for its scale.  Source pages add up.  (Other ways for 32 sequences to 2,048 tokens, 8 heads
 // of 128: a load from memory for each byte keeps the address unit busy, 107 us; rows through LDS and bytes there, a dim a
-// lane, 103; this way 92: the 252 MB that it cannot do without at 2.7 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
+// lane, 103; this way 90: the 252 MB that it cannot do without at 2.8 TB/s.)  K: 16 dims of a token a lane.  Bound by the chain of
 // ticket, list, codes and flag, which two workgroups of 88 registers on a CU do not hide; 80 registers spill (115), 16 dims a wave (52 registers) double the workgroups and draws (118), 1,024 threads are no better (101).
 constexpr int MOST_POLLS = 1 << 20;
 constexpr int MOVE_THREADS = 512;

@@ -61,7 +61,8 @@ constexpr int WEIGH_WAVES = 4;
 
 // At most 16 columns: one workgroup per (sequence, kv head, pps pages), its waves take the pages
 // in turn, the next page's keys under way; the query is an integer in three bytes, as in attention.  Bound by
-// the bytes of K: 64 rows of 1,025 to 8,190 tokens, 8 heads of 128, 321 MB in 74 us, 4.3 TB/s.
+// the bytes of K: 64 rows of 1,025 to 8,190 tokens, 8 heads of 128, 321 MB in 69 us, 4.6 TB/s.
+// All pages of the sequence are read, also those that a window hides from every row.
 template <int DP, class T>
 __global__ __launch_bounds__(64 * WEIGH_WAVES) void k_kv8_weigh(Kv8Weigh w, int g, int pps) {
     constexpr int KS = Tile<DP>::KS;
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(64 * WEIGH_WAVES) void k_kv8_weigh(Kv8Weigh w, int 
 // are (FP32 rows: two f16, hi + lo, under a power of two of the column's own).  sp pages a workgroup: with less than
 // eight, the waves of a page share the columns among them.  Bound by issue: a weight costs a multiply-add, an exponential
 // (four issue slots) and a sum, 55% of the clocks, the products 30%, and the two take turns: 2,047 rows of 16,000 tokens,
-// 32 heads over 8 of 128, 326 us, 770 TFLOP/s.  (One wave that reads its queries itself 588; exponentials
+// 32 heads over 8 of 128, 324 us, 775 TFLOP/s (FP32 rows, two products a score, 474).  (One wave that reads its queries itself 588; exponentials
 // between the next tile's products by hand 337.)
 template <class T> struct Half {
     typedef _Float16 one;

@@ -15,12 +15,13 @@
 // One pass sums what is left of p, max(e_p - r e_q, 0) with r = Z_p / Z_q, before r is known in 64 bits: the tokens that count
 // are those with e_p / e_q > r, and with r from the FP32 sums they are the same ones unless a token's ratio lies
 // between the two.  The pass keeps the sums of e_p and e_q over them, and how near to r the nearest ratio is; where the 64-bit r
-// turns out to be further away than that (one row of a hundred, or where p and q differ in a few tokens
-// only), the last workgroup sums the row again.
+// turns out to be further away than that, the last workgroup sums the row again: of FP32 rows of 131,072 tokens one in a hundred where
+// the draft's logits are 1 off the target's, a tenth at 0.03 to 0.1, a third at 0.01 (16-bit rows, whose ratios lie apart: none in a hundred).
+// That one workgroup needs 200 us (finish of 64 FP32 sequences 37 -> 240).
 //
-// 64 sequences of 3 to 7 drafts over 131,072 tokens (bfloat16): rows 30 us, bound by bytes (168 MB at 5.6 TB/s, a part from the
-// last-level cache), finish 37, bound by the 64-bit exponentials of 64 rows of p and q and three turns of dependent
-// loads; 8 drafted streams over 33 tokens (narrow) 4.5, a chain of loads and sums.
+// 64 sequences of 3 to 7 drafts over 131,072 tokens (bfloat16): rows 29 us, bound by bytes (168 MB at 5.7 TB/s, a part from the
+// last-level cache), finish 34, bound by the 64-bit exponentials of 64 rows of p and q and three turns of dependent
+// loads; 8 drafted streams over 33 tokens (narrow) 4.3, a chain of loads and sums.
 #include <float.h>
 
 #include <type_traits>
